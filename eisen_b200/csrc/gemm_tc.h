@@ -44,6 +44,14 @@ int gemm_bf16_pair_multi_n(cudaStream_t stream, int a_mn, int b_mn, int M, int K
                            const void* const* B, const long long* ldb, const int* N, void* const* C, const long long* ldc,
                            const int* out_mode, int split_k, float alpha, const float* rope_table, int seq_len,
                            int head_dim, int* status, const char** err);
+// head projection with a cross-entropy epilogue (linear_ce.cu): the logits' row statistics (grad = 0) or the
+// logits' gradients in bf16 (grad = 1) are written, the logits are not
+int gemm_bf16_pair_ce(cudaStream_t stream, int b_mn, int M, int N, int K, const void* A, long long lda, const void* B,
+                      long long ldb, int grad, const int* targets, int ignore_index, int vocab, int col_base, float2* stats,
+                      float* target_logit, const float* lse, const float* grad_out, float normalizer, void* D, long long ldd,
+                      int* status, const char** err);
+// columns of the output tile one statistics entry of gemm_bf16_pair_ce covers
+constexpr int GEMM_CE_COLS = 256;
 int gemm_pair_auto_split_k(int M, int N, int K);
 // m-tiles per band of the paired kernel's tile order; 0 = chosen by the DRAM-traffic model
 void gemm_pair_set_band(int band);

@@ -53,6 +53,14 @@ struct PairParams {
   int rope_s, rope_hd;
   float alpha;
   int* status;
+  // cross-entropy epilogues (the LCE instantiations): the product is a tile of logits that is never stored
+  const int* targets;
+  const float* lse;       // LCE_GRAD
+  const float* grad_out;  // LCE_GRAD, device scalar, null for 1
+  float2* stats;          // LCE_STATS: [n_tiles][M] (maximum, sum of exp(x - maximum)) of a row's 256 columns
+  float* target_logit;    // LCE_STATS: [M]
+  float normalizer;
+  int ignore_index, vocab, col_base;  // col_base: vocabulary index of column 0
   // segmented launches (the SEG instantiation of the kernel only).
   // K segments: the k-blocks from kseg[1] on come from the operand pair (A2, B2), those from kseg[2]
   // on from (A3, B3): C = A1 B1^T + A2 B2^T + A3 B3^T without intermediate roundings.
@@ -83,7 +91,34 @@ struct SegMaps {
   CUtensorMap b;     // B3 (B2 travels in the dual mode's slot)
 };
 
-template <bool SEG>
+// Epilogues of the head projection under a cross-entropy (linear_ce.cu).  A thread of the epilogue owns one
+// row of the tile, so both need no exchange between threads.
+//   LCE_STATS: running maximum and sum of exponentials over the row's 256 f32 accumulators -> stats; the
+//     target's logit -> target_logit.  About four instructions per entry on four warps (some 1500 clocks per
+//     tile) beside 8 * K clocks of tensor-core work: hidden from K = 256 on.
+//   LCE_GRAD: (exp(x - lse) - [column is the target]) * normalizer * grad_out, rounded once to bf16 (the
+//     operand type of the two gradient products) -> C.  Rows that do not count are written as zeros whatever
+//     their accumulators hold.
+constexpr int LCE_NONE = 0, LCE_STATS = 1, LCE_GRAD = 2;
+constexpr float LOG2E = 1.4426950408889634f;
+
+__device__ __forceinline__ float lce_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 32 accumulators of one row -> their gradients.  nl = -lse * log2(e), at = target column - first column.
+__device__ __forceinline__ void lce_grad32(uint32_t (&r)[32], float nl, float scale, bool counts, int at) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    float d = lce_ex2(fmaf(__uint_as_float(r[i]), LOG2E, nl));
+    if (i == at) d -= 1.0f;
+    r[i] = counts ? __float_as_uint(d * scale) : 0u;
+  }
+}
+
+template <bool SEG, int LCE = LCE_NONE>
 __global__ void __launch_bounds__(P_THREADS, 1)
 gemm_bf16_tc2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                      const __grid_constant__ CUtensorMap tmB2, const __grid_constant__ SegMaps seg_maps,
@@ -270,7 +305,100 @@ gemm_bf16_tc2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
                           row0 + 32 <= p.M && n0 + PN <= Nn && (ldc % 8) == 0 &&
                           (reinterpret_cast<uintptr_t>(Cp) & 15) == 0 &&
                           (!acc_bf16 || ((ldr % 8) == 0 && (reinterpret_cast<uintptr_t>(Rp) & 15) == 0));
-      if (p.dual) {
+      if constexpr (LCE == LCE_STATS) {
+        const int at = row_ok ? p.targets[row] : -1;
+        float m = -INFINITY, sum = 0.0f, xt = 0.0f;
+        bool found = false;
+#pragma unroll 1
+        for (int c = 0; c < PN / 32; ++c) {
+          const int left = Nn - n0 - c * 32;  // columns of this chunk that exist
+          if (left <= 0) break;
+          uint32_t r[32];
+          tmem_ld_32x32b_x32(taddr + c * 32, r);
+          tmem_ld_wait();
+          if (left < 32) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (i >= left) r[i] = 0xff800000u;
+          }
+          float cm = __uint_as_float(r[0]);
+#pragma unroll
+          for (int i = 1; i < 32; ++i) cm = fmaxf(cm, __uint_as_float(r[i]));
+          const float nm = fmaxf(m, cm);
+          const float nl = nm == -INFINITY ? 0.0f : -nm * LOG2E;
+          sum *= m == -INFINITY ? 0.0f : lce_ex2(fmaf(m, LOG2E, nl));
+          float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int i = 0; i < 32; ++i) part[i & 3] += lce_ex2(fmaf(__uint_as_float(r[i]), LOG2E, nl));
+          sum += (part[0] + part[1]) + (part[2] + part[3]);
+          m = nm;
+          const int in = at - n0 - c * 32;
+          if (in >= 0 && in < 32 && in < left) {
+            found = true;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (i == in) xt = __uint_as_float(r[i]);
+          }
+        }
+        if (row_ok) {
+          p.stats[(long long)nt * p.M + row] = make_float2(m, sum);
+          if (found) p.target_logit[row] = xt;
+        }
+      } else if constexpr (LCE == LCE_GRAD) {
+        const int tgt = row_ok ? p.targets[row] : -1;
+        const bool counts = row_ok && tgt != p.ignore_index && tgt >= 0 && tgt < p.vocab;
+        const float nl = counts ? -p.lse[row] * LOG2E : 0.0f;
+        const float scale = p.normalizer * (p.grad_out ? *p.grad_out : 1.0f);
+        const int at0 = tgt - p.col_base - n0;
+        if (staged) {
+          uint8_t* st = epi_stage + q * (32 * 128);
+          const int rr = lane >> 3, seg = lane & 7;
+          __nv_bfloat16* c_base = reinterpret_cast<__nv_bfloat16*>(Cp) + (long long)(row0 + rr) * ldc + n0 + seg * 8;
+#pragma unroll 1
+          for (int c = 0; c < PN / 64; ++c) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t r[32];
+              tmem_ld_32x32b_x32(taddr + c * 64 + h * 32, r);
+              tmem_ld_wait();
+              lce_grad32(r, nl, scale, counts, at0 - c * 64 - h * 32);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                uint4 o;
+                o.x = pack_bf16x2(__uint_as_float(r[8 * j + 0]), __uint_as_float(r[8 * j + 1]));
+                o.y = pack_bf16x2(__uint_as_float(r[8 * j + 2]), __uint_as_float(r[8 * j + 3]));
+                o.z = pack_bf16x2(__uint_as_float(r[8 * j + 4]), __uint_as_float(r[8 * j + 5]));
+                o.w = pack_bf16x2(__uint_as_float(r[8 * j + 6]), __uint_as_float(r[8 * j + 7]));
+                *reinterpret_cast<uint4*>(st + lane * 128 + (((j + 4 * h) ^ (lane & 7)) << 4)) = o;
+              }
+            }
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int rw = 4 * i + rr;
+              const uint4 o = *reinterpret_cast<const uint4*>(st + rw * 128 + ((seg ^ (rw & 7)) << 4));
+              *reinterpret_cast<uint4*>(c_base + (long long)(4 * i) * ldc + c * 64) = o;
+            }
+            __syncwarp();
+          }
+        } else {
+          const uint4 none[4] = {};
+#pragma unroll 1
+          for (int c = 0; c < PN / 32; ++c) {
+            const int col0 = n0 + c * 32;
+            uint32_t r[32];
+            tmem_ld_32x32b_x32(taddr + c * 32, r);
+            tmem_ld_wait();
+            if (row_ok && col0 < Nn) {
+              lce_grad32(r, nl, scale, counts, at0 - c * 32);
+              float v[32];
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+              gemm_store_chunk32(Cp, ldc, Cp, ldc, GEMM_OUT_BF16, row, col0, Nn, v, none, false);
+            }
+          }
+        }
+      } else if (p.dual) {
         // complete slabs only (the host checks M % 256 == 0 and N % 128 == 0).  Per 64 columns:
         // gate and up are rounded to bf16 first, H is computed from the rounded values (what the
         // separate SwiGLU kernel reads), then the three 32 x 64 slabs go through the staging tile
@@ -493,7 +621,7 @@ static int pair_band(int M, int N, int K, int m_tiles, int n_tiles) {
 }
 
 static int pair_launch(cudaStream_t stream, const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmB2,
-                       const PairParams& p, const char** err, const SegMaps* seg = nullptr) {
+                       const PairParams& p, const char** err, const SegMaps* seg = nullptr, int lce = LCE_NONE) {
   static bool attr_set[MAX_DEVICE_SLOTS] = {false};
   static const SegMaps no_seg = {};
   const int slot = device_slot();
@@ -501,6 +629,10 @@ static int pair_launch(cudaStream_t stream, const CUtensorMap& tmA, const CUtens
     cudaError_t e = cudaFuncSetAttribute(gemm_bf16_tc2_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, P_SMEM);
     if (e == cudaSuccess)
       e = cudaFuncSetAttribute(gemm_bf16_tc2_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, P_SMEM);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(gemm_bf16_tc2_kernel<false, LCE_STATS>, cudaFuncAttributeMaxDynamicSharedMemorySize, P_SMEM);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(gemm_bf16_tc2_kernel<false, LCE_GRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, P_SMEM);
     if (e != cudaSuccess) { if (err) *err = cudaGetErrorString(e); return 3; }
     attr_set[slot] = true;
   }
@@ -532,8 +664,11 @@ static int pair_launch(cudaStream_t stream, const CUtensorMap& tmA, const CUtens
   if (avail < 1) avail = 1;
   const int clusters = p.total_tiles < avail ? p.total_tiles : avail;
   cfg.gridDim = dim3(2 * clusters, 1, 1);
-  cudaError_t e = seg ? cudaLaunchKernelEx(&cfg, gemm_bf16_tc2_kernel<true>, tmA, tmB, tmB2, *seg, p)
-                      : cudaLaunchKernelEx(&cfg, gemm_bf16_tc2_kernel<false>, tmA, tmB, tmB2, no_seg, p);
+  cudaError_t e;
+  if (lce == LCE_STATS) e = cudaLaunchKernelEx(&cfg, gemm_bf16_tc2_kernel<false, LCE_STATS>, tmA, tmB, tmB2, no_seg, p);
+  else if (lce == LCE_GRAD) e = cudaLaunchKernelEx(&cfg, gemm_bf16_tc2_kernel<false, LCE_GRAD>, tmA, tmB, tmB2, no_seg, p);
+  else e = seg ? cudaLaunchKernelEx(&cfg, gemm_bf16_tc2_kernel<true>, tmA, tmB, tmB2, *seg, p)
+               : cudaLaunchKernelEx(&cfg, gemm_bf16_tc2_kernel<false>, tmA, tmB, tmB2, no_seg, p);
   if (e != cudaSuccess) { if (err) *err = cudaGetErrorString(e); return 3; }
   return 0;
 }
@@ -819,6 +954,39 @@ int gemm_bf16_pair_rope(cudaStream_t stream, int M, int N, int K, const void* A,
   p.alpha = 1.0f;
   p.status = status;
   return pair_launch(stream, tmA, tmB, tmB, p, err);
+}
+
+// Head projection with one of the cross-entropy epilogues.  A is h [M, K] (K contiguous); B the head's columns
+// from its vocabulary index col_base on, N of them: [K, vocab] (b_mn = 1) or the tied table [vocab, K] (b_mn = 0),
+// `B` pointing at the first of them.  grad = 0: stats / target_logit are written; grad != 0: D [M, N] bf16.
+int gemm_bf16_pair_ce(cudaStream_t stream, int b_mn, int M, int N, int K, const void* A, long long lda, const void* B,
+                      long long ldb, int grad, const int* targets, int ignore_index, int vocab, int col_base, float2* stats,
+                      float* target_logit, const float* lse, const float* grad_out, float normalizer, void* D, long long ldd,
+                      int* status, const char** err) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  CUtensorMap tmA, tmB;
+  if (make_tmap_bf16_2d(&tmA, A, K, M, lda, 64, PM)) { if (err) *err = "linear_ce: cuTensorMapEncodeTiled failed for h"; return 2; }
+  if (b_mn ? make_tmap_bf16_2d(&tmB, B, N, K, ldb, 64, BK) : make_tmap_bf16_2d(&tmB, B, K, N, ldb, 64, PN / 2)) {
+    if (err) *err = "linear_ce: cuTensorMapEncodeTiled failed for w";
+    return 2;
+  }
+  PairParams p = {};
+  p.M = M; p.N = N; p.K = K;
+  p.a_mn = 0; p.b_mn = b_mn;
+  p.C = D; p.ldc = ldd; p.out_mode = GEMM_OUT_BF16;
+  p.R = D; p.ldr = ldd;
+  p.m_tiles = (M + 2 * PM - 1) / (2 * PM);
+  p.n_tiles = (N + PN - 1) / PN;
+  p.kblocks_total = (K + BK - 1) / BK;
+  pair_set_split(p, 1);
+  p.band = pair_band(M, N, K, p.m_tiles, p.n_tiles);
+  p.rope_s = 1; p.rope_hd = 2;
+  p.alpha = 1.0f;
+  p.status = status;
+  p.targets = targets; p.ignore_index = ignore_index; p.vocab = vocab; p.col_base = col_base;
+  p.stats = stats; p.target_logit = target_logit;
+  p.lse = lse; p.grad_out = grad_out; p.normalizer = normalizer;
+  return pair_launch(stream, tmA, tmB, tmB, p, err, nullptr, grad ? LCE_GRAD : LCE_STATS);
 }
 
 int gemm_pair_clusters_hint() { return gemm_num_sms() / 2; }

@@ -1,0 +1,218 @@
+// Head projection and cross-entropy in pieces of the vocabulary: x = h W is never stored.
+//
+//   forward   every 256-column tile of the product leaves (maximum, sum of exponentials) per row, formed from
+//             the f32 accumulators in the GEMM's epilogue (gemm_tc2.cu, LCE_STATS); ce_join_kernel adds them up:
+//             lse = M + ln sum_t s_t exp(m_t - M),  row loss = -ln(exp(x_y - lse) + 1e-8) * normalizer.
+//             2 rows k vocab FLOPs, 8 bytes per row and tile instead of 512 for the logits.
+//   backward  per piece of the vocabulary the tile is formed again and leaves
+//             D = (exp(x - lse) - onehot) * normalizer * grad  in bf16 (LCE_GRAD), then dH += D W^T and dW = H^T D
+//             by the library's GEMM.  8 rows k vocab FLOPs (6 with the logits at hand).
+//
+// The row statistics come from unrounded logits; a [rows, vocab] tensor of bf16 logits carries a rounding of up to
+// 2^-9 of a logit, 3 % of a probability at |x| = 16.  D is the one value rounded to bf16 on the way to the
+// gradients: the tensor cores take bf16 operands.
+#include <algorithm>
+#include <cstdio>
+
+#include "common.cuh"
+#include "errors.h"
+#include "gemm_tc.h"
+#include "../../include/eisen_b200.h"
+
+namespace eisen {
+namespace {
+
+constexpr int CJ_ROWS = 32, CJ_SLICES = 8;
+
+// One warp-wide group of 32 rows per CTA (lane = row: the statistics of a tile are contiguous in the row), the
+// tiles are dealt to CJ_SLICES warps and joined in shared memory.  A launch of one CTA also adds up the loss.
+__global__ void __launch_bounds__(CJ_ROWS * CJ_SLICES)
+ce_join_kernel(const float2* __restrict__ stats, const float* __restrict__ target_logit, const int* __restrict__ targets,
+               float* __restrict__ loss, float* __restrict__ row_loss, float* __restrict__ lse, long long rows, int tiles,
+               int vocab, int ignore_index, float normalizer, int* __restrict__ bad_target_flag) {
+  __shared__ float sh_m[CJ_SLICES][CJ_ROWS], sh_s[CJ_SLICES][CJ_ROWS];
+  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
+  const long long row = (long long)blockIdx.x * CJ_ROWS + lane;
+  float m = -INFINITY, s = 0.0f;
+  if (row < rows) {
+#pragma unroll 4
+    for (int t = slice; t < tiles; t += CJ_SLICES) {
+      const float2 v = stats[(long long)t * rows + row];
+      const float nm = fmaxf(m, v.x), ref = nm == -INFINITY ? 0.0f : nm;
+      s = s * expf(m - ref) + v.y * expf(v.x - ref);
+      m = nm;
+    }
+  }
+  sh_m[slice][lane] = m;
+  sh_s[slice][lane] = s;
+  __syncthreads();
+  if (slice == 0) {
+    float l = 0.0f;
+    if (row < rows) {
+      float gm = -INFINITY, gs = 0.0f;
+#pragma unroll
+      for (int i = 0; i < CJ_SLICES; ++i) gm = fmaxf(gm, sh_m[i][lane]);
+      const float ref = gm == -INFINITY ? 0.0f : gm;
+#pragma unroll
+      for (int i = 0; i < CJ_SLICES; ++i) gs += sh_s[i][lane] * expf(sh_m[i][lane] - ref);
+      const int t = targets[row];
+      float e = 0.0f;
+      if (t != ignore_index && t >= 0 && t < vocab) {
+        e = ref + logf(gs);
+        l = -logf(expf(target_logit[row] - e) + 1e-8f) * normalizer;
+      } else if (t != ignore_index && bad_target_flag) {
+        *bad_target_flag = 1;
+      }
+      row_loss[row] = l;
+      lse[row] = e;
+    }
+    if (gridDim.x == 1 && loss) {
+      l = warp_sum(l);
+      if (lane == 0) *loss = l;
+    }
+  }
+}
+
+struct CePlan {
+  long long piece, ld;                 // vocabulary entries of a piece, row stride of D
+  long long stats_bytes, fwd_bytes;    // forward: tile statistics, then the target logits
+  long long d_bytes, bwd_bytes;        // backward: D, then dH in f32
+  bool dh_f32;                         // dH is added up in f32 over the pieces (or k slices) and then rounded
+};
+
+constexpr long long up256(long long n) { return (n + 255) & ~255LL; }
+
+CePlan ce_plan(long long rows, long long k, long long vocab, long long piece) {
+  CePlan p;
+  // D of the default piece takes about CE_D_BYTES
+  constexpr long long CE_D_BYTES = 256LL << 20;
+  const long long all = (vocab + GEMM_CE_COLS - 1) / GEMM_CE_COLS * GEMM_CE_COLS;
+  if (piece <= 0) piece = CE_D_BYTES / (2 * std::max<long long>(rows, 1));
+  piece = std::max<long long>(piece / GEMM_CE_COLS * GEMM_CE_COLS, GEMM_CE_COLS);
+  const long long n = (all + std::min(piece, all) - 1) / std::min(piece, all);
+  piece = ((all + n - 1) / n + GEMM_CE_COLS - 1) / GEMM_CE_COLS * GEMM_CE_COLS;  // pieces of about the same size
+  p.piece = piece;
+  p.ld = piece;
+  const long long tiles = all / GEMM_CE_COLS;
+  p.stats_bytes = up256(tiles * rows * 8);
+  p.fwd_bytes = p.stats_bytes + up256(rows * 4);
+  p.d_bytes = up256(rows * p.ld * 2);
+  // one piece and enough output tiles to fill the machine: dH leaves the product in bf16
+  const long long tiles_dh = ((rows + 255) / 256) * ((k + 255) / 256);
+  p.dh_f32 = n > 1 || tiles_dh < 48;
+  p.bwd_bytes = p.d_bytes + (p.dh_f32 ? up256(rows * k * 4) : 0);
+  return p;
+}
+
+int ce_check(const char* what, const void* h, long long ldh, const void* w, long long ldw, int trans_b, const void* targets,
+             const void* workspace, long long rows, long long k, long long vocab) {
+  static thread_local char msg[160];
+  auto bad = [&](int code, const char* why) {
+    snprintf(msg, sizeof(msg), "%s: %s", what, why);
+    return fail(code, msg);
+  };
+  if (rows < 0 || k <= 0 || vocab <= 0) return bad(EISEN_ERR_INVALID, "rows must not be negative, k and vocab must be positive");
+  if (rows > 0x7fffff00LL || k > 0x7fffff00LL || vocab > 0x7fffff00LL) return bad(EISEN_ERR_LIMIT, "a dimension exceeds 2^31 - 256");
+  if (!h || !w || !targets || !workspace) return bad(EISEN_ERR_INVALID, "h, w, targets and workspace must not be null");
+  if (ldh < k || ldw < (trans_b ? k : vocab)) return bad(EISEN_ERR_INVALID, "a leading dimension is shorter than its row");
+  if ((ldh % 8) || (ldw % 8) || !aligned16(h) || !aligned16(w) || !aligned16(workspace))
+    return bad(EISEN_ERR_INVALID, "h, w and workspace must be 16-byte aligned, leading dimensions multiples of 8");
+  return 0;
+}
+
+}  // namespace
+}  // namespace eisen
+
+extern "C" {
+
+long long eisen_linear_ce_workspace_bytes(long long rows, long long k, long long vocab, long long piece, int backward) {
+  using namespace eisen;
+  if (rows <= 0 || k <= 0 || vocab <= 0) return 256;
+  const CePlan p = ce_plan(rows, k, vocab, piece);
+  return backward ? std::max(p.fwd_bytes, p.bwd_bytes) : p.fwd_bytes;
+}
+
+int eisen_linear_ce_fwd(void* stream, const void* h, long long ldh, const void* w, long long ldw, int trans_b, const int* targets,
+                        float* loss, float* row_loss, float* lse, void* workspace, long long rows, long long k, long long vocab,
+                        int ignore_index, float normalizer, int* bad_target_flag, int* status) {
+  using namespace eisen;
+  if (rows == 0) {
+    if (loss && cudaMemsetAsync(loss, 0, 4, (cudaStream_t)stream) != cudaSuccess) return fail(EISEN_ERR_CUDA, "linear_ce_fwd: memset");
+    return 0;
+  }
+  int rc = ce_check("linear_ce_fwd", h, ldh, w, ldw, trans_b, targets, workspace, rows, k, vocab);
+  if (rc) return rc;
+  if (!row_loss || !lse) return fail(EISEN_ERR_INVALID, "linear_ce_fwd: row_loss and lse must not be null");
+  const CePlan p = ce_plan(rows, k, vocab, 0);
+  float2* stats = (float2*)workspace;
+  float* target_logit = (float*)((char*)workspace + p.stats_bytes);
+  const char* err = nullptr;
+  rc = gemm_bf16_pair_ce((cudaStream_t)stream, trans_b ? 0 : 1, (int)rows, (int)vocab, (int)k, h, ldh, w, ldw, 0, targets,
+                         ignore_index, (int)vocab, 0, stats, target_logit, nullptr, nullptr, 0.0f, nullptr, 0, status, &err);
+  if (rc) return fail(EISEN_ERR_CUDA, err ? err : "linear_ce_fwd failed");
+  count_launch();
+  const unsigned grid = (unsigned)((rows + CJ_ROWS - 1) / CJ_ROWS);
+  ce_join_kernel<<<grid, CJ_ROWS * CJ_SLICES, 0, (cudaStream_t)stream>>>(
+      stats, target_logit, targets, loss, row_loss, lse, rows, (int)((vocab + GEMM_CE_COLS - 1) / GEMM_CE_COLS), (int)vocab,
+      ignore_index, normalizer, bad_target_flag);
+  rc = check_launch("linear_ce_join");
+  if (rc || !loss || grid == 1) return rc;
+  return eisen_ce_loss_reduce(stream, row_loss, loss, rows);
+}
+
+int eisen_linear_ce_bwd(void* stream, const void* h, long long ldh, const void* w, long long ldw, int trans_b, const int* targets,
+                        const float* lse, const float* grad_out, void* dh, int accumulate_dh, void* dw, long long lddw,
+                        int dw_dtype, int accumulate_dw, void* workspace, long long rows, long long k, long long vocab,
+                        long long piece, int ignore_index, float normalizer, int* status) {
+  using namespace eisen;
+  cudaStream_t s = (cudaStream_t)stream;
+  const long long dw_rows = trans_b ? vocab : k, dw_cols = trans_b ? k : vocab;
+  if (dw && (dw_dtype != DT_F32 && dw_dtype != DT_BF16)) return fail(EISEN_ERR_INVALID, "linear_ce_bwd: dw must be f32 or bf16");
+  if (dw && lddw < dw_cols) return fail(EISEN_ERR_INVALID, "linear_ce_bwd: lddw is shorter than a row of dw");
+  if (rows == 0) {
+    const size_t es = dw_dtype == DT_F32 ? 4 : 2;
+    if (dw && !accumulate_dw && dw_cols > 0 && dw_rows > 0 &&
+        cudaMemset2DAsync(dw, (size_t)lddw * es, 0, (size_t)dw_cols * es, (size_t)dw_rows, s) != cudaSuccess)
+      return fail(EISEN_ERR_CUDA, "linear_ce_bwd: memset");
+    return 0;
+  }
+  int rc = ce_check("linear_ce_bwd", h, ldh, w, ldw, trans_b, targets, workspace, rows, k, vocab);
+  if (rc) return rc;
+  if (!lse || (!dh && !dw)) return fail(EISEN_ERR_INVALID, "linear_ce_bwd: lse and one of dh, dw must not be null");
+  if (!aligned16(dh) || !aligned16(dw)) return fail(EISEN_ERR_INVALID, "linear_ce_bwd: dh and dw must be 16-byte aligned");
+  if (k % 8) return fail(EISEN_ERR_INVALID, "linear_ce_bwd: k must be a multiple of 8");
+  const CePlan p = ce_plan(rows, k, vocab, piece);
+  char* d = (char*)workspace;
+  float* dh32 = (float*)(d + p.d_bytes);
+  if (dh && p.dh_f32 && cudaMemsetAsync(dh32, 0, (size_t)rows * k * 4, s) != cudaSuccess)
+    return fail(EISEN_ERR_CUDA, "linear_ce_bwd: memset");
+  for (long long c0 = 0; c0 < vocab; c0 += p.piece) {
+    const long long n = std::min(p.piece, vocab - c0);
+    const char* wp = (const char*)w + 2 * (trans_b ? c0 * ldw : c0);
+    const char* err = nullptr;
+    rc = gemm_bf16_pair_ce(s, trans_b ? 0 : 1, (int)rows, (int)n, (int)k, h, ldh, wp, ldw, 1, targets, ignore_index, (int)vocab,
+                           (int)c0, nullptr, nullptr, lse, grad_out, normalizer, d, p.ld, status, &err);
+    if (rc) return fail(EISEN_ERR_CUDA, err ? err : "linear_ce_bwd failed");
+    count_launch();
+    if (dh) {  // dH[rows, k] += D[rows, n] W_piece^T
+      rc = p.dh_f32 ? eisen_gemm_bf16(stream, 0, trans_b ? 1 : 0, rows, k, n, d, p.ld, wp, ldw, dh32, k, GEMM_OUT_F32_ATOMIC, 0,
+                                      1.0f, status)
+                    : eisen_gemm_bf16(stream, 0, trans_b ? 1 : 0, rows, k, n, d, p.ld, wp, ldw, dh, k,
+                                      accumulate_dh ? GEMM_OUT_BF16_ACC : GEMM_OUT_BF16, 1, 1.0f, status);
+      if (rc) return rc;
+    }
+    if (dw) {  // dW[k, piece] = H^T D, or with the tied table dW[piece, k] = D^T H
+      char* out = (char*)dw + (dw_dtype == DT_F32 ? 4 : 2) * (trans_b ? c0 * lddw : c0);
+      const int mode = dw_dtype == DT_F32 ? (accumulate_dw ? GEMM_OUT_F32_ATOMIC : GEMM_OUT_F32)
+                                          : (accumulate_dw ? GEMM_OUT_BF16_ACC : GEMM_OUT_BF16);
+      const int split = mode == GEMM_OUT_F32_ATOMIC ? 0 : 1;
+      rc = trans_b ? eisen_gemm_bf16(stream, 1, 1, n, k, rows, d, p.ld, h, ldh, out, lddw, mode, split, 1.0f, status)
+                   : eisen_gemm_bf16(stream, 1, 1, k, n, rows, h, ldh, d, p.ld, out, lddw, mode, split, 1.0f, status);
+      if (rc) return rc;
+    }
+  }
+  if (dh && p.dh_f32) return eisen_accumulate(stream, dh, DT_BF16, dh32, DT_F32, rows * k, accumulate_dh);
+  return 0;
+}
+
+}  // extern "C"

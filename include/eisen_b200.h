@@ -293,6 +293,74 @@ int eisen_ce_fused(void* stream, void* logits, const int* targets, float* loss, 
 int eisen_ce_loss_reduce(void* stream, const float* row_loss, float* loss, long long rows);
 
 /* ------------------------------------------------------------------------------------------
+ * The vocabulary end of a model: a teacher's top logits, the loss of a student against them, and head
+ * projection with cross-entropy without logits (no counterpart in the reference, whose only loss is the
+ * cross-entropy above)
+ * ------------------------------------------------------------------------------------------ */
+
+/* values [rows, k] (f32) and ids [rows, k]: the k largest logits of every row in descending order; equal
+ * values (-0 equals +0) come with the lowest id first, NaN counts as the largest value.  lse [rows] (may be
+ * null) = ln sum exp(x / temperature).  logits: rows of `vocab` entries, `ld` entries apart; a row may start at
+ * any element.  1 <= k <= min(vocab, 256). */
+int eisen_top_logits(void* stream, const void* logits, long long ld, float* values, int* ids, float* lse, long long rows,
+                     long long vocab, long long k, float temperature, int dtype);
+
+/* Distillation from a teacher's top logits, with the cross-entropy of hard targets beside it.  Per row
+ *   loss_r = kd_weight T^2 sum_j q_j (ln q_j - ln p_{id_j}) - ce_weight ln(softmax(x)_y + 1e-8)
+ * with p = softmax(x / T), T = temperature, and the teacher's distribution over its k entries
+ *   q_j = exp(t_j / T - l),  l = teacher_lse[r] (the log-sum-exp of its whole row at T), or, where teacher_lse is
+ *   null, the log-sum-exp of the entries themselves (q then sums to 1).
+ * Gradient of a row: kd_weight T (Q p_i - sum of q_j with id_j = i) + ce_weight (softmax(x)_i - [i = y]), Q = sum q_j;
+ * the 1e-8 takes no part in it (as in eisen_ce_bwd).
+ *   teacher_ids [rows, k] int32: negative entries are absent (their teacher_logits are not read); ids may repeat.
+ *     An id >= vocab raises *bad_id_flag and counts as absent.  A row without entries has no distillation term.
+ *   teacher_logits [rows, k] f32.  1 <= k <= 1024.
+ *   targets [rows] int32, or null (every row counts; ce_weight must then be 0).  Rows whose target is ignore_index
+ *     have loss 0 and gradient 0, whatever their logits hold; a target outside [0, vocab) raises *bad_id_flag and its
+ *     row is skipped the same way.
+ *   A weight of 0 removes its term.  A counted row needs a finite logit.
+ *   lse [2, rows]: log-sum-exp of x / T, then of x (0 for skipped rows); may be null except in eisen_distill_bwd,
+ *   which takes what the forward left.  *loss = sum of row_loss in a fixed order; loss may be null.
+ * eisen_distill_fused forms loss and dlogits (times grad_scale) in one pass over the logits, for an op that ends in
+ * the loss; eisen_distill_bwd forms dlogits (op)= gradient * (*grad_out) (null: 1).  dlogits may alias logits
+ * (same pointer, same row stride); otherwise the two must not overlap.  ld / ld_d: row strides in entries. */
+int eisen_distill_fwd(void* stream, const void* logits, long long ld, const int* teacher_ids, const float* teacher_logits,
+                      const float* teacher_lse, const int* targets, float* loss, float* row_loss, float* lse, long long rows,
+                      long long vocab, long long k, int ignore_index, float temperature, float kd_weight, float ce_weight, int dtype,
+                      int* bad_id_flag);
+int eisen_distill_bwd(void* stream, const void* logits, long long ld, const int* teacher_ids, const float* teacher_logits,
+                      const float* teacher_lse, const int* targets, const float* lse, void* dlogits, long long ld_d,
+                      const float* grad_out, long long rows, long long vocab, long long k, int ignore_index, float temperature,
+                      float kd_weight, float ce_weight, int dtype, int accumulate);
+int eisen_distill_fused(void* stream, const void* logits, long long ld, const int* teacher_ids, const float* teacher_logits,
+                        const float* teacher_lse, const int* targets, void* dlogits, long long ld_d, float* loss, float* row_loss,
+                        float* lse, long long rows, long long vocab, long long k, int ignore_index, float temperature, float kd_weight,
+                        float ce_weight, float grad_scale, int dtype, int* bad_id_flag);
+
+/* Head projection and cross-entropy in pieces of the vocabulary, bf16 operands, no logits kept:
+ *   x = h W (f32 accumulators, never stored or rounded), row loss = -ln(softmax(x)_t + 1e-8) * normalizer.
+ * h [rows, k] with leading dimension ldh; w [k, vocab], or with trans_b the tied table [vocab, k], leading dimension
+ * ldw.  targets, ignore_index, normalizer, loss, row_loss, lse and bad_target_flag as in eisen_ce_fwd (lse is required).
+ * The backward forms the logits again, `piece` vocabulary entries at a time (rounded to a multiple of 256; 0 = chosen
+ * so that one [rows, piece] bf16 slab takes about 256 MB), and
+ *   dh [rows, k] bf16 (op)= D W^T,  dw (layout of w, leading dimension lddw, dw_dtype EISEN_BF16 or EISEN_F32) (op)= H^T D,
+ *   D = bf16((softmax(x) - onehot) * normalizer * (*grad_out)), zero for rows that do not count; dh or dw may be null.
+ * Sums over tokens and vocabulary are f32; dh is added up in f32 over the pieces and rounded once.  Hidden states of
+ * rows that do not count must be finite where dw is asked for (their zero gradient multiplies them).
+ * ldh and ldw must be multiples of 8, k one of 8 in the backward; h, w, dh, dw and workspace 16-byte aligned.
+ * `workspace` holds eisen_linear_ce_workspace_bytes(rows, k, vocab, piece, backward) bytes of scratch; the amount
+ * for backward = 1 serves both calls.  Outside the fixed-order mode dh (and an f32 dw that is accumulated) may be
+ * summed over k slices in an order that varies.  status as in eisen_gemm_bf16. */
+long long eisen_linear_ce_workspace_bytes(long long rows, long long k, long long vocab, long long piece, int backward);
+int eisen_linear_ce_fwd(void* stream, const void* h, long long ldh, const void* w, long long ldw, int trans_b, const int* targets,
+                        float* loss, float* row_loss, float* lse, void* workspace, long long rows, long long k, long long vocab,
+                        int ignore_index, float normalizer, int* bad_target_flag, int* status);
+int eisen_linear_ce_bwd(void* stream, const void* h, long long ldh, const void* w, long long ldw, int trans_b, const int* targets,
+                        const float* lse, const float* grad_out, void* dh, int accumulate_dh, void* dw, long long lddw,
+                        int dw_dtype, int accumulate_dw, void* workspace, long long rows, long long k, long long vocab,
+                        long long piece, int ignore_index, float normalizer, int* status);
+
+/* ------------------------------------------------------------------------------------------
  * Elementwise / layout ops
  * ------------------------------------------------------------------------------------------ */
 int eisen_fill_f32(void* stream, float* p, float value, long long n);                  /* fill_f32, ops_f32.cu:101 */
