@@ -14,6 +14,7 @@
 
 #include "common.cuh"
 #include "errors.h"
+#include "row_slice.cuh"
 #include "../../include/eisen_b200.h"
 
 namespace eisen {
@@ -196,6 +197,7 @@ struct DistillParams {
   float temperature, inv_t, kd_weight, ce_weight, grad_scale;
   int accumulate;
   int* bad_id_flag;
+  int sum_kind, grad_kind, cluster;  // distill_row_kernel: see RowExp
 };
 
 constexpr int DS_FWD = 1, DS_BWD = 2;
@@ -334,6 +336,336 @@ distill_kernel(const DistillParams p) {
   }
 }
 
+// A row's exponentials exp((x - ref) / T) and exp(x - ref).  KIND says how they are formed:
+//   ONE   the first alone (temperature 1, or no cross-entropy term)
+//   TWO   both, each by itself
+//   PLAIN the f32 form, (x - ref) first and expf: rows of f32 logits, and rows whose largest entry is near the end of
+//         the type's range (all of it masked by the lowest value), where the products with ref would overflow
+//   10 a + b   bf16 rows whose temperature is b / a: h = exp((x - ref) / b), the exponentials are h^a and h^b.  The
+//         special-function unit gives 16 results per clock and SM: two exponentials in both passes over a row are 8000
+//         clocks per 32000 entries where the memory needs 5600, one is 4000.  A power multiplies the relative error of
+//         h (2^-22) by at most 7, far below the 2^-8 of the bf16 result.
+constexpr int ONE = 0, TWO = 1, PLAIN = 2;
+
+template <typename T, int KIND>
+struct RowExp {
+  float ref, inv_t, c, off, off1;
+  bool two;
+  __device__ __forceinline__ RowExp(float r, float it, bool both) : ref(r), inv_t(it), two(both) {
+    c = 1.4426950408889634f * (KIND < 10 ? it : 1.0f / (float)(KIND % 10));
+    off = -r * c;
+    off1 = -r * 1.4426950408889634f;
+  }
+  __device__ __forceinline__ void operator()(float x, float& et, float& e1) const {
+    if constexpr (KIND == PLAIN) {
+      et = expf((x - ref) * inv_t);
+      e1 = two ? expf(x - ref) : 0.0f;
+    } else if constexpr (KIND == ONE) {
+      et = exp2_approx(fmaf(x, c, off));
+      e1 = 0.0f;
+    } else if constexpr (KIND == TWO) {
+      et = exp2_approx(fmaf(x, c, off));
+      e1 = exp2_approx(fmaf(x, 1.4426950408889634f, off1));
+    } else {
+      constexpr int A = KIND / 10, B = KIND % 10;
+      const float h = exp2_approx(fmaf(x, c, off)), h2 = h * h;
+      et = A == 1 ? h : h2;
+      if constexpr (B == 1) e1 = h;
+      else if constexpr (B == 2) e1 = h2;
+      else if constexpr (B == 3) e1 = h2 * h;
+      else if constexpr (B == 4) e1 = h2 * h2;
+      else if constexpr (B == 5) e1 = h2 * h2 * h;
+      else e1 = h2 * h2 * (h2 * h);
+    }
+  }
+};
+
+// f(RowExp) for the kind that the row takes: one branch per pass, the same for the whole CTA
+template <typename T, typename F>
+__device__ __forceinline__ void with_exp(int kind, float ref, float inv_t, F f) {
+  if constexpr (sizeof(T) == 4) {
+    f(RowExp<T, PLAIN>(ref, inv_t, kind != ONE));
+  } else {
+    if (fabsf(ref) > 1e30f) return f(RowExp<T, PLAIN>(ref, inv_t, kind != ONE));
+    switch (kind) {
+      case ONE: return f(RowExp<T, ONE>(ref, inv_t, false));
+      case TWO: return f(RowExp<T, TWO>(ref, inv_t, true));
+      case 12: return f(RowExp<T, 12>(ref, inv_t, true));
+      case 13: return f(RowExp<T, 13>(ref, inv_t, true));
+      case 14: return f(RowExp<T, 14>(ref, inv_t, true));
+      case 21: return f(RowExp<T, 21>(ref, inv_t, true));
+      case 23: return f(RowExp<T, 23>(ref, inv_t, true));
+      case 25: return f(RowExp<T, 25>(ref, inv_t, true));
+      default: return f(RowExp<T, 27>(ref, inv_t, true));
+    }
+  }
+}
+
+// the kind for both exponentials at a temperature
+int exp_kind(float temperature, int dtype) {
+  if (dtype == DT_BF16)
+    for (int a = 1; a <= 2; ++a)
+      for (int b = 1; b <= (a == 1 ? 4 : 7); ++b)
+        if ((a == 1 || b % 2) && temperature * (float)a == (float)b && temperature != 1.0f) return 10 * a + b;
+  return TWO;
+}
+
+// A row in the registers of one CTA, or of a cluster of p.cluster CTAs with a slice of the vectors each: the
+// logits are read once, by loads that are all in flight together, and two CTAs per SM (eight of 128 threads for
+// short rows) work while the other one's loads are on their way.  The gradient pass takes the exponentials again
+// from the registers.  The teacher's entries go through shared memory beside the row's own maximum and sums;
+// entries with a term of their own are written after the dense pass, by the first thread among equal ids.
+template <typename T, int THREADS, int NV, int MODE>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
+distill_row_kernel(const DistillParams p) {
+  constexpr int V = VecOf<T>::N, WARPS = THREADS / 32;
+  constexpr int PAD = DS_MAX_K + 4;
+  constexpr bool FWD = (MODE & DS_FWD) != 0, BWD = (MODE & DS_BWD) != 0, ACC = BWD && !FWD;
+  __shared__ __align__(16) int s_id[PAD];  // the teacher's ids, -1: absent; entry k: the target
+  __shared__ float s_t[PAD];               // its logits / T
+  __shared__ float s_x[PAD];               // the student's logits there
+  __shared__ float s_old[ACC ? PAD : 1];   // what dlogits held there
+  __shared__ float s_max[2][WARPS], s_sum[4][WARPS];
+  __shared__ float s_xch[8][3];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int C = p.cluster, k = p.k, n = p.vocab;
+  const int rank = C > 1 ? (int)cluster_ctarank() : 0;
+  const long long row = C > 1 ? blockIdx.x / C : blockIdx.x;
+  if (FWD && C > 1) cluster_arrive();  // matched before the first access to a peer's shared memory
+  const T* xr = reinterpret_cast<const T*>(p.logits) + row * p.ld;
+  T* dr = BWD ? reinterpret_cast<T*>(p.dlogits) + row * p.ldd : nullptr;
+  const int y = p.targets ? p.targets[row] : -1;
+  // requested in front of the row, whose loads take their place behind them
+  const bool entries = BWD || rank == 0;
+  int id0 = -1;
+  float t0 = 0.0f;
+  if (entries && tid < k) {
+    id0 = p.t_ids[row * k + tid];
+    t0 = p.t_logits[row * k + tid];
+  }
+  const RowView<T> view(xr, n);
+  const int nvec = view.vectors(), per = (nvec + C - 1) / C;
+  const int lo = min(rank * per, nvec), hi = min(lo + per, nvec);
+  uint4 raw[NV];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int v = lo + tid + j * THREADS;
+    raw[j] = v < hi ? view.load(v) : minus_inf_vec<T>();
+  }
+  const bool aligned = BWD && ((reinterpret_cast<uintptr_t>(dr) ^ reinterpret_cast<uintptr_t>(xr)) & 15) == 0;
+  const bool ignored = p.targets && y == p.ignore_index;
+  const bool out = p.targets && !ignored && (y < 0 || y >= n);
+  if (ignored || out) {
+    if (FWD && tid == 0 && rank == 0) {
+      p.row_loss[row] = 0.0f;
+      if (p.lse) { p.lse[row] = 0.0f; p.lse[p.rows + row] = 0.0f; }
+      if (out && p.bad_id_flag) *p.bad_id_flag = 1;
+    }
+    if (BWD && !p.accumulate) {
+      for (int v = lo + tid; v < hi; v += THREADS) {
+        const int e = view.first(v);
+        if (aligned && view.whole(v)) *reinterpret_cast<uint4*>(dr + e) = make_uint4(0, 0, 0, 0);
+        else
+          for (int i = max(e, 0); i < min(e + V, n); ++i) dr[i] = from_f32<T>(0.0f);
+      }
+    }
+    if (FWD && C > 1) cluster_wait();
+    return;
+  }
+  float tm = -INFINITY;
+  if (entries) {
+    for (int j = tid; j < ((k + 4) & ~3); j += THREADS) {
+      int id = j == k ? y : -1;
+      float t = -INFINITY;
+      if (j < k) {
+        id = j < THREADS ? id0 : p.t_ids[row * k + j];
+        if (id >= n) {
+          if (FWD && p.bad_id_flag) *p.bad_id_flag = 1;
+          id = -1;
+        }
+        if (id >= 0) t = (j < THREADS ? t0 : p.t_logits[row * k + j]) * p.inv_t;
+      }
+      id = max(id, -1);
+      s_id[j] = id;
+      s_t[j] = t;
+      s_x[j] = id >= 0 ? to_f32(xr[id]) : 0.0f;
+      if (ACC && p.accumulate) s_old[j] = id >= 0 ? to_f32(dr[id]) : 0.0f;
+      tm = fmaxf(tm, t);
+    }
+  }
+  // the row's maximum and the teacher's
+  float ref = 0.0f;
+  if constexpr (FWD) {
+    const float m = warp_max(max_of<T, NV>(raw));
+    if (lane == 0) s_max[0][warp] = m;
+  }
+  tm = warp_max(tm);
+  if (lane == 0) s_max[1][warp] = tm;
+  __syncthreads();
+  if constexpr (FWD) {
+    ref = warp_max(s_max[0][lane % WARPS]);
+    if (ref == -INFINITY) ref = 0.0f;
+  }
+  // the teacher's sum: of exp(t - tref) = q_j S, where tref is its given log-sum-exp (S = 1) or its maximum
+  float tref;
+  if (p.t_lse) {
+    tref = p.t_lse[row];
+  } else {
+    tref = warp_max(s_max[1][lane % WARPS]);
+    if (tref == -INFINITY) tref = 0.0f;
+  }
+  float S = 0.0f;
+  if (entries)
+    for (int j = tid; j < k; j += THREADS) S += expf(s_t[j] - tref);
+  float st = 0.0f, s1 = 0.0f;
+  if constexpr (FWD) {
+    with_exp<T>(p.sum_kind, ref, p.inv_t, [&](const auto& ex) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        float x[V];
+        unpack_vec<T>(raw[j], x);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          float et, e1;
+          ex(x[i], et, e1);
+          st += et;
+          s1 += e1;
+        }
+      }
+    });
+    st = warp_sum(st);
+    s1 = warp_sum(s1);
+    if (lane == 0) { s_sum[0][warp] = st; s_sum[1][warp] = s1; }
+  }
+  S = warp_sum(S);
+  if (lane == 0) s_sum[2][warp] = S;
+  __syncthreads();
+  auto total = [&](int which) { return warp_sum(lane < WARPS ? s_sum[which][lane] : 0.0f); };
+  S = total(2);
+  // q_j = exp(t_j - tref) * inv_s,  Q = sum of them,  ln q_j = t_j - tl
+  const float tl = p.t_lse || S == 0.0f ? tref : tref + logf(S);
+  const float inv_s = p.t_lse || S == 0.0f ? 1.0f : 1.0f / S, Q = S * inv_s;
+  float lt, l1;
+  const bool has_kd = p.kd_weight != 0.0f, has_ce = p.ce_weight != 0.0f;
+  if constexpr (FWD) {
+    st = total(0);
+    s1 = total(1);
+    if (C > 1) {
+      cluster_wait();
+      if (tid < C) {
+        const uint32_t to = mapa_cluster(smem_u32(&s_xch[rank][0]), tid);
+        st_cluster_f32(to, st == 0.0f ? -INFINITY : ref);  // a slice without a finite entry has no say in the maximum
+        st_cluster_f32(to + 4, st);
+        st_cluster_f32(to + 8, s1);
+      }
+      cluster_arrive();
+      cluster_wait();
+      float gm = -INFINITY;
+      for (int r = 0; r < C; ++r) gm = fmaxf(gm, s_xch[r][0]);
+      ref = gm == -INFINITY ? 0.0f : gm;
+      st = s1 = 0.0f;
+      for (int r = 0; r < C; ++r) {
+        const float d = s_xch[r][0] - ref;
+        st += s_xch[r][1] * expf(d * p.inv_t);
+        s1 += s_xch[r][2] * expf(d);
+      }
+    }
+    lt = ref * p.inv_t + logf(st);
+    l1 = p.sum_kind == ONE ? (p.temperature == 1.0f ? lt : 0.0f) : ref + logf(s1);
+    if (warp == 0 && rank == 0) {
+      float kl = 0.0f;
+      for (int j = lane; j < k; j += 32) {
+        const float t = s_t[j], q = expf(t - tref) * inv_s;
+        if (q > 0.0f || q != q) kl += q * (t - tl - (s_x[j] * p.inv_t - lt));
+      }
+      kl = warp_sum(kl);
+      if (lane == 0) {
+        float l = 0.0f;
+        if (has_kd) l = p.kd_weight * p.temperature * p.temperature * kl;
+        if (has_ce) l -= p.ce_weight * logf(expf(s_x[k] - l1) + 1e-8f);
+        p.row_loss[row] = l;
+        if (p.lse) { p.lse[row] = lt; p.lse[p.rows + row] = l1; }
+      }
+    }
+  } else {
+    lt = p.lse[row];
+    l1 = p.lse[p.rows + row];
+    ref = l1;
+  }
+  if constexpr (BWD) {
+    // d = kt exp((x - ref) / T) + k1 exp(x - ref): kt, k1 turn the exponentials into weighted probabilities
+    const float g = p.grad_scale * (p.grad_out ? *p.grad_out : 1.0f);
+    const float kq = has_kd ? p.kd_weight * p.temperature * g : 0.0f, c1 = has_ce ? p.ce_weight * g : 0.0f;
+    float kt = 0.0f, k1 = 0.0f;
+    if (has_kd) kt = FWD ? kq * Q / st : kq * Q * expf(ref * p.inv_t - lt);
+    if (has_ce) k1 = FWD ? c1 / (p.grad_kind == ONE ? st : s1) : c1;
+    if (p.grad_kind == ONE) { kt += k1; k1 = 0.0f; }  // temperature 1: one exponential for both terms
+    with_exp<T>(p.grad_kind, ref, p.inv_t, [&](const auto& ex) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int v = lo + tid + j * THREADS;
+        if (v < hi) {
+          float d[V];
+          unpack_vec<T>(raw[j], d);
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            float et, e1;
+            ex(d[i], et, e1);
+            d[i] = kt * et + k1 * e1;
+          }
+          const int e = view.first(v);
+          if (aligned && view.whole(v)) {
+            if (ACC && p.accumulate) {
+              float o[V];
+              ld16(dr + e, o);
+#pragma unroll
+              for (int i = 0; i < V; ++i) d[i] += o[i];
+            }
+            st16(dr + e, d);
+          } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+              if (e + i >= 0 && e + i < n) {
+                if (ACC && p.accumulate) d[i] += to_f32(dr[e + i]);
+                dr[e + i] = from_f32<T>(d[i]);
+              }
+          }
+        }
+      }
+    });
+    __syncthreads();
+    // entries of this slice with a term of their own: the first of equal ids collects the probabilities of all
+    const int e_lo = max(view.first(lo), 0), e_hi = min(view.first(hi), n);
+    for (int j = tid; j <= k; j += THREADS) {
+      const int id = s_id[j];
+      if (id < e_lo || id >= e_hi) continue;
+      float w = 0.0f;
+      bool mine = true;
+      for (int i = 0; i <= k && mine; i += 4) {
+        const int4 o = *reinterpret_cast<const int4*>(s_id + i);
+        const int ids[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (ids[c] == id) {
+            if (i + c < j) mine = false;
+            if (i + c < k) w += expf(s_t[i + c] - tref);
+          }
+      }
+      if (!mine) continue;
+      float d = 0.0f;
+      with_exp<T>(p.grad_kind, ref, p.inv_t, [&](const auto& ex) {
+        float et, e1;
+        ex(s_x[j], et, e1);
+        d = kt * et + k1 * e1;
+      });
+      if (has_kd) d -= kq * w * inv_s;
+      if (id == y) d -= c1;
+      if (ACC && p.accumulate) d += s_old[j];
+      dr[id] = from_f32<T>(d);
+    }
+  }
+}
+
 int distill_check(const char* what, const DistillParams& p, int dtype, bool bwd) {
   static thread_local char msg[160];
   auto bad = [&](int code, const char* why) {
@@ -359,6 +691,38 @@ int distill_sizes(const char* what, long long rows, long long vocab, long long k
   if (rows >= 0 && rows <= 0x7fffffffLL && vocab > 0 && vocab <= 0x7fffff00LL && k >= 0 && k <= 0x7fffffffLL) return 0;
   snprintf(msg, sizeof(msg), "%s: rows must be in [0, 2^31), vocab in [1, 2^31 - 256]", what);
   return fail(EISEN_ERR_LIMIT, msg);
+}
+
+// Rows of up to 8 slices of 4096 vectors (262144 bf16 or 131072 f32 entries) stay in registers; longer ones take
+// distill_kernel, which reads them a second time.  Short rows in numbers get CTAs of 128 threads, whose barriers are
+// cheaper; few rows get more threads and CTAs each.
+template <typename T, int MODE>
+int distill_launch(const char* what, DistillParams& p, cudaStream_t s) {
+  const long long vectors = (p.vocab + VecOf<T>::N - 1) / VecOf<T>::N + 1;  // one more for a row that starts inside one
+  const bool few = p.rows < 2LL * sm_count();
+  p.cluster = cluster_for_row(p.rows, vectors, 4096, 512);
+  if (!p.cluster) {
+    distill_kernel<T, MODE><<<(unsigned)p.rows, DS_THREADS, 0, s>>>(p);
+    return check_launch(what);
+  }
+  const long long per = (vectors + p.cluster - 1) / p.cluster;
+  if (!few && per <= 256) return launch_rows(distill_row_kernel<T, 128, 2, MODE>, what, p.rows, p.cluster, 128, s, p);
+  if (!few && per <= 1024) return launch_rows(distill_row_kernel<T, 128, 8, MODE>, what, p.rows, p.cluster, 128, s, p);
+  if (per <= 1024) return launch_rows(distill_row_kernel<T, 512, 2, MODE>, what, p.rows, p.cluster, 512, s, p);
+  if (per <= 2048) return launch_rows(distill_row_kernel<T, 512, 4, MODE>, what, p.rows, p.cluster, 512, s, p);
+  return launch_rows(distill_row_kernel<T, 512, 8, MODE>, what, p.rows, p.cluster, 512, s, p);
+}
+
+int distill_run(const char* what, int mode, DistillParams& p, int dtype, cudaStream_t s) {
+  // both exponentials are summed where the caller takes both log-sum-exps or the cross-entropy needs its own
+  const bool one = p.temperature == 1.0f;
+  p.sum_kind = one || (!p.lse && p.ce_weight == 0.0f) ? ONE : exp_kind(p.temperature, dtype);
+  p.grad_kind = one || p.ce_weight == 0.0f ? ONE : exp_kind(p.temperature, dtype);
+  EISEN_DISPATCH_DTYPE(dtype, T, {
+    if (mode == DS_FWD) return distill_launch<T, DS_FWD>(what, p, s);
+    if (mode == DS_BWD) return distill_launch<T, DS_BWD>(what, p, s);
+    return distill_launch<T, DS_FWD | DS_BWD>(what, p, s);
+  });
 }
 
 }  // namespace
@@ -399,12 +763,9 @@ int eisen_distill_fwd(void* stream, const void* logits, long long ld, const int*
   }
   if (int rc = distill_check("distill_fwd", p, dtype, false)) return rc;
   if (!row_loss) return fail(EISEN_ERR_INVALID, "distill_fwd: row_loss must not be null");
-  EISEN_DISPATCH_DTYPE(dtype, T, {
-    distill_kernel<T, DS_FWD><<<(unsigned)rows, DS_THREADS, 0, (cudaStream_t)stream>>>(p);
-    int rc = check_launch("distill_fwd");
-    if (rc || !loss) return rc;
-    return eisen_ce_loss_reduce(stream, row_loss, loss, rows);
-  });
+  const int rc = distill_run("distill_fwd", DS_FWD, p, dtype, (cudaStream_t)stream);
+  if (rc || !loss) return rc;
+  return eisen_ce_loss_reduce(stream, row_loss, loss, rows);
 }
 
 int eisen_distill_bwd(void* stream, const void* logits, long long ld, const int* teacher_ids, const float* teacher_logits,
@@ -419,10 +780,7 @@ int eisen_distill_bwd(void* stream, const void* logits, long long ld, const int*
   if (rows == 0) return 0;
   if (int rc = distill_check("distill_bwd", p, dtype, true)) return rc;
   if (!lse) return fail(EISEN_ERR_INVALID, "distill_bwd: lse must not be null");
-  EISEN_DISPATCH_DTYPE(dtype, T, {
-    distill_kernel<T, DS_BWD><<<(unsigned)rows, DS_THREADS, 0, (cudaStream_t)stream>>>(p);
-    return check_launch("distill_bwd");
-  });
+  return distill_run("distill_bwd", DS_BWD, p, dtype, (cudaStream_t)stream);
 }
 
 int eisen_distill_fused(void* stream, const void* logits, long long ld, const int* teacher_ids, const float* teacher_logits,
@@ -439,12 +797,9 @@ int eisen_distill_fused(void* stream, const void* logits, long long ld, const in
   }
   if (int rc = distill_check("distill_fused", p, dtype, true)) return rc;
   if (!row_loss) return fail(EISEN_ERR_INVALID, "distill_fused: row_loss must not be null");
-  EISEN_DISPATCH_DTYPE(dtype, T, {
-    distill_kernel<T, DS_FWD | DS_BWD><<<(unsigned)rows, DS_THREADS, 0, (cudaStream_t)stream>>>(p);
-    int rc = check_launch("distill_fused");
-    if (rc || !loss) return rc;
-    return eisen_ce_loss_reduce(stream, row_loss, loss, rows);
-  });
+  const int rc = distill_run("distill_fused", DS_FWD | DS_BWD, p, dtype, (cudaStream_t)stream);
+  if (rc || !loss) return rc;
+  return eisen_ce_loss_reduce(stream, row_loss, loss, rows);
 }
 
 }  // extern "C"
