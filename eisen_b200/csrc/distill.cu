@@ -356,26 +356,43 @@ struct RowExp {
     off = -r * c;
     off1 = -r * 1.4426950408889634f;
   }
-  __device__ __forceinline__ void operator()(float x, float& et, float& e1) const {
+  // the exponentials of two elements, in packed arithmetic: et = exp((x - ref) / T), e1 = exp(x - ref)
+  __device__ __forceinline__ void operator()(float x, float y, float (&et)[2], float (&e1)[2]) const {
     if constexpr (KIND == PLAIN) {
-      et = expf((x - ref) * inv_t);
-      e1 = two ? expf(x - ref) : 0.0f;
-    } else if constexpr (KIND == ONE) {
-      et = exp2_approx(fmaf(x, c, off));
-      e1 = 0.0f;
-    } else if constexpr (KIND == TWO) {
-      et = exp2_approx(fmaf(x, c, off));
-      e1 = exp2_approx(fmaf(x, 1.4426950408889634f, off1));
+      et[0] = expf((x - ref) * inv_t);
+      et[1] = expf((y - ref) * inv_t);
+      e1[0] = two ? expf(x - ref) : 0.0f;
+      e1[1] = two ? expf(y - ref) : 0.0f;
     } else {
-      constexpr int A = KIND / 10, B = KIND % 10;
-      const float h = exp2_approx(fmaf(x, c, off)), h2 = h * h;
-      et = A == 1 ? h : h2;
-      if constexpr (B == 1) e1 = h;
-      else if constexpr (B == 2) e1 = h2;
-      else if constexpr (B == 3) e1 = h2 * h;
-      else if constexpr (B == 4) e1 = h2 * h2;
-      else if constexpr (B == 5) e1 = h2 * h2 * h;
-      else e1 = h2 * h2 * (h2 * h);
+      float h0, h1;
+      ffma2(h0, h1, x, y, c, c, off, off);
+      h0 = exp2_approx(h0);
+      h1 = exp2_approx(h1);
+      if constexpr (KIND == ONE) {
+        et[0] = h0; et[1] = h1;
+        e1[0] = e1[1] = 0.0f;
+      } else if constexpr (KIND == TWO) {
+        et[0] = h0; et[1] = h1;
+        ffma2(h0, h1, x, y, 1.4426950408889634f, 1.4426950408889634f, off1, off1);
+        e1[0] = exp2_approx(h0);
+        e1[1] = exp2_approx(h1);
+      } else {
+        constexpr int A = KIND / 10, B = KIND % 10;
+        float s0, s1, f0, f1;  // h^2, h^4
+        fmul2(s0, s1, h0, h1, h0, h1);
+        if constexpr (B >= 4) fmul2(f0, f1, s0, s1, s0, s1);
+        et[0] = A == 1 ? h0 : s0;
+        et[1] = A == 1 ? h1 : s1;
+        if constexpr (B == 1) { e1[0] = h0; e1[1] = h1; }
+        else if constexpr (B == 2) { e1[0] = s0; e1[1] = s1; }
+        else if constexpr (B == 3) fmul2(e1[0], e1[1], s0, s1, h0, h1);
+        else if constexpr (B == 4) { e1[0] = f0; e1[1] = f1; }
+        else if constexpr (B == 5) fmul2(e1[0], e1[1], f0, f1, h0, h1);
+        else {
+          fmul2(f0, f1, f0, f1, s0, s1);
+          fmul2(e1[0], e1[1], f0, f1, h0, h1);
+        }
+      }
     }
   }
 };
@@ -410,13 +427,24 @@ int exp_kind(float temperature, int dtype) {
   return TWO;
 }
 
+// the elements of a vector that reaches beyond an end of its row, or whose place in dlogits is not aligned
+template <typename T>
+__device__ __noinline__ void store_edge(T* dr, int e, int n, const float (&d)[VecOf<T>::N], bool accumulate) {
+#pragma unroll
+  for (int i = 0; i < VecOf<T>::N; ++i)
+    if (e + i >= 0 && e + i < n) dr[e + i] = from_f32<T>(accumulate ? d[i] + to_f32(dr[e + i]) : d[i]);
+}
+
 // A row in the registers of one CTA, or of a cluster of p.cluster CTAs with a slice of the vectors each: the
-// logits are read once, by loads that are all in flight together, and two CTAs per SM (eight of 128 threads for
-// short rows) work while the other one's loads are on their way.  The gradient pass takes the exponentials again
-// from the registers.  The teacher's entries go through shared memory beside the row's own maximum and sums;
-// entries with a term of their own are written after the dense pass, by the first thread among equal ids.
+// logits are read once, by loads that are all in flight together, and two CTAs per SM (more of shorter rows) work
+// while the other one's loads are on their way.  The gradient pass takes the exponentials again from the registers.
+// The teacher's entries go through shared memory beside the row's own maximum and sums; entries with a term of
+// their own are written after the dense pass, by the first thread among equal ids.  Few threads with many vectors
+// each: what a thread does beside its elements (addresses, three reductions, the row's scalars) is several hundred
+// instructions, as many as 60 elements take.
+constexpr int row_ctas(int threads, int nv) { return nv >= 16 ? 512 / threads : 1024 / threads; }
 template <typename T, int THREADS, int NV, int MODE>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
+__global__ void __launch_bounds__(THREADS, row_ctas(THREADS, NV))
 distill_row_kernel(const DistillParams p) {
   constexpr int V = VecOf<T>::N, WARPS = THREADS / 32;
   constexpr int PAD = DS_MAX_K + 4;
@@ -447,11 +475,7 @@ distill_row_kernel(const DistillParams p) {
   const int nvec = view.vectors(), per = (nvec + C - 1) / C;
   const int lo = min(rank * per, nvec), hi = min(lo + per, nvec);
   uint4 raw[NV];
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int v = lo + tid + j * THREADS;
-    raw[j] = v < hi ? view.load(v) : minus_inf_vec<T>();
-  }
+  load_slice<T, THREADS, NV>(view, lo, hi, raw);
   const bool aligned = BWD && ((reinterpret_cast<uintptr_t>(dr) ^ reinterpret_cast<uintptr_t>(xr)) & 15) == 0;
   const bool ignored = p.targets && y == p.ignore_index;
   const bool out = p.targets && !ignored && (y < 0 || y >= n);
@@ -464,7 +488,7 @@ distill_row_kernel(const DistillParams p) {
     if (BWD && !p.accumulate) {
       for (int v = lo + tid; v < hi; v += THREADS) {
         const int e = view.first(v);
-        if (aligned && view.whole(v)) *reinterpret_cast<uint4*>(dr + e) = make_uint4(0, 0, 0, 0);
+        if (aligned && e >= 0 && e + V <= n) *reinterpret_cast<uint4*>(dr + e) = make_uint4(0, 0, 0, 0);
         else
           for (int i = max(e, 0); i < min(e + V, n); ++i) dr[i] = from_f32<T>(0.0f);
       }
@@ -519,22 +543,23 @@ distill_row_kernel(const DistillParams p) {
     for (int j = tid; j < k; j += THREADS) S += expf(s_t[j] - tref);
   float st = 0.0f, s1 = 0.0f;
   if constexpr (FWD) {
+    float sa[2] = {0.0f, 0.0f}, sb[2] = {0.0f, 0.0f};
     with_exp<T>(p.sum_kind, ref, p.inv_t, [&](const auto& ex) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         float x[V];
         unpack_vec<T>(raw[j], x);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          float et, e1;
-          ex(x[i], et, e1);
-          st += et;
-          s1 += e1;
+        for (int i = 0; i < V; i += 2) {
+          float et[2], e1[2];
+          ex(x[i], x[i + 1], et, e1);
+          fadd2(sa[0], sa[1], sa[0], sa[1], et[0], et[1]);
+          if (ex.two) fadd2(sb[0], sb[1], sb[0], sb[1], e1[0], e1[1]);
         }
       }
     });
-    st = warp_sum(st);
-    s1 = warp_sum(s1);
+    st = warp_sum(sa[0] + sa[1]);
+    s1 = warp_sum(sb[0] + sb[1]);
     if (lane == 0) { s_sum[0][warp] = st; s_sum[1][warp] = s1; }
   }
   S = warp_sum(S);
@@ -542,10 +567,8 @@ distill_row_kernel(const DistillParams p) {
   __syncthreads();
   auto total = [&](int which) { return warp_sum(lane < WARPS ? s_sum[which][lane] : 0.0f); };
   S = total(2);
-  // q_j = exp(t_j - tref) * inv_s,  Q = sum of them,  ln q_j = t_j - tl
-  const float tl = p.t_lse || S == 0.0f ? tref : tref + logf(S);
-  const float inv_s = p.t_lse || S == 0.0f ? 1.0f : 1.0f / S, Q = S * inv_s;
-  float lt, l1;
+  // q_j = exp(t_j - tref) * inv_s,  Q = sum of them
+  const float inv_s = p.t_lse || S == 0.0f ? 1.0f : __fdividef(1.0f, S), Q = S * inv_s;
   const bool has_kd = p.kd_weight != 0.0f, has_ce = p.ce_weight != 0.0f;
   if constexpr (FWD) {
     st = total(0);
@@ -570,12 +593,13 @@ distill_row_kernel(const DistillParams p) {
         s1 += s_xch[r][2] * expf(d);
       }
     }
-    lt = ref * p.inv_t + logf(st);
-    l1 = p.sum_kind == ONE ? (p.temperature == 1.0f ? lt : 0.0f) : ref + logf(s1);
     if (warp == 0 && rank == 0) {
+      const float lt = ref * p.inv_t + logf(st);
+      const float l1 = p.sum_kind == ONE ? (p.temperature == 1.0f ? lt : 0.0f) : ref + logf(s1);
+      const float tl = p.t_lse || S == 0.0f ? tref : tref + logf(S);  // ln q_j = t_j - tl
       float kl = 0.0f;
       for (int j = lane; j < k; j += 32) {
-        const float t = s_t[j], q = expf(t - tref) * inv_s;
+        const float t = s_t[j], q = expf(t - tl);
         if (q > 0.0f || q != q) kl += q * (t - tl - (s_x[j] * p.inv_t - lt));
       }
       kl = warp_sum(kl);
@@ -588,47 +612,44 @@ distill_row_kernel(const DistillParams p) {
       }
     }
   } else {
-    lt = p.lse[row];
-    l1 = p.lse[p.rows + row];
-    ref = l1;
+    ref = p.lse[p.rows + row];
   }
   if constexpr (BWD) {
     // d = kt exp((x - ref) / T) + k1 exp(x - ref): kt, k1 turn the exponentials into weighted probabilities
     const float g = p.grad_scale * (p.grad_out ? *p.grad_out : 1.0f);
     const float kq = has_kd ? p.kd_weight * p.temperature * g : 0.0f, c1 = has_ce ? p.ce_weight * g : 0.0f;
     float kt = 0.0f, k1 = 0.0f;
-    if (has_kd) kt = FWD ? kq * Q / st : kq * Q * expf(ref * p.inv_t - lt);
-    if (has_ce) k1 = FWD ? c1 / (p.grad_kind == ONE ? st : s1) : c1;
+    if (has_kd) kt = FWD ? __fdividef(kq * Q, st) : kq * Q * expf(ref * p.inv_t - p.lse[row]);
+    if (has_ce) k1 = FWD ? __fdividef(c1, p.grad_kind == ONE ? st : s1) : c1;
     if (p.grad_kind == ONE) { kt += k1; k1 = 0.0f; }  // temperature 1: one exponential for both terms
+    const int w0 = aligned ? max(lo, view.whole_lo()) : hi, w1 = aligned ? min(hi, view.whole_hi()) : hi;
+    const int v0 = lo + tid;
+    T* to = dr + view.first(v0);
     with_exp<T>(p.grad_kind, ref, p.inv_t, [&](const auto& ex) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        const int v = lo + tid + j * THREADS;
+        const int v = v0 + j * THREADS;
         if (v < hi) {
           float d[V];
           unpack_vec<T>(raw[j], d);
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            float et, e1;
-            ex(d[i], et, e1);
-            d[i] = kt * et + k1 * e1;
+          for (int i = 0; i < V; i += 2) {
+            float et[2], e1[2];
+            ex(d[i], d[i + 1], et, e1);
+            fmul2(d[i], d[i + 1], et[0], et[1], kt, kt);
+            if (ex.two) ffma2(d[i], d[i + 1], e1[0], e1[1], k1, k1, d[i], d[i + 1]);
           }
-          const int e = view.first(v);
-          if (aligned && view.whole(v)) {
+          T* at = to + j * (THREADS * V);
+          if (v >= w0 && v < w1) {
             if (ACC && p.accumulate) {
               float o[V];
-              ld16(dr + e, o);
+              ld16(at, o);
 #pragma unroll
               for (int i = 0; i < V; ++i) d[i] += o[i];
             }
-            st16(dr + e, d);
+            st16(at, d);
           } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i)
-              if (e + i >= 0 && e + i < n) {
-                if (ACC && p.accumulate) d[i] += to_f32(dr[e + i]);
-                dr[e + i] = from_f32<T>(d[i]);
-              }
+            store_edge<T>(dr, view.first(v), n, d, ACC && p.accumulate);
           }
         }
       }
@@ -639,24 +660,25 @@ distill_row_kernel(const DistillParams p) {
     for (int j = tid; j <= k; j += THREADS) {
       const int id = s_id[j];
       if (id < e_lo || id >= e_hi) continue;
-      float w = 0.0f;
-      bool mine = true;
-      for (int i = 0; i <= k && mine; i += 4) {
+      int same = 0;
+      for (int i = 0; i <= k; i += 4) {
         const int4 o = *reinterpret_cast<const int4*>(s_id + i);
-        const int ids[4] = {o.x, o.y, o.z, o.w};
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          if (ids[c] == id) {
-            if (i + c < j) mine = false;
-            if (i + c < k) w += expf(s_t[i + c] - tref);
-          }
+        same += (o.x == id) + (o.y == id) + (o.z == id) + (o.w == id);
       }
-      if (!mine) continue;
+      float w = j < k ? expf(s_t[j] - tref) : 0.0f;
+      if (same > 1) {
+        int i = 0;
+        while (s_id[i] != id) ++i;
+        if (i < j) continue;
+        w = 0.0f;
+        for (; i < k; ++i)
+          if (s_id[i] == id) w += expf(s_t[i] - tref);
+      }
       float d = 0.0f;
       with_exp<T>(p.grad_kind, ref, p.inv_t, [&](const auto& ex) {
-        float et, e1;
-        ex(s_x[j], et, e1);
-        d = kt * et + k1 * e1;
+        float et[2], e1[2];
+        ex(s_x[j], s_x[j], et, e1);
+        d = kt * et[0] + k1 * e1[0];
       });
       if (has_kd) d -= kq * w * inv_s;
       if (id == y) d -= c1;
@@ -708,9 +730,9 @@ int distill_launch(const char* what, DistillParams& p, cudaStream_t s) {
   const long long per = (vectors + p.cluster - 1) / p.cluster;
   if (!few && per <= 256) return launch_rows(distill_row_kernel<T, 128, 2, MODE>, what, p.rows, p.cluster, 128, s, p);
   if (!few && per <= 1024) return launch_rows(distill_row_kernel<T, 128, 8, MODE>, what, p.rows, p.cluster, 128, s, p);
-  if (per <= 1024) return launch_rows(distill_row_kernel<T, 512, 2, MODE>, what, p.rows, p.cluster, 512, s, p);
-  if (per <= 2048) return launch_rows(distill_row_kernel<T, 512, 4, MODE>, what, p.rows, p.cluster, 512, s, p);
-  return launch_rows(distill_row_kernel<T, 512, 8, MODE>, what, p.rows, p.cluster, 512, s, p);
+  if (per <= 1024) return launch_rows(distill_row_kernel<T, 256, 4, MODE>, what, p.rows, p.cluster, 256, s, p);
+  if (per <= 2048) return launch_rows(distill_row_kernel<T, 256, 8, MODE>, what, p.rows, p.cluster, 256, s, p);
+  return launch_rows(distill_row_kernel<T, 256, 16, MODE>, what, p.rows, p.cluster, 256, s, p);
 }
 
 int distill_run(const char* what, int mode, DistillParams& p, int dtype, cudaStream_t s) {

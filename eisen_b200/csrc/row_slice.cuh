@@ -42,15 +42,17 @@ struct RowView {
   }
   __device__ __forceinline__ int vectors() const { return (lead + n + V - 1) / V; }
   __device__ __forceinline__ int first(int vec) const { return vec * V - lead; }  // row index of its first element
-  __device__ __forceinline__ bool whole(int vec) const { return first(vec) >= 0 && first(vec) + V <= n; }
-  __device__ __forceinline__ uint4 load(int vec) const {
-    if (whole(vec)) {
-      uint4 r;  // used once: kept out of L1
-      asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
-                   : "l"(base + (long long)vec * V));
-      return r;
-    }
+  // vectors inside the row: [whole_lo, whole_hi)
+  __device__ __forceinline__ int whole_lo() const { return lead ? 1 : 0; }
+  __device__ __forceinline__ int whole_hi() const { return (lead + n) / V; }
+  // a vector that lies in the row; used once, kept out of L1
+  __device__ __forceinline__ static uint4 load_whole(const T* at) {
+    uint4 r;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(at));
+    return r;
+  }
+  // one that reaches beyond an end of it
+  __device__ __noinline__ uint4 load_edge(int vec) const {
     uint32_t u[4];
     const int e0 = first(vec);
     if constexpr (sizeof(T) == 2) {
@@ -75,6 +77,28 @@ template <typename T>
 __device__ __forceinline__ uint4 minus_inf_vec() {
   constexpr uint32_t w = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
   return make_uint4(w, w, w, w);
+}
+
+// This thread's vectors lo + tid, lo + tid + THREADS, ... < hi of a row; -inf beyond
+template <typename T, int THREADS, int NV>
+__device__ __forceinline__ void load_slice(const RowView<T>& view, int lo, int hi, uint4 (&raw)[NV]) {
+  const int w0 = max(lo, view.whole_lo()), w1 = min(hi, view.whole_hi());
+  const int v0 = lo + (int)threadIdx.x;
+  const T* at = view.base + (long long)v0 * VecOf<T>::N;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int v = v0 + j * THREADS;
+    if (v >= w0 && v < w1) raw[j] = RowView<T>::load_whole(at + j * (THREADS * VecOf<T>::N));
+    else raw[j] = minus_inf_vec<T>();
+  }
+  // the one or two vectors at the row's ends, by the threads that own them
+  if (v0 < w0 || hi > w1) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int v = v0 + j * THREADS;
+      if (v < hi && (v < w0 || v >= w1)) raw[j] = view.load_edge(v);
+    }
+  }
 }
 
 // largest element of NV vectors; NaN where one of them is NaN
