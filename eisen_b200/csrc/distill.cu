@@ -14,7 +14,7 @@
 
 #include "common.cuh"
 #include "errors.h"
-#include "row_slice.cuh"
+#include "row_pipe.cuh"
 #include "../../include/eisen_b200.h"
 
 namespace eisen {
@@ -197,7 +197,8 @@ struct DistillParams {
   float temperature, inv_t, kd_weight, ce_weight, grad_scale;
   int accumulate;
   int* bad_id_flag;
-  int sum_kind, grad_kind, cluster;  // distill_row_kernel: see RowExp
+  int sum_kind, grad_kind;  // distill_pipe_kernel: see RowExp
+  RowShape shape;
 };
 
 constexpr int DS_FWD = 1, DS_BWD = 2;
@@ -427,264 +428,349 @@ int exp_kind(float temperature, int dtype) {
   return TWO;
 }
 
-// the elements of a vector that reaches beyond an end of its row, or whose place in dlogits is not aligned
-template <typename T>
-__device__ __noinline__ void store_edge(T* dr, int e, int n, const float (&d)[VecOf<T>::N], bool accumulate) {
-#pragma unroll
-  for (int i = 0; i < VecOf<T>::N; ++i)
-    if (e + i >= 0 && e + i < n) dr[e + i] = from_f32<T>(accumulate ? d[i] + to_f32(dr[e + i]) : d[i]);
-}
+// The frame of row_pipe.cuh with a row's work in one group of GT threads:
+//   maximum -> sums of the exponentials -> gradient over the logits in shared memory -> the entries with a term of
+//   their own (the teacher's ids and the target; the first of equal ids collects the probabilities of all).
+// The exponentials are taken again for the gradient.  A row's ids, teacher logits and target are requested while the
+// row before it is worked on.
+constexpr int pipe_threads(int gt, int groups) { return gt * groups + RP_EXTRA; }
+__host__ __device__ constexpr int entry_pad(int k) { return (k + 4) & ~3; }
+constexpr int entry_bytes(int k, int groups) { return groups * 2 * 3 * entry_pad(k) * 4; }
 
-// A row in the registers of one CTA, or of a cluster of p.cluster CTAs with a slice of the vectors each: the
-// logits are read once, by loads that are all in flight together, and two CTAs per SM (more of shorter rows) work
-// while the other one's loads are on their way.  The gradient pass takes the exponentials again from the registers.
-// The teacher's entries go through shared memory beside the row's own maximum and sums; entries with a term of
-// their own are written after the dense pass, by the first thread among equal ids.  Few threads with many vectors
-// each: what a thread does beside its elements (addresses, three reductions, the row's scalars) is several hundred
-// instructions, as many as 60 elements take.
-constexpr int row_ctas(int threads, int nv) { return nv >= 16 ? 512 / threads : 1024 / threads; }
-template <typename T, int THREADS, int NV, int MODE>
-__global__ void __launch_bounds__(THREADS, row_ctas(THREADS, NV))
-distill_row_kernel(const DistillParams p) {
-  constexpr int V = VecOf<T>::N, WARPS = THREADS / 32;
-  constexpr int PAD = DS_MAX_K + 4;
+template <typename T, int GT, int G, int MODE>
+__global__ void __launch_bounds__(GT * G + RP_EXTRA, 1)
+distill_pipe_kernel(const DistillParams p) {
+  constexpr int V = VecOf<T>::N, GW = GT / 32;
+  constexpr int PRE = GT >= 128 ? 1 : 4;  // entries per thread requested a row ahead
   constexpr bool FWD = (MODE & DS_FWD) != 0, BWD = (MODE & DS_BWD) != 0, ACC = BWD && !FWD;
-  __shared__ __align__(16) int s_id[PAD];  // the teacher's ids, -1: absent; entry k: the target
-  __shared__ float s_t[PAD];               // its logits / T
-  __shared__ float s_x[PAD];               // the student's logits there
-  __shared__ float s_old[ACC ? PAD : 1];   // what dlogits held there
-  __shared__ float s_max[2][WARPS], s_sum[4][WARPS];
-  __shared__ float s_xch[8][3];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int C = p.cluster, k = p.k, n = p.vocab;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ RowRing ring;
+  __shared__ uint64_t xbar[G];
+  __shared__ float s_max[G][2][GW], s_sum[G][3][GW];
+  __shared__ float s_xch[G][2][8][3];
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int C = p.shape.cluster, k = p.k, n = p.vocab, KP = entry_pad(k);
   const int rank = C > 1 ? (int)cluster_ctarank() : 0;
-  const long long row = C > 1 ? blockIdx.x / C : blockIdx.x;
-  if (FWD && C > 1) cluster_arrive();  // matched before the first access to a peer's shared memory
-  const T* xr = reinterpret_cast<const T*>(p.logits) + row * p.ld;
-  T* dr = BWD ? reinterpret_cast<T*>(p.dlogits) + row * p.ldd : nullptr;
-  const int y = p.targets ? p.targets[row] : -1;
-  // requested in front of the row, whose loads take their place behind them
-  const bool entries = BWD || rank == 0;
-  int id0 = -1;
-  float t0 = 0.0f;
-  if (entries && tid < k) {
-    id0 = p.t_ids[row * k + tid];
-    t0 = p.t_logits[row * k + tid];
+  const long long row0 = blockIdx.x / C, stride = gridDim.x / C;
+  const int n_mine = row0 < p.rows ? (int)((p.rows - row0 + stride - 1) / stride) : 0;
+  ring_init(ring, p.shape.stages, BWD ? 1 : GW, GW);
+  if (tid == 0) {
+    for (int g = 0; g < G; ++g) mbar_init(&xbar[g], C);
+    fence_mbar_init();
   }
-  const RowView<T> view(xr, n);
-  const int nvec = view.vectors(), per = (nvec + C - 1) / C;
-  const int lo = min(rank * per, nvec), hi = min(lo + per, nvec);
-  uint4 raw[NV];
-  load_slice<T, THREADS, NV>(view, lo, hi, raw);
-  const bool aligned = BWD && ((reinterpret_cast<uintptr_t>(dr) ^ reinterpret_cast<uintptr_t>(xr)) & 15) == 0;
-  const bool ignored = p.targets && y == p.ignore_index;
-  const bool out = p.targets && !ignored && (y < 0 || y >= n);
-  if (ignored || out) {
-    if (FWD && tid == 0 && rank == 0) {
-      p.row_loss[row] = 0.0f;
-      if (p.lse) { p.lse[row] = 0.0f; p.lse[p.rows + row] = 0.0f; }
-      if (out && p.bad_id_flag) *p.bad_id_flag = 1;
-    }
-    if (BWD && !p.accumulate) {
-      for (int v = lo + tid; v < hi; v += THREADS) {
-        const int e = view.first(v);
-        if (aligned && e >= 0 && e + V <= n) *reinterpret_cast<uint4*>(dr + e) = make_uint4(0, 0, 0, 0);
-        else
-          for (int i = max(e, 0); i < min(e + V, n); ++i) dr[i] = from_f32<T>(0.0f);
-      }
-    }
-    if (FWD && C > 1) cluster_wait();
-    return;
-  }
-  float tm = -INFINITY;
-  if (entries) {
-    for (int j = tid; j < ((k + 4) & ~3); j += THREADS) {
-      int id = j == k ? y : -1;
-      float t = -INFINITY;
-      if (j < k) {
-        id = j < THREADS ? id0 : p.t_ids[row * k + j];
-        if (id >= n) {
-          if (FWD && p.bad_id_flag) *p.bad_id_flag = 1;
-          id = -1;
-        }
-        if (id >= 0) t = (j < THREADS ? t0 : p.t_logits[row * k + j]) * p.inv_t;
-      }
-      id = max(id, -1);
-      s_id[j] = id;
-      s_t[j] = t;
-      s_x[j] = id >= 0 ? to_f32(xr[id]) : 0.0f;
-      if (ACC && p.accumulate) s_old[j] = id >= 0 ? to_f32(dr[id]) : 0.0f;
-      tm = fmaxf(tm, t);
-    }
-  }
-  // the row's maximum and the teacher's
-  float ref = 0.0f;
-  if constexpr (FWD) {
-    const float m = warp_max(max_of<T, NV>(raw));
-    if (lane == 0) s_max[0][warp] = m;
-  }
-  tm = warp_max(tm);
-  if (lane == 0) s_max[1][warp] = tm;
   __syncthreads();
-  if constexpr (FWD) {
-    ref = warp_max(s_max[0][lane % WARPS]);
-    if (ref == -INFINITY) ref = 0.0f;
-  }
-  // the teacher's sum: of exp(t - tref) = q_j S, where tref is its given log-sum-exp (S = 1) or its maximum
-  float tref;
-  if (p.t_lse) {
-    tref = p.t_lse[row];
+  if (C > 1) cluster_sync_all();
+  const T* logits = reinterpret_cast<const T*>(p.logits);
+  T* dlogits = reinterpret_cast<T*>(p.dlogits);
+  auto slice_of = [&](long long row) { return RowSlice<T>(logits + row * p.ld, n, rank, C); };
+  auto skipped = [&](int y) { return p.targets && (y == p.ignore_index || y < 0 || y >= n); };
+  auto skip_row = [&](long long row) { return p.targets && skipped(p.targets[row]); };
+
+  if (tid >= GT * G + 32) {
+    if constexpr (BWD)
+      ring_store<T>(ring, smem, p.shape.stages, p.shape.stage_bytes, n_mine, row0, stride, slice_of, skip_row,
+                    [&](long long row) { return dlogits + row * p.ldd; });
+  } else if (tid >= GT * G) {
+    ring_load<T>(ring, smem, p.shape.stages, p.shape.stage_bytes, n_mine, row0, stride, slice_of, skip_row);
   } else {
-    tref = warp_max(s_max[1][lane % WARPS]);
-    if (tref == -INFINITY) tref = 0.0f;
-  }
-  float S = 0.0f;
-  if (entries)
-    for (int j = tid; j < k; j += THREADS) S += expf(s_t[j] - tref);
-  float st = 0.0f, s1 = 0.0f;
-  if constexpr (FWD) {
-    float sa[2] = {0.0f, 0.0f}, sb[2] = {0.0f, 0.0f};
-    with_exp<T>(p.sum_kind, ref, p.inv_t, [&](const auto& ex) {
+    const int g = tid / GT, gt = tid % GT, warp = gt >> 5;
+    uint8_t* entries = smem + (size_t)p.shape.stages * p.shape.stage_bytes + (size_t)g * (2 * 3 * 4) * KP;
+    const bool has_kd = p.kd_weight != 0.0f, has_ce = p.ce_weight != 0.0f;
+    const float g_out = p.grad_scale * (BWD && p.grad_out ? *p.grad_out : 1.0f);
+    const bool want = BWD || rank == 0;  // this CTA looks at the teacher's entries
+    int y_next = -1, id_next[PRE];
+    float t_next[PRE], tl_next = 0.0f, lt_next = 0.0f, l1_next = 0.0f;
+    auto request = [&](int i) {
+      if (i >= n_mine) return;
+      const long long row = row0 + i * stride;
+      y_next = p.targets ? p.targets[row] : -1;
+      if (p.t_lse) tl_next = p.t_lse[row];
+      if constexpr (!FWD) { lt_next = p.lse[row]; l1_next = p.lse[p.rows + row]; }
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        float x[V];
-        unpack_vec<T>(raw[j], x);
-#pragma unroll
-        for (int i = 0; i < V; i += 2) {
-          float et[2], e1[2];
-          ex(x[i], x[i + 1], et, e1);
-          fadd2(sa[0], sa[1], sa[0], sa[1], et[0], et[1]);
-          if (ex.two) fadd2(sb[0], sb[1], sb[0], sb[1], e1[0], e1[1]);
+      for (int c = 0; c < PRE; ++c) {
+        const int j = gt + c * GT;
+        id_next[c] = -1;
+        t_next[c] = 0.0f;
+        if (want && j < k) {
+          id_next[c] = p.t_ids[row * k + j];
+          t_next[c] = p.t_logits[row * k + j];
         }
       }
-    });
-    st = warp_sum(sa[0] + sa[1]);
-    s1 = warp_sum(sb[0] + sb[1]);
-    if (lane == 0) { s_sum[0][warp] = st; s_sum[1][warp] = s1; }
-  }
-  S = warp_sum(S);
-  if (lane == 0) s_sum[2][warp] = S;
-  __syncthreads();
-  auto total = [&](int which) { return warp_sum(lane < WARPS ? s_sum[which][lane] : 0.0f); };
-  S = total(2);
-  // q_j = exp(t_j - tref) * inv_s,  Q = sum of them
-  const float inv_s = p.t_lse || S == 0.0f ? 1.0f : __fdividef(1.0f, S), Q = S * inv_s;
-  const bool has_kd = p.kd_weight != 0.0f, has_ce = p.ce_weight != 0.0f;
-  if constexpr (FWD) {
-    st = total(0);
-    s1 = total(1);
-    if (C > 1) {
-      cluster_wait();
-      if (tid < C) {
-        const uint32_t to = mapa_cluster(smem_u32(&s_xch[rank][0]), tid);
-        st_cluster_f32(to, st == 0.0f ? -INFINITY : ref);  // a slice without a finite entry has no say in the maximum
-        st_cluster_f32(to + 4, st);
-        st_cluster_f32(to + 8, s1);
-      }
-      cluster_arrive();
-      cluster_wait();
-      float gm = -INFINITY;
-      for (int r = 0; r < C; ++r) gm = fmaxf(gm, s_xch[r][0]);
-      ref = gm == -INFINITY ? 0.0f : gm;
-      st = s1 = 0.0f;
-      for (int r = 0; r < C; ++r) {
-        const float d = s_xch[r][0] - ref;
-        st += s_xch[r][1] * expf(d * p.inv_t);
-        s1 += s_xch[r][2] * expf(d);
-      }
-    }
-    if (warp == 0 && rank == 0) {
-      const float lt = ref * p.inv_t + logf(st);
-      const float l1 = p.sum_kind == ONE ? (p.temperature == 1.0f ? lt : 0.0f) : ref + logf(s1);
-      const float tl = p.t_lse || S == 0.0f ? tref : tref + logf(S);  // ln q_j = t_j - tl
-      float kl = 0.0f;
-      for (int j = lane; j < k; j += 32) {
-        const float t = s_t[j], q = expf(t - tl);
-        if (q > 0.0f || q != q) kl += q * (t - tl - (s_x[j] * p.inv_t - lt));
-      }
-      kl = warp_sum(kl);
-      if (lane == 0) {
-        float l = 0.0f;
-        if (has_kd) l = p.kd_weight * p.temperature * p.temperature * kl;
-        if (has_ce) l -= p.ce_weight * logf(expf(s_x[k] - l1) + 1e-8f);
-        p.row_loss[row] = l;
-        if (p.lse) { p.lse[row] = lt; p.lse[p.rows + row] = l1; }
-      }
-    }
-  } else {
-    ref = p.lse[p.rows + row];
-  }
-  if constexpr (BWD) {
-    // d = kt exp((x - ref) / T) + k1 exp(x - ref): kt, k1 turn the exponentials into weighted probabilities
-    const float g = p.grad_scale * (p.grad_out ? *p.grad_out : 1.0f);
-    const float kq = has_kd ? p.kd_weight * p.temperature * g : 0.0f, c1 = has_ce ? p.ce_weight * g : 0.0f;
-    float kt = 0.0f, k1 = 0.0f;
-    if (has_kd) kt = FWD ? __fdividef(kq * Q, st) : kq * Q * expf(ref * p.inv_t - p.lse[row]);
-    if (has_ce) k1 = FWD ? __fdividef(c1, p.grad_kind == ONE ? st : s1) : c1;
-    if (p.grad_kind == ONE) { kt += k1; k1 = 0.0f; }  // temperature 1: one exponential for both terms
-    const int w0 = aligned ? max(lo, view.whole_lo()) : hi, w1 = aligned ? min(hi, view.whole_hi()) : hi;
-    const int v0 = lo + tid;
-    T* to = dr + view.first(v0);
-    with_exp<T>(p.grad_kind, ref, p.inv_t, [&](const auto& ex) {
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int v = v0 + j * THREADS;
-        if (v < hi) {
-          float d[V];
-          unpack_vec<T>(raw[j], d);
-#pragma unroll
-          for (int i = 0; i < V; i += 2) {
-            float et[2], e1[2];
-            ex(d[i], d[i + 1], et, e1);
-            fmul2(d[i], d[i + 1], et[0], et[1], kt, kt);
-            if (ex.two) ffma2(d[i], d[i + 1], e1[0], e1[1], k1, k1, d[i], d[i + 1]);
+    };
+    request(g);
+    int turn = -1;  // rows this group has worked on (skipped ones do not count): its entries and slots alternate
+    for (int i = g; i < n_mine; i += G) {
+      const long long row = row0 + i * stride;
+      const int st_i = i % p.shape.stages;
+      const uint32_t ring_phase = (uint32_t)(i / p.shape.stages) & 1;
+      const int y = y_next;
+      const float tl_given = tl_next, lt_given = lt_next, l1_given = l1_next;
+      T* dr = BWD ? dlogits + row * p.ldd : nullptr;
+      const RowSlice<T> s = slice_of(row);
+      const bool aligned = BWD && (int)((reinterpret_cast<uintptr_t>(dr) & 15) / sizeof(T)) == s.lead;
+      if (skipped(y)) {
+        request(i + G);
+        if (FWD && gt == 0 && rank == 0) {
+          p.row_loss[row] = 0.0f;
+          if (p.lse) { p.lse[row] = 0.0f; p.lse[p.rows + row] = 0.0f; }
+          if (y != p.ignore_index && p.bad_id_flag) *p.bad_id_flag = 1;
+        }
+        if (BWD && !(ACC && p.accumulate)) {
+          for (int v = s.lo + gt; v < s.hi; v += GT) {
+            const int e = s.first(v);
+            if (aligned && v >= s.w0 && v < s.w1) *reinterpret_cast<uint4*>(dr + e) = make_uint4(0, 0, 0, 0);
+            else
+              for (int c = max(e, 0); c < min(e + V, n); ++c) dr[c] = from_f32<T>(0.0f);
           }
-          T* at = to + j * (THREADS * V);
-          if (v >= w0 && v < w1) {
-            if (ACC && p.accumulate) {
-              float o[V];
-              ld16(at, o);
+        }
+        ring_wait_row(ring, i, st_i, ring_phase);
+        mbar_arrive_warp(BWD ? &ring.done[st_i] : &ring.empty[st_i]);
+        continue;
+      }
+      ++turn;
+      int* s_id = reinterpret_cast<int*>(entries) + (turn & 1) * 3 * KP;
+      float* s_t = reinterpret_cast<float*>(s_id + KP);
+      float* s_x = s_t + KP;
+      float tm = -INFINITY;
+      if (want) {
+        auto entry = [&](int j, int id, float t) {
+          if (id >= n) {
+            if (FWD && p.bad_id_flag) *p.bad_id_flag = 1;
+            id = -1;
+          }
+          t = id >= 0 && j < k ? t * p.inv_t : -INFINITY;
+          s_id[j] = max(id, -1);
+          s_t[j] = t;
+          tm = fmaxf(tm, t);
+        };
 #pragma unroll
-              for (int i = 0; i < V; ++i) d[i] += o[i];
+        for (int c = 0; c < PRE; ++c) {
+          const int j = gt + c * GT;
+          if (j < KP) entry(j, j < k ? id_next[c] : (j == k ? y : -1), t_next[c]);
+        }
+        for (int j = gt + PRE * GT; j < KP; j += GT)
+          entry(j, j < k ? p.t_ids[row * k + j] : (j == k ? y : -1), j < k ? p.t_logits[row * k + j] : 0.0f);
+      }
+      request(i + G);
+      // the vectors at the row's ends, by the threads that walk over them
+      uint4 edge0 = make_uint4(0, 0, 0, 0), edge1 = edge0;
+      const bool own0 = s.w0 > s.lo && gt == 0, own1 = s.w1 < s.hi && s.hi - 1 >= s.w0 && gt == (s.hi - 1 - s.lo) % GT;
+      if (own0) edge0 = s.load_edge(s.lo);
+      if (own1) edge1 = s.load_edge(s.hi - 1);
+      uint4* vec = reinterpret_cast<uint4*>(smem + (size_t)st_i * p.shape.stage_bytes);
+      const int cnt = s.hi - s.lo;
+      ring_wait_row(ring, i, st_i, ring_phase);
+      if (own0) vec[0] = edge0;
+      if (own1) vec[cnt - 1] = edge1;
+
+      float ref = 0.0f;
+      if constexpr (FWD) {
+        float m = -INFINITY;
+        if constexpr (sizeof(T) == 2) {
+          const uint32_t lowest = 0xff80ff80u;
+          __nv_bfloat162 m2 = *reinterpret_cast<const __nv_bfloat162*>(&lowest), m3 = m2;
+#pragma unroll 4
+          for (int v = gt; v < cnt; v += GT) {
+            const uint4 r = vec[v];
+            m2 = __hmax2(m2, __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&r.x), *reinterpret_cast<const __nv_bfloat162*>(&r.y)));
+            m3 = __hmax2(m3, __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&r.z), *reinterpret_cast<const __nv_bfloat162*>(&r.w)));
+          }
+          m2 = __hmax2(m2, m3);
+          m = fmaxf(__low2float(m2), __high2float(m2));
+        } else {
+#pragma unroll 4
+          for (int v = gt; v < cnt; v += GT) {
+            const uint4 r = vec[v];
+            m = fmaxf(fmaxf(m, fmaxf(__uint_as_float(r.x), __uint_as_float(r.y))), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
+          }
+        }
+        m = warp_max(m);
+        if (lane == 0) s_max[g][0][warp] = m;
+      }
+      tm = warp_max(tm);
+      if (lane == 0) s_max[g][1][warp] = tm;
+      group_sync<GT>(g);
+      if constexpr (FWD) {
+        ref = lanes_max<GW>(s_max[g][0][lane % GW]);
+        if (ref == -INFINITY) ref = 0.0f;
+      }
+      // the teacher's sum: of exp(t - tref) = q_j S, where tref is its given log-sum-exp (S = 1) or its maximum
+      float tref = tl_given;
+      if (!p.t_lse) {
+        tref = lanes_max<GW>(s_max[g][1][lane % GW]);
+        if (tref == -INFINITY) tref = 0.0f;
+      }
+      float S = 0.0f;
+      const int e_lo = max(s.first(s.lo), 0), e_hi = min(s.first(s.hi), n);
+      if (want)
+        for (int j = gt; j <= k; j += GT) {
+          const int id = s_id[j];
+          float x = 0.0f;
+          if (id >= e_lo && id < e_hi) x = to_f32(reinterpret_cast<const T*>(vec)[id - s.first(s.lo)]);
+          else if (FWD && C > 1 && rank == 0 && id >= 0) x = to_f32(logits[row * p.ld + id]);
+          s_x[j] = x;
+          S += expf(s_t[j] - tref);
+        }
+      float st = 0.0f, s1 = 0.0f;
+      if constexpr (FWD) {
+        float sa[2] = {0.0f, 0.0f}, sb[2] = {0.0f, 0.0f};
+        with_exp<T>(p.sum_kind, ref, p.inv_t, [&](const auto& ex) {
+#pragma unroll 2
+          for (int v = gt; v < cnt; v += GT) {
+            float x[V];
+            unpack_vec<T>(vec[v], x);
+#pragma unroll
+            for (int c = 0; c < V; c += 2) {
+              float et[2], e1[2];
+              ex(x[c], x[c + 1], et, e1);
+              fadd2(sa[0], sa[1], sa[0], sa[1], et[0], et[1]);
+              if (ex.two) fadd2(sb[0], sb[1], sb[0], sb[1], e1[0], e1[1]);
             }
-            st16(at, d);
-          } else {
-            store_edge<T>(dr, view.first(v), n, d, ACC && p.accumulate);
+          }
+        });
+        st = warp_sum(sa[0] + sa[1]);
+        s1 = warp_sum(sb[0] + sb[1]);
+        if (lane == 0) { s_sum[g][0][warp] = st; s_sum[g][1][warp] = s1; }
+      }
+      S = warp_sum(S);
+      if (lane == 0) s_sum[g][2][warp] = S;
+      group_sync<GT>(g);
+      S = lanes_sum<GW>(s_sum[g][2][lane % GW]);
+      // q_j = exp(t_j - tref) * inv_s,  Q = sum of them
+      const float inv_s = p.t_lse || S == 0.0f ? 1.0f : __fdividef(1.0f, S), Q = S * inv_s;
+      if constexpr (FWD) {
+        st = lanes_sum<GW>(s_sum[g][0][lane % GW]);
+        s1 = lanes_sum<GW>(s_sum[g][1][lane % GW]);
+        if (C > 1) {
+          float(*mine)[3] = s_xch[g][turn & 1];
+          if (gt < C) {
+            const uint32_t to = mapa_cluster(smem_u32(&mine[rank][0]), gt);
+            st_cluster_f32(to, st == 0.0f ? -INFINITY : ref);  // a slice without a finite entry has no say in the maximum
+            st_cluster_f32(to + 4, st);
+            st_cluster_f32(to + 8, s1);
+            mbar_arrive_release_cluster(mapa_cluster(smem_u32(&xbar[g]), gt));
+          }
+          mbar_wait_cluster(&xbar[g], (uint32_t)(turn & 1), &ring.abort_flag);
+          float gm = -INFINITY;
+          for (int r = 0; r < C; ++r) gm = fmaxf(gm, mine[r][0]);
+          ref = gm == -INFINITY ? 0.0f : gm;
+          st = s1 = 0.0f;
+          for (int r = 0; r < C; ++r) {
+            const float d = mine[r][0] - ref;
+            st += mine[r][1] * expf(d * p.inv_t);
+            s1 += mine[r][2] * expf(d);
           }
         }
+        if (warp == GW - 1 && rank == 0) {
+          const float lt = ref * p.inv_t + logf(st);
+          const float l1 = p.sum_kind == ONE ? (p.temperature == 1.0f ? lt : 0.0f) : ref + logf(s1);
+          const float tl = p.t_lse || S == 0.0f ? tref : tref + logf(S);  // ln q_j = t_j - tl
+          float kl = 0.0f;
+          for (int j = lane; j < k; j += 32) {
+            const float t = s_t[j], q = expf(t - tl);
+            if (q > 0.0f || q != q) kl += q * (t - tl - (s_x[j] * p.inv_t - lt));
+          }
+          kl = warp_sum(kl);
+          if (lane == 0) {
+            float l = 0.0f;
+            if (has_kd) l = p.kd_weight * p.temperature * p.temperature * kl;
+            if (has_ce) l -= p.ce_weight * logf(expf(s_x[k] - l1) + 1e-8f);
+            p.row_loss[row] = l;
+            if (p.lse) { p.lse[row] = lt; p.lse[p.rows + row] = l1; }
+          }
+        }
+      } else {
+        ref = l1_given;
       }
-    });
-    __syncthreads();
-    // entries of this slice with a term of their own: the first of equal ids collects the probabilities of all
-    const int e_lo = max(view.first(lo), 0), e_hi = min(view.first(hi), n);
-    for (int j = tid; j <= k; j += THREADS) {
-      const int id = s_id[j];
-      if (id < e_lo || id >= e_hi) continue;
-      int same = 0;
-      for (int i = 0; i <= k; i += 4) {
-        const int4 o = *reinterpret_cast<const int4*>(s_id + i);
-        same += (o.x == id) + (o.y == id) + (o.z == id) + (o.w == id);
+      if constexpr (!BWD) {
+        fence_proxy_async_smem();  // the vectors at the ends, before a copy takes their place
+        mbar_arrive_warp(&ring.empty[st_i]);
+      } else {
+        // d = kt exp((x - ref) / T) + k1 exp(x - ref): kt, k1 turn the exponentials into weighted probabilities
+        const float kq = has_kd ? p.kd_weight * p.temperature * g_out : 0.0f, c1 = has_ce ? p.ce_weight * g_out : 0.0f;
+        float kt = 0.0f, k1 = 0.0f;
+        if (has_kd) kt = FWD ? __fdividef(kq * Q, st) : kq * Q * expf(ref * p.inv_t - lt_given);
+        if (has_ce) k1 = FWD ? __fdividef(c1, p.grad_kind == ONE ? st : s1) : c1;
+        if (p.grad_kind == ONE) { kt += k1; k1 = 0.0f; }  // temperature 1: one exponential for both terms
+        const bool acc = ACC && p.accumulate;
+        with_exp<T>(p.grad_kind, ref, p.inv_t, [&](const auto& ex) {
+#pragma unroll 2
+          for (int v = gt; v < cnt; v += GT) {
+            float d[V];
+            unpack_vec<T>(vec[v], d);
+#pragma unroll
+            for (int c = 0; c < V; c += 2) {
+              float et[2], e1[2];
+              ex(d[c], d[c + 1], et, e1);
+              fmul2(d[c], d[c + 1], et[0], et[1], kt, kt);
+              if (ex.two) ffma2(d[c], d[c + 1], e1[0], e1[1], k1, k1, d[c], d[c + 1]);
+            }
+            if (acc) {
+              const int e = s.first(s.lo + v);
+              if (aligned && s.lo + v >= s.w0 && s.lo + v < s.w1) {
+                float o[V];
+                ld16(dr + e, o);
+#pragma unroll
+                for (int c = 0; c < V; ++c) d[c] += o[c];
+              } else {
+#pragma unroll
+                for (int c = 0; c < V; ++c)
+                  if (e + c >= 0 && e + c < n) d[c] += to_f32(dr[e + c]);
+              }
+            }
+            st16(reinterpret_cast<T*>(vec + v), d);
+          }
+        });
+        group_sync<GT>(g);
+        T* out = reinterpret_cast<T*>(vec) - s.first(s.lo);  // out[id]: the entry of this slice
+        for (int j = gt; j <= k; j += GT) {
+          const int id = s_id[j];
+          if (id < e_lo || id >= e_hi) continue;
+          int same = 0;
+          for (int c = 0; c <= k; c += 4) {
+            const int4 o = *reinterpret_cast<const int4*>(s_id + c);
+            same += (o.x == id) + (o.y == id) + (o.z == id) + (o.w == id);
+          }
+          float w = j < k ? expf(s_t[j] - tref) : 0.0f;
+          if (same > 1) {
+            int c = 0;
+            while (s_id[c] != id) ++c;
+            if (c < j) continue;
+            w = 0.0f;
+            for (; c < k; ++c)
+              if (s_id[c] == id) w += expf(s_t[c] - tref);
+          }
+          float d = 0.0f;
+          with_exp<T>(p.grad_kind, ref, p.inv_t, [&](const auto& ex) {
+            float et[2], e1[2];
+            ex(s_x[j], s_x[j], et, e1);
+            d = kt * et[0] + k1 * e1[0];
+          });
+          if (has_kd) d -= kq * w * inv_s;
+          if (id == y) d -= c1;
+          if (acc) d += to_f32(dr[id]);
+          out[id] = from_f32<T>(d);
+        }
+        if (!aligned || s.edges()) {
+          group_sync<GT>(g);
+          if (!aligned) {
+            for (int e = e_lo + gt; e < e_hi; e += GT) dr[e] = out[e];
+          } else {
+            const int a = min(s.first(s.w0), e_hi), b = max(s.first(s.w1), a);
+            for (int e = e_lo + gt; e < a; e += GT) dr[e] = out[e];
+            for (int e = b + gt; e < e_hi; e += GT) dr[e] = out[e];
+          }
+        }
+        fence_proxy_async_smem();
+        mbar_arrive_warp(&ring.done[st_i]);
       }
-      float w = j < k ? expf(s_t[j] - tref) : 0.0f;
-      if (same > 1) {
-        int i = 0;
-        while (s_id[i] != id) ++i;
-        if (i < j) continue;
-        w = 0.0f;
-        for (; i < k; ++i)
-          if (s_id[i] == id) w += expf(s_t[i] - tref);
-      }
-      float d = 0.0f;
-      with_exp<T>(p.grad_kind, ref, p.inv_t, [&](const auto& ex) {
-        float et[2], e1[2];
-        ex(s_x[j], s_x[j], et, e1);
-        d = kt * et[0] + k1 * e1[0];
-      });
-      if (has_kd) d -= kq * w * inv_s;
-      if (id == y) d -= c1;
-      if (ACC && p.accumulate) d += s_old[j];
-      dr[id] = from_f32<T>(d);
     }
+  }
+  if (ring.abort_flag)
+    for (int i = 0; i < 64; ++i) __nanosleep(1000);  // copies in flight end before the CTA does
+  if (C > 1) {
+    __syncwarp();
+    cluster_sync_all();  // nobody leaves while a peer may still write to it
   }
 }
 
@@ -715,24 +801,26 @@ int distill_sizes(const char* what, long long rows, long long vocab, long long k
   return fail(EISEN_ERR_LIMIT, msg);
 }
 
-// Rows of up to 8 slices of 4096 vectors (262144 bf16 or 131072 f32 entries) stay in registers; longer ones take
-// distill_kernel, which reads them a second time.  Short rows in numbers get CTAs of 128 threads, whose barriers are
-// cheaper; few rows get more threads and CTAs each.
+// One warp per row for short rows in numbers, groups of 128 or 256 threads for longer ones (a group's reductions cost
+// the same whatever its row), all of a CTA's threads where there is at most one row per CTA.  Rows that do not fit the
+// shared memory of eight CTAs take distill_kernel, which reads them a second time.
 template <typename T, int MODE>
 int distill_launch(const char* what, DistillParams& p, cudaStream_t s) {
-  const long long vectors = (p.vocab + VecOf<T>::N - 1) / VecOf<T>::N + 1;  // one more for a row that starts inside one
-  const bool few = p.rows < 2LL * sm_count();
-  p.cluster = cluster_for_row(p.rows, vectors, 4096, 512);
-  if (!p.cluster) {
-    distill_kernel<T, MODE><<<(unsigned)p.rows, DS_THREADS, 0, s>>>(p);
-    return check_launch(what);
+  const long long bytes = (long long)p.vocab * sizeof(T);
+  auto shape = [&](int groups, int least) {
+    p.shape = row_shape(p.rows, p.vocab, sizeof(T), entry_bytes(p.k, groups), std::max(2 * groups, 3), least);
+    return p.shape.stages >= groups;
+  };
+  if (p.rows > 2LL * sm_count()) {
+    if (bytes <= 4096 && p.k <= 128 && shape(16, 1 << 30))
+      return launch_pipe<distill_pipe_kernel<T, 32, 16, MODE>>(what, p.shape, p.rows, pipe_threads(32, 16), s, p);
+    if (bytes <= 24 * 1024 && shape(4, 1 << 30))
+      return launch_pipe<distill_pipe_kernel<T, 128, 4, MODE>>(what, p.shape, p.rows, pipe_threads(128, 4), s, p);
+    if (shape(2, 1 << 30)) return launch_pipe<distill_pipe_kernel<T, 256, 2, MODE>>(what, p.shape, p.rows, pipe_threads(256, 2), s, p);
   }
-  const long long per = (vectors + p.cluster - 1) / p.cluster;
-  if (!few && per <= 256) return launch_rows(distill_row_kernel<T, 128, 2, MODE>, what, p.rows, p.cluster, 128, s, p);
-  if (!few && per <= 1024) return launch_rows(distill_row_kernel<T, 128, 8, MODE>, what, p.rows, p.cluster, 128, s, p);
-  if (per <= 1024) return launch_rows(distill_row_kernel<T, 256, 4, MODE>, what, p.rows, p.cluster, 256, s, p);
-  if (per <= 2048) return launch_rows(distill_row_kernel<T, 256, 8, MODE>, what, p.rows, p.cluster, 256, s, p);
-  return launch_rows(distill_row_kernel<T, 256, 16, MODE>, what, p.rows, p.cluster, 256, s, p);
+  if (shape(1, 8192)) return launch_pipe<distill_pipe_kernel<T, 512, 1, MODE>>(what, p.shape, p.rows, pipe_threads(512, 1), s, p);
+  distill_kernel<T, MODE><<<(unsigned)p.rows, DS_THREADS, 0, s>>>(p);
+  return check_launch(what);
 }
 
 int distill_run(const char* what, int mode, DistillParams& p, int dtype, cudaStream_t s) {

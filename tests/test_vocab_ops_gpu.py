@@ -315,6 +315,23 @@ def test_distill_in_place_accumulate_and_upstream_gradient(dtype, vocab):
     assert ((acc.double() - want).abs() <= c.d_tol + STEP[dtype] * (want.abs() + c.d_tol)).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab,k,ignored", [(1500, 700, 5, 0.5), (3000, 1001, 100, 0.05), (1111, 8200, 64, 0.6), (900, 5003, 3, 0.0),
+                                                  (700, 32000, 64, 0.4), (601, 24001, 700, 0.1), (400, 100003, 20, 0.3), (333, 50, 1024, 0.3)])
+def test_distill_many_rows(dtype, rows, vocab, k, ignored):
+    """Several rows per CTA, with rows in between that do not count."""
+    c = Case(dtype, rows, vocab, k, 2.0, 0.5, 0.5, ignored=ignored).expected()
+    d = torch.full_like(c.x, 5.0)
+    loss, row, lse = c.fused(d)
+    c.check_loss(loss, row, lse)
+    c.check_grad(d)
+    loss, row, lse = c.fwd()
+    c.check_loss(loss, row, lse)
+    d.fill_(5.0)
+    c.bwd(lse, d)
+    c.check_grad(d)
+
+
 def test_distill_without_targets_and_without_lse():
     c = Case(torch.float32, 5, 777, 6, 2.0, 0.8, 0.0).expected(targets=False)
     d = torch.empty_like(c.x)
