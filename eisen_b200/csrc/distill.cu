@@ -11,6 +11,9 @@
 #include <algorithm>
 #include <cfloat>
 #include <cstdio>
+#include <type_traits>
+
+#include <cuda_fp16.h>
 
 #include "common.cuh"
 #include "errors.h"
@@ -337,243 +340,484 @@ distill_kernel(const DistillParams p) {
   }
 }
 
-// A row's exponentials exp((x - ref) / T) and exp(x - ref).  KIND says how they are formed:
-//   ONE   the first alone (temperature 1, or no cross-entropy term)
-//   TWO   both, each by itself
-//   PLAIN the f32 form, (x - ref) first and expf: rows of f32 logits, and rows whose largest entry is near the end of
-//         the type's range (all of it masked by the lowest value), where the products with ref would overflow
-//   10 a + b   bf16 rows whose temperature is b / a: h = exp((x - ref) / b), the exponentials are h^a and h^b.  The
-//         special-function unit gives 16 results per clock and SM: two exponentials in both passes over a row are 8000
-//         clocks per 32000 entries where the memory needs 5600, one is 4000.  A power multiplies the relative error of
-//         h (2^-22) by at most 7, far below the 2^-8 of the bf16 result.
-constexpr int ONE = 0, TWO = 1, PLAIN = 2;
+// A row's exponentials et = exp((x - ref) / T) and e1 = exp(x - ref).  KIND says how they are formed:
+//   ONE     et alone (temperature 1, or no cross-entropy term and one log-sum-exp), as h^2 with h = exp((x - ref) / 2T)
+//   3 .. 8  bf16 rows with 2T a whole number: et = h^2, e1 = h^2T with the same h
+//   TWO     both, each by itself
+//   PLAIN1, PLAIN2   (x - ref) first and expf, et alone or both: rows of f32 logits, and rows whose largest entry is near
+//           the end of the type's range (all of it masked by the lowest value), where the products with ref would overflow
+// The special-function unit gives 16 results per clock and SM, 2000 clocks for 32000 entries.  Two exponentials in both
+// passes over a row would take 8000 where the memory needs 5600.  So the first pass of the fused form leaves h in the
+// row's place in shared memory for the second: f32 rows keep et itself, bf16 rows h in fp16 (half a step is 2^-11 of h;
+// et has twice that, a quarter of bf16's own half step, e1 2T <= 8 times, at most as much as bf16's half step).  h, not its square, so that fp16's
+// range covers et down to 2^-38 (2T = 8) or 2^-54 (2T <= 3) of the row's largest; smaller ones fade to 0.
+constexpr int ONE = 2, TWO = 1, PLAIN1 = 10, PLAIN2 = 11;
 
 template <typename T, int KIND>
 struct RowExp {
+  static constexpr bool ROOT = KIND >= ONE && KIND <= 8;
+  static constexpr bool BOTH = KIND != ONE && KIND != PLAIN1;
+  static constexpr bool KEEPS = sizeof(T) == 4 ? KIND == PLAIN1 : ROOT;  // what the first pass leaves serves the second
+  // h is held times 2^Z: et comes out times 2^2Z, e1 times 2^(KIND Z) (at most 2^40, so that a row's sum and its
+  // reciprocal stay in range)
+  static constexpr int Z = !ROOT ? 0 : 40 / KIND < 13 ? 40 / KIND : 13;
+  static constexpr float scale_t = 1.0f / (float)(1ll << (2 * Z)), scale_1 = 1.0f / (float)(1ll << (ROOT ? KIND * Z : 0));
   float ref, inv_t, c, off, off1;
-  bool two;
-  __device__ __forceinline__ RowExp(float r, float it, bool both) : ref(r), inv_t(it), two(both) {
-    c = 1.4426950408889634f * (KIND < 10 ? it : 1.0f / (float)(KIND % 10));
-    off = -r * c;
+  __device__ __forceinline__ RowExp(float r, float it) : ref(r), inv_t(it) {
+    c = 1.4426950408889634f * (ROOT ? 0.5f * it : it);
+    off = (float)Z - r * c;
     off1 = -r * 1.4426950408889634f;
   }
-  // the exponentials of two elements, in packed arithmetic: et = exp((x - ref) / T), e1 = exp(x - ref)
-  __device__ __forceinline__ void operator()(float x, float y, float (&et)[2], float (&e1)[2]) const {
-    if constexpr (KIND == PLAIN) {
-      et[0] = expf((x - ref) * inv_t);
-      et[1] = expf((y - ref) * inv_t);
-      e1[0] = two ? expf(x - ref) : 0.0f;
-      e1[1] = two ? expf(y - ref) : 0.0f;
+  // h of two elements, or et itself where there is no root
+  __device__ __forceinline__ void root(float x, float y, float& h0, float& h1) const {
+    if constexpr (KIND >= PLAIN1) {
+      h0 = expf((x - ref) * inv_t);
+      h1 = expf((y - ref) * inv_t);
     } else {
-      float h0, h1;
       ffma2(h0, h1, x, y, c, c, off, off);
       h0 = exp2_approx(h0);
       h1 = exp2_approx(h1);
-      if constexpr (KIND == ONE) {
-        et[0] = h0; et[1] = h1;
-        e1[0] = e1[1] = 0.0f;
-      } else if constexpr (KIND == TWO) {
-        et[0] = h0; et[1] = h1;
-        ffma2(h0, h1, x, y, 1.4426950408889634f, 1.4426950408889634f, off1, off1);
-        e1[0] = exp2_approx(h0);
-        e1[1] = exp2_approx(h1);
-      } else {
-        constexpr int A = KIND / 10, B = KIND % 10;
-        float s0, s1, f0, f1;  // h^2, h^4
-        fmul2(s0, s1, h0, h1, h0, h1);
-        if constexpr (B >= 4) fmul2(f0, f1, s0, s1, s0, s1);
-        et[0] = A == 1 ? h0 : s0;
-        et[1] = A == 1 ? h1 : s1;
-        if constexpr (B == 1) { e1[0] = h0; e1[1] = h1; }
-        else if constexpr (B == 2) { e1[0] = s0; e1[1] = s1; }
-        else if constexpr (B == 3) fmul2(e1[0], e1[1], s0, s1, h0, h1);
-        else if constexpr (B == 4) { e1[0] = f0; e1[1] = f1; }
-        else if constexpr (B == 5) fmul2(e1[0], e1[1], f0, f1, h0, h1);
-        else {
-          fmul2(f0, f1, f0, f1, s0, s1);
-          fmul2(e1[0], e1[1], f0, f1, h0, h1);
-        }
-      }
+    }
+  }
+  __device__ __forceinline__ void powers(float h0, float h1, float (&et)[2], float (&e1)[2]) const {
+    if constexpr (!ROOT) {
+      et[0] = h0; et[1] = h1;
+    } else {
+      fmul2(et[0], et[1], h0, h1, h0, h1);
+      float f0, f1;  // h^4
+      if constexpr (KIND >= 4) fmul2(f0, f1, et[0], et[1], et[0], et[1]);
+      if constexpr (KIND == 3) fmul2(e1[0], e1[1], et[0], et[1], h0, h1);
+      else if constexpr (KIND == 4) { e1[0] = f0; e1[1] = f1; }
+      else if constexpr (KIND == 5) fmul2(e1[0], e1[1], f0, f1, h0, h1);
+      else if constexpr (KIND == 6) fmul2(e1[0], e1[1], f0, f1, et[0], et[1]);
+      else if constexpr (KIND == 7) {
+        fmul2(f0, f1, f0, f1, et[0], et[1]);
+        fmul2(e1[0], e1[1], f0, f1, h0, h1);
+      } else if constexpr (KIND == 8) fmul2(e1[0], e1[1], f0, f1, f0, f1);
+    }
+  }
+  __device__ __forceinline__ void both(float x, float y, float (&et)[2], float (&e1)[2]) const {
+    float h0, h1;
+    root(x, y, h0, h1);
+    powers(h0, h1, et, e1);
+    apart(x, y, e1);
+  }
+  // e1 where it does not come from h
+  __device__ __forceinline__ void apart(float x, float y, float (&e1)[2]) const {
+    if constexpr (KIND == TWO) {
+      ffma2(e1[0], e1[1], x, y, 1.4426950408889634f, 1.4426950408889634f, off1, off1);
+      e1[0] = exp2_approx(e1[0]);
+      e1[1] = exp2_approx(e1[1]);
+    } else if constexpr (KIND == PLAIN2) {
+      e1[0] = expf(x - ref);
+      e1[1] = expf(y - ref);
     }
   }
 };
 
-// f(RowExp) for the kind that the row takes: one branch per pass, the same for the whole CTA
+// f(RowExp) for the kind that the row takes: one branch per pass, the same for all of its threads
 template <typename T, typename F>
 __device__ __forceinline__ void with_exp(int kind, float ref, float inv_t, F f) {
   if constexpr (sizeof(T) == 4) {
-    f(RowExp<T, PLAIN>(ref, inv_t, kind != ONE));
+    if (kind == ONE) f(RowExp<T, PLAIN1>(ref, inv_t));
+    else f(RowExp<T, PLAIN2>(ref, inv_t));
   } else {
-    if (fabsf(ref) > 1e30f) return f(RowExp<T, PLAIN>(ref, inv_t, kind != ONE));
+    if (fabsf(ref) > 1e30f) {
+      if (kind == ONE) f(RowExp<T, PLAIN1>(ref, inv_t));
+      else f(RowExp<T, PLAIN2>(ref, inv_t));
+      return;
+    }
     switch (kind) {
-      case ONE: return f(RowExp<T, ONE>(ref, inv_t, false));
-      case TWO: return f(RowExp<T, TWO>(ref, inv_t, true));
-      case 12: return f(RowExp<T, 12>(ref, inv_t, true));
-      case 13: return f(RowExp<T, 13>(ref, inv_t, true));
-      case 14: return f(RowExp<T, 14>(ref, inv_t, true));
-      case 21: return f(RowExp<T, 21>(ref, inv_t, true));
-      case 23: return f(RowExp<T, 23>(ref, inv_t, true));
-      case 25: return f(RowExp<T, 25>(ref, inv_t, true));
-      default: return f(RowExp<T, 27>(ref, inv_t, true));
+      case ONE: return f(RowExp<T, ONE>(ref, inv_t));
+      case 3: return f(RowExp<T, 3>(ref, inv_t));
+      case 4: return f(RowExp<T, 4>(ref, inv_t));
+      case 5: return f(RowExp<T, 5>(ref, inv_t));
+      case 6: return f(RowExp<T, 6>(ref, inv_t));
+      case 7: return f(RowExp<T, 7>(ref, inv_t));
+      case 8: return f(RowExp<T, 8>(ref, inv_t));
+      default: return f(RowExp<T, TWO>(ref, inv_t));
     }
   }
 }
 
-// the kind for both exponentials at a temperature
+// the kind for both exponentials at a temperature other than 1
 int exp_kind(float temperature, int dtype) {
   if (dtype == DT_BF16)
-    for (int a = 1; a <= 2; ++a)
-      for (int b = 1; b <= (a == 1 ? 4 : 7); ++b)
-        if ((a == 1 || b % 2) && temperature * (float)a == (float)b && temperature != 1.0f) return 10 * a + b;
+    for (int b = 3; b <= 8; ++b)
+      if (temperature * 2.0f == (float)b) return b;
   return TWO;
 }
 
-// The frame of row_pipe.cuh with a row's work in one group of GT threads:
-//   maximum -> sums of the exponentials -> gradient over the logits in shared memory -> the entries with a term of
-//   their own (the teacher's ids and the target; the first of equal ids collects the probabilities of all).
-// The exponentials are taken again for the gradient.  A row's ids, teacher logits and target are requested while the
-// row before it is worked on.
-constexpr int pipe_threads(int gt, int groups) { return gt * groups + RP_EXTRA; }
+// what the first pass leaves for the second: fp16 in the place of bf16, f32 in that of f32
+template <typename T>
+__device__ __forceinline__ uint4 keep_vec(const float (&x)[VecOf<T>::N]) {
+  uint32_t u[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 2) {
+      const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+      u[i] = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      u[i] = __float_as_uint(x[i]);
+    }
+  }
+  return make_uint4(u[0], u[1], u[2], u[3]);
+}
+template <typename T>
+__device__ __forceinline__ void kept_vec(const uint4& r, float (&x)[VecOf<T>::N]) {
+  const uint32_t u[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 2) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    } else {
+      x[i] = __uint_as_float(u[i]);
+    }
+  }
+}
+
+// The frame of row_pipe.cuh.  A group of GT threads walks over its row three times: maximum, sums of the exponentials,
+// gradient over the logits in shared memory.  Beside it two warps see to what the row has of single entries: one reads, a
+// row ahead, the teacher's ids and logits and forms their distribution; the other one, when the group has been through
+// the row, forms the loss and rewrites the entries that have a term of their own, the ids and the target.  In the
+// group's hands these were half of a row's time, latency after latency with most of its threads idle.
+constexpr int pipe_threads(int gt, int groups) { return (gt + 64) * groups + RP_EXTRA; }
 __host__ __device__ constexpr int entry_pad(int k) { return (k + 4) & ~3; }
-constexpr int entry_bytes(int k, int groups) { return groups * 2 * 3 * entry_pad(k) * 4; }
+// slots of the table that finds equal ids: at least twice the entries
+__host__ __device__ constexpr int entry_slots(int k) {
+  int n = 64;
+  while (n < 2 * k) n *= 2;
+  return n;
+}
+__host__ __device__ constexpr int entry_bytes(int k) { return 2 * 4 * 4 * entry_pad(k) + 2 * entry_slots(k); }
+
+// A row's entries in shared memory (two sets per group: one in use, one being read).
+struct Entries {
+  int* id;   // the teacher's ids, -1: absent or beyond the vocabulary
+  float* t;  // its logits / T
+  float* x;  // the student's logits there
+  float* w;  // exp(t - tref), of all equal ids in one of them; -1 in the others
+  __device__ __forceinline__ Entries(uint8_t* p, int set, int pad) {
+    id = reinterpret_cast<int*>(p) + set * 4 * pad;
+    t = reinterpret_cast<float*>(id + pad);
+    x = t + pad;
+    w = x + pad;
+  }
+};
+struct RowTeacher {  // exp(t - tref) = q_j S;  Q = sum of the q_j
+  float tref, S, Q;
+};
+struct RowStats {  // what the group found
+  float ref, kt, k1, lt, l1;
+};
 
 template <typename T, int GT, int G, int MODE>
-__global__ void __launch_bounds__(GT * G + RP_EXTRA, 1)
+__global__ void __launch_bounds__((GT + 64) * G + RP_EXTRA, 1)
 distill_pipe_kernel(const DistillParams p) {
   constexpr int V = VecOf<T>::N, GW = GT / 32;
-  constexpr int PRE = GT >= 128 ? 1 : 4;  // entries per thread requested a row ahead
   constexpr bool FWD = (MODE & DS_FWD) != 0, BWD = (MODE & DS_BWD) != 0, ACC = BWD && !FWD;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ RowRing ring;
-  __shared__ uint64_t xbar[G];
-  __shared__ float s_max[G][2][GW], s_sum[G][3][GW];
+  // a row's entries, its statistics and the barriers around them alternate between two sets
+  __shared__ uint64_t ready[G][2];     // the entries are prepared
+  __shared__ uint64_t through[G][2];   // the group is through the row (its warps)
+  __shared__ uint64_t finished[G][2];  // its entries are rewritten, the loss is formed: the set is free
+  __shared__ uint64_t xbar[G];         // the slices of a row have met (C arrivals)
+  __shared__ float s_red[G][3][GW];
+  __shared__ RowTeacher s_teacher[G][2];
+  __shared__ RowStats s_stats[G][2];
   __shared__ float s_xch[G][2][8][3];
   const int tid = threadIdx.x, lane = tid & 31;
-  const int C = p.shape.cluster, k = p.k, n = p.vocab, KP = entry_pad(k);
+  const int C = p.shape.cluster, k = p.k, n = p.vocab;
   const int rank = C > 1 ? (int)cluster_ctarank() : 0;
-  const long long row0 = blockIdx.x / C, stride = gridDim.x / C;
+  const long long row0 = blockIdx.x >> p.shape.cluster_log2, stride = gridDim.x >> p.shape.cluster_log2;
   const int n_mine = row0 < p.rows ? (int)((p.rows - row0 + stride - 1) / stride) : 0;
-  ring_init(ring, p.shape.stages, BWD ? 1 : GW, GW);
+  ring_init(ring, p.shape.stages, BWD ? 1 : GW, 1);
   if (tid == 0) {
-    for (int g = 0; g < G; ++g) mbar_init(&xbar[g], C);
+    for (int g = 0; g < G; ++g) {
+      mbar_init(&xbar[g], C);
+      for (int set = 0; set < 2; ++set) {
+        mbar_init(&ready[g][set], 1);
+        mbar_init(&through[g][set], GW);
+        mbar_init(&finished[g][set], 1);
+      }
+    }
     fence_mbar_init();
   }
   __syncthreads();
   if (C > 1) cluster_sync_all();
   const T* logits = reinterpret_cast<const T*>(p.logits);
   T* dlogits = reinterpret_cast<T*>(p.dlogits);
-  auto slice_of = [&](long long row) { return RowSlice<T>(logits + row * p.ld, n, rank, C); };
+  const bool has_kd = p.kd_weight != 0.0f, has_ce = p.ce_weight != 0.0f;
+  const float g_out = p.grad_scale * (BWD && p.grad_out ? *p.grad_out : 1.0f);
+  const float kq = has_kd ? p.kd_weight * p.temperature * g_out : 0.0f, c1 = has_ce ? p.ce_weight * g_out : 0.0f;
+  const bool acc = ACC && p.accumulate;
+  auto slice_of = [&](long long row) { return RowSlice<T>(logits + row * p.ld, n, rank, p.shape.cluster_log2); };
   auto skipped = [&](int y) { return p.targets && (y == p.ignore_index || y < 0 || y >= n); };
   auto skip_row = [&](long long row) { return p.targets && skipped(p.targets[row]); };
+  // dlogits' row starts like the logits' row: whole vectors go there as they are
+  auto like = [&](const RowSlice<T>& s, const T* dr) { return (int)(((uint32_t)reinterpret_cast<uintptr_t>(dr) & 15) / sizeof(T)) == s.lead; };
+  constexpr int ENTRY0 = GT * G, LOAD0 = ENTRY0 + 64 * G;
 
-  if (tid >= GT * G + 32) {
+  if (tid >= LOAD0 + 32) {
     if constexpr (BWD)
       ring_store<T>(ring, smem, p.shape.stages, p.shape.stage_bytes, n_mine, row0, stride, slice_of, skip_row,
                     [&](long long row) { return dlogits + row * p.ldd; });
-  } else if (tid >= GT * G) {
+  } else if (tid >= LOAD0) {
     ring_load<T>(ring, smem, p.shape.stages, p.shape.stage_bytes, n_mine, row0, stride, slice_of, skip_row);
-  } else {
-    const int g = tid / GT, gt = tid % GT, warp = gt >> 5;
-    uint8_t* entries = smem + (size_t)p.shape.stages * p.shape.stage_bytes + (size_t)g * (2 * 3 * 4) * KP;
-    const bool has_kd = p.kd_weight != 0.0f, has_ce = p.ce_weight != 0.0f;
-    const float g_out = p.grad_scale * (BWD && p.grad_out ? *p.grad_out : 1.0f);
-    const bool want = BWD || rank == 0;  // this CTA looks at the teacher's entries
-    int y_next = -1, id_next[PRE];
-    float t_next[PRE], tl_next = 0.0f, lt_next = 0.0f, l1_next = 0.0f;
-    auto request = [&](int i) {
-      if (i >= n_mine) return;
-      const long long row = row0 + i * stride;
-      y_next = p.targets ? p.targets[row] : -1;
-      if (p.t_lse) tl_next = p.t_lse[row];
-      if constexpr (!FWD) { lt_next = p.lse[row]; l1_next = p.lse[p.rows + row]; }
+  } else if (tid >= ENTRY0) {
+    // ---------------- the two entry warps of group g ----------------
+    const int g = (tid - ENTRY0) / 64;
+    const bool preparing = ((tid - ENTRY0) & 32) == 0;
+    const int KP = entry_pad(k), slots = entry_slots(k);
+    uint8_t* mine = smem + (size_t)p.shape.stages * p.shape.stage_bytes + (size_t)g * entry_bytes(k);
+    uint16_t* table = reinterpret_cast<uint16_t*>(mine + 2 * 4 * 4 * KP);
+    const bool want = BWD || rank == 0;  // this CTA has use for the entries
+    // the next row from i on that counts; n_mine or more: none
+    auto next_row = [&](int i, int& y) {
+      y = -1;
+      for (; i < n_mine; i += G) {
+        if (p.targets) y = p.targets[row0 + (long long)i * stride];
+        if (!skipped(y)) break;
+      }
+      return i;
+    };
+    auto prepare = [&](int i, int y, int set) {
+      const long long row = row0 + (long long)i * stride;
+      const T* xr = logits + row * p.ld;
+      const Entries e(mine, set, KP);
+      float ref = -INFINITY;
+      if (lane == 0) e.x[k] = y >= 0 ? to_f32(xr[y]) : 0.0f;
+      for (int j0 = lane; j0 < k; j0 += 128) {  // four entries' loads at a time
+        int id[4];
+        float t[4], x[4];
 #pragma unroll
-      for (int c = 0; c < PRE; ++c) {
-        const int j = gt + c * GT;
-        id_next[c] = -1;
-        t_next[c] = 0.0f;
-        if (want && j < k) {
-          id_next[c] = p.t_ids[row * k + j];
-          t_next[c] = p.t_logits[row * k + j];
+        for (int c = 0; c < 4; ++c) {
+          const int j = j0 + 32 * c;
+          id[c] = j < k ? p.t_ids[row * k + j] : -1;
+          t[c] = j < k ? p.t_logits[row * k + j] : 0.0f;
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          if (id[c] >= n) {
+            if (FWD && p.bad_id_flag) *p.bad_id_flag = 1;
+            id[c] = -1;
+          }
+          id[c] = max(id[c], -1);
+          x[c] = id[c] >= 0 ? to_f32(xr[id[c]]) : 0.0f;
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int j = j0 + 32 * c;
+          if (j < k) {
+            t[c] = id[c] >= 0 ? t[c] * p.inv_t : -INFINITY;
+            e.id[j] = id[c];
+            e.t[j] = t[c];
+            e.x[j] = x[c];
+            ref = fmaxf(ref, t[c]);
+          }
         }
       }
+      // exp(t - ref) = q_j S, where ref is the teacher's given log-sum-exp (S = 1) or its maximum
+      if (p.t_lse) {
+        ref = p.t_lse[row];
+      } else {
+        ref = warp_max(ref);
+        if (ref == -INFINITY) ref = 0.0f;
+      }
+      if constexpr (BWD)
+        for (int c = lane; c < slots / 8; c += 32) reinterpret_cast<uint4*>(table)[c] = make_uint4(~0u, ~0u, ~0u, ~0u);
+      __syncwarp();
+      float S = 0.0f;
+      bool again = false;
+      for (int j = lane; j < k; j += 32) {
+        const float w = expf(e.t[j] - ref);
+        S += w;
+        if constexpr (BWD) {
+          // equal ids find the same slot: whoever came first there stands for all of them (who it is does not matter)
+          const int id = e.id[j];
+          bool first = id >= 0;
+          if (id >= 0) {
+            int h = (int)(((uint32_t)id * 0x9e3779b1u) >> 16) & (slots - 1);
+            for (int tries = 0; tries < slots; ++tries) {
+              const uint16_t o = atomicCAS(table + h, (uint16_t)0xffff, (uint16_t)j);
+              if (o == 0xffff) break;
+              if (e.id[o] == id) { first = false; again = true; break; }
+              h = (h + 1) & (slots - 1);
+            }
+          }
+          e.w[j] = first ? w : -1.0f;
+        }
+      }
+      if (BWD && __any_sync(0xffffffffu, again)) {
+        __syncwarp();
+        for (int j = lane; j < k; j += 32)
+          if (e.w[j] != -1.0f) {  // in the order of the entries, so that the sum is the same every time
+            float w = 0.0f;
+            for (int c = 0; c < k; ++c)
+              if (e.id[c] == e.id[j]) w += expf(e.t[c] - ref);
+            e.w[j] = w;
+          }
+      }
+      S = warp_sum(S);
+      if (lane == 0) s_teacher[g][set] = {ref, S, p.t_lse || S == 0.0f ? S : 1.0f};
+    };
+    int y;
+    int i = next_row(g, y);
+    int stage = g, stage_i = g;  // stage of row i
+    for (int turn = 0; i < n_mine; ++turn) {
+      const int set = turn & 1;
+      const uint32_t phase = (uint32_t)(turn >> 1) & 1;
+      int y_after;
+      const int after = next_row(i + G, y_after);
+      if (preparing) {
+        if (turn >= 2) mbar_wait(&finished[g][set], phase ^ 1, &ring.abort_flag, nullptr, FAULT_WAIT_EMPTY);
+        if (want) prepare(i, y, set);
+        mbar_arrive_warp(&ready[g][set]);
+        i = after;
+        y = y_after;
+        continue;
+      }
+      while (stage_i < i) {
+        stage_i += G;
+        stage += G;
+        if (stage >= p.shape.stages) stage -= p.shape.stages;
+      }
+      mbar_wait(&ready[g][set], phase, &ring.abort_flag, nullptr, FAULT_WAIT_FULL);
+      mbar_wait(&through[g][set], phase, &ring.abort_flag, nullptr, FAULT_WAIT_FULL);
+      const long long row = row0 + (long long)i * stride;
+      const Entries e(mine, set, KP);
+      const RowStats st = s_stats[g][set];
+      const RowTeacher te = s_teacher[g][set];
+      const float S = te.S, inv_s = p.t_lse || S == 0.0f ? 1.0f : 1.0f / S;
+      if (FWD && rank == 0) {
+        const float tl = p.t_lse || S == 0.0f ? te.tref : te.tref + logf(S);  // ln q_j = t_j - tl
+        float kl = 0.0f;
+        for (int j = lane; j < k; j += 32) {
+          const float t = e.t[j], q = expf(t - tl);
+          if (q > 0.0f || q != q) kl += q * (t - tl - (e.x[j] * p.inv_t - st.lt));
+        }
+        kl = warp_sum(kl);
+        if (lane == 0) {
+          float l = 0.0f;
+          if (has_kd) l = p.kd_weight * p.temperature * p.temperature * kl;
+          if (has_ce) l -= p.ce_weight * logf(expf(e.x[k] - st.l1) + 1e-8f);
+          p.row_loss[row] = l;
+          if (p.lse) { p.lse[row] = st.lt; p.lse[p.rows + row] = st.l1; }
+        }
+      }
+      if constexpr (BWD) {
+        const RowSlice<T> s = slice_of(row);
+        T* dr = dlogits + row * p.ldd;
+        T* out = reinterpret_cast<T*>(smem + (size_t)stage * p.shape.stage_bytes) - s.first(s.lo);  // out[id]: the entry of this slice
+        const int e_lo = max(s.first(s.lo), 0), e_hi = min(s.first(s.hi), n);
+        auto rewrite = [&](int id, float x, float less) {
+          x -= st.ref;
+          float d = st.kt * expf(x * p.inv_t);
+          if (st.k1 != 0.0f) d += st.k1 * expf(x);
+          d -= less;
+          if (acc) d += to_f32(dr[id]);
+          out[id] = from_f32<T>(d);
+        };
+        bool met = false;  // the target is one of the ids
+        for (int j = lane; j < k; j += 32) {
+          const int id = e.id[j];
+          const float w = e.w[j];
+          met |= id >= 0 && id == y;
+          if (id >= e_lo && id < e_hi && w != -1.0f) rewrite(id, e.x[j], (has_kd ? kq * w * inv_s : 0.0f) + (id == y ? c1 : 0.0f));
+        }
+        met = __any_sync(0xffffffffu, met);
+        if (has_ce && !met && lane == 0 && y >= e_lo && y < e_hi) rewrite(y, e.x[k], c1);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (like(s, dr)) {
+          if (s.edges()) {  // the vectors at the row's ends
+            const int a = min(s.first(s.w0), e_hi), b = max(s.first(s.w1), a);
+            if (e_lo + lane < a) dr[e_lo + lane] = out[e_lo + lane];
+            if (b + lane < e_hi) dr[b + lane] = out[b + lane];
+          }
+          mbar_arrive_warp(&ring.done[stage]);
+        }  // else the group takes the row to its place
+      }
+      mbar_arrive_warp(&finished[g][set]);
+      i = after;
+      y = y_after;
+    }
+  } else {
+    // ---------------- a group ----------------
+    const int g = tid / GT, gt = tid % GT, warp = gt >> 5;
+    int y_next = -1;
+    float lt_next = 0.0f, l1_next = 0.0f;
+    auto request = [&](int i) {
+      if (i >= n_mine) return;
+      const long long row = row0 + (long long)i * stride;
+      y_next = p.targets ? p.targets[row] : -1;
+      if constexpr (!FWD) { lt_next = p.lse[row]; l1_next = p.lse[p.rows + row]; }
     };
     request(g);
-    int turn = -1;  // rows this group has worked on (skipped ones do not count): its entries and slots alternate
+    int turn = -1;       // rows this group has worked on (skipped ones do not count)
+    int stage = g - G;   // the stage of row i, and its phase; a ring has at least G stages
+    uint32_t phase = 0;
     for (int i = g; i < n_mine; i += G) {
-      const long long row = row0 + i * stride;
-      const int st_i = i % p.shape.stages;
-      const uint32_t ring_phase = (uint32_t)(i / p.shape.stages) & 1;
+      stage += G;
+      if (stage >= p.shape.stages) { stage -= p.shape.stages; phase ^= 1; }
+      const long long row = row0 + (long long)i * stride;
       const int y = y_next;
-      const float tl_given = tl_next, lt_given = lt_next, l1_given = l1_next;
+      const float lt_given = lt_next, l1_given = l1_next;
+      request(i + G);
       T* dr = BWD ? dlogits + row * p.ldd : nullptr;
       const RowSlice<T> s = slice_of(row);
-      const bool aligned = BWD && (int)((reinterpret_cast<uintptr_t>(dr) & 15) / sizeof(T)) == s.lead;
       if (skipped(y)) {
-        request(i + G);
         if (FWD && gt == 0 && rank == 0) {
           p.row_loss[row] = 0.0f;
           if (p.lse) { p.lse[row] = 0.0f; p.lse[p.rows + row] = 0.0f; }
           if (y != p.ignore_index && p.bad_id_flag) *p.bad_id_flag = 1;
         }
-        if (BWD && !(ACC && p.accumulate)) {
+        if (BWD && !acc) {
+          const bool whole = like(s, dr);
           for (int v = s.lo + gt; v < s.hi; v += GT) {
             const int e = s.first(v);
-            if (aligned && v >= s.w0 && v < s.w1) *reinterpret_cast<uint4*>(dr + e) = make_uint4(0, 0, 0, 0);
+            if (whole && v >= s.w0 && v < s.w1) *reinterpret_cast<uint4*>(dr + e) = make_uint4(0, 0, 0, 0);
             else
               for (int c = max(e, 0); c < min(e + V, n); ++c) dr[c] = from_f32<T>(0.0f);
           }
         }
-        ring_wait_row(ring, i, st_i, ring_phase);
-        mbar_arrive_warp(BWD ? &ring.done[st_i] : &ring.empty[st_i]);
+        ring_wait_row(ring, i, stage, phase);
+        if constexpr (BWD) {
+          group_sync<GT>(g);
+          if (gt == 0) mbar_arrive(&ring.done[stage]);
+        } else {
+          mbar_arrive_warp(&ring.empty[stage]);
+        }
         continue;
       }
       ++turn;
-      int* s_id = reinterpret_cast<int*>(entries) + (turn & 1) * 3 * KP;
-      float* s_t = reinterpret_cast<float*>(s_id + KP);
-      float* s_x = s_t + KP;
-      float tm = -INFINITY;
-      if (want) {
-        auto entry = [&](int j, int id, float t) {
-          if (id >= n) {
-            if (FWD && p.bad_id_flag) *p.bad_id_flag = 1;
-            id = -1;
-          }
-          t = id >= 0 && j < k ? t * p.inv_t : -INFINITY;
-          s_id[j] = max(id, -1);
-          s_t[j] = t;
-          tm = fmaxf(tm, t);
-        };
-#pragma unroll
-        for (int c = 0; c < PRE; ++c) {
-          const int j = gt + c * GT;
-          if (j < KP) entry(j, j < k ? id_next[c] : (j == k ? y : -1), t_next[c]);
-        }
-        for (int j = gt + PRE * GT; j < KP; j += GT)
-          entry(j, j < k ? p.t_ids[row * k + j] : (j == k ? y : -1), j < k ? p.t_logits[row * k + j] : 0.0f);
-      }
-      request(i + G);
+      const int set = turn & 1;
+      const uint32_t set_phase = (uint32_t)(turn >> 1) & 1;
       // the vectors at the row's ends, by the threads that walk over them
       uint4 edge0 = make_uint4(0, 0, 0, 0), edge1 = edge0;
       const bool own0 = s.w0 > s.lo && gt == 0, own1 = s.w1 < s.hi && s.hi - 1 >= s.w0 && gt == (s.hi - 1 - s.lo) % GT;
       if (own0) edge0 = s.load_edge(s.lo);
       if (own1) edge1 = s.load_edge(s.hi - 1);
-      uint4* vec = reinterpret_cast<uint4*>(smem + (size_t)st_i * p.shape.stage_bytes);
+      uint4* vec = reinterpret_cast<uint4*>(smem + (size_t)stage * p.shape.stage_bytes);
       const int cnt = s.hi - s.lo;
-      ring_wait_row(ring, i, st_i, ring_phase);
+      ring_wait_row(ring, i, stage, phase);
       if (own0) vec[0] = edge0;
       if (own1) vec[cnt - 1] = edge1;
 
-      float ref = 0.0f;
+      float ref = l1_given, own_ref = ref, st = 0.0f, s1 = 0.0f, own_st = 1.0f;
       if constexpr (FWD) {
         float m = -INFINITY;
         if constexpr (sizeof(T) == 2) {
-          const uint32_t lowest = 0xff80ff80u;
-          __nv_bfloat162 m2 = *reinterpret_cast<const __nv_bfloat162*>(&lowest), m3 = m2;
+          auto pair = [](uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); };
+          __nv_bfloat162 m2 = pair(0xff80ff80u), m3 = m2;
 #pragma unroll 4
           for (int v = gt; v < cnt; v += GT) {
             const uint4 r = vec[v];
-            m2 = __hmax2(m2, __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&r.x), *reinterpret_cast<const __nv_bfloat162*>(&r.y)));
-            m3 = __hmax2(m3, __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&r.z), *reinterpret_cast<const __nv_bfloat162*>(&r.w)));
+            m2 = __hmax2(m2, __hmax2(pair(r.x), pair(r.y)));
+            m3 = __hmax2(m3, __hmax2(pair(r.z), pair(r.w)));
           }
           m2 = __hmax2(m2, m3);
           m = fmaxf(__low2float(m2), __high2float(m2));
@@ -585,66 +829,51 @@ distill_pipe_kernel(const DistillParams p) {
           }
         }
         m = warp_max(m);
-        if (lane == 0) s_max[g][0][warp] = m;
-      }
-      tm = warp_max(tm);
-      if (lane == 0) s_max[g][1][warp] = tm;
-      group_sync<GT>(g);
-      if constexpr (FWD) {
-        ref = lanes_max<GW>(s_max[g][0][lane % GW]);
+        if (lane == 0) s_red[g][0][warp] = m;
+        group_sync<GT>(g);
+        ref = lanes_max<GW>(s_red[g][0][lane % GW]);
         if (ref == -INFINITY) ref = 0.0f;
-      }
-      // the teacher's sum: of exp(t - tref) = q_j S, where tref is its given log-sum-exp (S = 1) or its maximum
-      float tref = tl_given;
-      if (!p.t_lse) {
-        tref = lanes_max<GW>(s_max[g][1][lane % GW]);
-        if (tref == -INFINITY) tref = 0.0f;
-      }
-      float S = 0.0f;
-      const int e_lo = max(s.first(s.lo), 0), e_hi = min(s.first(s.hi), n);
-      if (want)
-        for (int j = gt; j <= k; j += GT) {
-          const int id = s_id[j];
-          float x = 0.0f;
-          if (id >= e_lo && id < e_hi) x = to_f32(reinterpret_cast<const T*>(vec)[id - s.first(s.lo)]);
-          else if (FWD && C > 1 && rank == 0 && id >= 0) x = to_f32(logits[row * p.ld + id]);
-          s_x[j] = x;
-          S += expf(s_t[j] - tref);
-        }
-      float st = 0.0f, s1 = 0.0f;
-      if constexpr (FWD) {
+        own_ref = ref;
         float sa[2] = {0.0f, 0.0f}, sb[2] = {0.0f, 0.0f};
         with_exp<T>(p.sum_kind, ref, p.inv_t, [&](const auto& ex) {
+          using Ex = std::remove_cv_t<std::remove_reference_t<decltype(ex)>>;
 #pragma unroll 2
           for (int v = gt; v < cnt; v += GT) {
             float x[V];
             unpack_vec<T>(vec[v], x);
 #pragma unroll
             for (int c = 0; c < V; c += 2) {
-              float et[2], e1[2];
-              ex(x[c], x[c + 1], et, e1);
+              float h0, h1, et[2], e1[2];
+              ex.root(x[c], x[c + 1], h0, h1);
+              ex.powers(h0, h1, et, e1);
+              ex.apart(x[c], x[c + 1], e1);
               fadd2(sa[0], sa[1], sa[0], sa[1], et[0], et[1]);
-              if (ex.two) fadd2(sb[0], sb[1], sb[0], sb[1], e1[0], e1[1]);
+              if constexpr (Ex::BOTH) fadd2(sb[0], sb[1], sb[0], sb[1], e1[0], e1[1]);
+              x[c] = h0;
+              x[c + 1] = h1;
             }
+            if constexpr (BWD && Ex::KEEPS) vec[v] = keep_vec<T>(x);
           }
+          st = (sa[0] + sa[1]) * Ex::scale_t;
+          s1 = (sb[0] + sb[1]) * Ex::scale_1;
         });
-        st = warp_sum(sa[0] + sa[1]);
-        s1 = warp_sum(sb[0] + sb[1]);
-        if (lane == 0) { s_sum[g][0][warp] = st; s_sum[g][1][warp] = s1; }
-      }
-      S = warp_sum(S);
-      if (lane == 0) s_sum[g][2][warp] = S;
-      group_sync<GT>(g);
-      S = lanes_sum<GW>(s_sum[g][2][lane % GW]);
-      // q_j = exp(t_j - tref) * inv_s,  Q = sum of them
-      const float inv_s = p.t_lse || S == 0.0f ? 1.0f : __fdividef(1.0f, S), Q = S * inv_s;
-      if constexpr (FWD) {
-        st = lanes_sum<GW>(s_sum[g][0][lane % GW]);
-        s1 = lanes_sum<GW>(s_sum[g][1][lane % GW]);
+        st = warp_sum(st);
+        s1 = warp_sum(s1);
+        if (lane == 0) { s_red[g][1][warp] = st; s_red[g][2][warp] = s1; }
+        group_sync<GT>(g);
+        if constexpr (!BWD) {
+          fence_proxy_async_smem();  // the vectors at the ends, before a copy takes their place
+          mbar_arrive_warp(&ring.empty[stage]);
+        }
+        st = lanes_sum<GW>(s_red[g][1][lane % GW]);
+        s1 = lanes_sum<GW>(s_red[g][2][lane % GW]);
         if (C > 1) {
-          float(*mine)[3] = s_xch[g][turn & 1];
+          own_st = st;
+          // the entry warp has read its logits: after the exchange the other CTAs may write theirs over them
+          mbar_wait(&ready[g][set], set_phase, &ring.abort_flag, nullptr, FAULT_WAIT_FULL);
+          float(*met)[3] = s_xch[g][set];
           if (gt < C) {
-            const uint32_t to = mapa_cluster(smem_u32(&mine[rank][0]), gt);
+            const uint32_t to = mapa_cluster(smem_u32(&met[rank][0]), gt);
             st_cluster_f32(to, st == 0.0f ? -INFINITY : ref);  // a slice without a finite entry has no say in the maximum
             st_cluster_f32(to + 4, st);
             st_cluster_f32(to + 8, s1);
@@ -652,62 +881,61 @@ distill_pipe_kernel(const DistillParams p) {
           }
           mbar_wait_cluster(&xbar[g], (uint32_t)(turn & 1), &ring.abort_flag);
           float gm = -INFINITY;
-          for (int r = 0; r < C; ++r) gm = fmaxf(gm, mine[r][0]);
+          for (int r = 0; r < C; ++r) gm = fmaxf(gm, met[r][0]);
           ref = gm == -INFINITY ? 0.0f : gm;
           st = s1 = 0.0f;
           for (int r = 0; r < C; ++r) {
-            const float d = mine[r][0] - ref;
-            st += mine[r][1] * expf(d * p.inv_t);
-            s1 += mine[r][2] * expf(d);
+            const float d = met[r][0] - ref;
+            st += met[r][1] * expf(d * p.inv_t);
+            s1 += met[r][2] * expf(d);
           }
         }
-        if (warp == GW - 1 && rank == 0) {
-          const float lt = ref * p.inv_t + logf(st);
-          const float l1 = p.sum_kind == ONE ? (p.temperature == 1.0f ? lt : 0.0f) : ref + logf(s1);
-          const float tl = p.t_lse || S == 0.0f ? tref : tref + logf(S);  // ln q_j = t_j - tl
-          float kl = 0.0f;
-          for (int j = lane; j < k; j += 32) {
-            const float t = s_t[j], q = expf(t - tl);
-            if (q > 0.0f || q != q) kl += q * (t - tl - (s_x[j] * p.inv_t - lt));
-          }
-          kl = warp_sum(kl);
-          if (lane == 0) {
-            float l = 0.0f;
-            if (has_kd) l = p.kd_weight * p.temperature * p.temperature * kl;
-            if (has_ce) l -= p.ce_weight * logf(expf(s_x[k] - l1) + 1e-8f);
-            p.row_loss[row] = l;
-            if (p.lse) { p.lse[row] = lt; p.lse[p.rows + row] = l1; }
-          }
-        }
-      } else {
-        ref = l1_given;
       }
-      if constexpr (!BWD) {
-        fence_proxy_async_smem();  // the vectors at the ends, before a copy takes their place
-        mbar_arrive_warp(&ring.empty[st_i]);
-      } else {
-        // d = kt exp((x - ref) / T) + k1 exp(x - ref): kt, k1 turn the exponentials into weighted probabilities
-        const float kq = has_kd ? p.kd_weight * p.temperature * g_out : 0.0f, c1 = has_ce ? p.ce_weight * g_out : 0.0f;
-        float kt = 0.0f, k1 = 0.0f;
+      if (!(FWD && C > 1)) mbar_wait(&ready[g][set], set_phase, &ring.abort_flag, nullptr, FAULT_WAIT_FULL);
+      // d = kt exp((x - ref) / T) + k1 exp(x - ref): kt, k1 turn the exponentials into weighted probabilities
+      float kt = 0.0f, k1 = 0.0f;
+      if constexpr (BWD) {
+        const float Q = s_teacher[g][set].Q;
         if (has_kd) kt = FWD ? __fdividef(kq * Q, st) : kq * Q * expf(ref * p.inv_t - lt_given);
         if (has_ce) k1 = FWD ? __fdividef(c1, p.grad_kind == ONE ? st : s1) : c1;
         if (p.grad_kind == ONE) { kt += k1; k1 = 0.0f; }  // temperature 1: one exponential for both terms
-        const bool acc = ACC && p.accumulate;
-        with_exp<T>(p.grad_kind, ref, p.inv_t, [&](const auto& ex) {
+      }
+      if (gt == 0) {
+        RowStats& o = s_stats[g][set];
+        o.ref = ref;
+        o.kt = kt;
+        o.k1 = k1;
+        if constexpr (FWD) {
+          o.lt = ref * p.inv_t + logf(st);
+          o.l1 = p.sum_kind == ONE ? (p.temperature == 1.0f ? o.lt : 0.0f) : ref + logf(s1);
+        }
+      }
+      if constexpr (!BWD) {
+        mbar_arrive_warp(&through[g][set]);
+      } else {
+        const bool whole = like(s, dr);
+        // a slice without a finite entry has nothing but zeros
+        const float at = C > 1 && FWD ? (own_st == 0.0f ? 0.0f : expf((own_ref - ref) * p.inv_t)) : 1.0f;
+        const float a1 = C > 1 && FWD ? (own_st == 0.0f ? 0.0f : expf(own_ref - ref)) : 1.0f;
+        with_exp<T>(FWD ? p.sum_kind : p.grad_kind, own_ref, p.inv_t, [&](const auto& ex) {
+          using Ex = std::remove_cv_t<std::remove_reference_t<decltype(ex)>>;
+          const float mt = kt * at * Ex::scale_t, m1 = k1 * a1 * Ex::scale_1;
 #pragma unroll 2
           for (int v = gt; v < cnt; v += GT) {
             float d[V];
-            unpack_vec<T>(vec[v], d);
+            if constexpr (FWD && Ex::KEEPS) kept_vec<T>(vec[v], d);
+            else unpack_vec<T>(vec[v], d);
 #pragma unroll
             for (int c = 0; c < V; c += 2) {
               float et[2], e1[2];
-              ex(d[c], d[c + 1], et, e1);
-              fmul2(d[c], d[c + 1], et[0], et[1], kt, kt);
-              if (ex.two) ffma2(d[c], d[c + 1], e1[0], e1[1], k1, k1, d[c], d[c + 1]);
+              if constexpr (FWD && Ex::KEEPS) ex.powers(d[c], d[c + 1], et, e1);
+              else ex.both(d[c], d[c + 1], et, e1);
+              fmul2(d[c], d[c + 1], et[0], et[1], mt, mt);
+              if constexpr (Ex::BOTH) ffma2(d[c], d[c + 1], e1[0], e1[1], m1, m1, d[c], d[c + 1]);
             }
             if (acc) {
               const int e = s.first(s.lo + v);
-              if (aligned && s.lo + v >= s.w0 && s.lo + v < s.w1) {
+              if (whole && s.lo + v >= s.w0 && s.lo + v < s.w1) {
                 float o[V];
                 ld16(dr + e, o);
 #pragma unroll
@@ -721,48 +949,15 @@ distill_pipe_kernel(const DistillParams p) {
             st16(reinterpret_cast<T*>(vec + v), d);
           }
         });
-        group_sync<GT>(g);
-        T* out = reinterpret_cast<T*>(vec) - s.first(s.lo);  // out[id]: the entry of this slice
-        for (int j = gt; j <= k; j += GT) {
-          const int id = s_id[j];
-          if (id < e_lo || id >= e_hi) continue;
-          int same = 0;
-          for (int c = 0; c <= k; c += 4) {
-            const int4 o = *reinterpret_cast<const int4*>(s_id + c);
-            same += (o.x == id) + (o.y == id) + (o.z == id) + (o.w == id);
-          }
-          float w = j < k ? expf(s_t[j] - tref) : 0.0f;
-          if (same > 1) {
-            int c = 0;
-            while (s_id[c] != id) ++c;
-            if (c < j) continue;
-            w = 0.0f;
-            for (; c < k; ++c)
-              if (s_id[c] == id) w += expf(s_t[c] - tref);
-          }
-          float d = 0.0f;
-          with_exp<T>(p.grad_kind, ref, p.inv_t, [&](const auto& ex) {
-            float et[2], e1[2];
-            ex(s_x[j], s_x[j], et, e1);
-            d = kt * et[0] + k1 * e1[0];
-          });
-          if (has_kd) d -= kq * w * inv_s;
-          if (id == y) d -= c1;
-          if (acc) d += to_f32(dr[id]);
-          out[id] = from_f32<T>(d);
-        }
-        if (!aligned || s.edges()) {
-          group_sync<GT>(g);
-          if (!aligned) {
-            for (int e = e_lo + gt; e < e_hi; e += GT) dr[e] = out[e];
-          } else {
-            const int a = min(s.first(s.w0), e_hi), b = max(s.first(s.w1), a);
-            for (int e = e_lo + gt; e < a; e += GT) dr[e] = out[e];
-            for (int e = b + gt; e < e_hi; e += GT) dr[e] = out[e];
-          }
-        }
         fence_proxy_async_smem();
-        mbar_arrive_warp(&ring.done[st_i]);
+        mbar_arrive_warp(&through[g][set]);
+        if (!whole) {
+          mbar_wait(&finished[g][set], set_phase, &ring.abort_flag, nullptr, FAULT_WAIT_FULL);
+          const T* out = reinterpret_cast<const T*>(vec) - s.first(s.lo);
+          for (int e = max(s.first(s.lo), 0) + gt; e < min(s.first(s.hi), n); e += GT) dr[e] = out[e];
+          group_sync<GT>(g);
+          if (gt == 0) mbar_arrive(&ring.done[stage]);
+        }
       }
     }
   }
@@ -802,18 +997,18 @@ int distill_sizes(const char* what, long long rows, long long vocab, long long k
 }
 
 // One warp per row for short rows in numbers, groups of 128 or 256 threads for longer ones (a group's reductions cost
-// the same whatever its row), all of a CTA's threads where there is at most one row per CTA.  Rows that do not fit the
-// shared memory of eight CTAs take distill_kernel, which reads them a second time.
+// the same whatever its row), all of a CTA's threads where there is at most one row or two per CTA.  Rows that do not fit
+// the shared memory of eight CTAs take distill_kernel, which reads them a second time.
 template <typename T, int MODE>
 int distill_launch(const char* what, DistillParams& p, cudaStream_t s) {
   const long long bytes = (long long)p.vocab * sizeof(T);
   auto shape = [&](int groups, int least) {
-    p.shape = row_shape(p.rows, p.vocab, sizeof(T), entry_bytes(p.k, groups), std::max(2 * groups, 3), least);
+    p.shape = row_shape(p.rows, p.vocab, sizeof(T), groups * entry_bytes(p.k), std::max(2 * groups, 3), least);
     return p.shape.stages >= groups;
   };
   if (p.rows > 2LL * sm_count()) {
-    if (bytes <= 4096 && p.k <= 128 && shape(16, 1 << 30))
-      return launch_pipe<distill_pipe_kernel<T, 32, 16, MODE>>(what, p.shape, p.rows, pipe_threads(32, 16), s, p);
+    if (bytes <= 4096 && shape(8, 1 << 30))
+      return launch_pipe<distill_pipe_kernel<T, 32, 8, MODE>>(what, p.shape, p.rows, pipe_threads(32, 8), s, p);
     if (bytes <= 24 * 1024 && shape(4, 1 << 30))
       return launch_pipe<distill_pipe_kernel<T, 128, 4, MODE>>(what, p.shape, p.rows, pipe_threads(128, 4), s, p);
     if (shape(2, 1 << 30)) return launch_pipe<distill_pipe_kernel<T, 256, 2, MODE>>(what, p.shape, p.rows, pipe_threads(256, 2), s, p);

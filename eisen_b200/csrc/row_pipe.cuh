@@ -51,11 +51,12 @@ struct RowSlice {
   int n;          // elements of the row
   int lo, hi;     // vectors of this CTA
   int w0, w1;     // those of them that lie in the row
-  __device__ __forceinline__ RowSlice(const T* row, int len, int rank, int parts) {
-    lead = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+  // the rank-th of 2^parts_log2 slices
+  __device__ __forceinline__ RowSlice(const T* row, int len, int rank, int parts_log2) {
+    lead = (int)(((uint32_t)reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
     base = row - lead;
     n = len;
-    const int all = (lead + n + V - 1) / V, per = (all + parts - 1) / parts;
+    const int all = (lead + n + V - 1) / V, per = (all + (1 << parts_log2) - 1) >> parts_log2;
     lo = min(rank * per, all);
     hi = min(lo + per, all);
     w0 = max(lo, lead ? 1 : 0);
@@ -257,7 +258,7 @@ __device__ __forceinline__ void ring_store(RowRing& r, uint8_t* smem, int stages
 
 // ---- host: shape of a launch
 struct RowShape {
-  int cluster, stages, stage_bytes, smem;
+  int cluster, cluster_log2, stages, stage_bytes, smem;
 };
 
 // Shared memory a CTA may use, less a little for its static part.
@@ -276,6 +277,7 @@ inline RowShape row_shape(long long rows, long long vocab, int elem, int extra, 
   while (c < 8 && rows * c * 2 <= sm_count() && row_bytes / (2 * c) >= least) c *= 2;
   if (slice(c) > room || slice(c) > (1 << 20)) return s;
   s.cluster = c;
+  s.cluster_log2 = c == 1 ? 0 : c == 2 ? 1 : c == 4 ? 2 : 3;
   s.stage_bytes = (int)slice(c);
   s.stages = (int)std::min<long long>(std::min<long long>(want_stages, RP_MAX_STAGES), room / s.stage_bytes);
   s.smem = s.stages * s.stage_bytes + extra;
@@ -306,7 +308,7 @@ int launch_pipe(const char* what, const RowShape& s, long long rows, int threads
   cfg.numAttrs = s.cluster > 1 ? 1 : 0;
   // the rows are dealt out over clusters that are all resident (a cluster's CTAs share a group of SMs, and the groups
   // do not divide evenly): one more would start when another ends, and take as long again
-  int& n = resident[slot][s.cluster == 1 ? 0 : s.cluster == 2 ? 1 : s.cluster == 4 ? 2 : 3];
+  int& n = resident[slot][s.cluster_log2];
   if (!n) {
     int most = sm_count();
     if (s.cluster > 1 && (cudaOccupancyMaxActiveClusters(&most, KERNEL, &cfg) != cudaSuccess || most <= 0)) {
