@@ -524,6 +524,7 @@ distill_pipe_kernel(const DistillParams p) {
   __shared__ uint64_t ready[G][2];     // the entries are prepared
   __shared__ uint64_t through[G][2];   // the group is through the row (its warps)
   __shared__ uint64_t finished[G][2];  // its entries are rewritten, the loss is formed: the set is free
+  __shared__ uint64_t rewritten[G];    // a row that its group takes to dlogits is ready for that
   __shared__ uint64_t xbar[G];         // the slices of a row have met (C arrivals)
   __shared__ float s_red[G][3][GW];
   __shared__ RowTeacher s_teacher[G][2];
@@ -538,6 +539,7 @@ distill_pipe_kernel(const DistillParams p) {
   if (tid == 0) {
     for (int g = 0; g < G; ++g) {
       mbar_init(&xbar[g], C);
+      mbar_init(&rewritten[g], 1);
       for (int set = 0; set < 2; ++set) {
         mbar_init(&ready[g][set], 1);
         mbar_init(&through[g][set], GW);
@@ -584,20 +586,35 @@ distill_pipe_kernel(const DistillParams p) {
       }
       return i;
     };
-    auto prepare = [&](int i, int y, int set) {
+    // The first 128 entries of a row (four per lane) are requested while the row before it is prepared.
+    int id_next[4];
+    float t_next[4], tl_next = 0.0f;
+    auto request = [&](int i) {
+      if (i >= n_mine) return;
+      const long long row = row0 + (long long)i * stride;
+      if (p.t_lse) tl_next = p.t_lse[row];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int j = lane + 32 * c;
+        id_next[c] = j < k ? p.t_ids[row * k + j] : -1;
+        t_next[c] = j < k ? p.t_logits[row * k + j] : 0.0f;
+      }
+    };
+    auto prepare = [&](int i, int y, int set, int after) {
       const long long row = row0 + (long long)i * stride;
       const T* xr = logits + row * p.ld;
       const Entries e(mine, set, KP);
       float ref = -INFINITY;
-      if (lane == 0) e.x[k] = y >= 0 ? to_f32(xr[y]) : 0.0f;
-      for (int j0 = lane; j0 < k; j0 += 128) {  // four entries' loads at a time
+      const float xy = lane == 0 && y >= 0 ? to_f32(xr[y]) : 0.0f;
+      const float tl_given = tl_next;
+      for (int j0 = lane; j0 - lane < k; j0 += 128) {  // four entries' loads at a time
         int id[4];
         float t[4], x[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           const int j = j0 + 32 * c;
-          id[c] = j < k ? p.t_ids[row * k + j] : -1;
-          t[c] = j < k ? p.t_logits[row * k + j] : 0.0f;
+          id[c] = j0 == lane ? id_next[c] : (j < k ? p.t_ids[row * k + j] : -1);
+          t[c] = j0 == lane ? t_next[c] : (j < k ? p.t_logits[row * k + j] : 0.0f);
         }
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -608,6 +625,7 @@ distill_pipe_kernel(const DistillParams p) {
           id[c] = max(id[c], -1);
           x[c] = id[c] >= 0 ? to_f32(xr[id[c]]) : 0.0f;
         }
+        if (j0 == lane) request(after);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           const int j = j0 + 32 * c;
@@ -620,9 +638,10 @@ distill_pipe_kernel(const DistillParams p) {
           }
         }
       }
+      if (lane == 0) e.x[k] = xy;
       // exp(t - ref) = q_j S, where ref is the teacher's given log-sum-exp (S = 1) or its maximum
       if (p.t_lse) {
-        ref = p.t_lse[row];
+        ref = tl_given;
       } else {
         ref = warp_max(ref);
         if (ref == -INFINITY) ref = 0.0f;
@@ -667,6 +686,7 @@ distill_pipe_kernel(const DistillParams p) {
     int y;
     int i = next_row(g, y);
     int stage = g, stage_i = g;  // stage of row i
+    if (preparing && want) request(i);
     for (int turn = 0; i < n_mine; ++turn) {
       const int set = turn & 1;
       const uint32_t phase = (uint32_t)(turn >> 1) & 1;
@@ -674,7 +694,7 @@ distill_pipe_kernel(const DistillParams p) {
       const int after = next_row(i + G, y_after);
       if (preparing) {
         if (turn >= 2) mbar_wait(&finished[g][set], phase ^ 1, &ring.abort_flag, nullptr, FAULT_WAIT_EMPTY);
-        if (want) prepare(i, y, set);
+        if (want) prepare(i, y, set, after);
         mbar_arrive_warp(&ready[g][set]);
         i = after;
         y = y_after;
@@ -692,22 +712,6 @@ distill_pipe_kernel(const DistillParams p) {
       const RowStats st = s_stats[g][set];
       const RowTeacher te = s_teacher[g][set];
       const float S = te.S, inv_s = p.t_lse || S == 0.0f ? 1.0f : 1.0f / S;
-      if (FWD && rank == 0) {
-        const float tl = p.t_lse || S == 0.0f ? te.tref : te.tref + logf(S);  // ln q_j = t_j - tl
-        float kl = 0.0f;
-        for (int j = lane; j < k; j += 32) {
-          const float t = e.t[j], q = expf(t - tl);
-          if (q > 0.0f || q != q) kl += q * (t - tl - (e.x[j] * p.inv_t - st.lt));
-        }
-        kl = warp_sum(kl);
-        if (lane == 0) {
-          float l = 0.0f;
-          if (has_kd) l = p.kd_weight * p.temperature * p.temperature * kl;
-          if (has_ce) l -= p.ce_weight * logf(expf(e.x[k] - st.l1) + 1e-8f);
-          p.row_loss[row] = l;
-          if (p.lse) { p.lse[row] = st.lt; p.lse[p.rows + row] = st.l1; }
-        }
-      }
       if constexpr (BWD) {
         const RowSlice<T> s = slice_of(row);
         T* dr = dlogits + row * p.ldd;
@@ -739,7 +743,25 @@ distill_pipe_kernel(const DistillParams p) {
             if (b + lane < e_hi) dr[b + lane] = out[b + lane];
           }
           mbar_arrive_warp(&ring.done[stage]);
-        }  // else the group takes the row to its place
+        } else {
+          mbar_arrive_warp(&rewritten[g]);  // the group takes the row to its place
+        }
+      }
+      if (FWD && rank == 0) {
+        const float tl = p.t_lse || S == 0.0f ? te.tref : te.tref + logf(S);  // ln q_j = t_j - tl
+        float kl = 0.0f;
+        for (int j = lane; j < k; j += 32) {
+          const float t = e.t[j], q = expf(t - tl);
+          if (q > 0.0f || q != q) kl += q * (t - tl - (e.x[j] * p.inv_t - st.lt));
+        }
+        kl = warp_sum(kl);
+        if (lane == 0) {
+          float l = 0.0f;
+          if (has_kd) l = p.kd_weight * p.temperature * p.temperature * kl;
+          if (has_ce) l -= p.ce_weight * logf(expf(e.x[k] - st.l1) + 1e-8f);
+          p.row_loss[row] = l;
+          if (p.lse) { p.lse[row] = st.lt; p.lse[p.rows + row] = st.l1; }
+        }
       }
       mbar_arrive_warp(&finished[g][set]);
       i = after;
@@ -758,6 +780,7 @@ distill_pipe_kernel(const DistillParams p) {
     };
     request(g);
     int turn = -1;       // rows this group has worked on (skipped ones do not count)
+    uint32_t odd = 0;    // phase of `rewritten`
     int stage = g - G;   // the stage of row i, and its phase; a ring has at least G stages
     uint32_t phase = 0;
     for (int i = g; i < n_mine; i += G) {
@@ -837,7 +860,7 @@ distill_pipe_kernel(const DistillParams p) {
         float sa[2] = {0.0f, 0.0f}, sb[2] = {0.0f, 0.0f};
         with_exp<T>(p.sum_kind, ref, p.inv_t, [&](const auto& ex) {
           using Ex = std::remove_cv_t<std::remove_reference_t<decltype(ex)>>;
-#pragma unroll 2
+#pragma unroll 1
           for (int v = gt; v < cnt; v += GT) {
             float x[V];
             unpack_vec<T>(vec[v], x);
@@ -920,7 +943,7 @@ distill_pipe_kernel(const DistillParams p) {
         with_exp<T>(FWD ? p.sum_kind : p.grad_kind, own_ref, p.inv_t, [&](const auto& ex) {
           using Ex = std::remove_cv_t<std::remove_reference_t<decltype(ex)>>;
           const float mt = kt * at * Ex::scale_t, m1 = k1 * a1 * Ex::scale_1;
-#pragma unroll 2
+#pragma unroll 1
           for (int v = gt; v < cnt; v += GT) {
             float d[V];
             if constexpr (FWD && Ex::KEEPS) kept_vec<T>(vec[v], d);
@@ -952,7 +975,8 @@ distill_pipe_kernel(const DistillParams p) {
         fence_proxy_async_smem();
         mbar_arrive_warp(&through[g][set]);
         if (!whole) {
-          mbar_wait(&finished[g][set], set_phase, &ring.abort_flag, nullptr, FAULT_WAIT_FULL);
+          mbar_wait(&rewritten[g], odd, &ring.abort_flag, nullptr, FAULT_WAIT_FULL);
+          odd ^= 1;
           const T* out = reinterpret_cast<const T*>(vec) - s.first(s.lo);
           for (int e = max(s.first(s.lo), 0) + gt; e < min(s.first(s.hi), n); e += GT) dr[e] = out[e];
           group_sync<GT>(g);
