@@ -1,13 +1,10 @@
-// A teacher's top logits and the loss of a student against them.
+// The loss of a student against a teacher's top logits (top_logits.cu), and its gradient:
+//   kd T^2 sum_j q_j (ln q_j - ln p_j) - ce ln(softmax(x)_y + 1e-8)  with p = softmax(x / T) and q the teacher's
+//   distribution over the entries it gives; gradient
+//   kd T (Q p_i - sum_{id_j = i} q_j) + ce (softmax(x)_i - [i = y]),  Q = sum_j q_j
 //
-//   eisen_top_logits     the k largest entries of every row in descending order (equal values: the lowest index
-//                        first), and the row's log-sum-exp at a temperature
-//   eisen_distill_*      kd T^2 sum_j q_j (ln q_j - ln p_j) - ce ln(softmax(x)_y + 1e-8) with p = softmax(x / T) and q
-//                        the teacher's distribution over the entries it gives; gradient
-//                        kd T (Q p_i - sum_{id_j = i} q_j) + ce (softmax(x)_i - [i = y]),  Q = sum_j q_j
-//
-// All of them read a row of `vocab` logits once or twice and are bound by that traffic.  Maxima, sums and
-// probabilities are f32; only dlogits of bf16 logits is rounded, once.
+// A row of `vocab` logits is read once, and written once where there is a gradient: bound by that traffic.  Maxima,
+// sums and statistics are f32.
 #include <algorithm>
 #include <cfloat>
 #include <cstdio>
@@ -23,8 +20,6 @@
 namespace eisen {
 namespace {
 
-constexpr int TOP_THREADS = 512;
-constexpr int TOP_MAX_K = 256;
 constexpr int DS_THREADS = 512;
 constexpr int DS_MAX_K = 1024;
 
@@ -52,17 +47,6 @@ __device__ __forceinline__ void for_row(const T* __restrict__ xr, int n, int tid
   if (at < n) f(at, to_f32(xr[at]));
 }
 
-// order of the values as unsigned integers: -0 equals +0, NaN comes first
-__device__ __forceinline__ uint32_t order_key(float x) {
-  if (x != x) return 0xffffffffu;
-  const uint32_t u = __float_as_uint(x + 0.0f);
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-}
-__device__ __forceinline__ float key_value(uint32_t k) {
-  if (k == 0xffffffffu) return __uint_as_float(0x7fffffffu);
-  return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
-}
-
 // running maximum and sum of exp((x - m) * inv_t)
 struct OnlineSum {
   float m = -INFINITY, s = 0.0f;
@@ -75,113 +59,6 @@ struct OnlineSum {
     s += exp_row<T>((x - (m == -INFINITY ? 0.0f : m)) * inv_t);
   }
 };
-
-// The digit (of 256) of the threshold: the highest bin at which the count from the top reaches `want`.
-// Returns the count above that bin and leaves the bin in sh[0].
-__device__ __forceinline__ void pick_bin(const int* hist, int want, int* out) {
-  // one warp: lane l owns bins 255 - 8 l ... 255 - 8 l - 7
-  const int lane = threadIdx.x & 31;
-  int c[8], total = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) { c[i] = hist[255 - lane * 8 - i]; total += c[i]; }
-  int before = total;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, before, o);
-    if (lane >= o) before += v;
-  }
-  before -= total;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (before < want && before + c[i] >= want) { out[0] = 255 - lane * 8 - i; out[1] = before; out[2] = c[i]; }
-    before += c[i];
-  }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(TOP_THREADS)
-top_logits_kernel(const T* __restrict__ logits, long long ld, float* __restrict__ values, int* __restrict__ ids,
-                  float* __restrict__ lse, int vocab, int k, float inv_t) {
-  __shared__ int hist[256];
-  __shared__ int pick[3];
-  __shared__ int count;
-  __shared__ float sh[32];
-  __shared__ uint64_t cand[TOP_MAX_K];
-  const long long row = blockIdx.x;
-  const T* xr = logits + row * ld;
-  const int tid = threadIdx.x;
-  // threshold by digits of eight bits, first of the value, then (where the last bin holds more than are
-  // wanted) of the index from the low end
-  uint32_t prefix = 0, mask = 0;
-  int want = k, in_bin = vocab;
-  OnlineSum os;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (tid < 256) hist[tid] = 0;
-    __syncthreads();
-    const bool first = shift == 24;
-    for_row(xr, vocab, tid, TOP_THREADS, [&](int, float x) {
-      if (first && lse) os.add<T>(x, inv_t);
-      const uint32_t key = order_key(x);
-      if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255], 1);
-    });
-    __syncthreads();
-    if (tid < 32) pick_bin(hist, want, pick);
-    __syncthreads();
-    prefix |= (uint32_t)pick[0] << shift;
-    mask |= 255u << shift;
-    want -= pick[1];
-    in_bin = pick[2];
-    __syncthreads();
-  }
-  if (lse) {
-    const float gm = block_max(os.m, sh);
-    const float ref = gm == -INFINITY ? 0.0f : gm;
-    const float s = block_sum(os.s * (os.m == -INFINITY && os.s == 0.0f ? 0.0f : exp_row<T>((os.m == -INFINITY ? 0.0f : os.m - ref) * inv_t)), sh);
-    if (tid == 0) lse[row] = ref * inv_t + logf(s);
-    __syncthreads();
-  }
-  uint32_t last = 0xffffffffu;  // highest index taken among the entries equal to the threshold
-  if (in_bin > want) {
-    uint32_t ip = 0, im = 0;  // on the complement of the index: the largest complements are the lowest indices
-    int iw = want;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) hist[tid] = 0;
-      __syncthreads();
-      for_row(xr, vocab, tid, TOP_THREADS, [&](int i, float x) {
-        const uint32_t c = ~(uint32_t)i;
-        if (order_key(x) == prefix && (c & im) == ip) atomicAdd(&hist[(c >> shift) & 255], 1);
-      });
-      __syncthreads();
-      if (tid < 32) pick_bin(hist, iw, pick);
-      __syncthreads();
-      ip |= (uint32_t)pick[0] << shift;
-      im |= 255u << shift;
-      iw -= pick[1];
-      __syncthreads();
-    }
-    last = ~ip;
-  }
-  if (tid == 0) count = 0;
-  __syncthreads();
-  for_row(xr, vocab, tid, TOP_THREADS, [&](int i, float x) {
-    const uint32_t key = order_key(x);
-    if (key > prefix || (key == prefix && (uint32_t)i <= last)) {
-      const int at = atomicAdd(&count, 1);
-      if (at < TOP_MAX_K) cand[at] = ((uint64_t)key << 32) | (uint32_t)~i;
-    }
-  });
-  __syncthreads();
-  // rank by counting: the composites are distinct, so the result does not depend on the order of arrival
-  if (tid < k) {
-    const uint64_t c = cand[tid];
-    int r = 0;
-    for (int j = 0; j < k; ++j) r += cand[j] > c;
-    const float v = key_value((uint32_t)(c >> 32));
-    if (r == 0 && lse && v == INFINITY) lse[row] = v;  // where the sum ran into inf - inf
-    values[row * k + r] = v;
-    ids[row * k + r] = (int)~(uint32_t)c;
-  }
-}
 
 struct DistillParams {
   const void* logits;
@@ -1058,25 +935,6 @@ int distill_run(const char* what, int mode, DistillParams& p, int dtype, cudaStr
 }  // namespace eisen
 
 extern "C" {
-
-int eisen_top_logits(void* stream, const void* logits, long long ld, float* values, int* ids, float* lse, long long rows,
-                     long long vocab, long long k, float temperature, int dtype) {
-  using namespace eisen;
-  if (int rc = distill_sizes("top_logits", rows, vocab, k)) return rc;
-  if (dtype != DT_F32 && dtype != DT_BF16) return fail(EISEN_ERR_INVALID, "top_logits: logits must be f32 or bf16");
-  if (k < 1 || k > TOP_MAX_K || k > vocab) return fail(EISEN_ERR_LIMIT, "top_logits: k must be in [1, min(vocab, 256)]");
-  if (ld < vocab) return fail(EISEN_ERR_INVALID, "top_logits: the row stride is shorter than a row");
-  if (!(temperature > 0.0f) || !(temperature <= FLT_MAX) || !(1.0f / temperature <= FLT_MAX))
-    return fail(EISEN_ERR_INVALID, "top_logits: the temperature must be positive and finite");
-  if (rows == 0) return 0;
-  if (!logits || !values || !ids) return fail(EISEN_ERR_INVALID, "top_logits: logits, values and ids must not be null");
-  if (reinterpret_cast<uintptr_t>(logits) % (dtype == DT_F32 ? 4 : 2)) return fail(EISEN_ERR_INVALID, "top_logits: unaligned pointer");
-  EISEN_DISPATCH_DTYPE(dtype, T, {
-    top_logits_kernel<T><<<(unsigned)rows, TOP_THREADS, 0, (cudaStream_t)stream>>>((const T*)logits, ld, values, ids, lse, (int)vocab,
-                                                                                  (int)k, 1.0f / temperature);
-    return check_launch("top_logits");
-  });
-}
 
 int eisen_distill_fwd(void* stream, const void* logits, long long ld, const int* teacher_ids, const float* teacher_logits,
                       const float* teacher_lse, const int* targets, float* loss, float* row_loss, float* lse, long long rows,

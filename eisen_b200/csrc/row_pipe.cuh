@@ -262,7 +262,7 @@ struct RowShape {
 };
 
 // Shared memory a CTA may use, less a little for its static part.
-constexpr int RP_SMEM = 220 * 1024;
+constexpr int RP_SMEM = 216 * 1024;
 
 // `extra`: dynamic shared memory beside the stages.  A row of up to a third of the stage memory stays whole (three
 // stages keep the memory busy while two groups work); longer rows are split over 2, 4 or 8 CTAs, and so are rows that

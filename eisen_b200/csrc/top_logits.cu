@@ -1,0 +1,480 @@
+// The k largest logits of every row in descending order (equal values: the lowest index first), and the row's
+// log-sum-exp at a temperature: what a teacher hands to a student (distill.cu).
+//
+// A row is read once, into shared memory (row_pipe.cuh).  A group of GT threads then
+//   1. takes the largest element of every thread's share: the k-th largest of these is a threshold that at least k
+//      elements of the row reach and, on rows in no special order, few more do;
+//   2. lists the elements that reach it, and adds up the exponentials in the same pass;
+//   3. ranks the listed ones against each other.
+// Keys are 64 bits, value above complemented index, so every two differ and nothing depends on the order of arrival.
+// Rows whose large values sit in a few threads' shares (or are equal in thousands) overflow the list; for them the
+// exact threshold is found digit by digit over all elements, first of the value, then of the index.
+#include <algorithm>
+#include <cfloat>
+#include <cstdio>
+
+#include "common.cuh"
+#include "errors.h"
+#include "row_pipe.cuh"
+#include "../../include/eisen_b200.h"
+
+namespace eisen {
+namespace {
+
+constexpr int TOP_THREADS = 512;
+constexpr int TOP_MAX_K = 256;
+
+struct TopParams {
+  const void* logits;
+  long long ld;
+  float* values;
+  int* ids;
+  float* lse;
+  long long rows;
+  int vocab, k;
+  float inv_t;
+  RowShape shape;
+};
+
+// order of the values as unsigned integers: -0 equals +0, NaN comes first
+__device__ __forceinline__ uint32_t order_key(float x) {
+  if (x != x) return 0xffffffffu;
+  const uint32_t u = __float_as_uint(x + 0.0f);
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  if (k == 0xffffffffu) return __uint_as_float(0x7fffffffu);
+  return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+// largest element of a vector; NaN where one of them is NaN
+template <typename T>
+__device__ __forceinline__ float vec_max(const uint4& r) {
+  if constexpr (sizeof(T) == 2) {
+    auto pair = [](uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); };
+    const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(pair(r.x), pair(r.y)), __hmax2_nan(pair(r.z), pair(r.w)));
+    return max_nan(__low2float(m), __high2float(m));
+  } else {
+    return max_nan(max_nan(__uint_as_float(r.x), __uint_as_float(r.y)), max_nan(__uint_as_float(r.z), __uint_as_float(r.w)));
+  }
+}
+
+// how many of a group's threads say so (a barrier of the group)
+template <int GT>
+__device__ __forceinline__ int group_count(int g, bool yes) {
+  if constexpr (GT == 32) {
+    return __popc(__ballot_sync(0xffffffffu, yes));
+  } else {
+    int n;
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.u32 p, %1, 0;\nbar.red.popc.u32 %0, %2, %3, p;\n}"
+        : "=r"(n)
+        : "r"((uint32_t)yes), "r"(1 + g), "n"(GT)
+        : "memory");
+    return n;
+  }
+}
+
+// One warp: the bin of 256 at which the count from the top reaches `want`.  out = bin, count above it, count in it.
+__device__ __forceinline__ void pick_bin(const int* hist, int want, int* out) {
+  const int lane = threadIdx.x & 31;
+  int c[8], total = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) { c[i] = hist[255 - lane * 8 - i]; total += c[i]; }
+  int before = total;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += v;
+  }
+  before -= total;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (before < want && before + c[i] >= want) { out[0] = 255 - lane * 8 - i; out[1] = before; out[2] = c[i]; }
+    before += c[i];
+  }
+}
+
+struct TopSelect {
+  int hist[256];
+  int pick[3];
+};
+
+// The k-th largest key of a set by digits of eight bits, first of the value, then (where the last bin holds more than are
+// wanted) of the complemented index.  each(f): f(index, value) for every element that the calling thread owns; sync(): a
+// barrier of the threads that share the set; tid: this thread's number among them (at least 32 of them).
+template <int THREADS, typename Each, typename Sync>
+__device__ void exact_threshold(TopSelect& s, int tid, int k, int all, uint32_t& value, uint32_t& last, Each each, Sync sync) {
+  uint32_t prefix = 0, mask = 0;
+  int want = k, in_bin = all;
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    for (int i = tid; i < 256; i += THREADS) s.hist[i] = 0;
+    sync();
+    each([&](int, float x) {
+      const uint32_t key = order_key(x);
+      if ((key & mask) == prefix) atomicAdd(&s.hist[(key >> shift) & 255], 1);
+    });
+    sync();
+    if (tid < 32) pick_bin(s.hist, want, s.pick);
+    sync();
+    prefix |= (uint32_t)s.pick[0] << shift;
+    mask |= 255u << shift;
+    want -= s.pick[1];
+    in_bin = s.pick[2];
+    sync();
+  }
+  value = prefix;
+  last = 0xffffffffu;  // highest index taken among the elements equal to the threshold
+  if (in_bin > want) {
+    uint32_t ip = 0, im = 0;  // the largest complements are the lowest indices
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      for (int i = tid; i < 256; i += THREADS) s.hist[i] = 0;
+      sync();
+      each([&](int i, float x) {
+        const uint32_t c = ~(uint32_t)i;
+        if (order_key(x) == prefix && (c & im) == ip) atomicAdd(&s.hist[(c >> shift) & 255], 1);
+      });
+      sync();
+      if (tid < 32) pick_bin(s.hist, want, s.pick);
+      sync();
+      ip |= (uint32_t)s.pick[0] << shift;
+      im |= 255u << shift;
+      want -= s.pick[1];
+      sync();
+    }
+    last = ~ip;
+  }
+}
+
+// f(index, value) for the vectors of a slice in shared memory that belong to thread gt of GT; places outside the row
+// are left out
+template <typename T, int GT, typename F>
+__device__ __forceinline__ void each_element(const RowSlice<T>& s, const uint4* vec, int gt, F f) {
+  constexpr int V = RowSlice<T>::V;
+  const int cnt = s.hi - s.lo;
+#pragma unroll 1
+  for (int v = gt; v < cnt; v += GT) {
+    float x[V];
+    unpack_vec<T>(vec[v], x);
+    const int e = s.first(s.lo + v);
+#pragma unroll
+    for (int c = 0; c < V; ++c)
+      if (e + c >= 0 && e + c < s.n) f(e + c, x[c]);
+  }
+}
+
+__host__ __device__ constexpr int top_list(int k) { return k <= 64 ? 256 : 1024; }  // entries of a group's list
+
+template <typename T, int GT, int G>
+__global__ void __launch_bounds__(GT * G + 32, 1)
+top_pipe_kernel(const TopParams p) {
+  constexpr int V = VecOf<T>::N, GW = GT / 32;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ RowRing ring;
+  __shared__ uint64_t xbar[G], xdone[G];  // all slices' lists are there; the first CTA has read them
+  __shared__ float s_max[G][GW], s_sum[G][GW];
+  __shared__ int s_count[G];
+  __shared__ __align__(8) float s_slice[G][2];  // a slice's maximum and sum
+  __shared__ TopSelect s_sel[G];
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int C = p.shape.cluster, k = p.k, n = p.vocab, cap = top_list(k);
+  const int rank = C > 1 ? (int)cluster_ctarank() : 0;
+  const long long row0 = blockIdx.x >> p.shape.cluster_log2, stride = gridDim.x >> p.shape.cluster_log2;
+  const int n_mine = row0 < p.rows ? (int)((p.rows - row0 + stride - 1) / stride) : 0;
+  ring_init(ring, p.shape.stages, GW, 1);
+  if (tid == 0) {
+    for (int g = 0; g < G; ++g) {
+      mbar_init(&xbar[g], C);
+      mbar_init(&xdone[g], 1);
+    }
+    fence_mbar_init();
+  }
+  __syncthreads();
+  if (C > 1) cluster_sync_all();
+  const T* logits = reinterpret_cast<const T*>(p.logits);
+  auto slice_of = [&](long long row) { return RowSlice<T>(logits + row * p.ld, n, rank, p.shape.cluster_log2); };
+  if (tid >= GT * G) {
+    ring_load<T>(ring, smem, p.shape.stages, p.shape.stage_bytes, n_mine, row0, stride, slice_of, [](long long) { return false; });
+  } else {
+    const int g = tid / GT, gt = tid % GT, warp = gt >> 5;
+    uint64_t* list = reinterpret_cast<uint64_t*>(smem + (size_t)p.shape.stages * p.shape.stage_bytes) + (size_t)g * (cap + TOP_MAX_K);
+    uint64_t* best = list + cap;  // this slice's k largest in descending order (clusters)
+    int stage = g - G;  // the stage of row i, and its phase; a ring has at least G stages
+    uint32_t phase = 0, turn = 0;
+    for (int i = g; i < n_mine; i += G, ++turn) {
+      stage += G;
+      if (stage >= p.shape.stages) { stage -= p.shape.stages; phase ^= 1; }
+      const long long row = row0 + (long long)i * stride;
+      const RowSlice<T> s = slice_of(row);
+      // the vectors at the row's ends, by the threads that walk over them
+      uint4 edge0 = make_uint4(0, 0, 0, 0), edge1 = edge0;
+      const bool own0 = s.w0 > s.lo && gt == 0, own1 = s.w1 < s.hi && s.hi - 1 >= s.w0 && gt == (s.hi - 1 - s.lo) % GT;
+      if (own0) edge0 = s.load_edge(s.lo);
+      if (own1) edge1 = s.load_edge(s.hi - 1);
+      uint4* vec = reinterpret_cast<uint4*>(smem + (size_t)stage * p.shape.stage_bytes);
+      const int cnt = s.hi - s.lo;
+      const int e_lo = max(s.first(s.lo), 0), here = max(min(s.first(s.hi), n) - e_lo, 0);  // elements of this slice
+      const int kk = min(k, here);
+      ring_wait_row(ring, i, stage, phase);
+      if (own0) vec[0] = edge0;
+      if (own1) vec[cnt - 1] = edge1;
+
+      // ---- largest elements of this thread's four shares; NaN counts as the largest
+      float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+      for (int v = gt; v < cnt; v += 4 * GT) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (v + q * GT < cnt) m[q] = max_nan(m[q], vec_max<T>(vec[v + q * GT]));
+      }
+      const float most = max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3]));
+      if (gt == 0) s_count[g] = 0;
+      const float wm = warp_max(most);  // drops NaN, which the sum brings back
+      if (lane == 0) s_max[g][warp] = wm;
+      // ---- threshold: the kk-th largest of the threads' maxima in their upper 16 bits, by bisection.  Where kk is more than
+      // half of the threads, the lesser of so many maxima would let too much through: then of the four shares' maxima
+      uint32_t tau = 0;
+      if (2 * kk <= min(cnt, GT)) {
+        const uint32_t key = order_key(most) >> 16;
+#pragma unroll 1
+        for (int bit = 15; bit >= 0; --bit) {
+          const uint32_t trial = tau | (1u << bit);
+          if (group_count<GT>(g, gt < cnt && key >= trial) >= kk) tau = trial;
+        }
+      } else if (kk <= min(cnt, 4 * GT)) {
+        uint32_t key[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) key[q] = gt + q * GT < cnt ? order_key(m[q]) >> 16 : 0;
+#pragma unroll 1
+        for (int bit = 15; bit >= 0; --bit) {
+          const uint32_t trial = tau | (1u << bit);  // never 0: places without a share do not count
+          int total = 0;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) total += group_count<GT>(g, key[q] >= trial);
+          if (total >= kk) tau = trial;
+        }
+      }
+      group_sync<GT>(g);
+      float ref = lanes_max<GW>(s_max[g][lane % GW]);
+      if (ref == -INFINITY) ref = 0.0f;
+      // every element whose key reaches tau; NaN does, and so does everything where tau is 0
+      const float floor_value = key_value(tau << 16);
+      const float c2 = 1.4426950408889634f * p.inv_t, off = -ref * c2;
+      const bool far = sizeof(T) == 4 || fabsf(ref) > 1e30f;
+      float sum = 0.0f;
+#pragma unroll 1
+      for (int v = gt; v < cnt; v += GT) {
+        float x[V];
+        unpack_vec<T>(vec[v], x);
+        bool any = false;
+#pragma unroll
+        for (int c = 0; c < V; ++c) any |= !(x[c] < floor_value);
+        if (any) {
+          const int e = s.first(s.lo + v);
+#pragma unroll
+          for (int c = 0; c < V; ++c)
+            if (!(x[c] < floor_value) && e + c >= 0 && e + c < n) {
+              const int at = atomicAdd(&s_count[g], 1);
+              if (at < cap) list[at] = ((uint64_t)order_key(x[c]) << 32) | (uint32_t)~(e + c);
+            }
+        }
+        if (p.lse) {
+          if (far) {
+#pragma unroll
+            for (int c = 0; c < V; ++c) sum += expf((x[c] - ref) * p.inv_t);
+          } else {
+#pragma unroll
+            for (int c = 0; c < V; ++c) sum += exp2_approx(fmaf(x[c], c2, off));
+          }
+        }
+      }
+      sum = warp_sum(sum);
+      if (lane == 0) s_sum[g][warp] = sum;
+      group_sync<GT>(g);
+      sum = lanes_sum<GW>(s_sum[g][lane % GW]);
+      int listed = s_count[g];
+      if (listed > cap) {
+        uint32_t value, last;
+        exact_threshold<GT>(s_sel[g], gt, kk, here, value, last, [&](auto f) { each_element<T, GT>(s, vec, gt, f); },
+                            [&]() { group_sync<GT>(g); });
+        if (gt == 0) s_count[g] = 0;
+        group_sync<GT>(g);
+        each_element<T, GT>(s, vec, gt, [&](int e, float x) {
+          const uint32_t q = order_key(x);
+          if (q > value || (q == value && (uint32_t)e <= last)) {
+            const int at = atomicAdd(&s_count[g], 1);
+            if (at < cap) list[at] = ((uint64_t)q << 32) | (uint32_t)~e;
+          }
+        });
+        group_sync<GT>(g);
+        listed = min(s_count[g], cap);
+      }
+      fence_proxy_async_smem();  // the vectors at the ends, before a copy takes their place
+      mbar_arrive_warp(&ring.empty[stage]);
+
+      // ---- ranks.  Places of a slice's list that no element takes hold 0, below every key
+      float top = ref;  // the row's largest
+      auto put = [&](int r, uint64_t c) {
+        const float v = key_value((uint32_t)(c >> 32));
+        p.values[row * k + r] = v;
+        p.ids[row * k + r] = (int)~(uint32_t)c;
+        if (r == 0 && p.lse && top == INFINITY) p.lse[row] = v;  // inf or NaN, where the sum ran into inf - inf
+      };
+      if (C == 1) {
+        if (gt == 0 && p.lse && top != INFINITY) p.lse[row] = ref * p.inv_t + logf(sum);
+        for (int j = gt; j < listed; j += GT) {
+          const uint64_t c = list[j];
+          int r = 0;
+#pragma unroll 4
+          for (int o = 0; o < listed; ++o) r += list[o] > c;
+          if (r < k) put(r, c);
+        }
+        group_sync<GT>(g);  // the list is read before the next row's takes its place
+      } else {
+        if (gt == 0) { s_slice[g][0] = sum == 0.0f ? -INFINITY : ref; s_slice[g][1] = sum; }
+        for (int j = gt + kk; j < k; j += GT) best[j] = 0;
+        for (int j = gt; j < listed; j += GT) {
+          const uint64_t c = list[j];
+          int r = 0;
+#pragma unroll 4
+          for (int o = 0; o < listed; ++o) r += list[o] > c;
+          if (r < k) best[r] = c;
+        }
+        group_sync<GT>(g);
+        if (gt == 0) mbar_arrive_release_cluster(mapa_cluster(smem_u32(&xbar[g]), 0));
+        if (rank == 0) {
+          mbar_wait_cluster(&xbar[g], turn & 1, &ring.abort_flag);
+          const uint32_t b0 = smem_u32(best), s0 = smem_u32(&s_slice[g][0]);
+          top = -INFINITY;
+          for (int o = 0; o < C; ++o) top = fmaxf(top, __uint_as_float((uint32_t)ld_cluster_u64(mapa_cluster(s0, o))));
+          for (int j = gt; j < C * k; j += GT) {
+            const int from = j / k, at = j - from * k;
+            const uint64_t c = ld_cluster_u64(mapa_cluster(b0 + 8 * at, from));
+            if (c == 0) continue;
+            int r = at;  // before it in its own list, and in every other one
+            for (int o = 0; o < C && r < k; ++o) {
+              if (o == from) continue;
+              const uint32_t other = mapa_cluster(b0, o);
+              int lo = 0, hi = k;
+              while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (ld_cluster_u64(other + 8 * mid) > c) lo = mid + 1;
+                else hi = mid;
+              }
+              r += lo;
+            }
+            if (r < k) put(r, c);
+          }
+          if (gt == 0 && p.lse && top != INFINITY) {
+            const float r0 = top == -INFINITY ? 0.0f : top;
+            float gs = 0.0f;
+            for (int o = 0; o < C; ++o) {
+              const uint64_t ms = ld_cluster_u64(mapa_cluster(s0, o));
+              gs += __uint_as_float((uint32_t)(ms >> 32)) * expf((__uint_as_float((uint32_t)ms) - r0) * p.inv_t);
+            }
+            p.lse[row] = r0 * p.inv_t + logf(gs);
+          }
+          group_sync<GT>(g);
+          if (gt < C) mbar_arrive_release_cluster(mapa_cluster(smem_u32(&xdone[g]), gt));
+        }
+        mbar_wait_cluster(&xdone[g], turn & 1, &ring.abort_flag);  // `best` may be written again
+      }
+    }
+  }
+  if (ring.abort_flag)
+    for (int i = 0; i < 64; ++i) __nanosleep(1000);  // copies in flight end before the CTA does
+  if (C > 1) {
+    __syncwarp();
+    cluster_sync_all();  // nobody leaves while a peer may still read its lists
+  }
+}
+
+// Rows beyond the shared memory of eight CTAs: read from global memory again for every digit.
+template <typename T>
+__global__ void __launch_bounds__(TOP_THREADS)
+top_long_kernel(const TopParams p) {
+  __shared__ TopSelect sel;
+  __shared__ int count;
+  __shared__ float sh[32];
+  __shared__ uint64_t cand[TOP_MAX_K];
+  const long long row = blockIdx.x;
+  const T* xr = reinterpret_cast<const T*>(p.logits) + row * p.ld;
+  const int tid = threadIdx.x, k = p.k;
+  auto each = [&](auto f) {
+    for (int i = tid; i < p.vocab; i += TOP_THREADS) f(i, to_f32(xr[i]));
+  };
+  float m = -INFINITY;
+  each([&](int, float x) { m = fmaxf(m, x); });
+  m = block_max(m, sh);
+  const float ref = m == -INFINITY ? 0.0f : m;
+  float s = 0.0f;
+  each([&](int, float x) { s += expf((x - ref) * p.inv_t); });
+  s = block_sum(s, sh);
+  if (tid == 0) {
+    count = 0;
+    if (p.lse) p.lse[row] = ref * p.inv_t + logf(s);
+  }
+  uint32_t value, last;
+  exact_threshold<TOP_THREADS>(sel, tid, k, p.vocab, value, last, each, []() { __syncthreads(); });
+  each([&](int i, float x) {
+    const uint32_t key = order_key(x);
+    if (key > value || (key == value && (uint32_t)i <= last)) {
+      const int at = atomicAdd(&count, 1);
+      if (at < TOP_MAX_K) cand[at] = ((uint64_t)key << 32) | (uint32_t)~i;
+    }
+  });
+  __syncthreads();
+  if (tid < k) {
+    const uint64_t c = cand[tid];
+    int r = 0;
+    for (int j = 0; j < k; ++j) r += cand[j] > c;
+    const float v = key_value((uint32_t)(c >> 32));
+    if (r == 0 && p.lse && m == INFINITY) p.lse[row] = v;  // inf or NaN, where the sum ran into inf - inf
+    p.values[row * k + r] = v;
+    p.ids[row * k + r] = (int)~(uint32_t)c;
+  }
+}
+
+template <typename T>
+int top_launch(TopParams& p, cudaStream_t s) {
+  const long long bytes = (long long)p.vocab * sizeof(T);
+  auto shape = [&](int groups, int least) {
+    p.shape = row_shape(p.rows, p.vocab, sizeof(T), groups * 8 * (top_list(p.k) + TOP_MAX_K), std::max(2 * groups, 3), least);
+    return p.shape.stages >= groups;
+  };
+  if (p.rows > 2LL * sm_count()) {
+    if (bytes <= 4096 && p.k <= 32 && shape(8, 1 << 30))
+      return launch_pipe<top_pipe_kernel<T, 32, 8>>("top_logits", p.shape, p.rows, 32 * 8 + 32, s, p);
+    if (bytes <= 24 * 1024 && shape(4, 1 << 30))
+      return launch_pipe<top_pipe_kernel<T, 128, 4>>("top_logits", p.shape, p.rows, 128 * 4 + 32, s, p);
+    if (shape(2, 1 << 30)) return launch_pipe<top_pipe_kernel<T, 256, 2>>("top_logits", p.shape, p.rows, 256 * 2 + 32, s, p);
+  }
+  if (shape(1, 8192)) return launch_pipe<top_pipe_kernel<T, 512, 1>>("top_logits", p.shape, p.rows, 512 + 32, s, p);
+  top_long_kernel<T><<<(unsigned)p.rows, TOP_THREADS, 0, s>>>(p);
+  return check_launch("top_logits");
+}
+
+}  // namespace
+}  // namespace eisen
+
+extern "C" int eisen_top_logits(void* stream, const void* logits, long long ld, float* values, int* ids, float* lse, long long rows,
+                                long long vocab, long long k, float temperature, int dtype) {
+  using namespace eisen;
+  if (rows < 0 || rows > 0x7fffffffLL || vocab <= 0 || vocab > 0x7fffff00LL)
+    return fail(EISEN_ERR_LIMIT, "top_logits: rows must be in [0, 2^31), vocab in [1, 2^31 - 256]");
+  if (dtype != DT_F32 && dtype != DT_BF16) return fail(EISEN_ERR_INVALID, "top_logits: logits must be f32 or bf16");
+  if (k < 1 || k > TOP_MAX_K || k > vocab) return fail(EISEN_ERR_LIMIT, "top_logits: k must be in [1, min(vocab, 256)]");
+  if (ld < vocab) return fail(EISEN_ERR_INVALID, "top_logits: the row stride is shorter than a row");
+  if (!(temperature > 0.0f) || !(temperature <= FLT_MAX) || !(1.0f / temperature <= FLT_MAX))
+    return fail(EISEN_ERR_INVALID, "top_logits: the temperature must be positive and finite");
+  if (rows == 0) return 0;
+  if (!logits || !values || !ids) return fail(EISEN_ERR_INVALID, "top_logits: logits, values and ids must not be null");
+  if (reinterpret_cast<uintptr_t>(logits) % (dtype == DT_F32 ? 4 : 2)) return fail(EISEN_ERR_INVALID, "top_logits: unaligned pointer");
+  TopParams p = {logits, ld, values, ids, lse, rows, (int)vocab, (int)k, 1.0f / temperature, {}};
+  EISEN_DISPATCH_DTYPE(dtype, T, { return top_launch<T>(p, (cudaStream_t)stream); });
+}

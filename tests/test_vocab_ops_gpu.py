@@ -65,9 +65,8 @@ def check_top(x, k, temperature=1.0):
     want = d.gather(1, order)
     assert torch.equal(torch.nan_to_num(v.double(), nan=1e300), torch.nan_to_num(want, nan=1e300))
     lse = torch.logsumexp(d / temperature, 1)
-    same = torch.isnan(lse) == torch.isnan(s)
-    assert same.all()
-    ok = ~torch.isnan(lse) & torch.isfinite(lse)
+    assert (torch.isnan(lse) == torch.isnan(s)).all() and ((lse == math.inf) == (s == math.inf)).all()
+    ok = torch.isfinite(lse)
     assert ((s.double() - lse)[ok].abs() <= EPS_P + 4 * 2.0 ** -24 * lse[ok].abs()).all()
 
 
@@ -120,6 +119,24 @@ def test_top_logits_orders(dtype, kind):
 def test_top_logits_strides(dtype, ld, shift):
     x = torch.randn(6, 1003, generator=gen(ld), device=dev()).to(dtype)
     check_top(rows_at(x, ld, shift), 17, 2.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab,k", [(1500, 700, 5), (1200, 1001, 32), (900, 2000, 200), (700, 8200, 64), (601, 5003, 256), (500, 32000, 64),
+                                          (400, 32000, 256), (333, 100003, 20), (310, 300, 300 - 44)])
+def test_top_logits_many_rows(dtype, rows, vocab, k):
+    """Several rows per CTA; every third row constant, every fifth ascending."""
+    x = torch.randn(rows, vocab, generator=gen(rows + vocab + k), device=dev()) * 2
+    x[::3] = x[::3, :1]
+    x[::5] = (torch.arange(vocab, device=dev()) // 3).float()
+    check_top(x.to(dtype), k, 1.5)
+
+
+def test_top_logits_longer_than_shared_memory():
+    x = torch.randn(2, 700001, generator=gen(2), device=dev())
+    x[1, 5000:6000] = 9.0
+    check_top(x, 100, 2.0)
+    check_top(x.to(torch.bfloat16), 256)
 
 
 def test_top_logits_no_rows_no_lse():
