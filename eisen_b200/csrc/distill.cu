@@ -737,10 +737,12 @@ distill_pipe_kernel(const DistillParams p) {
         float sa[2] = {0.0f, 0.0f}, sb[2] = {0.0f, 0.0f};
         with_exp<T>(p.sum_kind, ref, p.inv_t, [&](const auto& ex) {
           using Ex = std::remove_cv_t<std::remove_reference_t<decltype(ex)>>;
+          uint4 next = gt < cnt ? vec[gt] : make_uint4(0, 0, 0, 0);
 #pragma unroll 1
           for (int v = gt; v < cnt; v += GT) {
             float x[V];
-            unpack_vec<T>(vec[v], x);
+            unpack_vec<T>(next, x);
+            if (v + GT < cnt) next = vec[v + GT];  // on its way while this one is worked on
 #pragma unroll
             for (int c = 0; c < V; c += 2) {
               float h0, h1, et[2], e1[2];
@@ -820,11 +822,13 @@ distill_pipe_kernel(const DistillParams p) {
         with_exp<T>(FWD ? p.sum_kind : p.grad_kind, own_ref, p.inv_t, [&](const auto& ex) {
           using Ex = std::remove_cv_t<std::remove_reference_t<decltype(ex)>>;
           const float mt = kt * at * Ex::scale_t, m1 = k1 * a1 * Ex::scale_1;
+          uint4 next = gt < cnt ? vec[gt] : make_uint4(0, 0, 0, 0);
 #pragma unroll 1
           for (int v = gt; v < cnt; v += GT) {
             float d[V];
-            if constexpr (FWD && Ex::KEEPS) kept_vec<T>(vec[v], d);
-            else unpack_vec<T>(vec[v], d);
+            if constexpr (FWD && Ex::KEEPS) kept_vec<T>(next, d);
+            else unpack_vec<T>(next, d);
+            if (v + GT < cnt) next = vec[v + GT];
 #pragma unroll
             for (int c = 0; c < V; c += 2) {
               float et[2], e1[2];

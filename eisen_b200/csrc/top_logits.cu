@@ -178,6 +178,7 @@ top_pipe_kernel(const TopParams p) {
   __shared__ RowRing ring;
   __shared__ uint64_t xbar[G], xdone[G];  // all slices' lists are there; the first CTA has read them
   __shared__ float s_max[G][GW], s_sum[G][GW];
+  __shared__ uint32_t s_range[G][GW];
   __shared__ int s_count[G];
   __shared__ __align__(8) float s_slice[G][2];  // a slice's maximum and sum
   __shared__ TopSelect s_sel[G];
@@ -234,17 +235,29 @@ top_pipe_kernel(const TopParams p) {
       }
       const float most = max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3]));
       if (gt == 0) s_count[g] = 0;
+      const uint32_t top_key = gt < cnt ? order_key(most) >> 16 : 0;
       const float wm = warp_max(most);  // drops NaN, which the sum brings back
-      if (lane == 0) s_max[g][warp] = wm;
+      const uint32_t k_hi = __reduce_max_sync(0xffffffffu, top_key);
+      const uint32_t k_lo = __reduce_min_sync(0xffffffffu, gt < cnt ? top_key : 0xffffu);
+      if (lane == 0) { s_max[g][warp] = wm; s_range[g][warp] = (k_hi << 16) | k_lo; }
+      group_sync<GT>(g);
+      // the bits in which the threads' maxima agree are the threshold's too
+      uint32_t hi16 = 0, lo16 = 0xffffu;
+#pragma unroll
+      for (int w = 0; w < GW; ++w) {
+        hi16 = max(hi16, s_range[g][w] >> 16);
+        lo16 = min(lo16, s_range[g][w] & 0xffffu);
+      }
+      const int bits = 32 - __clz(hi16 ^ lo16);
       // ---- threshold: the kk-th largest of the threads' maxima in their upper 16 bits, by bisection.  Where kk is more than
       // half of the threads, the lesser of so many maxima would let too much through: then of the four shares' maxima
       uint32_t tau = 0;
       if (2 * kk <= min(cnt, GT)) {
-        const uint32_t key = order_key(most) >> 16;
+        tau = (hi16 >> bits) << bits;
 #pragma unroll 1
-        for (int bit = 15; bit >= 0; --bit) {
+        for (int bit = bits - 1; bit >= 0; --bit) {
           const uint32_t trial = tau | (1u << bit);
-          if (group_count<GT>(g, gt < cnt && key >= trial) >= kk) tau = trial;
+          if (group_count<GT>(g, top_key >= trial) >= kk) tau = trial;  // trial is not 0: threads without a share do not count
         }
       } else if (kk <= min(cnt, 4 * GT)) {
         uint32_t key[4];
@@ -266,11 +279,13 @@ top_pipe_kernel(const TopParams p) {
       const float floor_value = key_value(tau << 16);
       const float c2 = 1.4426950408889634f * p.inv_t, off = -ref * c2;
       const bool far = sizeof(T) == 4 || fabsf(ref) > 1e30f;
-      float sum = 0.0f;
+      float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      uint4 next = gt < cnt ? vec[gt] : make_uint4(0, 0, 0, 0);
 #pragma unroll 1
       for (int v = gt; v < cnt; v += GT) {
         float x[V];
-        unpack_vec<T>(vec[v], x);
+        unpack_vec<T>(next, x);
+        if (v + GT < cnt) next = vec[v + GT];  // on its way while this one is worked on
         bool any = false;
 #pragma unroll
         for (int c = 0; c < V; ++c) any |= !(x[c] < floor_value);
@@ -286,13 +301,14 @@ top_pipe_kernel(const TopParams p) {
         if (p.lse) {
           if (far) {
 #pragma unroll
-            for (int c = 0; c < V; ++c) sum += expf((x[c] - ref) * p.inv_t);
+            for (int c = 0; c < V; ++c) acc[c & 3] += expf((x[c] - ref) * p.inv_t);
           } else {
 #pragma unroll
-            for (int c = 0; c < V; ++c) sum += exp2_approx(fmaf(x[c], c2, off));
+            for (int c = 0; c < V; ++c) acc[c & 3] += exp2_approx(fmaf(x[c], c2, off));
           }
         }
       }
+      float sum = (acc[0] + acc[1]) + (acc[2] + acc[3]);
       sum = warp_sum(sum);
       if (lane == 0) s_sum[g][warp] = sum;
       group_sync<GT>(g);
