@@ -64,6 +64,40 @@ __device__ __forceinline__ float vec_max(const uint4& r) {
   }
 }
 
+// whether an element of a vector is not below `floor` (its upper 16 bits are the threshold's: for bf16 they are all that
+// counts)
+template <typename T>
+__device__ __forceinline__ bool reaches(const uint4& r, float floor) {
+  if constexpr (sizeof(T) == 2) {
+    const uint32_t f = __float_as_uint(floor) >> 16, ff = f | (f << 16);
+    auto pair = [](uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); };
+    const uint32_t below = __hlt2_mask(pair(r.x), pair(ff)) & __hlt2_mask(pair(r.y), pair(ff)) & __hlt2_mask(pair(r.z), pair(ff)) &
+                           __hlt2_mask(pair(r.w), pair(ff));
+    return below != 0xffffffffu;
+  } else {
+    return !(__uint_as_float(r.x) < floor) || !(__uint_as_float(r.y) < floor) || !(__uint_as_float(r.z) < floor) ||
+           !(__uint_as_float(r.w) < floor);
+  }
+}
+
+// f(rank, key) for the listed keys: how many of them are larger.  2 or 4 threads share a key's comparisons where there
+// are threads enough.
+template <int GT, typename F>
+__device__ __forceinline__ void each_rank(const uint64_t* list, int listed, int gt, F f) {
+  const int share = 4 * listed <= GT ? 2 : 2 * listed <= GT ? 1 : 0;  // log2
+  const int part = gt & ((1 << share) - 1);
+  for (int j0 = 0; j0 < listed; j0 += GT >> share) {
+    const int j = j0 + (gt >> share);
+    const uint64_t c = j < listed ? list[j] : ~0ull;
+    int r = 0;
+#pragma unroll 4
+    for (int o = part; o < listed; o += 1 << share) r += list[o] > c;
+    if (share > 0) r += __shfl_xor_sync(0xffffffffu, r, 1);
+    if (share > 1) r += __shfl_xor_sync(0xffffffffu, r, 2);
+    if (j < listed && part == 0) f(r, c);
+  }
+}
+
 // how many of a group's threads say so (a barrier of the group)
 template <int GT>
 __device__ __forceinline__ int group_count(int g, bool yes) {
@@ -179,7 +213,7 @@ top_pipe_kernel(const TopParams p) {
   __shared__ uint64_t xbar[G], xdone[G];  // all slices' lists are there; the first CTA has read them
   __shared__ float s_max[G][GW], s_sum[G][GW];
   __shared__ uint32_t s_range[G][GW];
-  __shared__ int s_count[G];
+  __shared__ int s_count[G], s_hits[G];
   __shared__ __align__(8) float s_slice[G][2];  // a slice's maximum and sum
   __shared__ TopSelect s_sel[G];
   const int tid = threadIdx.x, lane = tid & 31;
@@ -203,8 +237,9 @@ top_pipe_kernel(const TopParams p) {
     ring_load<T>(ring, smem, p.shape.stages, p.shape.stage_bytes, n_mine, row0, stride, slice_of, [](long long) { return false; });
   } else {
     const int g = tid / GT, gt = tid % GT, warp = gt >> 5;
-    uint64_t* list = reinterpret_cast<uint64_t*>(smem + (size_t)p.shape.stages * p.shape.stage_bytes) + (size_t)g * (cap + TOP_MAX_K);
-    uint64_t* best = list + cap;  // this slice's k largest in descending order (clusters)
+    uint64_t* list = reinterpret_cast<uint64_t*>(smem + (size_t)p.shape.stages * p.shape.stage_bytes) + (size_t)g * (cap + cap / 2 + TOP_MAX_K);
+    int* hits = reinterpret_cast<int*>(list + cap);  // vectors with an element that reaches the threshold
+    uint64_t* best = list + cap + cap / 2;  // this slice's k largest in descending order (clusters)
     int stage = g - G;  // the stage of row i, and its phase; a ring has at least G stages
     uint32_t phase = 0, turn = 0;
     for (int i = g; i < n_mine; i += G, ++turn) {
@@ -234,7 +269,7 @@ top_pipe_kernel(const TopParams p) {
           if (v + q * GT < cnt) m[q] = max_nan(m[q], vec_max<T>(vec[v + q * GT]));
       }
       const float most = max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3]));
-      if (gt == 0) s_count[g] = 0;
+      if (gt == 0) { s_count[g] = 0; s_hits[g] = 0; }
       const uint32_t top_key = gt < cnt ? order_key(most) >> 16 : 0;
       const float wm = warp_max(most);  // drops NaN, which the sum brings back
       const uint32_t k_hi = __reduce_max_sync(0xffffffffu, top_key);
@@ -281,39 +316,68 @@ top_pipe_kernel(const TopParams p) {
       const bool far = sizeof(T) == 4 || fabsf(ref) > 1e30f;
       float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
       uint4 next = gt < cnt ? vec[gt] : make_uint4(0, 0, 0, 0);
+      // a thread notes which of its vectors hold such an element (32 at a time); looking into them here would hold up
+      // the other 31 lanes of the warp
 #pragma unroll 1
-      for (int v = gt; v < cnt; v += GT) {
-        float x[V];
-        unpack_vec<T>(next, x);
-        if (v + GT < cnt) next = vec[v + GT];  // on its way while this one is worked on
-        bool any = false;
+      for (int v0 = gt; v0 - gt < cnt; v0 += 32 * GT) {
+        uint32_t noted = 0;
+#pragma unroll 1
+        for (int j = 0; j < 32; ++j) {
+          const int v = v0 + j * GT;
+          if (v >= cnt) break;
+          const uint4 r = next;
+          if (v + GT < cnt) next = vec[v + GT];  // on its way while this one is worked on
+          noted |= (uint32_t)reaches<T>(r, floor_value) << j;
+          if (p.lse) {
+            float x[V];
+            unpack_vec<T>(r, x);
+            if (far) {
 #pragma unroll
-        for (int c = 0; c < V; ++c) any |= !(x[c] < floor_value);
-        if (any) {
-          const int e = s.first(s.lo + v);
+              for (int c = 0; c < V; ++c) acc[c & 3] += expf((x[c] - ref) * p.inv_t);
+            } else {
 #pragma unroll
-          for (int c = 0; c < V; ++c)
-            if (!(x[c] < floor_value) && e + c >= 0 && e + c < n) {
-              const int at = atomicAdd(&s_count[g], 1);
-              if (at < cap) list[at] = ((uint64_t)order_key(x[c]) << 32) | (uint32_t)~(e + c);
+              for (int c = 0; c < V; ++c) acc[c & 3] += exp2_approx(fmaf(x[c], c2, off));
             }
-        }
-        if (p.lse) {
-          if (far) {
-#pragma unroll
-            for (int c = 0; c < V; ++c) acc[c & 3] += expf((x[c] - ref) * p.inv_t);
-          } else {
-#pragma unroll
-            for (int c = 0; c < V; ++c) acc[c & 3] += exp2_approx(fmaf(x[c], c2, off));
           }
         }
+        // the notes of a warp, one after the other, into the group's list of vectors
+        int mine = __popc(noted), before = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int up = __shfl_up_sync(0xffffffffu, before, o);
+          if (lane >= o) before += up;
+        }
+        int at = 0;
+        if (lane == 31 && before) at = atomicAdd(&s_hits[g], before);
+        at = __shfl_sync(0xffffffffu, at, 31) + before - mine;
+        for (; noted; noted &= noted - 1, ++at)
+          if (at < cap) hits[at] = v0 + (__ffs(noted) - 1) * GT;
       }
       float sum = (acc[0] + acc[1]) + (acc[2] + acc[3]);
       sum = warp_sum(sum);
       if (lane == 0) s_sum[g][warp] = sum;
       group_sync<GT>(g);
       sum = lanes_sum<GW>(s_sum[g][lane % GW]);
-      int listed = s_count[g];
+      const int noted = s_hits[g];
+      if (noted <= cap) {
+        for (int j = gt; j < noted; j += GT) {
+          float x[V];
+          const int v = hits[j], e = s.first(s.lo + v);
+          unpack_vec<T>(vec[v], x);
+          uint32_t in = 0;
+#pragma unroll
+          for (int c = 0; c < V; ++c) in |= (uint32_t)(!(x[c] < floor_value) && e + c >= 0 && e + c < n) << c;
+          int at = atomicAdd(&s_count[g], __popc(in));
+#pragma unroll
+          for (int c = 0; c < V; ++c)
+            if ((in >> c) & 1) {
+              if (at < cap) list[at] = ((uint64_t)order_key(x[c]) << 32) | (uint32_t)~(e + c);
+              ++at;
+            }
+        }
+      }
+      group_sync<GT>(g);
+      int listed = noted <= cap ? s_count[g] : cap + 1;
       if (listed > cap) {
         uint32_t value, last;
         exact_threshold<GT>(s_sel[g], gt, kk, here, value, last, [&](auto f) { each_element<T, GT>(s, vec, gt, f); },
@@ -343,24 +407,12 @@ top_pipe_kernel(const TopParams p) {
       };
       if (C == 1) {
         if (gt == 0 && p.lse && top != INFINITY) p.lse[row] = ref * p.inv_t + logf(sum);
-        for (int j = gt; j < listed; j += GT) {
-          const uint64_t c = list[j];
-          int r = 0;
-#pragma unroll 4
-          for (int o = 0; o < listed; ++o) r += list[o] > c;
-          if (r < k) put(r, c);
-        }
+        each_rank<GT>(list, listed, gt, [&](int r, uint64_t c) { if (r < k) put(r, c); });
         group_sync<GT>(g);  // the list is read before the next row's takes its place
       } else {
         if (gt == 0) { s_slice[g][0] = sum == 0.0f ? -INFINITY : ref; s_slice[g][1] = sum; }
         for (int j = gt + kk; j < k; j += GT) best[j] = 0;
-        for (int j = gt; j < listed; j += GT) {
-          const uint64_t c = list[j];
-          int r = 0;
-#pragma unroll 4
-          for (int o = 0; o < listed; ++o) r += list[o] > c;
-          if (r < k) best[r] = c;
-        }
+        each_rank<GT>(list, listed, gt, [&](int r, uint64_t c) { if (r < k) best[r] = c; });
         group_sync<GT>(g);
         if (gt == 0) mbar_arrive_release_cluster(mapa_cluster(smem_u32(&xbar[g]), 0));
         if (rank == 0) {
@@ -460,7 +512,7 @@ template <typename T>
 int top_launch(TopParams& p, cudaStream_t s) {
   const long long bytes = (long long)p.vocab * sizeof(T);
   auto shape = [&](int groups, int least) {
-    p.shape = row_shape(p.rows, p.vocab, sizeof(T), groups * 8 * (top_list(p.k) + TOP_MAX_K), std::max(2 * groups, 3), least);
+    p.shape = row_shape(p.rows, p.vocab, sizeof(T), groups * 8 * (top_list(p.k) * 3 / 2 + TOP_MAX_K), std::max(2 * groups, 3), least);
     return p.shape.stages >= groups;
   };
   if (p.rows > 2LL * sm_count()) {
