@@ -356,11 +356,12 @@ __device__ __forceinline__ void kept_vec(const uint4& r, float (&x)[VecOf<T>::N]
 }
 
 // The frame of row_pipe.cuh.  A group of GT threads walks over its row three times: maximum, sums of the exponentials,
-// gradient over the logits in shared memory.  Beside it two warps see to what the row has of single entries: one reads, a
+// gradient, which goes from registers to global memory: a row of 64 KB sent off from shared memory would hold its stage,
+// one of three, for another 5000 clocks.  Beside it two warps see to what the row has of single entries: one reads, a
 // row ahead, the teacher's ids and logits and forms their distribution; the other one, when the group has been through
 // the row, forms the loss and rewrites the entries that have a term of their own, the ids and the target.  In the
 // group's hands these were half of a row's time, latency after latency with most of its threads idle.
-constexpr int pipe_threads(int gt, int groups) { return (gt + 64) * groups + RP_EXTRA; }
+constexpr int pipe_threads(int gt, int groups) { return (gt + 64) * groups + 32; }
 __host__ __device__ constexpr int entry_pad(int k) { return (k + 4) & ~3; }
 // slots of the table that finds equal ids: at least twice the entries
 __host__ __device__ constexpr int entry_slots(int k) {
@@ -368,7 +369,7 @@ __host__ __device__ constexpr int entry_slots(int k) {
   while (n < 2 * k) n *= 2;
   return n;
 }
-__host__ __device__ constexpr int entry_bytes(int k) { return 2 * 4 * 4 * entry_pad(k) + 2 * entry_slots(k); }
+__host__ __device__ constexpr int entry_bytes(int k) { return 2 * 5 * 4 * entry_pad(k) + 2 * entry_slots(k); }
 
 // A row's entries in shared memory (two sets per group: one in use, one being read).
 struct Entries {
@@ -376,11 +377,13 @@ struct Entries {
   float* t;  // its logits / T
   float* x;  // the student's logits there
   float* w;  // exp(t - tref), of all equal ids in one of them; -1 in the others
+  float* o;  // what dlogits held there (accumulate)
   __device__ __forceinline__ Entries(uint8_t* p, int set, int pad) {
-    id = reinterpret_cast<int*>(p) + set * 4 * pad;
+    id = reinterpret_cast<int*>(p) + set * 5 * pad;
     t = reinterpret_cast<float*>(id + pad);
     x = t + pad;
     w = x + pad;
+    o = w + pad;
   }
 };
 struct RowTeacher {  // exp(t - tref) = q_j S;  Q = sum of the q_j
@@ -391,7 +394,7 @@ struct RowStats {  // what the group found
 };
 
 template <typename T, int GT, int G, int MODE>
-__global__ void __launch_bounds__((GT + 64) * G + RP_EXTRA, 1)
+__global__ void __launch_bounds__((GT + 64) * G + 32, 1)
 distill_pipe_kernel(const DistillParams p) {
   constexpr int V = VecOf<T>::N, GW = GT / 32;
   constexpr bool FWD = (MODE & DS_FWD) != 0, BWD = (MODE & DS_BWD) != 0, ACC = BWD && !FWD;
@@ -401,7 +404,6 @@ distill_pipe_kernel(const DistillParams p) {
   __shared__ uint64_t ready[G][2];     // the entries are prepared
   __shared__ uint64_t through[G][2];   // the group is through the row (its warps)
   __shared__ uint64_t finished[G][2];  // its entries are rewritten, the loss is formed: the set is free
-  __shared__ uint64_t rewritten[G];    // a row that its group takes to dlogits is ready for that
   __shared__ uint64_t xbar[G];         // the slices of a row have met (C arrivals)
   __shared__ float s_red[G][3][GW];
   __shared__ RowTeacher s_teacher[G][2];
@@ -412,11 +414,10 @@ distill_pipe_kernel(const DistillParams p) {
   const int rank = C > 1 ? (int)cluster_ctarank() : 0;
   const long long row0 = blockIdx.x >> p.shape.cluster_log2, stride = gridDim.x >> p.shape.cluster_log2;
   const int n_mine = row0 < p.rows ? (int)((p.rows - row0 + stride - 1) / stride) : 0;
-  ring_init(ring, p.shape.stages, BWD ? 1 : GW, 1);
+  ring_init(ring, p.shape.stages, GW);
   if (tid == 0) {
     for (int g = 0; g < G; ++g) {
       mbar_init(&xbar[g], C);
-      mbar_init(&rewritten[g], 1);
       for (int set = 0; set < 2; ++set) {
         mbar_init(&ready[g][set], 1);
         mbar_init(&through[g][set], GW);
@@ -440,11 +441,7 @@ distill_pipe_kernel(const DistillParams p) {
   auto like = [&](const RowSlice<T>& s, const T* dr) { return (int)(((uint32_t)reinterpret_cast<uintptr_t>(dr) & 15) / sizeof(T)) == s.lead; };
   constexpr int ENTRY0 = GT * G, LOAD0 = ENTRY0 + 64 * G;
 
-  if (tid >= LOAD0 + 32) {
-    if constexpr (BWD)
-      ring_store<T>(ring, smem, p.shape.stages, p.shape.stage_bytes, n_mine, row0, stride, slice_of, skip_row,
-                    [&](long long row) { return dlogits + row * p.ldd; });
-  } else if (tid >= LOAD0) {
+  if (tid >= LOAD0) {
     ring_load<T>(ring, smem, p.shape.stages, p.shape.stage_bytes, n_mine, row0, stride, slice_of, skip_row);
   } else if (tid >= ENTRY0) {
     // ---------------- the two entry warps of group g ----------------
@@ -452,7 +449,7 @@ distill_pipe_kernel(const DistillParams p) {
     const bool preparing = ((tid - ENTRY0) & 32) == 0;
     const int KP = entry_pad(k), slots = entry_slots(k);
     uint8_t* mine = smem + (size_t)p.shape.stages * p.shape.stage_bytes + (size_t)g * entry_bytes(k);
-    uint16_t* table = reinterpret_cast<uint16_t*>(mine + 2 * 4 * 4 * KP);
+    uint16_t* table = reinterpret_cast<uint16_t*>(mine + 2 * 5 * 4 * KP);
     const bool want = BWD || rank == 0;  // this CTA has use for the entries
     // the next row from i on that counts; n_mine or more: none
     auto next_row = [&](int i, int& y) {
@@ -483,6 +480,8 @@ distill_pipe_kernel(const DistillParams p) {
       const Entries e(mine, set, KP);
       float ref = -INFINITY;
       const float xy = lane == 0 && y >= 0 ? to_f32(xr[y]) : 0.0f;
+      const T* dr = dlogits + row * p.ldd;
+      if (ACC && acc && lane == 0) e.o[k] = y >= 0 ? to_f32(dr[y]) : 0.0f;
       const float tl_given = tl_next;
       for (int j0 = lane; j0 - lane < k; j0 += 128) {  // four entries' loads at a time
         int id[4];
@@ -511,6 +510,7 @@ distill_pipe_kernel(const DistillParams p) {
             e.id[j] = id[c];
             e.t[j] = t[c];
             e.x[j] = x[c];
+            if (ACC && acc) e.o[j] = id[c] >= 0 ? to_f32(dr[id[c]]) : 0.0f;
             ref = fmaxf(ref, t[c]);
           }
         }
@@ -562,7 +562,6 @@ distill_pipe_kernel(const DistillParams p) {
     };
     int y;
     int i = next_row(g, y);
-    int stage = g, stage_i = g;  // stage of row i
     if (preparing && want) request(i);
     for (int turn = 0; i < n_mine; ++turn) {
       const int set = turn & 1;
@@ -577,11 +576,6 @@ distill_pipe_kernel(const DistillParams p) {
         y = y_after;
         continue;
       }
-      while (stage_i < i) {
-        stage_i += G;
-        stage += G;
-        if (stage >= p.shape.stages) stage -= p.shape.stages;
-      }
       mbar_wait(&ready[g][set], phase, &ring.abort_flag, nullptr, FAULT_WAIT_FULL);
       mbar_wait(&through[g][set], phase, &ring.abort_flag, nullptr, FAULT_WAIT_FULL);
       const long long row = row0 + (long long)i * stride;
@@ -592,37 +586,25 @@ distill_pipe_kernel(const DistillParams p) {
       if constexpr (BWD) {
         const RowSlice<T> s = slice_of(row);
         T* dr = dlogits + row * p.ldd;
-        T* out = reinterpret_cast<T*>(smem + (size_t)stage * p.shape.stage_bytes) - s.first(s.lo);  // out[id]: the entry of this slice
         const int e_lo = max(s.first(s.lo), 0), e_hi = min(s.first(s.hi), n);
-        auto rewrite = [&](int id, float x, float less) {
+        auto rewrite = [&](int j, int id, float less) {
+          float x = e.x[j];
           x -= st.ref;
           float d = st.kt * expf(x * p.inv_t);
           if (st.k1 != 0.0f) d += st.k1 * expf(x);
           d -= less;
-          if (acc) d += to_f32(dr[id]);
-          out[id] = from_f32<T>(d);
+          if (ACC && acc) d += e.o[j];
+          dr[id] = from_f32<T>(d);
         };
         bool met = false;  // the target is one of the ids
         for (int j = lane; j < k; j += 32) {
           const int id = e.id[j];
           const float w = e.w[j];
           met |= id >= 0 && id == y;
-          if (id >= e_lo && id < e_hi && w != -1.0f) rewrite(id, e.x[j], (has_kd ? kq * w * inv_s : 0.0f) + (id == y ? c1 : 0.0f));
+          if (id >= e_lo && id < e_hi && w != -1.0f) rewrite(j, id, (has_kd ? kq * w * inv_s : 0.0f) + (id == y ? c1 : 0.0f));
         }
         met = __any_sync(0xffffffffu, met);
-        if (has_ce && !met && lane == 0 && y >= e_lo && y < e_hi) rewrite(y, e.x[k], c1);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (like(s, dr)) {
-          if (s.edges()) {  // the vectors at the row's ends
-            const int a = min(s.first(s.w0), e_hi), b = max(s.first(s.w1), a);
-            if (e_lo + lane < a) dr[e_lo + lane] = out[e_lo + lane];
-            if (b + lane < e_hi) dr[b + lane] = out[b + lane];
-          }
-          mbar_arrive_warp(&ring.done[stage]);
-        } else {
-          mbar_arrive_warp(&rewritten[g]);  // the group takes the row to its place
-        }
+        if (has_ce && !met && lane == 0 && y >= e_lo && y < e_hi) rewrite(k, y, c1);
       }
       if (FWD && rank == 0) {
         const float tl = p.t_lse || S == 0.0f ? te.tref : te.tref + logf(S);  // ln q_j = t_j - tl
@@ -657,7 +639,6 @@ distill_pipe_kernel(const DistillParams p) {
     };
     request(g);
     int turn = -1;       // rows this group has worked on (skipped ones do not count)
-    uint32_t odd = 0;    // phase of `rewritten`
     int stage = g - G;   // the stage of row i, and its phase; a ring has at least G stages
     uint32_t phase = 0;
     for (int i = g; i < n_mine; i += G) {
@@ -685,12 +666,7 @@ distill_pipe_kernel(const DistillParams p) {
           }
         }
         ring_wait_row(ring, i, stage, phase);
-        if constexpr (BWD) {
-          group_sync<GT>(g);
-          if (gt == 0) mbar_arrive(&ring.done[stage]);
-        } else {
-          mbar_arrive_warp(&ring.empty[stage]);
-        }
+        mbar_arrive_warp(&ring.empty[stage]);
         continue;
       }
       ++turn;
@@ -815,7 +791,8 @@ distill_pipe_kernel(const DistillParams p) {
       if constexpr (!BWD) {
         mbar_arrive_warp(&through[g][set]);
       } else {
-        const bool whole = like(s, dr);
+        // vectors that go to dlogits as they are
+        const int w0 = like(s, dr) ? s.w0 : s.hi, w1 = like(s, dr) ? s.w1 : s.hi;
         // a slice without a finite entry has nothing but zeros
         const float at = C > 1 && FWD ? (own_st == 0.0f ? 0.0f : expf((own_ref - ref) * p.inv_t)) : 1.0f;
         const float a1 = C > 1 && FWD ? (own_st == 0.0f ? 0.0f : expf(own_ref - ref)) : 1.0f;
@@ -837,32 +814,28 @@ distill_pipe_kernel(const DistillParams p) {
               fmul2(d[c], d[c + 1], et[0], et[1], mt, mt);
               if constexpr (Ex::BOTH) ffma2(d[c], d[c + 1], e1[0], e1[1], m1, m1, d[c], d[c + 1]);
             }
-            if (acc) {
-              const int e = s.first(s.lo + v);
-              if (whole && s.lo + v >= s.w0 && s.lo + v < s.w1) {
+            const int e = s.first(s.lo + v);
+            if (s.lo + v >= w0 && s.lo + v < w1) {
+              if (ACC && acc) {
                 float o[V];
                 ld16(dr + e, o);
 #pragma unroll
                 for (int c = 0; c < V; ++c) d[c] += o[c];
-              } else {
-#pragma unroll
-                for (int c = 0; c < V; ++c)
-                  if (e + c >= 0 && e + c < n) d[c] += to_f32(dr[e + c]);
               }
+              st16(dr + e, d);
+            } else {
+#pragma unroll
+              for (int c = 0; c < V; ++c)
+                if (e + c >= 0 && e + c < n) {
+                  if (ACC && acc) d[c] += to_f32(dr[e + c]);
+                  dr[e + c] = from_f32<T>(d[c]);
+                }
             }
-            st16(reinterpret_cast<T*>(vec + v), d);
           }
         });
-        fence_proxy_async_smem();
+        fence_proxy_async_smem();  // what was kept in the row's place, before a copy takes it
+        mbar_arrive_warp(&ring.empty[stage]);
         mbar_arrive_warp(&through[g][set]);
-        if (!whole) {
-          mbar_wait(&rewritten[g], odd, &ring.abort_flag, nullptr, FAULT_WAIT_FULL);
-          odd ^= 1;
-          const T* out = reinterpret_cast<const T*>(vec) - s.first(s.lo);
-          for (int e = max(s.first(s.lo), 0) + gt; e < min(s.first(s.hi), n); e += GT) dr[e] = out[e];
-          group_sync<GT>(g);
-          if (gt == 0) mbar_arrive(&ring.done[stage]);
-        }
       }
     }
   }

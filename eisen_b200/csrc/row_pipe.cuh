@@ -2,10 +2,9 @@
 //
 // A persistent CTA (one per SM) takes every n-th row.  One warp keeps a ring of stages filled with bulk
 // asynchronous copies of whole rows; G groups of GT threads take the rows in turn and walk over them in shared
-// memory as often as they need; where a row is rewritten in place, another warp sends it off by a bulk copy.  The
-// memory stays busy while the groups sit at their reductions, a group's loops are a few instructions long, and
-// random access to a row (a target, a teacher's ids) costs a shared-memory access.  A row that is too long for a
-// stage is split over the CTAs of a cluster.
+// memory as often as they need.  The memory stays busy while the groups sit at their reductions, and a group's loops
+// are a few instructions long.  A row that is too long for a third of the shared memory is split over the CTAs of a
+// cluster.
 //
 // A row may start at any element: the copies take the 16-byte vectors that lie in it, the one or two vectors at
 // its ends are read and written element by element.
@@ -19,7 +18,6 @@
 namespace eisen {
 
 constexpr int RP_MAX_STAGES = 32;
-constexpr int RP_EXTRA = 64;  // threads of the loading and the storing warp
 
 template <typename T>
 __device__ __forceinline__ void unpack_vec(const uint4& r, float (&v)[VecOf<T>::N]) {
@@ -148,18 +146,16 @@ __device__ __forceinline__ float lanes_max(float v) {
 // barriers of a CTA's ring
 struct RowRing {
   uint64_t full[RP_MAX_STAGES];   // 1 arrival and the bytes of the copy
-  uint64_t empty[RP_MAX_STAGES];  // the storing warp, or the warps of the group that read the stage
-  uint64_t done[RP_MAX_STAGES];   // the warps of the group that rewrote the stage
+  uint64_t empty[RP_MAX_STAGES];  // the warps of the group that read the stage
   volatile int issued;            // rows the loading warp has sent for
   int abort_flag;
 };
 
-__device__ __forceinline__ void ring_init(RowRing& r, int stages, int empty_arrivals, int done_arrivals) {
+__device__ __forceinline__ void ring_init(RowRing& r, int stages, int group_warps) {
   if (threadIdx.x == 0) {
     for (int i = 0; i < stages; ++i) {
       mbar_init(&r.full[i], 1);
-      mbar_init(&r.empty[i], empty_arrivals);
-      mbar_init(&r.done[i], done_arrivals);
+      mbar_init(&r.empty[i], group_warps);
     }
     r.abort_flag = 0;
     r.issued = 0;
@@ -217,43 +213,6 @@ __device__ __forceinline__ void ring_load(RowRing& r, uint8_t* smem, int stages,
     }
     if (__any_sync(0xffffffffu, given_up)) return;  // nothing more is sent for
   }
-}
-
-// The storing warp: sends the whole vectors of a rewritten stage to `dst(row)` (the address of the row's first element;
-// where it is not aligned like the row it came from, the group writes the row itself) and frees the stage.
-template <typename T, typename Slice, typename Skip, typename Dst>
-__device__ __forceinline__ void ring_store(RowRing& r, uint8_t* smem, int stages, int stage_bytes, int n_mine, long long row0,
-                                           long long stride, Slice slice, Skip skip, Dst dst) {
-  const int lane = threadIdx.x & 31;
-  int st = 0;
-  uint32_t phase = 0;
-  for (int i0 = 0; i0 < n_mine; i0 += 32) {
-    const bool mine = i0 + lane < n_mine && skip(row0 + (long long)(i0 + lane) * stride);
-    const uint32_t skips = __ballot_sync(0xffffffffu, mine);
-    bool given_up = false;
-    if (lane == 0) {
-      const int m = min(32, n_mine - i0);
-      for (int i = 0; i < m; ++i) {
-        given_up = !mbar_wait(&r.done[st], phase, &r.abort_flag, nullptr, FAULT_WAIT_FULL);
-        if (given_up) break;
-        const long long row = row0 + (long long)(i0 + i) * stride;
-        const RowSlice<T> s = slice(row);
-        T* to = dst(row);
-        const uint32_t bytes = (uint32_t)(s.w1 - s.w0) * 16;
-        if (!((skips >> i) & 1) && bytes && (reinterpret_cast<uintptr_t>(to) & 15) / sizeof(T) == s.lead) {
-          asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to + s.first(s.w0)),
-                       "r"(smem_u32(smem + (size_t)st * stage_bytes + (size_t)(s.w0 - s.lo) * 16)), "r"(bytes)
-                       : "memory");
-          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-          asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-        }
-        mbar_arrive(&r.empty[st]);
-        if (++st == stages) { st = 0; phase ^= 1; }
-      }
-    }
-    if (__any_sync(0xffffffffu, given_up)) break;
-  }
-  if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 
 // ---- host: shape of a launch

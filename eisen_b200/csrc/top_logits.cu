@@ -221,7 +221,7 @@ top_pipe_kernel(const TopParams p) {
   const int rank = C > 1 ? (int)cluster_ctarank() : 0;
   const long long row0 = blockIdx.x >> p.shape.cluster_log2, stride = gridDim.x >> p.shape.cluster_log2;
   const int n_mine = row0 < p.rows ? (int)((p.rows - row0 + stride - 1) / stride) : 0;
-  ring_init(ring, p.shape.stages, GW, 1);
+  ring_init(ring, p.shape.stages, GW);
   if (tid == 0) {
     for (int g = 0; g < G; ++g) {
       mbar_init(&xbar[g], C);
@@ -520,7 +520,7 @@ int top_launch(TopParams& p, cudaStream_t s) {
       return launch_pipe<top_pipe_kernel<T, 32, 8>>("top_logits", p.shape, p.rows, 32 * 8 + 32, s, p);
     if (bytes <= 24 * 1024 && shape(4, 1 << 30))
       return launch_pipe<top_pipe_kernel<T, 128, 4>>("top_logits", p.shape, p.rows, 128 * 4 + 32, s, p);
-    if (shape(2, 1 << 30)) return launch_pipe<top_pipe_kernel<T, 256, 2>>("top_logits", p.shape, p.rows, 256 * 2 + 32, s, p);
+    if (shape(3, 1 << 30)) return launch_pipe<top_pipe_kernel<T, 256, 3>>("top_logits", p.shape, p.rows, 256 * 3 + 32, s, p);
   }
   if (shape(1, 8192)) return launch_pipe<top_pipe_kernel<T, 512, 1>>("top_logits", p.shape, p.rows, 512 + 32, s, p);
   top_long_kernel<T><<<(unsigned)p.rows, TOP_THREADS, 0, s>>>(p);
