@@ -363,10 +363,10 @@ __device__ __forceinline__ void kept_vec(const uint4& r, float (&x)[VecOf<T>::N]
 // group's hands these were half of a row's time, latency after latency with most of its threads idle.
 constexpr int pipe_threads(int gt, int groups) { return (gt + 64) * groups + 32; }
 __host__ __device__ constexpr int entry_pad(int k) { return (k + 4) & ~3; }
-// slots of the table that finds equal ids: at least twice the entries
+// slots of the table that finds equal ids: at least four times the entries
 __host__ __device__ constexpr int entry_slots(int k) {
   int n = 64;
-  while (n < 2 * k) n *= 2;
+  while (n < 4 * k) n *= 2;
   return n;
 }
 __host__ __device__ constexpr int entry_bytes(int k) { return 2 * 5 * 4 * entry_pad(k) + 2 * entry_slots(k); }
@@ -451,59 +451,78 @@ distill_pipe_kernel(const DistillParams p) {
     uint8_t* mine = smem + (size_t)p.shape.stages * p.shape.stage_bytes + (size_t)g * entry_bytes(k);
     uint16_t* table = reinterpret_cast<uint16_t*>(mine + 2 * 5 * 4 * KP);
     const bool want = BWD || rank == 0;  // this CTA has use for the entries
-    // the next row from i on that counts; n_mine or more: none
-    auto next_row = [&](int i, int& y) {
-      y = -1;
-      for (; i < n_mine; i += G) {
-        if (p.targets) y = p.targets[row0 + (long long)i * stride];
-        if (!skipped(y)) break;
+    // the next row of this group that counts (n_mine or more: none) and its target; the targets are requested one ahead
+    int cand = g, y_cand = p.targets && g < n_mine ? p.targets[row0 + (long long)g * stride] : -1;
+    auto next_row = [&](int& y) {
+      while (cand < n_mine) {
+        const int i = cand;
+        y = y_cand;
+        cand += G;
+        if (p.targets && cand < n_mine) y_cand = p.targets[row0 + (long long)cand * stride];
+        if (!skipped(y)) return i;
       }
-      return i;
+      return n_mine;
     };
-    // The first 128 entries of a row (four per lane) are requested while the row before it is prepared.
-    int id_next[4];
-    float t_next[4], tl_next = 0.0f;
+    // The first 64 entries of a row (two per lane) are requested while the row before it is prepared, and the student's
+    // logits there at the end of that.
+    int id_next[2], id[2];
+    float t_next[2], x_next[2], t[2], x[2], tl_next = 0.0f, xy_next = 0.0f;
+    auto clean = [&](int v) {
+      if (v >= n) {
+        if (FWD && p.bad_id_flag) *p.bad_id_flag = 1;
+        return -1;
+      }
+      return max(v, -1);
+    };
     auto request = [&](int i) {
       if (i >= n_mine) return;
       const long long row = row0 + (long long)i * stride;
+      const int* ids = p.t_ids + row * k + lane;
+      const float* tv = p.t_logits + row * k + lane;
       if (p.t_lse) tl_next = p.t_lse[row];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int j = lane + 32 * c;
-        id_next[c] = j < k ? p.t_ids[row * k + j] : -1;
-        t_next[c] = j < k ? p.t_logits[row * k + j] : 0.0f;
+      for (int c = 0; c < 2; ++c) {
+        const bool in = lane + 32 * c < k;
+        id_next[c] = in ? ids[32 * c] : -1;
+        t_next[c] = in ? tv[32 * c] : 0.0f;
       }
     };
-    auto prepare = [&](int i, int y, int set, int after) {
+    auto gather = [&](int i, int y) {
+      if (i >= n_mine) return;
+      const T* xr = logits + (row0 + (long long)i * stride) * p.ld;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        id_next[c] = clean(id_next[c]);
+        x_next[c] = id_next[c] >= 0 ? to_f32(xr[id_next[c]]) : 0.0f;
+      }
+      xy_next = y >= 0 ? to_f32(xr[y]) : 0.0f;
+    };
+    auto prepare = [&](int i, int y, int set, int after, int y_after) {
       const long long row = row0 + (long long)i * stride;
       const T* xr = logits + row * p.ld;
+      const T* dr = dlogits + row * p.ldd;
       const Entries e(mine, set, KP);
       float ref = -INFINITY;
-      const float xy = lane == 0 && y >= 0 ? to_f32(xr[y]) : 0.0f;
-      const T* dr = dlogits + row * p.ldd;
-      if (ACC && acc && lane == 0) e.o[k] = y >= 0 ? to_f32(dr[y]) : 0.0f;
-      const float tl_given = tl_next;
-      for (int j0 = lane; j0 - lane < k; j0 += 128) {  // four entries' loads at a time
-        int id[4];
-        float t[4], x[4];
+      const float tl_given = tl_next, xy = xy_next;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int j = j0 + 32 * c;
-          id[c] = j0 == lane ? id_next[c] : (j < k ? p.t_ids[row * k + j] : -1);
-          t[c] = j0 == lane ? t_next[c] : (j < k ? p.t_logits[row * k + j] : 0.0f);
-        }
+      for (int c = 0; c < 2; ++c) { id[c] = id_next[c]; t[c] = t_next[c]; x[c] = x_next[c]; }
+      request(after);
+      if (lane == 0) {
+        e.x[k] = xy;
+        if (ACC && acc) e.o[k] = y >= 0 ? to_f32(dr[y]) : 0.0f;
+      }
+      for (int j0 = lane; j0 - lane < k; j0 += 64) {
+        if (j0 >= 64) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          if (id[c] >= n) {
-            if (FWD && p.bad_id_flag) *p.bad_id_flag = 1;
-            id[c] = -1;
+          for (int c = 0; c < 2; ++c) {
+            const int j = j0 + 32 * c;
+            id[c] = j < k ? clean(p.t_ids[row * k + j]) : -1;
+            t[c] = j < k ? p.t_logits[row * k + j] : 0.0f;
+            x[c] = id[c] >= 0 ? to_f32(xr[id[c]]) : 0.0f;
           }
-          id[c] = max(id[c], -1);
-          x[c] = id[c] >= 0 ? to_f32(xr[id[c]]) : 0.0f;
         }
-        if (j0 == lane) request(after);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 2; ++c) {
           const int j = j0 + 32 * c;
           if (j < k) {
             t[c] = id[c] >= 0 ? t[c] * p.inv_t : -INFINITY;
@@ -515,7 +534,6 @@ distill_pipe_kernel(const DistillParams p) {
           }
         }
       }
-      if (lane == 0) e.x[k] = xy;
       // exp(t - ref) = q_j S, where ref is the teacher's given log-sum-exp (S = 1) or its maximum
       if (p.t_lse) {
         ref = tl_given;
@@ -559,18 +577,21 @@ distill_pipe_kernel(const DistillParams p) {
       }
       S = warp_sum(S);
       if (lane == 0) s_teacher[g][set] = {ref, S, p.t_lse || S == 0.0f ? S : 1.0f};
+      gather(after, y_after);
     };
-    int y;
-    int i = next_row(g, y);
-    if (preparing && want) request(i);
+    int y = -1, y_after = -1;
+    int i = next_row(y);
+    if (preparing && want) {
+      request(i);
+      gather(i, y);
+    }
     for (int turn = 0; i < n_mine; ++turn) {
       const int set = turn & 1;
       const uint32_t phase = (uint32_t)(turn >> 1) & 1;
-      int y_after;
-      const int after = next_row(i + G, y_after);
+      const int after = next_row(y_after);
       if (preparing) {
         if (turn >= 2) mbar_wait(&finished[g][set], phase ^ 1, &ring.abort_flag, nullptr, FAULT_WAIT_EMPTY);
-        if (want) prepare(i, y, set, after);
+        if (want) prepare(i, y, set, after, y_after);
         mbar_arrive_warp(&ready[g][set]);
         i = after;
         y = y_after;
@@ -889,7 +910,12 @@ int distill_launch(const char* what, DistillParams& p, cudaStream_t s) {
       return launch_pipe<distill_pipe_kernel<T, 32, 8, MODE>>(what, p.shape, p.rows, pipe_threads(32, 8), s, p);
     if (bytes <= 24 * 1024 && shape(4, 1 << 30))
       return launch_pipe<distill_pipe_kernel<T, 128, 4, MODE>>(what, p.shape, p.rows, pipe_threads(128, 4), s, p);
-    if (shape(2, 1 << 30)) return launch_pipe<distill_pipe_kernel<T, 256, 2, MODE>>(what, p.shape, p.rows, pipe_threads(256, 2), s, p);
+    // where nothing is written three groups leave no stage idle; a gradient wants one that is being filled
+    if constexpr (MODE == DS_FWD) {
+      if (shape(3, 1 << 30)) return launch_pipe<distill_pipe_kernel<T, 128, 3, MODE>>(what, p.shape, p.rows, pipe_threads(128, 3), s, p);
+    } else {
+      if (shape(2, 1 << 30)) return launch_pipe<distill_pipe_kernel<T, 256, 2, MODE>>(what, p.shape, p.rows, pipe_threads(256, 2), s, p);
+    }
   }
   if (shape(1, 8192)) return launch_pipe<distill_pipe_kernel<T, 512, 1, MODE>>(what, p.shape, p.rows, pipe_threads(512, 1), s, p);
   distill_kernel<T, MODE><<<(unsigned)p.rows, DS_THREADS, 0, s>>>(p);
