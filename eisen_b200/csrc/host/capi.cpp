@@ -253,6 +253,86 @@ int eisen_graph_lm_head_cross_entropy(void* g, long long h, long long w, long lo
     *out = G(g).lm_head_cross_entropy(h, w, target_ids, n_valid > 0 ? 1.0f / (float)n_valid : 0.0f, trans_b != 0, chunk_rows);
   });
 }
+int eisen_graph_linear_cross_entropy(void* g, long long h, long long w, long long target_ids, long long n_valid, int trans_b,
+                                     long long piece, long long* out) {
+  return guarded([&] {
+    *out = G(g).linear_cross_entropy(h, w, target_ids, n_valid > 0 ? 1.0f / (float)n_valid : 0.0f, trans_b != 0, piece);
+  });
+}
+int eisen_graph_top_logits(void* g, long long logits, long long k, float temperature, long long* out3) {
+  return guarded([&] {
+    int64_t o[3];
+    G(g).top_logits(logits, k, temperature, o);
+    for (int i = 0; i < 3; ++i) out3[i] = o[i];
+  });
+}
+int eisen_graph_lm_head_top_logits(void* g, long long h, long long w, long long k, float temperature, int trans_b, long long chunk_rows,
+                                   long long* out3) {
+  return guarded([&] {
+    int64_t o[3];
+    G(g).lm_head_top_logits(h, w, k, temperature, trans_b != 0, chunk_rows, o);
+    for (int i = 0; i < 3; ++i) out3[i] = o[i];
+  });
+}
+static Graph::Teacher teacher_of(long long ids, long long logits, long long lse, float temperature, float kd_weight, float ce_weight) {
+  Graph::Teacher t;
+  t.ids = ids; t.logits = logits; t.lse = lse;
+  t.temperature = temperature; t.kd_weight = kd_weight; t.ce_weight = ce_weight;
+  return t;
+}
+int eisen_graph_distill(void* g, long long logits, long long teacher_ids, long long teacher_logits, long long teacher_lse,
+                        long long target_ids, long long n_valid, float temperature, float kd_weight, float ce_weight, long long* out) {
+  return guarded([&] {
+    *out = G(g).distill(logits, teacher_of(teacher_ids, teacher_logits, teacher_lse, temperature, kd_weight, ce_weight), target_ids,
+                        n_valid > 0 ? 1.0f / (float)n_valid : 0.0f);
+  });
+}
+int eisen_graph_lm_head_distill(void* g, long long h, long long w, long long teacher_ids, long long teacher_logits, long long teacher_lse,
+                                long long target_ids, long long n_valid, float temperature, float kd_weight, float ce_weight, int trans_b,
+                                long long chunk_rows, long long* out) {
+  return guarded([&] {
+    *out = G(g).lm_head_distill(h, w, teacher_of(teacher_ids, teacher_logits, teacher_lse, temperature, kd_weight, ce_weight), target_ids,
+                                n_valid > 0 ? 1.0f / (float)n_valid : 0.0f, trans_b != 0, chunk_rows);
+  });
+}
+int eisen_graph_copy_from(void* g, void* src, long long src_id, long long* out) {
+  return guarded([&] {
+    Graph& to = G(g);
+    Graph& from = G(src);
+    const HTensor t = from.tensors.at(src_id);
+    const bool apart = to.stream != from.stream;
+    if (apart && (to.capturing || from.capturing)) throw EisenException(EISEN_ERR_INVALID, "copy_from: a capture may not wait on another graph's stream");
+    cudaEvent_t ev = nullptr;
+    struct Free { cudaEvent_t& e; ~Free() { if (e) cudaEventDestroy(e); } } free_ev{ev};
+    auto must = [](cudaError_t e) {
+      if (e != cudaSuccess) throw EisenException(EISEN_ERR_CUDA, std::string("copy_from: ") + cudaGetErrorString(e));
+    };
+    const int64_t id = to.alloc_pooled_dtype(t.shape, t.dtype);
+    to.tensors[id].constant = true;
+    if (apart) {  // the copy comes after what the other stream has queued, and before what it queues from here on
+      must(cudaEventCreateWithFlags(&ev, cudaEventDisableTiming));
+      must(cudaEventRecord(ev, from.stream));
+      must(cudaStreamWaitEvent(to.stream, ev, 0));
+    }
+    if (t.numel > 0) must(cudaMemcpyAsync(to.tensors[id].data, t.data, (size_t)t.numel * (t.dtype == 1 ? 2 : 4), cudaMemcpyDefault, to.stream));
+    if (apart) {
+      must(cudaEventRecord(ev, to.stream));
+      must(cudaStreamWaitEvent(from.stream, ev, 0));
+    }
+    *out = id;
+  });
+}
+int eisen_graph_sync_ids_to_cpu(void* g, long long id, int* out) {
+  return guarded([&] {
+    Graph& gr = G(g);
+    const HTensor& t = gr.tensors.at(id);
+    if (t.dtype != DT_I32) throw EisenException(EISEN_ERR_INVALID, "sync_ids_to_cpu: not an id tensor");
+    if (!out) throw EisenException(EISEN_ERR_INVALID, "sync_ids_to_cpu: null output");
+    if (cudaMemcpyAsync(out, t.data, (size_t)t.numel * 4, cudaMemcpyDefault, gr.stream) != cudaSuccess ||
+        cudaStreamSynchronize(gr.stream) != cudaSuccess)
+      throw EisenException(EISEN_ERR_CUDA, "sync_ids_to_cpu: copy failed");
+  });
+}
 int eisen_graph_rms_norm(void* g, long long x, long long w, float eps, long long* out) {
   return guarded([&] { *out = G(g).rms_norm(x, w, eps); });
 }
@@ -294,6 +374,27 @@ int eisen_lm_set_head_fusion(void* lm, int fused, long long chunk_rows) {
     TransformerLM* m = static_cast<TransformerLM*>(lm);
     m->fused_head = fused != 0;
     m->head_chunk_rows = chunk_rows;
+  });
+}
+int eisen_lm_set_head_pieces(void* lm, long long piece) {
+  return guarded([&] { static_cast<TransformerLM*>(lm)->head_piece = piece < 0 ? -1 : piece; });
+}
+int eisen_lm_top_logits(void* lm, void* g, long long x_ids, long long k, float temperature, long long chunk_rows, long long* out3) {
+  return guarded([&] {
+    int64_t o[3];
+    static_cast<TransformerLM*>(lm)->top_logits(G(g), x_ids, k, temperature, chunk_rows, o);
+    for (int i = 0; i < 3; ++i) out3[i] = o[i];
+  });
+}
+int eisen_lm_distill_micro_step_dev(void* lm, void* g, long long x_ids, long long teacher_ids, long long teacher_logits,
+                                    long long teacher_lse, long long target_ids, long long n_valid, float temperature, float kd_weight,
+                                    float ce_weight, int checkpoint, eisen_block_cb after_block, void* user, long long* loss_id) {
+  return guarded([&] {
+    std::function<void(int64_t)> cb;
+    if (after_block) cb = [after_block, user](int64_t l) { after_block((long long)l, user); };
+    *loss_id = static_cast<TransformerLM*>(lm)->distill_micro_step_dev(
+        G(g), x_ids, teacher_of(teacher_ids, teacher_logits, teacher_lse, temperature, kd_weight, ce_weight), target_ids, n_valid,
+        checkpoint != 0, cb);
   });
 }
 int eisen_lm_forward(void* lm, void* g, long long x, long long* out) {

@@ -1296,6 +1296,204 @@ int64_t Graph::lm_head_cross_entropy(int64_t h, int64_t w, int64_t tid, float no
   return o;
 }
 
+// Rows, width and vocabulary of a head projection, checked.
+namespace {
+struct HeadShape {
+  int64_t rows, k, vocab;
+};
+}  // namespace
+static HeadShape head_shape(const char* what, const HTensor& th, const HTensor& tw, bool trans_b) {
+  if (tw.shape.size() != 2 || th.shape.empty()) invalid(std::string(what) + ": the head weight must have rank 2");
+  const int64_t k = th.shape.back();
+  if (k <= 0 || (trans_b ? tw.shape[1] : tw.shape[0]) != k) invalid(std::string(what) + ": inner dims differ");
+  return {th.numel / k, k, trans_b ? tw.shape[0] : tw.shape[1]};
+}
+
+int64_t Graph::linear_cross_entropy(int64_t h, int64_t w, int64_t tid, float normalizer, bool trans_b, int64_t piece) {
+  if (precision != Precision::Bf16Mixed) invalid("linear_cross_entropy: bf16 operands only (Bf16Mixed)");
+  const HeadShape d = head_shape("linear_cross_entropy", tensors.at(h), tensors.at(w), trans_b);
+  if (tensors.at(tid).dtype != DT_I32 || tensors[tid].numel != d.rows) invalid("linear_cross_entropy: one int32 target per row expected");
+  if (tensors[w].host_homed) invalid("linear_cross_entropy: the head weight must be on the device");
+  if (piece < 0) invalid("linear_cross_entropy: piece must be >= 0");
+  const int64_t ldw = trans_b ? d.k : d.vocab;
+  const int64_t lse = alloc_pooled_dtype({d.rows}, 0), row_loss = alloc_pooled_dtype({d.rows}, 0), o = alloc_pooled_dtype({}, 0);
+  tensors[lse].constant = tensors[row_loss].constant = true;
+  {
+    const size_t bytes = (size_t)eisen_linear_ce_workspace_bytes(d.rows, d.k, d.vocab, piece, 0);
+    void* ws = pool_get(bytes);
+    struct Release { Graph& g; void* p; size_t b; ~Release() { g.pool_put(p, b); } } release{*this, ws, bytes};
+    prof_begin(0, 2.0 * (double)d.rows * (double)d.k * (double)d.vocab);
+    ck(eisen_linear_ce_fwd(stream, operand(tensors[h]), d.k, operand(tensors[w]), ldw, trans_b, (const int*)tensors[tid].data,
+                           (float*)tensors[o].data, (float*)tensors[row_loss].data, (float*)tensors[lse].data, ws, d.rows, d.k,
+                           d.vocab, -1, normalizer, bad_id_dev + 1, status_dev),
+       "linear_cross_entropy");
+    prof_end();
+  }
+  if (!no_grad) {
+    tape.push_back({{h, w}, o, [this, h, w, tid, lse, o, d, ldw, trans_b, piece, normalizer]() {
+      OUT_GRAD_OR_RETURN(o);
+      const bool dw = !tensors[w].constant;
+      ensure_grad(h);
+      if (dw) ensure_grad(w);
+      HTensor& gh = tensors[h];
+      HTensor& gw = tensors[w];
+      if (gh.grad_dtype != 1) invalid("linear_cross_entropy: the hidden-state gradient must be bf16");
+      const size_t bytes = (size_t)eisen_linear_ce_workspace_bytes(d.rows, d.k, d.vocab, piece, 1);
+      void* ws = pool_get(bytes);
+      struct Release { Graph& g; void* p; size_t b; ~Release() { g.pool_put(p, b); } } release{*this, ws, bytes};
+      prof_begin(0, (dw ? 6.0 : 4.0) * (double)d.rows * (double)d.k * (double)d.vocab);
+      ck(eisen_linear_ce_bwd(stream, operand(gh), d.k, operand(gw), ldw, trans_b, (const int*)tensors[tid].data,
+                             (const float*)tensors[lse].data, (const float*)to.grad, gh.grad, gh.grad_init, dw ? gw.grad : nullptr, ldw,
+                             gw.grad_dtype, gw.grad_init, ws, d.rows, d.k, d.vocab, piece, -1, normalizer, status_dev),
+         "linear_cross_entropy.bwd");
+      prof_end();
+      gh.grad_init = true;
+      if (dw) gw.grad_init = true;
+    }});
+  }
+  return o;
+}
+
+void Graph::top_logits(int64_t logits, int64_t k, float temperature, int64_t out3[3]) {
+  const std::vector<int64_t> shape = tensors.at(logits).shape;
+  if (shape.empty()) invalid("top_logits: logits must be [.., vocab]");
+  const int64_t vocab = shape.back(), rows = tensors[logits].numel / std::max<int64_t>(vocab, 1);
+  if (k < 1 || k > vocab) invalid("top_logits: k must be in [1, vocab]");
+  std::vector<int64_t> ks = shape, ls = shape;
+  ks.back() = k;
+  ls.pop_back();
+  out3[0] = alloc_pooled_dtype(ks, 0);
+  out3[1] = alloc_pooled_dtype(ks, DT_I32);
+  out3[2] = alloc_pooled_dtype(ls, 0);
+  for (int i = 0; i < 3; ++i) tensors[out3[i]].constant = true;
+  ck(eisen_top_logits(stream, operand(tensors[logits]), vocab, (float*)tensors[out3[0]].data, (int*)tensors[out3[1]].data,
+                      (float*)tensors[out3[2]].data, rows, vocab, k, temperature, act_dtype()),
+     "top_logits");
+}
+
+void Graph::lm_head_top_logits(int64_t h, int64_t w, int64_t k, float temperature, bool trans_b, int64_t chunk_rows, int64_t out3[3]) {
+  const HeadShape d = head_shape("lm_head_top_logits", tensors.at(h), tensors.at(w), trans_b);
+  if (k < 1 || k > d.vocab) invalid("lm_head_top_logits: k must be in [1, vocab]");
+  if (chunk_rows <= 0 || chunk_rows > d.rows) chunk_rows = d.rows;
+  const int dt = act_dtype();
+  std::vector<int64_t> ks = tensors[h].shape, ls = ks;
+  ks.back() = k;
+  ls.pop_back();
+  out3[0] = alloc_pooled_dtype(ks, 0);
+  out3[1] = alloc_pooled_dtype(ks, DT_I32);
+  out3[2] = alloc_pooled_dtype(ls, 0);
+  for (int i = 0; i < 3; ++i) tensors[out3[i]].constant = true;
+  const size_t slab_bytes = (size_t)std::max<int64_t>(chunk_rows, 1) * d.vocab * dsize(dt);
+  void* slab = pool_get(slab_bytes);
+  struct Release { Graph& g; void* p; size_t b; ~Release() { g.pool_put(p, b); } } release{*this, slab, slab_bytes};
+  for (int64_t r0 = 0; r0 < d.rows; r0 += chunk_rows) {
+    const int64_t m = std::min(chunk_rows, d.rows - r0);
+    gemm(*this, false, !trans_b, m, d.vocab, d.k, (const char*)operand(tensors[h]) + (size_t)r0 * d.k * dsize(dt), weight_operand(w), slab,
+         dt, false);
+    ck(eisen_top_logits(stream, slab, d.vocab, (float*)tensors[out3[0]].data + r0 * k, (int*)tensors[out3[1]].data + r0 * k,
+                        (float*)tensors[out3[2]].data + r0, m, d.vocab, k, temperature, dt),
+       "lm_head_top_logits");
+  }
+}
+
+// k of a teacher whose tensors belong to `rows` rows
+static int64_t teacher_k(const Graph& g, const char* what, const Graph::Teacher& t, int64_t tid, int64_t rows) {
+  const HTensor& ids = g.tensors.at(t.ids);
+  const HTensor& lg = g.tensors.at(t.logits);
+  if (ids.dtype != DT_I32 || lg.dtype != 0 || ids.numel != lg.numel || rows <= 0 || ids.numel % rows || ids.numel == 0)
+    invalid(std::string(what) + ": the teacher's ids (int32) and logits (f32) must be [rows, k]");
+  if (t.lse >= 0 && (g.tensors.at(t.lse).dtype != 0 || g.tensors[t.lse].numel != rows))
+    invalid(std::string(what) + ": one f32 teacher log-sum-exp per row expected");
+  if (tid >= 0 && (g.tensors.at(tid).dtype != DT_I32 || g.tensors[tid].numel != rows))
+    invalid(std::string(what) + ": one int32 target per row expected");
+  return ids.numel / rows;
+}
+
+int64_t Graph::distill(int64_t logits, const Teacher& t, int64_t tid, float normalizer) {
+  const HTensor& tl = tensors.at(logits);
+  if (tl.shape.size() != 2) invalid("distill: logits must be [rows, vocab]");
+  const int64_t rows = tl.shape[0], vocab = tl.shape[1], k = teacher_k(*this, "distill", t, tid, rows);
+  const int dt = act_dtype();
+  const int64_t lse = alloc_pooled_dtype({2, rows}, 0), row_loss = alloc_pooled_dtype({rows}, 0), o = alloc_pooled_dtype({}, 0);
+  tensors[lse].constant = tensors[row_loss].constant = true;
+  const int* targets = tid >= 0 ? (const int*)tensors[tid].data : nullptr;
+  const float* t_lse = t.lse >= 0 ? (const float*)tensors[t.lse].data : nullptr;
+  ck(eisen_distill_fwd(stream, operand(tensors[logits]), vocab, (const int*)tensors[t.ids].data, (const float*)tensors[t.logits].data, t_lse,
+                       targets, (float*)tensors[o].data, (float*)tensors[row_loss].data, (float*)tensors[lse].data, rows, vocab, k, -1,
+                       t.temperature, t.kd_weight * normalizer, t.ce_weight * normalizer, dt, bad_id_dev + 1),
+     "distill");
+  if (!no_grad) {
+    tape.push_back({{logits}, o, [this, logits, t, tid, lse, o, rows, vocab, k, normalizer, dt]() {
+      OUT_GRAD_OR_RETURN(o);
+      HTensor& gl = tensors[logits];
+      ensure_grad(logits);
+      ck(eisen_distill_bwd(stream, operand(gl), vocab, (const int*)tensors[t.ids].data, (const float*)tensors[t.logits].data,
+                           t.lse >= 0 ? (const float*)tensors[t.lse].data : nullptr, tid >= 0 ? (const int*)tensors[tid].data : nullptr,
+                           (const float*)tensors[lse].data, gl.grad, vocab, (const float*)to.grad, rows, vocab, k, -1, t.temperature,
+                           t.kd_weight * normalizer, t.ce_weight * normalizer, dt, gl.grad_init),
+         "distill.bwd");
+      gl.grad_init = true;
+    }});
+  }
+  return o;
+}
+
+int64_t Graph::lm_head_distill(int64_t h, int64_t w, const Teacher& t, int64_t tid, float normalizer, bool trans_b, int64_t chunk_rows) {
+  const HeadShape d = head_shape("lm_head_distill", tensors.at(h), tensors.at(w), trans_b);
+  const int64_t k = teacher_k(*this, "lm_head_distill", t, tid, d.rows);
+  if (chunk_rows <= 0 || chunk_rows > d.rows) chunk_rows = d.rows;
+  const int dt = act_dtype();
+  const bool grads = !no_grad;
+  const int64_t row_loss = alloc_pooled_dtype({d.rows}, 0), o = alloc_pooled_dtype({}, 0);
+  tensors[row_loss].constant = true;
+  if (grads) {
+    ensure_grad(h);
+    if (!tensors[w].constant) ensure_grad(w);
+    if (tensors[h].grad_dtype != dt) invalid("lm_head_distill: the hidden-state gradient must have the activation dtype");
+  }
+  const size_t slab_bytes = (size_t)chunk_rows * d.vocab * dsize(dt);
+  void* slab = pool_get(slab_bytes);
+  struct Release { Graph& g; void* p; size_t b; ~Release() { g.pool_put(p, b); } } release{*this, slab, slab_bytes};
+  float* rl = (float*)tensors[row_loss].data;
+  for (int64_t r0 = 0; r0 < d.rows; r0 += chunk_rows) {
+    const int64_t m = std::min(chunk_rows, d.rows - r0);
+    const char* hrows = (const char*)operand(tensors[h]) + (size_t)r0 * d.k * dsize(dt);
+    gemm(*this, false, !trans_b, m, d.vocab, d.k, hrows, weight_operand(w), slab, dt, false);
+    const int* ids = (const int*)tensors[t.ids].data + r0 * k;
+    const float* tv = (const float*)tensors[t.logits].data + r0 * k;
+    const float* t_lse = t.lse >= 0 ? (const float*)tensors[t.lse].data + r0 : nullptr;
+    const int* targets = tid >= 0 ? (const int*)tensors[tid].data + r0 : nullptr;
+    const float kd = t.kd_weight * normalizer, ce = t.ce_weight * normalizer;
+    if (!grads) {
+      ck(eisen_distill_fwd(stream, slab, d.vocab, ids, tv, t_lse, targets, nullptr, rl + r0, nullptr, m, d.vocab, k, -1, t.temperature, kd, ce,
+                           dt, bad_id_dev + 1),
+         "lm_head_distill(loss)");
+      continue;
+    }
+    ck(eisen_distill_fused(stream, slab, d.vocab, ids, tv, t_lse, targets, slab, d.vocab, nullptr, rl + r0, nullptr, m, d.vocab, k, -1,
+                           t.temperature, kd, ce, 1.0f, dt, bad_id_dev + 1),
+       "lm_head_distill");
+    HTensor& gh = tensors[h];
+    char* dh = (char*)gh.grad + (size_t)r0 * d.k * dsize(gh.grad_dtype);
+    gemm(*this, false, trans_b, m, d.k, d.vocab, slab, weight_operand(w), dh, gh.grad_dtype, gh.grad_init);
+    if (!tensors[w].constant) {
+      if (!trans_b) dw_gemm(*this, true, true, d.k, d.vocab, m, hrows, slab, w);
+      else dw_gemm(*this, true, true, d.vocab, d.k, m, slab, hrows, w);
+    }
+  }
+  if (grads) tensors[h].grad_init = true;
+  ck(eisen_ce_loss_reduce(stream, rl, (float*)tensors[o].data, d.rows), "lm_head_distill(reduce)");
+  if (grads) {
+    tape.push_back({{h, w}, o, [this, o]() {
+      OUT_GRAD_OR_RETURN(o);
+      if (!to.grad_is_ones)
+        invalid("lm_head_distill: its gradients are formed in the forward with a loss gradient of 1; "
+                "the loss must be the tensor backward() starts from");
+    }});
+  }
+  return o;
+}
+
 // src/graph/ops/reduction.rs:529-719: mean over rows of -ln(p_target + 1e-8)
 int64_t Graph::cross_entropy(int64_t logits, const int64_t* targets, int64_t n) {
   for (int64_t i = 0; i < n; ++i)

@@ -178,6 +178,22 @@ class Graph {
   int64_t lm_head_cross_entropy(int64_t h, int64_t w, int64_t target_ids, float normalizer, bool trans_b,
                                 int64_t chunk_rows);
 
+  // The same loss without logits (Bf16Mixed): head projection and cross-entropy in pieces of `piece` vocabulary entries
+  // (0 = the library's choice), eisen_linear_ce_fwd here and eisen_linear_ce_bwd in the backward pass.  Any loss gradient
+  // may come in: nothing is formed ahead.
+  int64_t linear_cross_entropy(int64_t h, int64_t w, int64_t target_ids, float normalizer, bool trans_b, int64_t piece);
+  // The k largest logits of every row, their ids and the row's log-sum-exp at a temperature: {values f32 [.., k],
+  // ids int32 [.., k], lse f32 [..]}, none of which takes a gradient.  The second form works through the head in chunks of
+  // token rows, so that only a [chunk_rows, vocab] slab of logits exists.
+  void top_logits(int64_t logits, int64_t k, float temperature, int64_t out3[3]);
+  void lm_head_top_logits(int64_t h, int64_t w, int64_t k, float temperature, bool trans_b, int64_t chunk_rows, int64_t out3[3]);
+  // Distillation from a teacher's top logits (eisen_distill_*).  teacher.lse and target_ids may be -1.
+  struct Teacher { int64_t ids = -1, logits = -1, lse = -1; float temperature = 1.0f, kd_weight = 1.0f, ce_weight = 0.0f; };
+  int64_t distill(int64_t logits, const Teacher& teacher, int64_t target_ids, float normalizer);
+  // ... with the LM head, in chunks of token rows like lm_head_cross_entropy: its gradients are formed in the forward
+  int64_t lm_head_distill(int64_t h, int64_t w, const Teacher& teacher, int64_t target_ids, float normalizer, bool trans_b,
+                          int64_t chunk_rows);
+
   // event-based timing of the tensor-core kernels (class 0 GEMM, 1 attention fwd, 2 attention bwd)
   bool prof_on = false;
   struct ProfRec { cudaEvent_t a, b; double flops; int cls; };
@@ -261,6 +277,9 @@ class TransformerLM {
   TransformerLM(Graph& g, int64_t vocab, int64_t hidden, int64_t heads, int64_t kv_heads, int64_t ffn,
                 int64_t layers, bool tie);
   int64_t forward(Graph& g, int64_t x_ids);                       // :184-196
+  int64_t hidden_forward(Graph& g, int64_t x_ids);                // up to the final norm
+  // What this model, as a teacher, hands to a student: Graph::lm_head_top_logits of its last hidden states, no tape
+  void top_logits(Graph& g, int64_t x_ids, int64_t k, float temperature, int64_t chunk_rows, int64_t out3[3]);
   // skip_dead_tail: leave out the forward kernels whose results no backward node reads
   // kv_out (optional): receives the ids of the rotated key projection and of the value projection,
   // [B, S, kv_heads * head_dim] each (what a KV cache keeps)
@@ -289,6 +308,9 @@ class TransformerLM {
                            const std::function<void(int64_t)>& after_block);
   int64_t train_micro_step_dev(Graph& g, int64_t x_ids, int64_t target_ids, int64_t n_valid, bool checkpoint,
                                const std::function<void(int64_t)>& after_block);
+  // The same micro-step under the distillation loss (Graph::lm_head_distill; target_ids may be -1)
+  int64_t distill_micro_step_dev(Graph& g, int64_t x_ids, const Graph::Teacher& teacher, int64_t target_ids, int64_t n_valid,
+                                 bool checkpoint, const std::function<void(int64_t)>& after_block);
   int64_t vocab, hidden, heads, kv_heads, ffn, layers;
   bool tie;
   bool fused = true;  // fused attention / SwiGLU ops (always the reference chain in Fp32 mode when false)
@@ -303,8 +325,15 @@ class TransformerLM {
   std::function<void(int64_t)> before_block;
   bool fused_head = true;
   int64_t head_chunk_rows = 0;
+  // >= 0: train_micro_step takes Graph::linear_cross_entropy with pieces of this many vocabulary entries (0 = chosen)
+  int64_t head_piece = -1;
   int64_t emb, norm_f, head;
   std::vector<BlockParams> blocks;
+
+ private:
+  // forward up to the final norm, loss_of(hidden states) -> loss, backward
+  int64_t micro_step(Graph& g, int64_t x_ids, bool checkpoint, const std::function<void(int64_t)>& after_block,
+                     const std::function<int64_t(int64_t)>& loss_of);
 };
 
 // examples/export_hf_pipeline.rs, src/tools/huggingface.rs: model.safetensors + config.json (export_hf.cpp)

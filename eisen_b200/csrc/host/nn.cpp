@@ -232,13 +232,35 @@ int64_t TransformerLM::block_forward(Graph& g, const BlockParams& b, int64_t x, 
   return out;
 }
 
-int64_t TransformerLM::forward(Graph& g, int64_t x) {
+int64_t TransformerLM::hidden_forward(Graph& g, int64_t x) {
   int64_t h = g.gather(emb, x);
   for (int64_t l = 0; l < layers; ++l) {
     prefetch_block(g, l + 1);
     h = block_forward(g, blocks[(size_t)l], h);
   }
-  h = g.rms_norm(h, norm_f, 1e-5f);
+  return g.rms_norm(h, norm_f, 1e-5f);
+}
+
+void TransformerLM::top_logits(Graph& g, int64_t x, int64_t k, float temperature, int64_t chunk_rows, int64_t out3[3]) {
+  if (k < 1 || k > vocab) throw EisenException(EISEN_ERR_INVALID, "lm_top_logits: k must be in [1, vocab]");
+  const int64_t rows = g.tensors.at(x).numel;
+  int64_t keep[3] = {g.alloc_pooled_dtype({rows, k}, 0), g.alloc_pooled_dtype({rows, k}, DT_I32), g.alloc_pooled_dtype({rows}, 0)};
+  const int64_t sp = g.mark_save_point();
+  {
+    FlagGuard ng(g.no_grad, true);
+    int64_t made[3];
+    g.lm_head_top_logits(hidden_forward(g, x), tie ? emb : head, k, temperature, tie, chunk_rows, made);
+    for (int i = 0; i < 3; ++i) {
+      std::swap(g.tensors[keep[i]].data, g.tensors[made[i]].data);
+      g.tensors[keep[i]].constant = true;
+      out3[i] = keep[i];
+    }
+  }
+  g.restore_save_point(sp);  // the forward pass leaves nothing behind
+}
+
+int64_t TransformerLM::forward(Graph& g, int64_t x) {
+  int64_t h = hidden_forward(g, x);
   if (tie) return g.matmul_trans_b(h, emb);
   return linear_fwd(g, h, head);
 }
@@ -258,8 +280,29 @@ int64_t TransformerLM::train_micro_step(Graph& g, int64_t x, const int64_t* targ
 
 int64_t TransformerLM::train_micro_step_dev(Graph& g, int64_t x, int64_t target_ids, int64_t n_valid, bool checkpoint,
                                             const std::function<void(int64_t)>& after_block) {
-  if (g.no_grad) throw EisenException(EISEN_ERR_INVALID, "train_micro_step: graph is in no_grad mode");
   const int64_t n_targets = g.tensors.at(target_ids).numel;
+  // src/graph/ops/reduction.rs:724-737: mean over the valid rows; all rows masked -> loss 0, no gradient
+  const float normalizer = n_valid > 0 ? 1.0f / (float)n_valid : 0.0f;
+  return micro_step(g, x, checkpoint, after_block, [&](int64_t hn) {
+    if (head_piece >= 0) return g.linear_cross_entropy(hn, tie ? emb : head, target_ids, normalizer, tie, head_piece);
+    if (fused_head) return g.lm_head_cross_entropy(hn, tie ? emb : head, target_ids, normalizer, tie, head_chunk_rows);
+    int64_t logits = tie ? g.matmul_trans_b(hn, emb) : linear_fwd(g, hn, head);
+    g.reinterpret_shape(logits, {n_targets, vocab});
+    return g.ce_device(logits, target_ids, normalizer);
+  });
+}
+
+int64_t TransformerLM::distill_micro_step_dev(Graph& g, int64_t x, const Graph::Teacher& teacher, int64_t target_ids, int64_t n_valid,
+                                              bool checkpoint, const std::function<void(int64_t)>& after_block) {
+  const float normalizer = n_valid > 0 ? 1.0f / (float)n_valid : 0.0f;
+  return micro_step(g, x, checkpoint, after_block, [&](int64_t hn) {
+    return g.lm_head_distill(hn, tie ? emb : head, teacher, target_ids, normalizer, tie, head_chunk_rows);
+  });
+}
+
+int64_t TransformerLM::micro_step(Graph& g, int64_t x, bool checkpoint, const std::function<void(int64_t)>& after_block,
+                                  const std::function<int64_t(int64_t)>& loss_of) {
+  if (g.no_grad) throw EisenException(EISEN_ERR_INVALID, "train_micro_step: graph is in no_grad mode");
   const int64_t tape0 = (int64_t)g.tape.size();
   const bool stash = checkpoint && keep_attention && fused;
   struct StashScope {  // whatever happens, no stashed buffer outlives the step and the mode is off again
@@ -300,16 +343,7 @@ int64_t TransformerLM::train_micro_step_dev(Graph& g, int64_t x, int64_t target_
   block_tape[layers] = (int64_t)g.tape.size();
   if (before_block) before_block(layers);
   int64_t hn = g.rms_norm(h, norm_f, 1e-5f);
-  // src/graph/ops/reduction.rs:724-737: mean over the valid rows; all rows masked -> loss 0, no gradient
-  const float normalizer = n_valid > 0 ? 1.0f / (float)n_valid : 0.0f;
-  int64_t loss;
-  if (fused_head) {
-    loss = g.lm_head_cross_entropy(hn, tie ? emb : head, target_ids, normalizer, tie, head_chunk_rows);
-  } else {
-    int64_t logits = tie ? g.matmul_trans_b(hn, emb) : linear_fwd(g, hn, head);
-    g.reinterpret_shape(logits, {n_targets, vocab});
-    loss = g.ce_device(logits, target_ids, normalizer);
-  }
+  const int64_t loss = loss_of(hn);
 
   // ---- backward
   g.seed_grad_ones(loss);

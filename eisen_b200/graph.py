@@ -287,6 +287,41 @@ class Graph:
     def lm_head_cross_entropy(self, h, w, target_ids, n_valid, trans_b=False, chunk_rows=0):
         return self._op("lm_head_cross_entropy", h, w, target_ids, n_valid, 1 if trans_b else 0, chunk_rows)
 
+    def linear_cross_entropy(self, h, w, target_ids, n_valid, trans_b=False, piece=0):
+        """lm_head_cross_entropy without a logits slab, in pieces of the vocabulary (Bf16Mixed)."""
+        return self._op("linear_cross_entropy", h, w, target_ids, n_valid, 1 if trans_b else 0, piece)
+
+    def _op3(self, name, *args):
+        out = (C.c_longlong * 3)()
+        call("eisen_graph_" + name, self._h, *args, out)
+        return out[0], out[1], out[2]
+
+    def top_logits(self, logits, k, temperature=1.0):
+        """(values, ids, lse): the k largest logits of every row, their ids, the row's log-sum-exp at the temperature."""
+        return self._op3("top_logits", logits, k, temperature)
+
+    def lm_head_top_logits(self, h, w, k, temperature=1.0, trans_b=False, chunk_rows=0):
+        return self._op3("lm_head_top_logits", h, w, k, temperature, 1 if trans_b else 0, chunk_rows)
+
+    def distill(self, logits, teacher_ids, teacher_logits, n_valid, teacher_lse=-1, target_ids=-1, temperature=1.0, kd_weight=1.0,
+                ce_weight=0.0):
+        """Distillation loss against a teacher's top logits, with the cross-entropy of the targets beside it."""
+        return self._op("distill", logits, teacher_ids, teacher_logits, teacher_lse, target_ids, n_valid, temperature, kd_weight, ce_weight)
+
+    def lm_head_distill(self, h, w, teacher_ids, teacher_logits, n_valid, teacher_lse=-1, target_ids=-1, temperature=1.0, kd_weight=1.0,
+                        ce_weight=0.0, trans_b=False, chunk_rows=0):
+        return self._op("lm_head_distill", h, w, teacher_ids, teacher_logits, teacher_lse, target_ids, n_valid, temperature, kd_weight,
+                        ce_weight, 1 if trans_b else 0, chunk_rows)
+
+    def copy_from(self, other, i):
+        """Tensor i of another graph as an activation of this one (no gradient)."""
+        return self._op("copy_from", other._h, i)
+
+    def ids_to_cpu(self, i):
+        out = np.empty(self.numel(i), dtype=np.int32)
+        call("eisen_graph_sync_ids_to_cpu", self._h, i, out.ctypes.data)
+        return out
+
     def attention(self, q, k, v, num_heads, num_kv_heads, causal=True):
         return self._op("attention", q, k, v, num_heads, num_kv_heads, 1 if causal else 0)
 
@@ -322,6 +357,25 @@ class TransformerLM:
     def set_head_fusion(self, fused=True, chunk_rows=0):
         """Head projection + cross-entropy as one chunked op in train_micro_step (default on)."""
         call("eisen_lm_set_head_fusion", self._h, 1 if fused else 0, chunk_rows)
+
+    def set_head_pieces(self, piece=0):
+        """Head projection + cross-entropy in pieces of the vocabulary, no logits kept (None: off, 0: chosen)."""
+        call("eisen_lm_set_head_pieces", self._h, -1 if piece is None else piece)
+
+    def top_logits(self, x_id, k, temperature=1.0, chunk_rows=0):
+        """(values, ids, lse) of every position: this model as a teacher."""
+        out = (C.c_longlong * 3)()
+        call("eisen_lm_top_logits", self._h, self.g._h, x_id, k, temperature, chunk_rows, out)
+        return out[0], out[1], out[2]
+
+    def distill_micro_step_dev(self, x_id, teacher_ids, teacher_logits, n_valid, teacher_lse=-1, target_ids_id=-1, temperature=1.0,
+                               kd_weight=1.0, ce_weight=0.0, checkpoint=False, after_block=None):
+        """train_micro_step_dev under the distillation loss against a teacher's top logits (top_logits of another model)."""
+        cb = BLOCK_CB(lambda layer, user: after_block(layer)) if after_block else None
+        out = C.c_longlong()
+        call("eisen_lm_distill_micro_step_dev", self._h, self.g._h, x_id, teacher_ids, teacher_logits, teacher_lse, target_ids_id, n_valid,
+             temperature, kd_weight, ce_weight, 1 if checkpoint else 0, C.cast(cb, C.c_void_p) if cb else None, None, C.byref(out))
+        return out.value
 
     def forward(self, x_id):
         out = C.c_longlong()

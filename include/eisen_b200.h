@@ -566,6 +566,29 @@ int eisen_graph_cross_entropy_masked(void* g, long long logits, const long long*
  * eisen_graph_backward is called on (checked there).  With no_grad set only the loss is computed. */
 int eisen_graph_lm_head_cross_entropy(void* g, long long h, long long w, long long target_ids, long long n_valid,
                                       int trans_b, long long chunk_rows, long long* out);
+/* The same loss without a logits slab (Bf16Mixed): eisen_linear_ce_fwd now, eisen_linear_ce_bwd in the backward pass, in
+ * pieces of `piece` vocabulary entries (0 = chosen).  The logits are formed twice and never rounded; the loss may have any
+ * gradient.  An untied head needs a vocabulary that is a multiple of 8; a host-homed head weight is refused. */
+int eisen_graph_linear_cross_entropy(void* g, long long h, long long w, long long target_ids, long long n_valid, int trans_b,
+                                     long long piece, long long* out);
+/* eisen_top_logits as graph ops; out3 = ids of {values f32 [.., k], ids int32 [.., k], lse f32 [..]}, which take no
+ * gradient and live like activations.  The second form projects h [.., width] through the head in chunks of chunk_rows
+ * token rows (0 = all at once). */
+int eisen_graph_top_logits(void* g, long long logits, long long k, float temperature, long long* out3);
+int eisen_graph_lm_head_top_logits(void* g, long long h, long long w, long long k, float temperature, int trans_b, long long chunk_rows,
+                                   long long* out3);
+/* eisen_distill_* as graph ops: mean over n_valid rows (both weights are divided by it).  teacher_ids (int32) and
+ * teacher_logits (f32) [rows, k]; teacher_lse (f32 [rows]) and target_ids (int32 [rows], -1 = ignored) may be -1.  The second
+ * form is eisen_graph_lm_head_cross_entropy with this loss: one [chunk_rows, vocab] slab, gradients formed in the forward. */
+int eisen_graph_distill(void* g, long long logits, long long teacher_ids, long long teacher_logits, long long teacher_lse,
+                        long long target_ids, long long n_valid, float temperature, float kd_weight, float ce_weight, long long* out);
+int eisen_graph_lm_head_distill(void* g, long long h, long long w, long long teacher_ids, long long teacher_logits, long long teacher_lse,
+                                long long target_ids, long long n_valid, float temperature, float kd_weight, float ce_weight, int trans_b,
+                                long long chunk_rows, long long* out);
+int eisen_graph_sync_ids_to_cpu(void* g, long long id, int* out);   /* an id tensor to the host */
+/* A tensor of another graph (a teacher's top logits) as an activation without gradient of this one: a copy on this graph's
+ * stream, ordered behind the other stream's work so far. */
+int eisen_graph_copy_from(void* g, void* src_graph, long long src_id, long long* out);
 int eisen_graph_rms_norm(void* g, long long x, long long w, float eps, long long* out);
 int eisen_graph_rope(void* g, long long a, long long head_dim, long long* out);
 int eisen_graph_gather(void* g, long long weights, long long indices, long long* out);
@@ -597,6 +620,12 @@ int eisen_lm_set_keep_attention(void* lm, int keep);
  * eisen_graph_lm_head_cross_entropy in chunks of chunk_rows token rows (0 = all rows at once);
  * fused == 0 runs matmul + cross_entropy_masked as the reference does. */
 int eisen_lm_set_head_fusion(void* lm, int fused, long long chunk_rows);
+/* eisen_lm_train_micro_step[_dev]: piece >= 0 takes eisen_graph_linear_cross_entropy for the head and the loss (0 = the
+ * library's pieces); negative (default) leaves the choice to eisen_lm_set_head_fusion. */
+int eisen_lm_set_head_pieces(void* lm, long long piece);
+/* This model as a teacher: forward pass without a tape, then eisen_graph_lm_head_top_logits of every position.  out3 = ids of
+ * {values f32 [tokens, k], ids int32 [tokens, k], lse f32 [tokens]}; nothing else of the pass is kept. */
+int eisen_lm_top_logits(void* lm, void* g, long long x_ids, long long k, float temperature, long long chunk_rows, long long* out3);
 int eisen_lm_forward(void* lm, void* g, long long x_ids, long long* logits_out);       /* Module::forward, :184-196 */
 int eisen_lm_params(void* lm, long long* ids_out, int* n_out);                         /* Module::params, :198-210 */
 /* Greedy generation, the loop of examples/train_llm.rs:560-584: max_new_tokens times the argmax of
@@ -632,6 +661,13 @@ int eisen_lm_train_micro_step(void* lm, void* g, long long x_ids, const long lon
  * -1 for ignored rows) and their number of valid rows */
 int eisen_lm_train_micro_step_dev(void* lm, void* g, long long x_ids, long long target_ids, long long n_valid,
                                   int checkpoint, eisen_block_cb after_block, void* user, long long* loss_id);
+
+/* eisen_lm_train_micro_step_dev under the distillation loss of eisen_graph_lm_head_distill (chunks of token rows as set by
+ * eisen_lm_set_head_fusion).  The teacher's tensors come from eisen_lm_top_logits of another model by
+ * eisen_graph_copy_from, or from eisen_graph_alloc / eisen_graph_alloc_ids; teacher_lse and target_ids may be -1.  n_valid: rows that count. */
+int eisen_lm_distill_micro_step_dev(void* lm, void* g, long long x_ids, long long teacher_ids, long long teacher_logits,
+                                    long long teacher_lse, long long target_ids, long long n_valid, float temperature, float kd_weight,
+                                    float ce_weight, int checkpoint, eisen_block_cb after_block, void* user, long long* loss_id);
 
 /* Per-class device timing of the tensor-core kernels of a graph, taken with CUDA events on the
  * graph's stream around each launch while enabled.  eisen_graph_prof_read synchronises the
