@@ -21,10 +21,11 @@ int gemm_bf16_tc(cudaStream_t stream, int a_mn, int b_mn, int M, int N, int K, c
                  long long lda, const void* B, long long ldb, void* C, long long ldc, const void* R, long long ldr,
                  int out_mode, int split_k, float alpha, int* status, const char** err);
 
-// paired-CTA (cta_group::2) variant: 256 x 256 tile per cluster of two CTAs (gemm_tc2.cu)
+// paired-CTA (cta_group::2) variant: 256 x 256 tile per cluster of two CTAs (gemm_tc2.cu).  alpha_dev: a device scalar that
+// alpha is multiplied by, null for none
 int gemm_bf16_tc_pair(cudaStream_t stream, int a_mn, int b_mn, int M, int N, int K, const void* A, long long lda,
                       const void* B, long long ldb, void* C, long long ldc, const void* R, long long ldr, int out_mode,
-                      int split_k, float alpha, int* status, const char** err);
+                      int split_k, float alpha, int* status, const char** err, const float* alpha_dev = nullptr);
 // gate / up projections with the SwiGLU product in the epilogue (dual mode of the paired kernel)
 int gemm_bf16_pair_swiglu(cudaStream_t stream, int M, int N, int K, const void* A, long long lda, const void* Bg,
                           const void* Bu, long long ldb, void* G, void* U, void* H, long long ldo, int* status,
@@ -48,8 +49,7 @@ int gemm_bf16_pair_multi_n(cudaStream_t stream, int a_mn, int b_mn, int M, int K
 // logits' gradients in bf16 (grad = 1) are written, the logits are not
 int gemm_bf16_pair_ce(cudaStream_t stream, int b_mn, int M, int N, int K, const void* A, long long lda, const void* B,
                       long long ldb, int grad, const int* targets, int ignore_index, int vocab, int col_base, float2* stats,
-                      float* target_logit, const float* lse, const float* grad_out, float normalizer, void* D, long long ldd,
-                      int* status, const char** err);
+                      float* target_logit, const float* lse, void* D, long long ldd, int* status, const char** err);
 // columns of the output tile one statistics entry of gemm_bf16_pair_ce covers
 constexpr int GEMM_CE_COLS = 256;
 int gemm_pair_auto_split_k(int M, int N, int K);

@@ -56,10 +56,9 @@ struct PairParams {
   // cross-entropy epilogues (the LCE instantiations): the product is a tile of logits that is never stored
   const int* targets;
   const float* lse;       // LCE_GRAD
-  const float* grad_out;  // LCE_GRAD, device scalar, null for 1
+  const float* grad_out;  // LCE_SCALED, device scalar
   float2* stats;          // LCE_STATS: [n_tiles][M] (maximum, sum of exp(x - maximum)) of a row's 256 columns
   float* target_logit;    // LCE_STATS: [M]
-  float normalizer;
   int ignore_index, vocab, col_base;  // col_base: vocabulary index of column 0
   // segmented launches (the SEG instantiation of the kernel only).
   // K segments: the k-blocks from kseg[1] on come from the operand pair (A2, B2), those from kseg[2]
@@ -96,10 +95,12 @@ struct SegMaps {
 //   LCE_STATS: running maximum and sum of exponentials over the row's 256 f32 accumulators -> stats; the
 //     target's logit -> target_logit.  About four instructions per entry on four warps (some 1500 clocks per
 //     tile) beside 8 * K clocks of tensor-core work: hidden from K = 256 on.
-//   LCE_GRAD: (exp(x - lse) - [column is the target]) * normalizer * grad_out, rounded once to bf16 (the
-//     operand type of the two gradient products) -> C.  Rows that do not count are written as zeros whatever
-//     their accumulators hold.
-constexpr int LCE_NONE = 0, LCE_STATS = 1, LCE_GRAD = 2;
+//   LCE_GRAD: exp(x - lse) - [column is the target], rounded once to bf16 (the operand type of the two gradient
+//     products) -> C = D.  Rows that do not count are written as zeros whatever their accumulators hold.  The factor
+//     normalizer * grad_out comes in behind the products: on D it would take every target's entry, about -1, off the
+//     numbers that bf16 has, all of them by the same rounding error.
+//   LCE_SCALED: the plain epilogues with alpha times *grad_out, for the products whose operand D is.
+constexpr int LCE_NONE = 0, LCE_STATS = 1, LCE_GRAD = 2, LCE_SCALED = 3;
 constexpr float LOG2E = 1.4426950408889634f;
 
 __device__ __forceinline__ float lce_ex2(float x) {
@@ -109,12 +110,12 @@ __device__ __forceinline__ float lce_ex2(float x) {
 }
 
 // 32 accumulators of one row -> their gradients.  nl = -lse * log2(e), at = target column - first column.
-__device__ __forceinline__ void lce_grad32(uint32_t (&r)[32], float nl, float scale, bool counts, int at) {
+__device__ __forceinline__ void lce_grad32(uint32_t (&r)[32], float nl, bool counts, int at) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) {
     float d = lce_ex2(fmaf(__uint_as_float(r[i]), LOG2E, nl));
     if (i == at) d -= 1.0f;
-    r[i] = counts ? __float_as_uint(d * scale) : 0u;
+    r[i] = counts ? __float_as_uint(d) : 0u;
   }
 }
 
@@ -172,6 +173,7 @@ gemm_bf16_tc2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
   grid_launch_dependents();
   grid_dependency_wait();
 
+  const float alpha = LCE == LCE_SCALED ? p.alpha * *p.grad_out : p.alpha;
   const int tiles_mn = p.m_tiles * p.n_tiles;
   const int cluster_id = blockIdx.x >> 1;
   const int n_clusters = gridDim.x >> 1;
@@ -348,7 +350,6 @@ gemm_bf16_tc2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         const int tgt = row_ok ? p.targets[row] : -1;
         const bool counts = row_ok && tgt != p.ignore_index && tgt >= 0 && tgt < p.vocab;
         const float nl = counts ? -p.lse[row] * LOG2E : 0.0f;
-        const float scale = p.normalizer * (p.grad_out ? *p.grad_out : 1.0f);
         const int at0 = tgt - p.col_base - n0;
         if (staged) {
           uint8_t* st = epi_stage + q * (32 * 128);
@@ -361,7 +362,7 @@ gemm_bf16_tc2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
               uint32_t r[32];
               tmem_ld_32x32b_x32(taddr + c * 64 + h * 32, r);
               tmem_ld_wait();
-              lce_grad32(r, nl, scale, counts, at0 - c * 64 - h * 32);
+              lce_grad32(r, nl, counts, at0 - c * 64 - h * 32);
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
                 uint4 o;
@@ -390,7 +391,7 @@ gemm_bf16_tc2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
             tmem_ld_32x32b_x32(taddr + c * 32, r);
             tmem_ld_wait();
             if (row_ok && col0 < Nn) {
-              lce_grad32(r, nl, scale, counts, at0 - c * 32);
+              lce_grad32(r, nl, counts, at0 - c * 32);
               float v[32];
 #pragma unroll
               for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
@@ -416,16 +417,16 @@ gemm_bf16_tc2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
             tmem_ld_wait();
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              gq[i] = pack_bf16x2(__uint_as_float(r0[2 * i]) * p.alpha, __uint_as_float(r0[2 * i + 1]) * p.alpha);
-              gq[16 + i] = pack_bf16x2(__uint_as_float(r1[2 * i]) * p.alpha, __uint_as_float(r1[2 * i + 1]) * p.alpha);
+              gq[i] = pack_bf16x2(__uint_as_float(r0[2 * i]) * alpha, __uint_as_float(r0[2 * i + 1]) * alpha);
+              gq[16 + i] = pack_bf16x2(__uint_as_float(r1[2 * i]) * alpha, __uint_as_float(r1[2 * i + 1]) * alpha);
             }
             tmem_ld_32x32b_x32(taddr + PN / 2 + c * 64, r0);
             tmem_ld_32x32b_x32(taddr + PN / 2 + c * 64 + 32, r1);
             tmem_ld_wait();
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              uq[i] = pack_bf16x2(__uint_as_float(r0[2 * i]) * p.alpha, __uint_as_float(r0[2 * i + 1]) * p.alpha);
-              uq[16 + i] = pack_bf16x2(__uint_as_float(r1[2 * i]) * p.alpha, __uint_as_float(r1[2 * i + 1]) * p.alpha);
+              uq[i] = pack_bf16x2(__uint_as_float(r0[2 * i]) * alpha, __uint_as_float(r0[2 * i + 1]) * alpha);
+              uq[16 + i] = pack_bf16x2(__uint_as_float(r1[2 * i]) * alpha, __uint_as_float(r1[2 * i + 1]) * alpha);
             }
           }
 #pragma unroll
@@ -497,8 +498,8 @@ gemm_bf16_tc2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
               for (int i = 0; i < 8; ++i) {
                 const int rw = 4 * i + rr;
                 const uint4 x = *reinterpret_cast<const uint4*>(st + rw * 128 + ((seg ^ (rw & 7)) << 4));
-                const float x0 = __uint_as_float(x.x) * p.alpha, y0 = __uint_as_float(x.y) * p.alpha;
-                const float x1 = __uint_as_float(x.z) * p.alpha, y1 = __uint_as_float(x.w) * p.alpha;
+                const float x0 = __uint_as_float(x.x) * alpha, y0 = __uint_as_float(x.y) * alpha;
+                const float x1 = __uint_as_float(x.z) * alpha, y1 = __uint_as_float(x.w) * alpha;
                 const float c0 = __uint_as_float(ang[i].x), s0 = __uint_as_float(ang[i].y);
                 const float c1 = __uint_as_float(ang[i].z), s1 = __uint_as_float(ang[i].w);
                 uint2 o;
@@ -513,15 +514,15 @@ gemm_bf16_tc2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             uint4 o;
-            o.x = pack_bf16x2(__uint_as_float(r0[8 * j + 0]) * p.alpha, __uint_as_float(r0[8 * j + 1]) * p.alpha);
-            o.y = pack_bf16x2(__uint_as_float(r0[8 * j + 2]) * p.alpha, __uint_as_float(r0[8 * j + 3]) * p.alpha);
-            o.z = pack_bf16x2(__uint_as_float(r0[8 * j + 4]) * p.alpha, __uint_as_float(r0[8 * j + 5]) * p.alpha);
-            o.w = pack_bf16x2(__uint_as_float(r0[8 * j + 6]) * p.alpha, __uint_as_float(r0[8 * j + 7]) * p.alpha);
+            o.x = pack_bf16x2(__uint_as_float(r0[8 * j + 0]) * alpha, __uint_as_float(r0[8 * j + 1]) * alpha);
+            o.y = pack_bf16x2(__uint_as_float(r0[8 * j + 2]) * alpha, __uint_as_float(r0[8 * j + 3]) * alpha);
+            o.z = pack_bf16x2(__uint_as_float(r0[8 * j + 4]) * alpha, __uint_as_float(r0[8 * j + 5]) * alpha);
+            o.w = pack_bf16x2(__uint_as_float(r0[8 * j + 6]) * alpha, __uint_as_float(r0[8 * j + 7]) * alpha);
             *reinterpret_cast<uint4*>(st + lane * 128 + ((j ^ (lane & 7)) << 4)) = o;
-            o.x = pack_bf16x2(__uint_as_float(r1[8 * j + 0]) * p.alpha, __uint_as_float(r1[8 * j + 1]) * p.alpha);
-            o.y = pack_bf16x2(__uint_as_float(r1[8 * j + 2]) * p.alpha, __uint_as_float(r1[8 * j + 3]) * p.alpha);
-            o.z = pack_bf16x2(__uint_as_float(r1[8 * j + 4]) * p.alpha, __uint_as_float(r1[8 * j + 5]) * p.alpha);
-            o.w = pack_bf16x2(__uint_as_float(r1[8 * j + 6]) * p.alpha, __uint_as_float(r1[8 * j + 7]) * p.alpha);
+            o.x = pack_bf16x2(__uint_as_float(r1[8 * j + 0]) * alpha, __uint_as_float(r1[8 * j + 1]) * alpha);
+            o.y = pack_bf16x2(__uint_as_float(r1[8 * j + 2]) * alpha, __uint_as_float(r1[8 * j + 3]) * alpha);
+            o.z = pack_bf16x2(__uint_as_float(r1[8 * j + 4]) * alpha, __uint_as_float(r1[8 * j + 5]) * alpha);
+            o.w = pack_bf16x2(__uint_as_float(r1[8 * j + 6]) * alpha, __uint_as_float(r1[8 * j + 7]) * alpha);
             *reinterpret_cast<uint4*>(st + lane * 128 + (((j + 4) ^ (lane & 7)) << 4)) = o;
           }
           __syncwarp();
@@ -565,7 +566,7 @@ gemm_bf16_tc2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         if (row_ok && col0 < Nn && has_k) {
           float v[32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]) * p.alpha;
+          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]) * alpha;
           gemm_store_chunk32(Cp, ldc, Rp, ldr, out_mode, row, col0, Nn, v, pre_cur, have_cur);
         }
 #pragma unroll
@@ -633,6 +634,8 @@ static int pair_launch(cudaStream_t stream, const CUtensorMap& tmA, const CUtens
       e = cudaFuncSetAttribute(gemm_bf16_tc2_kernel<false, LCE_STATS>, cudaFuncAttributeMaxDynamicSharedMemorySize, P_SMEM);
     if (e == cudaSuccess)
       e = cudaFuncSetAttribute(gemm_bf16_tc2_kernel<false, LCE_GRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, P_SMEM);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(gemm_bf16_tc2_kernel<false, LCE_SCALED>, cudaFuncAttributeMaxDynamicSharedMemorySize, P_SMEM);
     if (e != cudaSuccess) { if (err) *err = cudaGetErrorString(e); return 3; }
     attr_set[slot] = true;
   }
@@ -667,6 +670,7 @@ static int pair_launch(cudaStream_t stream, const CUtensorMap& tmA, const CUtens
   cudaError_t e;
   if (lce == LCE_STATS) e = cudaLaunchKernelEx(&cfg, gemm_bf16_tc2_kernel<false, LCE_STATS>, tmA, tmB, tmB2, no_seg, p);
   else if (lce == LCE_GRAD) e = cudaLaunchKernelEx(&cfg, gemm_bf16_tc2_kernel<false, LCE_GRAD>, tmA, tmB, tmB2, no_seg, p);
+  else if (lce == LCE_SCALED) e = cudaLaunchKernelEx(&cfg, gemm_bf16_tc2_kernel<false, LCE_SCALED>, tmA, tmB, tmB2, no_seg, p);
   else e = seg ? cudaLaunchKernelEx(&cfg, gemm_bf16_tc2_kernel<true>, tmA, tmB, tmB2, *seg, p)
                : cudaLaunchKernelEx(&cfg, gemm_bf16_tc2_kernel<false>, tmA, tmB, tmB2, no_seg, p);
   if (e != cudaSuccess) { if (err) *err = cudaGetErrorString(e); return 3; }
@@ -835,7 +839,7 @@ int gemm_bf16_pair_multi_n(cudaStream_t stream, int a_mn, int b_mn, int M, int K
 
 int gemm_bf16_tc_pair(cudaStream_t stream, int a_mn, int b_mn, int M, int N, int K, const void* A, long long lda,
                       const void* B, long long ldb, void* C, long long ldc, const void* R, long long ldr, int out_mode, int split_k,
-                      float alpha, int* status, const char** err) {
+                      float alpha, int* status, const char** err, const float* alpha_dev) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
   if ((lda % 8) || (ldb % 8) || (reinterpret_cast<uintptr_t>(A) & 15) || (reinterpret_cast<uintptr_t>(B) & 15)) {
     if (err) *err = "gemm_bf16_tc: operand rows must be 16-byte aligned (leading dimension % 8 == 0)";
@@ -873,7 +877,8 @@ int gemm_bf16_tc_pair(cudaStream_t stream, int a_mn, int b_mn, int M, int N, int
   p.status = status;
   p.dual = 0; p.C2 = nullptr; p.H = nullptr;
   p.rope_tab = nullptr; p.rope_s = 1; p.rope_hd = 2;
-  return pair_launch(stream, tmA, tmB, tmB, p, err);
+  p.grad_out = alpha_dev;
+  return pair_launch(stream, tmA, tmB, tmB, p, err, nullptr, alpha_dev ? LCE_SCALED : LCE_NONE);
 }
 
 // Gate / up projections with the SwiGLU product in the epilogue (dual mode of the kernel):
@@ -961,8 +966,7 @@ int gemm_bf16_pair_rope(cudaStream_t stream, int M, int N, int K, const void* A,
 // `B` pointing at the first of them.  grad = 0: stats / target_logit are written; grad != 0: D [M, N] bf16.
 int gemm_bf16_pair_ce(cudaStream_t stream, int b_mn, int M, int N, int K, const void* A, long long lda, const void* B,
                       long long ldb, int grad, const int* targets, int ignore_index, int vocab, int col_base, float2* stats,
-                      float* target_logit, const float* lse, const float* grad_out, float normalizer, void* D, long long ldd,
-                      int* status, const char** err) {
+                      float* target_logit, const float* lse, void* D, long long ldd, int* status, const char** err) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
   CUtensorMap tmA, tmB;
   if (make_tmap_bf16_2d(&tmA, A, K, M, lda, 64, PM)) { if (err) *err = "linear_ce: cuTensorMapEncodeTiled failed for h"; return 2; }
@@ -985,7 +989,7 @@ int gemm_bf16_pair_ce(cudaStream_t stream, int b_mn, int M, int N, int K, const 
   p.status = status;
   p.targets = targets; p.ignore_index = ignore_index; p.vocab = vocab; p.col_base = col_base;
   p.stats = stats; p.target_logit = target_logit;
-  p.lse = lse; p.grad_out = grad_out; p.normalizer = normalizer;
+  p.lse = lse;
   return pair_launch(stream, tmA, tmB, tmB, p, err, nullptr, grad ? LCE_GRAD : LCE_STATS);
 }
 

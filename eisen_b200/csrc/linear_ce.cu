@@ -4,9 +4,9 @@
 //             the f32 accumulators in the GEMM's epilogue (gemm_tc2.cu, LCE_STATS); ce_join_kernel adds them up:
 //             lse = M + ln sum_t s_t exp(m_t - M),  row loss = -ln(exp(x_y - lse) + 1e-8) * normalizer.
 //             2 rows k vocab FLOPs, 8 bytes per row and tile instead of 512 for the logits.
-//   backward  per piece of the vocabulary the tile is formed again and leaves
-//             D = (exp(x - lse) - onehot) * normalizer * grad  in bf16 (LCE_GRAD), then dH += D W^T and dW = H^T D
-//             by the library's GEMM.  8 rows k vocab FLOPs (6 with the logits at hand).
+//   backward  per piece of the vocabulary the tile is formed again and leaves D = exp(x - lse) - onehot in bf16
+//             (LCE_GRAD), then dH += c D W^T and dW = c H^T D with c = normalizer * grad by the library's GEMM.
+//             8 rows k vocab FLOPs (6 with the logits at hand).
 //
 // The row statistics come from unrounded logits; a [rows, vocab] tensor of bf16 logits carries a rounding of up to
 // 2^-9 of a logit, 3 % of a probability at |x| = 16.  D is the one value rounded to bf16 on the way to the
@@ -148,7 +148,7 @@ int eisen_linear_ce_fwd(void* stream, const void* h, long long ldh, const void* 
   float* target_logit = (float*)((char*)workspace + p.stats_bytes);
   const char* err = nullptr;
   rc = gemm_bf16_pair_ce((cudaStream_t)stream, trans_b ? 0 : 1, (int)rows, (int)vocab, (int)k, h, ldh, w, ldw, 0, targets,
-                         ignore_index, (int)vocab, 0, stats, target_logit, nullptr, nullptr, 0.0f, nullptr, 0, status, &err);
+                         ignore_index, (int)vocab, 0, stats, target_logit, nullptr, nullptr, 0, status, &err);
   if (rc) return fail(EISEN_ERR_CUDA, err ? err : "linear_ce_fwd failed");
   count_launch();
   const unsigned grid = (unsigned)((rows + CJ_ROWS - 1) / CJ_ROWS);
@@ -186,28 +186,35 @@ int eisen_linear_ce_bwd(void* stream, const void* h, long long ldh, const void* 
   float* dh32 = (float*)(d + p.d_bytes);
   if (dh && p.dh_f32 && cudaMemsetAsync(dh32, 0, (size_t)rows * k * 4, s) != cudaSuccess)
     return fail(EISEN_ERR_CUDA, "linear_ce_bwd: memset");
+  // C (op)= normalizer * (*grad_out) * A B^T on the paired-CTA kernel, whatever the size: its k slices fill the machine
+  auto product = [&](int a_mn, int b_mn, long long M, long long N, long long K, const void* A, long long lda, const void* B,
+                     long long ldb, void* C, long long ldc, int mode) {
+    const int split = mode == GEMM_OUT_F32_ATOMIC && !deterministic() ? gemm_pair_auto_split_k((int)M, (int)N, (int)K) : 1;
+    const char* err = nullptr;
+    if (gemm_bf16_tc_pair(s, a_mn, b_mn, (int)M, (int)N, (int)K, A, lda, B, ldb, C, ldc, nullptr, 0, mode, split, normalizer, status, &err,
+                          grad_out))
+      return fail(EISEN_ERR_CUDA, err ? err : "linear_ce_bwd failed");
+    count_launch();
+    return 0;
+  };
   for (long long c0 = 0; c0 < vocab; c0 += p.piece) {
     const long long n = std::min(p.piece, vocab - c0);
     const char* wp = (const char*)w + 2 * (trans_b ? c0 * ldw : c0);
     const char* err = nullptr;
     rc = gemm_bf16_pair_ce(s, trans_b ? 0 : 1, (int)rows, (int)n, (int)k, h, ldh, wp, ldw, 1, targets, ignore_index, (int)vocab,
-                           (int)c0, nullptr, nullptr, lse, grad_out, normalizer, d, p.ld, status, &err);
+                           (int)c0, nullptr, nullptr, lse, d, p.ld, status, &err);
     if (rc) return fail(EISEN_ERR_CUDA, err ? err : "linear_ce_bwd failed");
     count_launch();
     if (dh) {  // dH[rows, k] += D[rows, n] W_piece^T
-      rc = p.dh_f32 ? eisen_gemm_bf16(stream, 0, trans_b ? 1 : 0, rows, k, n, d, p.ld, wp, ldw, dh32, k, GEMM_OUT_F32_ATOMIC, 0,
-                                      1.0f, status)
-                    : eisen_gemm_bf16(stream, 0, trans_b ? 1 : 0, rows, k, n, d, p.ld, wp, ldw, dh, k,
-                                      accumulate_dh ? GEMM_OUT_BF16_ACC : GEMM_OUT_BF16, 1, 1.0f, status);
+      const int mode = p.dh_f32 ? GEMM_OUT_F32_ATOMIC : accumulate_dh ? GEMM_OUT_BF16_ACC : GEMM_OUT_BF16;
+      rc = product(0, trans_b ? 1 : 0, rows, k, n, d, p.ld, wp, ldw, p.dh_f32 ? (void*)dh32 : dh, k, mode);
       if (rc) return rc;
     }
     if (dw) {  // dW[k, piece] = H^T D, or with the tied table dW[piece, k] = D^T H
       char* out = (char*)dw + (dw_dtype == DT_F32 ? 4 : 2) * (trans_b ? c0 * lddw : c0);
       const int mode = dw_dtype == DT_F32 ? (accumulate_dw ? GEMM_OUT_F32_ATOMIC : GEMM_OUT_F32)
                                           : (accumulate_dw ? GEMM_OUT_BF16_ACC : GEMM_OUT_BF16);
-      const int split = mode == GEMM_OUT_F32_ATOMIC ? 0 : 1;
-      rc = trans_b ? eisen_gemm_bf16(stream, 1, 1, n, k, rows, d, p.ld, h, ldh, out, lddw, mode, split, 1.0f, status)
-                   : eisen_gemm_bf16(stream, 1, 1, k, n, rows, h, ldh, d, p.ld, out, lddw, mode, split, 1.0f, status);
+      rc = trans_b ? product(1, 1, n, k, rows, d, p.ld, h, ldh, out, lddw, mode) : product(1, 1, k, n, rows, h, ldh, d, p.ld, out, lddw, mode);
       if (rc) return rc;
     }
   }

@@ -343,8 +343,8 @@ int eisen_distill_fused(void* stream, const void* logits, long long ld, const in
  * ldw.  targets, ignore_index, normalizer, loss, row_loss, lse and bad_target_flag as in eisen_ce_fwd (lse is required).
  * The backward forms the logits again, `piece` vocabulary entries at a time (rounded to a multiple of 256; 0 = chosen
  * so that one [rows, piece] bf16 slab takes about 256 MB), and
- *   dh [rows, k] bf16 (op)= D W^T,  dw (layout of w, leading dimension lddw, dw_dtype EISEN_BF16 or EISEN_F32) (op)= H^T D,
- *   D = bf16((softmax(x) - onehot) * normalizer * (*grad_out)), zero for rows that do not count; dh or dw may be null.
+ *   dh [rows, k] bf16 (op)= c D W^T,  dw (layout of w, leading dimension lddw, dw_dtype EISEN_BF16 or EISEN_F32) (op)= c H^T D,
+ *   D = bf16(softmax(x) - onehot), zero for rows that do not count, c = normalizer * (*grad_out); dh or dw may be null.
  * Sums over tokens and vocabulary are f32; dh is added up in f32 over the pieces and rounded once.  Hidden states of
  * rows that do not count must be finite where dw is asked for (their zero gradient multiplies them).
  * ldh and ldw must be multiples of 8, k one of 8 in the backward; h, w, dh, dw and workspace 16-byte aligned.
