@@ -868,6 +868,140 @@ distill_pipe_kernel(const DistillParams p) {
   }
 }
 
+// The loss alone: nothing has to be kept of a row, so it is not staged.  A CTA of 256 threads reads it once, four
+// vectors of every thread in flight, with a running maximum and sums that are brought to a new maximum four vectors at
+// a time; up to six CTAs per SM cover each other's latencies (the entries' gathers, four reductions).
+constexpr int DF_THREADS = 256, DF_FLIGHT = 4;
+
+template <typename T>
+__global__ void __launch_bounds__(DF_THREADS, 5)
+distill_stream_kernel(const DistillParams p) {
+  constexpr int V = VecOf<T>::N, WARPS = DF_THREADS / 32;
+  __shared__ float s_t[DS_MAX_K], s_x[DS_MAX_K];
+  __shared__ float s_red[4][WARPS];
+  const long long row = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = p.vocab, k = p.k;
+  const T* xr = reinterpret_cast<const T*>(p.logits) + row * p.ld;
+  const int y = p.targets ? p.targets[row] : -1;
+  const bool ignored = p.targets && y == p.ignore_index;
+  const bool out = p.targets && !ignored && (y < 0 || y >= n);
+  if (ignored || out) {
+    if (tid == 0) {
+      p.row_loss[row] = 0.0f;
+      if (p.lse) { p.lse[row] = 0.0f; p.lse[p.rows + row] = 0.0f; }
+      if (out && p.bad_id_flag) *p.bad_id_flag = 1;
+    }
+    return;
+  }
+  // the teacher's entries, absent ones at -inf
+  float tm = -INFINITY;
+  for (int j = tid; j < k; j += DF_THREADS) {
+    int id = p.t_ids[row * k + j];
+    float t = p.t_logits[row * k + j] * p.inv_t;
+    if (id >= n) {
+      if (p.bad_id_flag) *p.bad_id_flag = 1;
+      id = -1;
+    }
+    if (id < 0) t = -INFINITY;
+    s_t[j] = t;
+    s_x[j] = id >= 0 ? to_f32(xr[id]) : 0.0f;
+    tm = fmaxf(tm, t);
+  }
+  const float xy = tid == 0 && y >= 0 ? to_f32(xr[y]) : 0.0f;
+  const RowSlice<T> s(xr, n, 0, 0);
+  float m = -INFINITY, st = 0.0f, s1 = 0.0f;
+#pragma unroll 1
+  for (int v0 = tid; v0 < s.hi; v0 += DF_FLIGHT * DF_THREADS) {
+    uint4 raw[DF_FLIGHT];
+#pragma unroll
+    for (int q = 0; q < DF_FLIGHT; ++q) {
+      const int v = v0 + q * DF_THREADS;
+      constexpr uint32_t low = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
+      raw[q] = make_uint4(low, low, low, low);
+      if (v >= s.w0 && v < s.w1) {
+        asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(raw[q].x), "=r"(raw[q].y), "=r"(raw[q].z), "=r"(raw[q].w)
+                     : "l"(s.base + (long long)v * V));
+      } else if (v < s.hi) {
+        raw[q] = s.load_edge(v);
+      }
+    }
+    float bm = m;
+#pragma unroll
+    for (int q = 0; q < DF_FLIGHT; ++q) {
+      float x[V];
+      unpack_vec<T>(raw[q], x);
+#pragma unroll
+      for (int c = 0; c < V; ++c) bm = fmaxf(bm, x[c]);
+    }
+    const float ref = bm == -INFINITY ? 0.0f : bm;
+    if (bm > m) {
+      st *= m == -INFINITY ? 0.0f : expf((m - ref) * p.inv_t);  // a NaN of st stays one
+      s1 *= m == -INFINITY ? 0.0f : expf(m - ref);
+      m = bm;
+    }
+    with_exp<T>(p.sum_kind, ref, p.inv_t, [&](const auto& ex) {
+      using Ex = std::remove_cv_t<std::remove_reference_t<decltype(ex)>>;
+      float sa[2] = {0.0f, 0.0f}, sb[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int q = 0; q < DF_FLIGHT; ++q) {
+        float x[V];
+        unpack_vec<T>(raw[q], x);
+#pragma unroll
+        for (int c = 0; c < V; c += 2) {
+          float et[2], e1[2];
+          ex.both(x[c], x[c + 1], et, e1);
+          fadd2(sa[0], sa[1], sa[0], sa[1], et[0], et[1]);
+          if constexpr (Ex::BOTH) fadd2(sb[0], sb[1], sb[0], sb[1], e1[0], e1[1]);
+        }
+      }
+      st += (sa[0] + sa[1]) * Ex::scale_t;
+      s1 += (sb[0] + sb[1]) * Ex::scale_1;
+    });
+  }
+  // maxima, then the sums relative to them
+  const float wm = warp_max(m);
+  tm = warp_max(tm);
+  if (lane == 0) { s_red[0][warp] = wm; s_red[1][warp] = tm; }
+  __syncthreads();
+  const float gm = lanes_max<WARPS>(s_red[0][lane % WARPS]), ref = gm == -INFINITY ? 0.0f : gm;
+  float tref = lanes_max<WARPS>(s_red[1][lane % WARPS]);
+  if (p.t_lse) tref = p.t_lse[row];
+  else if (tref == -INFINITY) tref = 0.0f;
+  const float mine = m == -INFINITY ? 0.0f : m - ref;
+  st = warp_sum(st * expf(mine * p.inv_t));
+  s1 = warp_sum(s1 * expf(mine));
+  float S = 0.0f;
+  for (int j = tid; j < k; j += DF_THREADS) S += expf(s_t[j] - tref);
+  S = warp_sum(S);
+  __syncthreads();
+  if (lane == 0) { s_red[0][warp] = st; s_red[1][warp] = s1; s_red[2][warp] = S; }
+  __syncthreads();
+  st = lanes_sum<WARPS>(s_red[0][lane % WARPS]);
+  s1 = lanes_sum<WARPS>(s_red[1][lane % WARPS]);
+  S = lanes_sum<WARPS>(s_red[2][lane % WARPS]);
+  const float lt = ref * p.inv_t + logf(st);
+  const float l1 = p.sum_kind == ONE ? (p.temperature == 1.0f ? lt : 0.0f) : ref + logf(s1);
+  const float tl = p.t_lse || S == 0.0f ? tref : tref + logf(S);  // ln q_j = t_j - tl
+  float kl = 0.0f;
+  for (int j = tid; j < k; j += DF_THREADS) {
+    const float q = expf(s_t[j] - tl);
+    if (q > 0.0f || q != q) kl += q * (s_t[j] - tl - (s_x[j] * p.inv_t - lt));
+  }
+  kl = warp_sum(kl);
+  if (lane == 0) s_red[3][warp] = kl;
+  __syncthreads();
+  if (tid == 0) {
+    kl = 0.0f;
+    for (int w = 0; w < WARPS; ++w) kl += s_red[3][w];
+    float l = 0.0f;
+    if (p.kd_weight != 0.0f) l = p.kd_weight * p.temperature * p.temperature * kl;
+    if (p.ce_weight != 0.0f) l -= p.ce_weight * logf(expf(xy - l1) + 1e-8f);
+    p.row_loss[row] = l;
+    if (p.lse) { p.lse[row] = lt; p.lse[p.rows + row] = l1; }
+  }
+}
+
 int distill_check(const char* what, const DistillParams& p, int dtype, bool bwd) {
   static thread_local char msg[160];
   auto bad = [&](int code, const char* why) {
@@ -905,17 +1039,19 @@ int distill_launch(const char* what, DistillParams& p, cudaStream_t s) {
     p.shape = row_shape(p.rows, p.vocab, sizeof(T), groups * entry_bytes(p.k), std::max(2 * groups, 3), least);
     return p.shape.stages >= groups;
   };
+  if constexpr (MODE == DS_FWD) {
+    // rows in numbers, or too long to be staged
+    if (p.rows > 2LL * sm_count() || !shape(1, 8192)) {
+      distill_stream_kernel<T><<<(unsigned)p.rows, DF_THREADS, 0, s>>>(p);
+      return check_launch(what);
+    }
+  }
   if (p.rows > 2LL * sm_count()) {
     if (bytes <= 4096 && shape(8, 1 << 30))
       return launch_pipe<distill_pipe_kernel<T, 32, 8, MODE>>(what, p.shape, p.rows, pipe_threads(32, 8), s, p);
     if (bytes <= 24 * 1024 && shape(4, 1 << 30))
       return launch_pipe<distill_pipe_kernel<T, 128, 4, MODE>>(what, p.shape, p.rows, pipe_threads(128, 4), s, p);
-    // where nothing is written three groups leave no stage idle; a gradient wants one that is being filled
-    if constexpr (MODE == DS_FWD) {
-      if (shape(3, 1 << 30)) return launch_pipe<distill_pipe_kernel<T, 128, 3, MODE>>(what, p.shape, p.rows, pipe_threads(128, 3), s, p);
-    } else {
-      if (shape(2, 1 << 30)) return launch_pipe<distill_pipe_kernel<T, 256, 2, MODE>>(what, p.shape, p.rows, pipe_threads(256, 2), s, p);
-    }
+    if (shape(2, 1 << 30)) return launch_pipe<distill_pipe_kernel<T, 256, 2, MODE>>(what, p.shape, p.rows, pipe_threads(256, 2), s, p);
   }
   if (shape(1, 8192)) return launch_pipe<distill_pipe_kernel<T, 512, 1, MODE>>(what, p.shape, p.rows, pipe_threads(512, 1), s, p);
   distill_kernel<T, MODE><<<(unsigned)p.rows, DS_THREADS, 0, s>>>(p);
