@@ -868,13 +868,13 @@ distill_pipe_kernel(const DistillParams p) {
   }
 }
 
-// The loss alone: nothing has to be kept of a row, so it is not staged.  A CTA of 256 threads reads it once, four
-// vectors of every thread in flight, with a running maximum and sums that are brought to a new maximum four vectors at
-// a time; up to six CTAs per SM cover each other's latencies (the entries' gathers, four reductions).
-constexpr int DF_THREADS = 256, DF_FLIGHT = 4;
+// The loss alone: nothing has to be kept of a row, so it is not staged.  A CTA reads it once, four vectors of every
+// thread in flight, with a running maximum and sums that are brought to a new maximum four vectors at a time; five CTAs
+// per SM (20 of 64 threads, for short rows) cover each other's latencies: the entries' gathers, the reductions.
+constexpr int DF_FLIGHT = 4;
 
-template <typename T>
-__global__ void __launch_bounds__(DF_THREADS, 5)
+template <typename T, int DF_THREADS>
+__global__ void __launch_bounds__(DF_THREADS, 1280 / DF_THREADS)
 distill_stream_kernel(const DistillParams p) {
   constexpr int V = VecOf<T>::N, WARPS = DF_THREADS / 32;
   __shared__ float s_t[DS_MAX_K], s_x[DS_MAX_K];
@@ -913,19 +913,7 @@ distill_stream_kernel(const DistillParams p) {
 #pragma unroll 1
   for (int v0 = tid; v0 < s.hi; v0 += DF_FLIGHT * DF_THREADS) {
     uint4 raw[DF_FLIGHT];
-#pragma unroll
-    for (int q = 0; q < DF_FLIGHT; ++q) {
-      const int v = v0 + q * DF_THREADS;
-      constexpr uint32_t low = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
-      raw[q] = make_uint4(low, low, low, low);
-      if (v >= s.w0 && v < s.w1) {
-        asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(raw[q].x), "=r"(raw[q].y), "=r"(raw[q].z), "=r"(raw[q].w)
-                     : "l"(s.base + (long long)v * V));
-      } else if (v < s.hi) {
-        raw[q] = s.load_edge(v);
-      }
-    }
+    load_vectors<T>(s, v0, DF_THREADS, raw);
     float bm = m;
 #pragma unroll
     for (int q = 0; q < DF_FLIGHT; ++q) {
@@ -1042,7 +1030,8 @@ int distill_launch(const char* what, DistillParams& p, cudaStream_t s) {
   if constexpr (MODE == DS_FWD) {
     // rows in numbers, or too long to be staged
     if (p.rows > 2LL * sm_count() || !shape(1, 8192)) {
-      distill_stream_kernel<T><<<(unsigned)p.rows, DF_THREADS, 0, s>>>(p);
+      if (bytes <= 8192) distill_stream_kernel<T, 64><<<(unsigned)p.rows, 64, 0, s>>>(p);
+      else distill_stream_kernel<T, 256><<<(unsigned)p.rows, 256, 0, s>>>(p);
       return check_launch(what);
     }
   }

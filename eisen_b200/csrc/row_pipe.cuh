@@ -83,6 +83,25 @@ struct RowSlice {
   }
 };
 
+// N vectors of a row, `step` apart, all in flight together; -inf in the places that are not in the slice.  Past the L1
+// cache: a row does not fit there.
+template <typename T, int N>
+__device__ __forceinline__ void load_vectors(const RowSlice<T>& s, int v0, int step, uint4 (&raw)[N]) {
+  constexpr uint32_t low = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
+#pragma unroll
+  for (int q = 0; q < N; ++q) {
+    const int v = v0 + q * step;
+    raw[q] = make_uint4(low, low, low, low);
+    if (v >= s.w0 && v < s.w1) {
+      asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(raw[q].x), "=r"(raw[q].y), "=r"(raw[q].z), "=r"(raw[q].w)
+                   : "l"(s.base + (long long)v * RowSlice<T>::V));
+    } else if (v < s.hi) {
+      raw[q] = s.load_edge(v);
+    }
+  }
+}
+
 // ---- clusters of CTAs that share a row
 __device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");

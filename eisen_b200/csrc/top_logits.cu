@@ -21,7 +21,6 @@
 namespace eisen {
 namespace {
 
-constexpr int TOP_THREADS = 512;
 constexpr int TOP_MAX_K = 256;
 
 struct TopParams {
@@ -462,68 +461,212 @@ top_pipe_kernel(const TopParams p) {
   }
 }
 
-// Rows beyond the shared memory of eight CTAs: read from global memory again for every digit.
-template <typename T>
-__global__ void __launch_bounds__(TOP_THREADS)
-top_long_kernel(const TopParams p) {
-  __shared__ TopSelect sel;
-  __shared__ int count;
-  __shared__ float sh[32];
-  __shared__ uint64_t cand[TOP_MAX_K];
+// Rows in numbers, or rows that no cluster holds: nothing is staged.  A CTA reads its row once for the threads' maxima and
+// the sum (a running maximum, brought up to date four vectors at a time), and again, out of the L2 cache for the most part,
+// for the elements that reach the threshold.  Five CTAs per SM (20 of 64 threads, for short rows) cover each other's
+// latencies; the staged form above has two or three rows at work on an SM.
+constexpr int TS_FLIGHT = 4;
+
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1280 / THREADS)
+top_stream_kernel(const TopParams p) {
+  constexpr int V = VecOf<T>::N, WARPS = THREADS / 32;
+  extern __shared__ __align__(16) uint64_t list[];
+  __shared__ float s_max[WARPS], s_sum[WARPS];
+  __shared__ uint32_t s_range[WARPS];
+  __shared__ int s_count, s_hits;
+  __shared__ TopSelect s_sel;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int k = p.k, n = p.vocab, cap = top_list(k);
+  int* hits = reinterpret_cast<int*>(list + cap);
   const long long row = blockIdx.x;
-  const T* xr = reinterpret_cast<const T*>(p.logits) + row * p.ld;
-  const int tid = threadIdx.x, k = p.k;
-  auto each = [&](auto f) {
-    for (int i = tid; i < p.vocab; i += TOP_THREADS) f(i, to_f32(xr[i]));
-  };
-  float m = -INFINITY;
-  each([&](int, float x) { m = fmaxf(m, x); });
-  m = block_max(m, sh);
-  const float ref = m == -INFINITY ? 0.0f : m;
-  float s = 0.0f;
-  each([&](int, float x) { s += expf((x - ref) * p.inv_t); });
-  s = block_sum(s, sh);
-  if (tid == 0) {
-    count = 0;
-    if (p.lse) p.lse[row] = ref * p.inv_t + logf(s);
-  }
-  uint32_t value, last;
-  exact_threshold<TOP_THREADS>(sel, tid, k, p.vocab, value, last, each, []() { __syncthreads(); });
-  each([&](int i, float x) {
-    const uint32_t key = order_key(x);
-    if (key > value || (key == value && (uint32_t)i <= last)) {
-      const int at = atomicAdd(&count, 1);
-      if (at < TOP_MAX_K) cand[at] = ((uint64_t)key << 32) | (uint32_t)~i;
+  const RowSlice<T> s(reinterpret_cast<const T*>(p.logits) + row * p.ld, n, 0, 0);
+  const float scale = 1.4426950408889634f * p.inv_t;
+  float m[TS_FLIGHT], ref = -INFINITY, sum = 0.0f;  // the shares' maxima; the running maximum without NaN, the sum
+#pragma unroll
+  for (int q = 0; q < TS_FLIGHT; ++q) m[q] = -INFINITY;
+#pragma unroll 1
+  for (int v0 = tid; v0 < s.hi; v0 += TS_FLIGHT * THREADS) {
+    uint4 raw[TS_FLIGHT];
+    load_vectors<T>(s, v0, THREADS, raw);
+    float bm = ref;
+#pragma unroll
+    for (int q = 0; q < TS_FLIGHT; ++q) {
+      const float x = vec_max<T>(raw[q]);
+      m[q] = max_nan(m[q], x);
+      bm = fmaxf(bm, x);
     }
-  });
+    if (p.lse) {
+      const float r0 = bm == -INFINITY ? 0.0f : bm;
+      if (bm > ref) {
+        sum *= ref == -INFINITY ? 0.0f : expf((ref - r0) * p.inv_t);
+        ref = bm;
+      }
+      const float off = -r0 * scale;
+      const bool far = sizeof(T) == 4 || fabsf(r0) > 1e30f;
+      float acc[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int q = 0; q < TS_FLIGHT; ++q) {
+        float x[V];
+        unpack_vec<T>(raw[q], x);
+        if (far) {
+#pragma unroll
+          for (int c = 0; c < V; ++c) acc[c & 1] += expf((x[c] - r0) * p.inv_t);
+        } else {
+#pragma unroll
+          for (int c = 0; c < V; ++c) acc[c & 1] += exp2_approx(fmaf(x[c], scale, off));
+        }
+      }
+      sum += acc[0] + acc[1];
+    } else {
+      ref = bm;
+    }
+  }
+  // ---- threshold, as above
+  const float most = max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3]));
+  const uint32_t top_key = tid < s.hi ? order_key(most) >> 16 : 0;
+  const float wm = warp_max(ref);
+  const uint32_t k_hi = __reduce_max_sync(0xffffffffu, top_key);
+  const uint32_t k_lo = __reduce_min_sync(0xffffffffu, tid < s.hi ? top_key : 0xffffu);
+  if (lane == 0) { s_max[warp] = wm; s_range[warp] = (k_hi << 16) | k_lo; }
+  if (tid == 0) { s_count = 0; s_hits = 0; }
   __syncthreads();
-  if (tid < k) {
-    const uint64_t c = cand[tid];
-    int r = 0;
-    for (int j = 0; j < k; ++j) r += cand[j] > c;
+  const float top = lanes_max<WARPS>(s_max[lane % WARPS]), base = top == -INFINITY ? 0.0f : top;
+  sum = warp_sum(sum * (ref == -INFINITY ? 1.0f : expf((ref - base) * p.inv_t)));
+  if (lane == 0) s_sum[warp] = sum;
+  uint32_t hi16 = 0, lo16 = 0xffffu;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    hi16 = max(hi16, s_range[w] >> 16);
+    lo16 = min(lo16, s_range[w] & 0xffffu);
+  }
+  const int bits = 32 - __clz(hi16 ^ lo16);
+  uint32_t tau = 0;
+  if (2 * k <= min(s.hi, THREADS)) {
+    tau = (hi16 >> bits) << bits;
+#pragma unroll 1
+    for (int bit = bits - 1; bit >= 0; --bit) {
+      const uint32_t trial = tau | (1u << bit);
+      if (__syncthreads_count(top_key >= trial) >= k) tau = trial;
+    }
+  } else if (k <= min(s.hi, TS_FLIGHT * THREADS)) {
+    uint32_t key[TS_FLIGHT];
+#pragma unroll
+    for (int q = 0; q < TS_FLIGHT; ++q) key[q] = tid + q * THREADS < s.hi ? order_key(m[q]) >> 16 : 0;
+#pragma unroll 1
+    for (int bit = 15; bit >= 0; --bit) {
+      const uint32_t trial = tau | (1u << bit);
+      int total = 0;
+#pragma unroll
+      for (int q = 0; q < TS_FLIGHT; ++q) total += __syncthreads_count(key[q] >= trial);
+      if (total >= k) tau = trial;
+    }
+  }
+  __syncthreads();  // s_sum, the counters
+  if (tid == 0 && p.lse && top != INFINITY) {
+    float all = 0.0f;
+    for (int w = 0; w < WARPS; ++w) all += s_sum[w];
+    p.lse[row] = base * p.inv_t + logf(all);
+  }
+  // ---- the vectors that hold an element at or above it
+  const float floor_value = key_value(tau << 16);
+#pragma unroll 1
+  for (int v0 = tid; v0 - tid < s.hi; v0 += 8 * TS_FLIGHT * THREADS) {
+    uint32_t noted = 0;
+#pragma unroll 1
+    for (int b = 0; b < 8; ++b) {
+      uint4 raw[TS_FLIGHT];
+      const int v = v0 + b * TS_FLIGHT * THREADS;
+      if (v >= s.hi) break;
+      load_vectors<T>(s, v, THREADS, raw);
+#pragma unroll
+      for (int q = 0; q < TS_FLIGHT; ++q) noted |= (uint32_t)(v + q * THREADS < s.hi && reaches<T>(raw[q], floor_value)) << (b * TS_FLIGHT + q);
+    }
+    int mine = __popc(noted), before = mine;
+    if (__any_sync(0xffffffffu, mine)) {
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += up;
+      }
+      int at = 0;
+      if (lane == 31) at = atomicAdd(&s_hits, before);
+      at = __shfl_sync(0xffffffffu, at, 31) + before - mine;
+      for (; noted; noted &= noted - 1, ++at)
+        if (at < cap) hits[at] = v0 + (__ffs(noted) - 1) * THREADS;
+    }
+  }
+  __syncthreads();
+  const int noted = s_hits;
+  if (noted <= cap) {
+    for (int j = tid; j < noted; j += THREADS) {
+      uint4 raw[1];
+      float x[V];
+      const int v = hits[j], e = s.first(v);
+      load_vectors<T>(s, v, 0, raw);
+      unpack_vec<T>(raw[0], x);
+      uint32_t in = 0;
+#pragma unroll
+      for (int c = 0; c < V; ++c) in |= (uint32_t)(!(x[c] < floor_value) && e + c >= 0 && e + c < n) << c;
+      int at = atomicAdd(&s_count, __popc(in));
+#pragma unroll
+      for (int c = 0; c < V; ++c)
+        if ((in >> c) & 1) {
+          if (at < cap) list[at] = ((uint64_t)order_key(x[c]) << 32) | (uint32_t)~(e + c);
+          ++at;
+        }
+    }
+  }
+  __syncthreads();
+  int listed = noted <= cap ? s_count : cap + 1;
+  if (listed > cap) {
+    auto each = [&](auto f) {
+#pragma unroll 1
+      for (int v = tid; v < s.hi; v += THREADS) {
+        uint4 raw[1];
+        float x[V];
+        load_vectors<T>(s, v, 0, raw);
+        unpack_vec<T>(raw[0], x);
+        const int e = s.first(v);
+#pragma unroll
+        for (int c = 0; c < V; ++c)
+          if (e + c >= 0 && e + c < n) f(e + c, x[c]);
+      }
+    };
+    uint32_t value, last;
+    exact_threshold<THREADS>(s_sel, tid, k, n, value, last, each, []() { __syncthreads(); });
+    if (tid == 0) s_count = 0;
+    __syncthreads();
+    each([&](int e, float x) {
+      const uint32_t q = order_key(x);
+      if (q > value || (q == value && (uint32_t)e <= last)) {
+        const int at = atomicAdd(&s_count, 1);
+        if (at < cap) list[at] = ((uint64_t)q << 32) | (uint32_t)~e;
+      }
+    });
+    __syncthreads();
+    listed = min(s_count, cap);
+  }
+  each_rank<THREADS>(list, listed, tid, [&](int r, uint64_t c) {
+    if (r >= k) return;
     const float v = key_value((uint32_t)(c >> 32));
-    if (r == 0 && p.lse && m == INFINITY) p.lse[row] = v;  // inf or NaN, where the sum ran into inf - inf
     p.values[row * k + r] = v;
     p.ids[row * k + r] = (int)~(uint32_t)c;
-  }
+    if (r == 0 && p.lse && top == INFINITY) p.lse[row] = v;  // inf or NaN, where the sum ran into inf - inf
+  });
 }
 
 template <typename T>
 int top_launch(TopParams& p, cudaStream_t s) {
   const long long bytes = (long long)p.vocab * sizeof(T);
-  auto shape = [&](int groups, int least) {
-    p.shape = row_shape(p.rows, p.vocab, sizeof(T), groups * 8 * (top_list(p.k) * 3 / 2 + TOP_MAX_K), std::max(2 * groups, 3), least);
-    return p.shape.stages >= groups;
-  };
-  if (p.rows > 2LL * sm_count()) {
-    if (bytes <= 4096 && p.k <= 32 && shape(8, 1 << 30))
-      return launch_pipe<top_pipe_kernel<T, 32, 8>>("top_logits", p.shape, p.rows, 32 * 8 + 32, s, p);
-    if (bytes <= 24 * 1024 && shape(4, 1 << 30))
-      return launch_pipe<top_pipe_kernel<T, 128, 4>>("top_logits", p.shape, p.rows, 128 * 4 + 32, s, p);
-    if (shape(3, 1 << 30)) return launch_pipe<top_pipe_kernel<T, 256, 3>>("top_logits", p.shape, p.rows, 256 * 3 + 32, s, p);
+  const int lists = 8 * (top_list(p.k) * 3 / 2);
+  // few rows: all of a CTA's threads, and up to eight CTAs, for each of them
+  if (p.rows <= 2LL * sm_count()) {
+    p.shape = row_shape(p.rows, p.vocab, sizeof(T), lists + 8 * TOP_MAX_K, 3, 8192);
+    if (p.shape.stages) return launch_pipe<top_pipe_kernel<T, 512, 1>>("top_logits", p.shape, p.rows, 512 + 32, s, p);
   }
-  if (shape(1, 8192)) return launch_pipe<top_pipe_kernel<T, 512, 1>>("top_logits", p.shape, p.rows, 512 + 32, s, p);
-  top_long_kernel<T><<<(unsigned)p.rows, TOP_THREADS, 0, s>>>(p);
+  if (bytes <= 8192) top_stream_kernel<T, 64><<<(unsigned)p.rows, 64, lists, s>>>(p);
+  else top_stream_kernel<T, 256><<<(unsigned)p.rows, 256, lists, s>>>(p);
   return check_launch("top_logits");
 }
 
