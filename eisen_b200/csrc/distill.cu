@@ -20,45 +20,8 @@
 namespace eisen {
 namespace {
 
-constexpr int DS_THREADS = 512;
 constexpr int DS_MAX_K = 1024;
 
-template <typename T>
-__device__ __forceinline__ float exp_row(float x) {
-  if constexpr (sizeof(T) == 2) return __expf(x);
-  else return expf(x);
-}
-
-// f(index, value) for every element of a row that may start at any element boundary: 16-byte reads between a
-// scalar head and a scalar tail
-template <typename T, typename F>
-__device__ __forceinline__ void for_row(const T* __restrict__ xr, int n, int tid, int threads, F f) {
-  constexpr int V = VecOf<T>::N;
-  const int head = min(n, (int)(((16 - (reinterpret_cast<uintptr_t>(xr) & 15)) & 15) / sizeof(T)));
-  if (tid < head) f(tid, to_f32(xr[tid]));
-  const int nvec = (n - head) / V;
-  for (int i = tid; i < nvec; i += threads) {
-    float v[V];
-    ld16(xr + head + i * V, v);
-#pragma unroll
-    for (int e = 0; e < V; ++e) f(head + i * V + e, v[e]);
-  }
-  const int at = head + nvec * V + tid;
-  if (at < n) f(at, to_f32(xr[at]));
-}
-
-// running maximum and sum of exp((x - m) * inv_t)
-struct OnlineSum {
-  float m = -INFINITY, s = 0.0f;
-  template <typename T>
-  __device__ __forceinline__ void add(float x, float inv_t) {
-    if (x > m) {
-      s *= m == -INFINITY ? 0.0f : exp_row<T>((m - x) * inv_t);
-      m = x;
-    }
-    s += exp_row<T>((x - (m == -INFINITY ? 0.0f : m)) * inv_t);
-  }
-};
 
 struct DistillParams {
   const void* logits;
@@ -82,140 +45,6 @@ struct DistillParams {
 };
 
 constexpr int DS_FWD = 1, DS_BWD = 2;
-
-// The entries of one row that need more than p_i: the teacher's ids and the target (entry k).
-struct RowEntries {
-  int id[DS_MAX_K + 1];    // -1: absent
-  float q[DS_MAX_K + 1];
-  float x[DS_MAX_K + 1];   // the student's logits there
-  float old[DS_MAX_K + 1]; // accumulate: what dlogits holds there
-};
-
-template <typename T, int MODE>
-__global__ void __launch_bounds__(DS_THREADS)
-distill_kernel(const DistillParams p) {
-  __shared__ RowEntries en;
-  __shared__ float sh[32];
-  const long long row = blockIdx.x;
-  const int tid = threadIdx.x, V_ = p.vocab, k = p.k;
-  const T* xr = reinterpret_cast<const T*>(p.logits) + row * p.ld;
-  T* dr = (MODE & DS_BWD) ? reinterpret_cast<T*>(p.dlogits) + row * p.ldd : nullptr;
-  const int y = p.targets ? p.targets[row] : -1;
-  const bool ignored = p.targets && y == p.ignore_index;
-  const bool out = p.targets && !ignored && (y < 0 || y >= V_);
-  if (ignored || out) {
-    if constexpr (MODE & DS_FWD) {
-      if (tid == 0) {
-        p.row_loss[row] = 0.0f;
-        if (p.lse) { p.lse[row] = 0.0f; p.lse[p.rows + row] = 0.0f; }
-        if (out && p.bad_id_flag) *p.bad_id_flag = 1;
-      }
-    }
-    if constexpr (MODE & DS_BWD) {
-      if (!p.accumulate)
-        for (int i = tid; i < V_; i += DS_THREADS) dr[i] = from_f32<T>(0.0f);
-    }
-    return;
-  }
-  // ---- the teacher's distribution
-  const float inv_t = p.inv_t;
-  float tm = -INFINITY;
-  for (int j = tid; j <= k; j += DS_THREADS) {
-    int id = j < k ? p.t_ids[row * k + j] : y;
-    if (j < k && id >= V_) {
-      if ((MODE & DS_FWD) && p.bad_id_flag) *p.bad_id_flag = 1;
-      id = -1;
-    }
-    id = id < 0 ? -1 : id;
-    float t = -INFINITY;
-    if (j < k && id >= 0) t = p.t_logits[row * k + j] * inv_t;
-    en.id[j] = id;
-    en.q[j] = t;
-    en.x[j] = id >= 0 ? to_f32(xr[id]) : 0.0f;
-    if ((MODE & DS_BWD) && p.accumulate) en.old[j] = id >= 0 ? to_f32(dr[id]) : 0.0f;
-    tm = t != t ? t : fmaxf(tm, t);
-  }
-  float tl;
-  if (p.t_lse) {
-    tl = p.t_lse[row];
-    __syncthreads();
-  } else {
-    tm = block_max(tm, sh);
-    const float ref = tm == -INFINITY ? 0.0f : tm;
-    float s = 0.0f;
-    for (int j = tid; j < k; j += DS_THREADS) s += expf(en.q[j] - ref);
-    s = block_sum(s, sh);
-    tl = s > 0.0f || s != s ? ref + logf(s) : 0.0f;  // no entry: every q is 0
-  }
-  float Q = 0.0f;
-  for (int j = tid; j <= k; j += DS_THREADS) Q += (en.q[j] = expf(en.q[j] - tl));
-  Q = block_sum(Q, sh);
-
-  const bool two = p.ce_weight != 0.0f && p.temperature != 1.0f;
-  float lt, l1;
-  if constexpr (MODE & DS_FWD) {
-    OnlineSum os, o1;
-    for_row(xr, V_, tid, DS_THREADS, [&](int, float x) {
-      os.add<T>(x, inv_t);
-      if (two || p.lse) o1.add<T>(x, 1.0f);
-    });
-    const float gm = block_max(os.m, sh), ref = gm == -INFINITY ? 0.0f : gm;
-    const float mine = os.m == -INFINITY ? 0.0f : os.m - ref;
-    const float st = block_sum(os.s * exp_row<T>(mine * inv_t), sh);
-    const float s1 = block_sum(o1.s * exp_row<T>(mine), sh);
-    lt = ref * inv_t + logf(st);
-    l1 = ref + logf(two || p.lse ? s1 : st);
-    float kl = 0.0f;
-    for (int j = tid; j < k; j += DS_THREADS) {
-      const float q = en.q[j];
-      if (q > 0.0f || q != q) kl += q * (p.t_logits[row * k + j] * inv_t - tl - (en.x[j] * inv_t - lt));
-    }
-    kl = block_sum(kl, sh);
-    if (tid == 0) {
-      float l = 0.0f;
-      if (p.kd_weight != 0.0f) l = p.kd_weight * p.temperature * p.temperature * kl;
-      if (p.ce_weight != 0.0f) l -= p.ce_weight * logf(expf(en.x[k] - l1) + 1e-8f);
-      p.row_loss[row] = l;
-      if (p.lse) { p.lse[row] = lt; p.lse[p.rows + row] = l1; }
-    }
-  } else {
-    lt = p.lse[row];
-    l1 = p.lse[p.rows + row];
-  }
-  if constexpr (MODE & DS_BWD) {
-    const float g = p.grad_scale * (p.grad_out ? *p.grad_out : 1.0f);
-    const float kq = p.kd_weight * p.temperature * g, kp = kq * Q, c1 = p.ce_weight * g;
-    auto grad = [&](float x) {
-      float d = kp * exp_row<T>(x * inv_t - lt);
-      if (p.ce_weight != 0.0f) d += c1 * exp_row<T>(x - l1);
-      return d;
-    };
-    for (int i = tid; i < V_; i += DS_THREADS) {
-      float d = grad(to_f32(xr[i]));
-      if (p.accumulate) d += to_f32(dr[i]);
-      dr[i] = from_f32<T>(d);
-    }
-    __syncthreads();
-    // entries with a term of their own: the first of equal ids collects them all and writes last
-    for (int j = tid; j <= k; j += DS_THREADS) {
-      const int id = en.id[j];
-      if (id < 0) continue;
-      float q = 0.0f;
-      bool first = true;
-      for (int i = 0; i <= k; ++i) {
-        if (en.id[i] == id) {
-          if (i < j) first = false;
-          if (i < k) q += en.q[i];
-        }
-      }
-      if (!first) continue;
-      float d = grad(en.x[j]) - kq * q;
-      if (id == y && p.ce_weight != 0.0f) d -= c1;
-      if (p.accumulate) d += en.old[j];
-      dr[id] = from_f32<T>(d);
-    }
-  }
-}
 
 // A row's exponentials et = exp((x - ref) / T) and e1 = exp(x - ref).  KIND says how they are formed:
 //   ONE     et alone (temperature 1, or no cross-entropy term and one log-sum-exp), as h^2 with h = exp((x - ref) / 2T)
@@ -868,125 +697,266 @@ distill_pipe_kernel(const DistillParams p) {
   }
 }
 
-// The loss alone: nothing has to be kept of a row, so it is not staged.  A CTA reads it once, four vectors of every
-// thread in flight, with a running maximum and sums that are brought to a new maximum four vectors at a time; five CTAs
-// per SM (20 of 64 threads, for short rows) cover each other's latencies: the entries' gathers, the reductions.
-constexpr int DF_FLIGHT = 4;
+// largest element of a vector
+template <typename T>
+__device__ __forceinline__ float largest(const uint4& r) {
+  if constexpr (sizeof(T) == 2) {
+    auto pair = [](uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); };
+    const __nv_bfloat162 m = __hmax2(__hmax2(pair(r.x), pair(r.y)), __hmax2(pair(r.z), pair(r.w)));
+    return fmaxf(__low2float(m), __high2float(m));
+  } else {
+    return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
+  }
+}
 
-template <typename T, int DF_THREADS>
-__global__ void __launch_bounds__(DF_THREADS, 1280 / DF_THREADS)
+// Rows in numbers: nothing is staged.  A CTA reads its row once for a running maximum and sums (four vectors of every
+// thread in flight, brought to a new maximum four vectors at a time), and where there is a gradient once more, out of the
+// L2 cache.  Ten CTAs of 128 threads per SM (32 of one warp for short rows, five of 256 for long f32 rows: 600 x 131072, loss and
+// then gradient, 181 us against 215) cover each other's latencies: the entries' gathers, the reductions, the entries that
+// are written last.  The staged form has two or three rows at work on an SM.
+constexpr int DF_FLIGHT = 4;
+constexpr int stream_bytes(int k) { return 5 * 4 * entry_pad(k) + 2 * entry_slots(k); }
+
+template <typename T, int DF_THREADS, int MODE>
+__global__ void __launch_bounds__(DF_THREADS, DF_THREADS == 32 ? 32 : 1280 / DF_THREADS)
 distill_stream_kernel(const DistillParams p) {
   constexpr int V = VecOf<T>::N, WARPS = DF_THREADS / 32;
-  __shared__ float s_t[DS_MAX_K], s_x[DS_MAX_K];
+  constexpr bool FWD = (MODE & DS_FWD) != 0, BWD = (MODE & DS_BWD) != 0, ACC = BWD && !FWD;
+  extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float s_red[4][WARPS];
   const long long row = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = p.vocab, k = p.k;
+  const Entries e(smem, 0, entry_pad(k));
+  uint16_t* table = reinterpret_cast<uint16_t*>(smem + 5 * 4 * entry_pad(k));
   const T* xr = reinterpret_cast<const T*>(p.logits) + row * p.ld;
+  T* dr = BWD ? reinterpret_cast<T*>(p.dlogits) + row * p.ldd : nullptr;
+  const RowSlice<T> s(xr, n, 0, 0);
+  // vectors that go to dlogits as they are
+  const bool like = BWD && (int)(((uint32_t)reinterpret_cast<uintptr_t>(dr) & 15) / sizeof(T)) == s.lead;
+  const int w0 = like ? s.w0 : s.hi, w1 = like ? s.w1 : s.hi;
+  const bool acc = ACC && p.accumulate;
   const int y = p.targets ? p.targets[row] : -1;
   const bool ignored = p.targets && y == p.ignore_index;
   const bool out = p.targets && !ignored && (y < 0 || y >= n);
   if (ignored || out) {
-    if (tid == 0) {
+    if (FWD && tid == 0) {
       p.row_loss[row] = 0.0f;
       if (p.lse) { p.lse[row] = 0.0f; p.lse[p.rows + row] = 0.0f; }
       if (out && p.bad_id_flag) *p.bad_id_flag = 1;
     }
+    if (BWD && !acc)
+      for (int v = tid; v < s.hi; v += DF_THREADS) {
+        const int at = s.first(v);
+        if (v >= w0 && v < w1) *reinterpret_cast<uint4*>(dr + at) = make_uint4(0, 0, 0, 0);
+        else
+          for (int c = max(at, 0); c < min(at + V, n); ++c) dr[c] = from_f32<T>(0.0f);
+      }
     return;
   }
-  // the teacher's entries, absent ones at -inf
+  // the teacher's entries, absent ones at -inf; entry k is the target
   float tm = -INFINITY;
-  for (int j = tid; j < k; j += DF_THREADS) {
-    int id = p.t_ids[row * k + j];
-    float t = p.t_logits[row * k + j] * p.inv_t;
+  for (int j = tid; j <= k; j += DF_THREADS) {
+    int id = j < k ? p.t_ids[row * k + j] : y;
+    float t = j < k ? p.t_logits[row * k + j] * p.inv_t : -INFINITY;
     if (id >= n) {
-      if (p.bad_id_flag) *p.bad_id_flag = 1;
+      if (FWD && p.bad_id_flag) *p.bad_id_flag = 1;
       id = -1;
     }
+    id = max(id, -1);
     if (id < 0) t = -INFINITY;
-    s_t[j] = t;
-    s_x[j] = id >= 0 ? to_f32(xr[id]) : 0.0f;
+    e.id[j] = id;
+    e.t[j] = t;
+    e.x[j] = id >= 0 ? to_f32(xr[id]) : 0.0f;
+    if (ACC && acc) e.o[j] = id >= 0 ? to_f32(dr[id]) : 0.0f;
     tm = fmaxf(tm, t);
   }
-  const float xy = tid == 0 && y >= 0 ? to_f32(xr[y]) : 0.0f;
-  const RowSlice<T> s(xr, n, 0, 0);
+  if constexpr (BWD)
+    for (int c = tid; c < entry_slots(k) / 8; c += DF_THREADS) reinterpret_cast<uint4*>(table)[c] = make_uint4(~0u, ~0u, ~0u, ~0u);
   float m = -INFINITY, st = 0.0f, s1 = 0.0f;
+  if constexpr (FWD) {
 #pragma unroll 1
-  for (int v0 = tid; v0 < s.hi; v0 += DF_FLIGHT * DF_THREADS) {
-    uint4 raw[DF_FLIGHT];
-    load_vectors<T>(s, v0, DF_THREADS, raw);
-    float bm = m;
+    for (int v0 = tid; v0 < s.hi; v0 += DF_FLIGHT * DF_THREADS) {
+      uint4 raw[DF_FLIGHT];
+      load_vectors<T>(s, v0, DF_THREADS, raw);
+      float bm = m;
 #pragma unroll
-    for (int q = 0; q < DF_FLIGHT; ++q) {
-      float x[V];
-      unpack_vec<T>(raw[q], x);
-#pragma unroll
-      for (int c = 0; c < V; ++c) bm = fmaxf(bm, x[c]);
-    }
-    const float ref = bm == -INFINITY ? 0.0f : bm;
-    if (bm > m) {
-      st *= m == -INFINITY ? 0.0f : expf((m - ref) * p.inv_t);  // a NaN of st stays one
-      s1 *= m == -INFINITY ? 0.0f : expf(m - ref);
-      m = bm;
-    }
-    with_exp<T>(p.sum_kind, ref, p.inv_t, [&](const auto& ex) {
-      using Ex = std::remove_cv_t<std::remove_reference_t<decltype(ex)>>;
-      float sa[2] = {0.0f, 0.0f}, sb[2] = {0.0f, 0.0f};
-#pragma unroll
-      for (int q = 0; q < DF_FLIGHT; ++q) {
-        float x[V];
-        unpack_vec<T>(raw[q], x);
-#pragma unroll
-        for (int c = 0; c < V; c += 2) {
-          float et[2], e1[2];
-          ex.both(x[c], x[c + 1], et, e1);
-          fadd2(sa[0], sa[1], sa[0], sa[1], et[0], et[1]);
-          if constexpr (Ex::BOTH) fadd2(sb[0], sb[1], sb[0], sb[1], e1[0], e1[1]);
-        }
+      for (int q = 0; q < DF_FLIGHT; ++q) bm = fmaxf(bm, largest<T>(raw[q]));
+      const float ref = bm == -INFINITY ? 0.0f : bm;
+      if (bm > m) {
+        st *= m == -INFINITY ? 0.0f : expf((m - ref) * p.inv_t);  // a NaN of st stays one
+        s1 *= m == -INFINITY ? 0.0f : expf(m - ref);
+        m = bm;
       }
-      st += (sa[0] + sa[1]) * Ex::scale_t;
-      s1 += (sb[0] + sb[1]) * Ex::scale_1;
-    });
+      with_exp<T>(p.sum_kind, ref, p.inv_t, [&](const auto& ex) {
+        using Ex = std::remove_cv_t<std::remove_reference_t<decltype(ex)>>;
+        float sa[2] = {0.0f, 0.0f}, sb[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int q = 0; q < DF_FLIGHT; ++q) {
+          float x[V];
+          unpack_vec<T>(raw[q], x);
+#pragma unroll
+          for (int c = 0; c < V; c += 2) {
+            float et[2], e1[2];
+            ex.both(x[c], x[c + 1], et, e1);
+            fadd2(sa[0], sa[1], sa[0], sa[1], et[0], et[1]);
+            if constexpr (Ex::BOTH) fadd2(sb[0], sb[1], sb[0], sb[1], e1[0], e1[1]);
+          }
+        }
+        st += (sa[0] + sa[1]) * Ex::scale_t;
+        s1 += (sb[0] + sb[1]) * Ex::scale_1;
+      });
+    }
   }
   // maxima, then the sums relative to them
-  const float wm = warp_max(m);
+  if constexpr (FWD) {
+    const float wm = warp_max(m);
+    if (lane == 0) s_red[0][warp] = wm;
+  }
   tm = warp_max(tm);
-  if (lane == 0) { s_red[0][warp] = wm; s_red[1][warp] = tm; }
+  if (lane == 0) s_red[1][warp] = tm;
   __syncthreads();
-  const float gm = lanes_max<WARPS>(s_red[0][lane % WARPS]), ref = gm == -INFINITY ? 0.0f : gm;
+  float ref = FWD ? lanes_max<WARPS>(s_red[0][lane % WARPS]) : p.lse[p.rows + row];
+  if (ref == -INFINITY) ref = 0.0f;
+  // exp(t - tref) = q_j S, where tref is the teacher's given log-sum-exp (S = 1) or its maximum
   float tref = lanes_max<WARPS>(s_red[1][lane % WARPS]);
   if (p.t_lse) tref = p.t_lse[row];
   else if (tref == -INFINITY) tref = 0.0f;
-  const float mine = m == -INFINITY ? 0.0f : m - ref;
-  st = warp_sum(st * expf(mine * p.inv_t));
-  s1 = warp_sum(s1 * expf(mine));
   float S = 0.0f;
-  for (int j = tid; j < k; j += DF_THREADS) S += expf(s_t[j] - tref);
+  bool again = false;
+  for (int j = tid; j < k; j += DF_THREADS) {
+    const float w = expf(e.t[j] - tref);
+    S += w;
+    if constexpr (BWD) {
+      // equal ids find the same slot: whoever came first there stands for all of them (who it is does not matter)
+      const int id = e.id[j];
+      bool first = id >= 0;
+      if (id >= 0) {
+        const int slots = entry_slots(k);
+        int h = (int)(((uint32_t)id * 0x9e3779b1u) >> 16) & (slots - 1);
+        for (int tries = 0; tries < slots; ++tries) {
+          const uint16_t o = atomicCAS(table + h, (uint16_t)0xffff, (uint16_t)j);
+          if (o == 0xffff) break;
+          if (e.id[o] == id) { first = false; again = true; break; }
+          h = (h + 1) & (slots - 1);
+        }
+      }
+      e.w[j] = first ? w : -1.0f;
+    }
+  }
   S = warp_sum(S);
+  if constexpr (FWD) {
+    const float mine = m == -INFINITY ? 0.0f : m - ref;
+    st = warp_sum(st * expf(mine * p.inv_t));
+    s1 = warp_sum(s1 * expf(mine));
+  }
   __syncthreads();
   if (lane == 0) { s_red[0][warp] = st; s_red[1][warp] = s1; s_red[2][warp] = S; }
-  __syncthreads();
+  again = __syncthreads_or(again);
   st = lanes_sum<WARPS>(s_red[0][lane % WARPS]);
   s1 = lanes_sum<WARPS>(s_red[1][lane % WARPS]);
   S = lanes_sum<WARPS>(s_red[2][lane % WARPS]);
-  const float lt = ref * p.inv_t + logf(st);
-  const float l1 = p.sum_kind == ONE ? (p.temperature == 1.0f ? lt : 0.0f) : ref + logf(s1);
-  const float tl = p.t_lse || S == 0.0f ? tref : tref + logf(S);  // ln q_j = t_j - tl
+  const bool has_kd = p.kd_weight != 0.0f, has_ce = p.ce_weight != 0.0f;
   float kl = 0.0f;
-  for (int j = tid; j < k; j += DF_THREADS) {
-    const float q = expf(s_t[j] - tl);
-    if (q > 0.0f || q != q) kl += q * (s_t[j] - tl - (s_x[j] * p.inv_t - lt));
+  if constexpr (FWD) {
+    if (warp == 0 || !BWD) {  // the loss; beside a gradient in the hands of one warp
+      const float lt = ref * p.inv_t + logf(st);
+      const float tl = p.t_lse || S == 0.0f ? tref : tref + logf(S);  // ln q_j = t_j - tl
+      for (int j = BWD ? lane : tid; j < k; j += BWD ? 32 : DF_THREADS) {
+        const float q = expf(e.t[j] - tl);
+        if (q > 0.0f || q != q) kl += q * (e.t[j] - tl - (e.x[j] * p.inv_t - lt));
+      }
+      kl = warp_sum(kl);
+    }
+    if constexpr (!BWD) {
+      if (lane == 0) s_red[3][warp] = kl;
+      __syncthreads();
+      kl = lanes_sum<WARPS>(s_red[3][lane % WARPS]);
+    }
+    if (tid == 0) {
+      const float lt = ref * p.inv_t + logf(st);
+      const float l1 = p.sum_kind == ONE ? (p.temperature == 1.0f ? lt : 0.0f) : ref + logf(s1);
+      float l = 0.0f;
+      if (has_kd) l = p.kd_weight * p.temperature * p.temperature * kl;
+      if (has_ce) l -= p.ce_weight * logf(expf(e.x[k] - l1) + 1e-8f);
+      p.row_loss[row] = l;
+      if (p.lse) { p.lse[row] = lt; p.lse[p.rows + row] = l1; }
+    }
   }
-  kl = warp_sum(kl);
-  if (lane == 0) s_red[3][warp] = kl;
-  __syncthreads();
-  if (tid == 0) {
-    kl = 0.0f;
-    for (int w = 0; w < WARPS; ++w) kl += s_red[3][w];
-    float l = 0.0f;
-    if (p.kd_weight != 0.0f) l = p.kd_weight * p.temperature * p.temperature * kl;
-    if (p.ce_weight != 0.0f) l -= p.ce_weight * logf(expf(xy - l1) + 1e-8f);
-    p.row_loss[row] = l;
-    if (p.lse) { p.lse[row] = lt; p.lse[p.rows + row] = l1; }
+  if constexpr (BWD) {
+    // d = kt exp((x - ref) / T) + k1 exp(x - ref): kt, k1 turn the exponentials into weighted probabilities
+    const float g = p.grad_scale * (p.grad_out ? *p.grad_out : 1.0f);
+    const float kq = has_kd ? p.kd_weight * p.temperature * g : 0.0f, c1 = has_ce ? p.ce_weight * g : 0.0f;
+    const float Q = p.t_lse || S == 0.0f ? S : 1.0f;
+    float kt = 0.0f, k1 = 0.0f;
+    if (has_kd) kt = FWD ? __fdividef(kq * Q, st) : kq * Q * expf(ref * p.inv_t - p.lse[row]);
+    if (has_ce) k1 = FWD ? __fdividef(c1, p.grad_kind == ONE ? st : s1) : c1;
+    if (p.grad_kind == ONE) { kt += k1; k1 = 0.0f; }  // temperature 1: one exponential for both terms
+#pragma unroll 1
+    for (int v0 = tid; v0 < s.hi; v0 += DF_FLIGHT * DF_THREADS) {
+      uint4 raw[DF_FLIGHT];
+      load_vectors<T>(s, v0, DF_THREADS, raw);
+      with_exp<T>(p.grad_kind, ref, p.inv_t, [&](const auto& ex) {
+        using Ex = std::remove_cv_t<std::remove_reference_t<decltype(ex)>>;
+        const float mt = kt * Ex::scale_t, m1 = k1 * Ex::scale_1;
+#pragma unroll
+        for (int q = 0; q < DF_FLIGHT; ++q) {
+          const int v = v0 + q * DF_THREADS;
+          if (v >= s.hi) break;
+          float d[V];
+          unpack_vec<T>(raw[q], d);
+#pragma unroll
+          for (int c = 0; c < V; c += 2) {
+            float et[2], e1[2];
+            ex.both(d[c], d[c + 1], et, e1);
+            fmul2(d[c], d[c + 1], et[0], et[1], mt, mt);
+            if constexpr (Ex::BOTH) ffma2(d[c], d[c + 1], e1[0], e1[1], m1, m1, d[c], d[c + 1]);
+          }
+          const int at = s.first(v);
+          if (v >= w0 && v < w1) {
+            if (ACC && acc) {
+              float o[V];
+              ld16(dr + at, o);
+#pragma unroll
+              for (int c = 0; c < V; ++c) d[c] += o[c];
+            }
+            st16(dr + at, d);
+          } else {
+#pragma unroll
+            for (int c = 0; c < V; ++c)
+              if (at + c >= 0 && at + c < n) {
+                if (ACC && acc) d[c] += to_f32(dr[at + c]);
+                dr[at + c] = from_f32<T>(d[c]);
+              }
+          }
+        }
+      });
+    }
+    if (again) {  // sums over equal ids, in the order of the entries, so that they are the same every time
+      for (int j = tid; j < k; j += DF_THREADS)
+        if (e.w[j] != -1.0f) {
+          float w = 0.0f;
+          for (int c = 0; c < k; ++c)
+            if (e.id[c] == e.id[j]) w += expf(e.t[c] - tref);
+          e.w[j] = w;
+        }
+    }
+    // the target is one of the ids
+    bool met = false;
+    for (int j = tid; j < k; j += DF_THREADS) met |= y >= 0 && e.id[j] == y;
+    met = __syncthreads_or(met);  // and all of the row is written: the entries with a term of their own come last
+    const float inv_s = p.t_lse || S == 0.0f ? 1.0f : 1.0f / S;
+    for (int j = tid; j <= k; j += DF_THREADS) {
+      const int id = e.id[j];
+      const float w = j < k ? e.w[j] : 0.0f;
+      if (id < 0 || w == -1.0f || (j == k && (met || !has_ce))) continue;
+      const float x = e.x[j] - ref;
+      float d = kt * expf(x * p.inv_t);
+      if (k1 != 0.0f) d += k1 * expf(x);
+      if (has_kd) d -= kq * w * inv_s;
+      if (id == y) d -= c1;
+      if (ACC && acc) d += e.o[j];
+      dr[id] = from_f32<T>(d);
+    }
   }
 }
 
@@ -1017,9 +987,9 @@ int distill_sizes(const char* what, long long rows, long long vocab, long long k
   return fail(EISEN_ERR_LIMIT, msg);
 }
 
-// One warp per row for short rows in numbers, groups of 128 or 256 threads for longer ones (a group's reductions cost
-// the same whatever its row), all of a CTA's threads where there is at most one row or two per CTA.  Rows that do not fit
-// the shared memory of eight CTAs take distill_kernel, which reads them a second time.
+// Which form.  Few rows (two per SM at most): staged, all of a CTA's threads and up to eight CTAs for each of them.  Loss and
+// gradient together over rows of more than 16 KB: staged, so that the row is read once (4096 x 32000 bf16: 111 us against
+// 146 read twice; 8192 x 4096: 80 against 54).  All else: not staged (the loss alone, 1023 x 100003 bf16: 57 us against 84).
 template <typename T, int MODE>
 int distill_launch(const char* what, DistillParams& p, cudaStream_t s) {
   const long long bytes = (long long)p.vocab * sizeof(T);
@@ -1027,23 +997,16 @@ int distill_launch(const char* what, DistillParams& p, cudaStream_t s) {
     p.shape = row_shape(p.rows, p.vocab, sizeof(T), groups * entry_bytes(p.k), std::max(2 * groups, 3), least);
     return p.shape.stages >= groups;
   };
-  if constexpr (MODE == DS_FWD) {
-    // rows in numbers, or too long to be staged
-    if (p.rows > 2LL * sm_count() || !shape(1, 8192)) {
-      if (bytes <= 8192) distill_stream_kernel<T, 64><<<(unsigned)p.rows, 64, 0, s>>>(p);
-      else distill_stream_kernel<T, 256><<<(unsigned)p.rows, 256, 0, s>>>(p);
-      return check_launch(what);
-    }
+  if (p.rows <= 2LL * sm_count() && shape(1, 8192))
+    return launch_pipe<distill_pipe_kernel<T, 512, 1, MODE>>(what, p.shape, p.rows, pipe_threads(512, 1), s, p);
+  if constexpr (MODE == (DS_FWD | DS_BWD)) {
+    if (bytes > 16384 && shape(2, 1 << 30))
+      return launch_pipe<distill_pipe_kernel<T, 256, 2, MODE>>(what, p.shape, p.rows, pipe_threads(256, 2), s, p);
   }
-  if (p.rows > 2LL * sm_count()) {
-    if (bytes <= 4096 && shape(8, 1 << 30))
-      return launch_pipe<distill_pipe_kernel<T, 32, 8, MODE>>(what, p.shape, p.rows, pipe_threads(32, 8), s, p);
-    if (bytes <= 24 * 1024 && shape(4, 1 << 30))
-      return launch_pipe<distill_pipe_kernel<T, 128, 4, MODE>>(what, p.shape, p.rows, pipe_threads(128, 4), s, p);
-    if (shape(2, 1 << 30)) return launch_pipe<distill_pipe_kernel<T, 256, 2, MODE>>(what, p.shape, p.rows, pipe_threads(256, 2), s, p);
-  }
-  if (shape(1, 8192)) return launch_pipe<distill_pipe_kernel<T, 512, 1, MODE>>(what, p.shape, p.rows, pipe_threads(512, 1), s, p);
-  distill_kernel<T, MODE><<<(unsigned)p.rows, DS_THREADS, 0, s>>>(p);
+  const int smem = stream_bytes(p.k);
+  if (bytes <= 8192) distill_stream_kernel<T, 32, MODE><<<(unsigned)p.rows, 32, smem, s>>>(p);
+  else if (sizeof(T) == 2 || bytes <= 65536) distill_stream_kernel<T, 128, MODE><<<(unsigned)p.rows, 128, smem, s>>>(p);
+  else distill_stream_kernel<T, 256, MODE><<<(unsigned)p.rows, 256, smem, s>>>(p);
   return check_launch(what);
 }
 

@@ -93,7 +93,7 @@ __device__ __forceinline__ void load_vectors(const RowSlice<T>& s, int v0, int s
     const int v = v0 + q * step;
     raw[q] = make_uint4(low, low, low, low);
     if (v >= s.w0 && v < s.w1) {
-      asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+      asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
                    : "=r"(raw[q].x), "=r"(raw[q].y), "=r"(raw[q].z), "=r"(raw[q].w)
                    : "l"(s.base + (long long)v * RowSlice<T>::V));
     } else if (v < s.hi) {

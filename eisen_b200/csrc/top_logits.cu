@@ -32,6 +32,7 @@ struct TopParams {
   long long rows;
   int vocab, k;
   float inv_t;
+  int keyed;  // top_stream_kernel: there is room for the vectors' keys
   RowShape shape;
 };
 
@@ -462,13 +463,16 @@ top_pipe_kernel(const TopParams p) {
 }
 
 // Rows in numbers, or rows that no cluster holds: nothing is staged.  A CTA reads its row once for the threads' maxima and
-// the sum (a running maximum, brought up to date four vectors at a time), and again, out of the L2 cache for the most part,
-// for the elements that reach the threshold.  Five CTAs per SM (20 of 64 threads, for short rows) cover each other's
-// latencies; the staged form above has two or three rows at work on an SM.
-constexpr int TS_FLIGHT = 4;
+// the sum (a running maximum, brought up to date four vectors at a time), and notes the key of every vector's largest
+// element, so that it knows where to look for the elements that reach the threshold; rows of more than TS_KEYS vectors
+// are read again for that, out of the L2 cache for the most part.  Ten CTAs of 128 threads per SM (32 of
+// one warp for short rows: 16384 x 1000 bf16 31 us, 54 with two) cover each other's latencies, where the staged form above has three rows at work on an SM; and a thread's
+// work beside its elements, some 500 instructions, is shared by more of them than in larger CTAs (4096 x 32000 bf16, k 64:
+// 92 us with 256 threads, 78 with 128).
+constexpr int TS_FLIGHT = 4, TS_KEYS = 16384;
 
 template <typename T, int THREADS>
-__global__ void __launch_bounds__(THREADS, 1280 / THREADS)
+__global__ void __launch_bounds__(THREADS, THREADS == 32 ? 32 : 1280 / THREADS)
 top_stream_kernel(const TopParams p) {
   constexpr int V = VecOf<T>::N, WARPS = THREADS / 32;
   extern __shared__ __align__(16) uint64_t list[];
@@ -479,12 +483,15 @@ top_stream_kernel(const TopParams p) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int k = p.k, n = p.vocab, cap = top_list(k);
   int* hits = reinterpret_cast<int*>(list + cap);
+  uint16_t* keys = reinterpret_cast<uint16_t*>(list + cap + cap / 2);
   const long long row = blockIdx.x;
   const RowSlice<T> s(reinterpret_cast<const T*>(p.logits) + row * p.ld, n, 0, 0);
   const float scale = 1.4426950408889634f * p.inv_t;
-  float m[TS_FLIGHT], ref = -INFINITY, sum = 0.0f;  // the shares' maxima; the running maximum without NaN, the sum
+  const bool keyed = p.keyed;
+  uint32_t m[TS_FLIGHT];  // keys of the shares' maxima, upper 16 bits; 0: no share
+  float ref = -INFINITY, sum = 0.0f;  // the running maximum without NaN, the sum
 #pragma unroll
-  for (int q = 0; q < TS_FLIGHT; ++q) m[q] = -INFINITY;
+  for (int q = 0; q < TS_FLIGHT; ++q) m[q] = 0;
 #pragma unroll 1
   for (int v0 = tid; v0 < s.hi; v0 += TS_FLIGHT * THREADS) {
     uint4 raw[TS_FLIGHT];
@@ -492,8 +499,13 @@ top_stream_kernel(const TopParams p) {
     float bm = ref;
 #pragma unroll
     for (int q = 0; q < TS_FLIGHT; ++q) {
+      const int v = v0 + q * THREADS;
       const float x = vec_max<T>(raw[q]);
-      m[q] = max_nan(m[q], x);
+      if (v < s.hi) {
+        const uint32_t key = order_key(x) >> 16;
+        m[q] = max(m[q], key);
+        if (keyed) keys[v] = (uint16_t)key;
+      }
       bm = fmaxf(bm, x);
     }
     if (p.lse) {
@@ -514,7 +526,11 @@ top_stream_kernel(const TopParams p) {
           for (int c = 0; c < V; ++c) acc[c & 1] += expf((x[c] - r0) * p.inv_t);
         } else {
 #pragma unroll
-          for (int c = 0; c < V; ++c) acc[c & 1] += exp2_approx(fmaf(x[c], scale, off));
+          for (int c = 0; c < V; c += 2) {
+            float h0, h1;
+            ffma2(h0, h1, x[c], x[c + 1], scale, scale, off, off);
+            fadd2(acc[0], acc[1], acc[0], acc[1], exp2_approx(h0), exp2_approx(h1));
+          }
         }
       }
       sum += acc[0] + acc[1];
@@ -523,8 +539,7 @@ top_stream_kernel(const TopParams p) {
     }
   }
   // ---- threshold, as above
-  const float most = max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3]));
-  const uint32_t top_key = tid < s.hi ? order_key(most) >> 16 : 0;
+  const uint32_t top_key = max(max(m[0], m[1]), max(m[2], m[3]));
   const float wm = warp_max(ref);
   const uint32_t k_hi = __reduce_max_sync(0xffffffffu, top_key);
   const uint32_t k_lo = __reduce_min_sync(0xffffffffu, tid < s.hi ? top_key : 0xffffu);
@@ -550,15 +565,12 @@ top_stream_kernel(const TopParams p) {
       if (__syncthreads_count(top_key >= trial) >= k) tau = trial;
     }
   } else if (k <= min(s.hi, TS_FLIGHT * THREADS)) {
-    uint32_t key[TS_FLIGHT];
-#pragma unroll
-    for (int q = 0; q < TS_FLIGHT; ++q) key[q] = tid + q * THREADS < s.hi ? order_key(m[q]) >> 16 : 0;
 #pragma unroll 1
     for (int bit = 15; bit >= 0; --bit) {
       const uint32_t trial = tau | (1u << bit);
       int total = 0;
 #pragma unroll
-      for (int q = 0; q < TS_FLIGHT; ++q) total += __syncthreads_count(key[q] >= trial);
+      for (int q = 0; q < TS_FLIGHT; ++q) total += __syncthreads_count(m[q] >= trial);
       if (total >= k) tau = trial;
     }
   }
@@ -573,14 +585,22 @@ top_stream_kernel(const TopParams p) {
 #pragma unroll 1
   for (int v0 = tid; v0 - tid < s.hi; v0 += 8 * TS_FLIGHT * THREADS) {
     uint32_t noted = 0;
+    if (keyed) {
+#pragma unroll 4
+      for (int b = 0; b < 8 * TS_FLIGHT; ++b) {
+        const int v = v0 + b * THREADS;
+        if (v < s.hi) noted |= (uint32_t)(keys[v] >= tau) << b;  // this thread's own notes
+      }
+    } else {
 #pragma unroll 1
-    for (int b = 0; b < 8; ++b) {
-      uint4 raw[TS_FLIGHT];
-      const int v = v0 + b * TS_FLIGHT * THREADS;
-      if (v >= s.hi) break;
-      load_vectors<T>(s, v, THREADS, raw);
+      for (int b = 0; b < 8; ++b) {
+        uint4 raw[TS_FLIGHT];
+        const int v = v0 + b * TS_FLIGHT * THREADS;
+        if (v >= s.hi) break;
+        load_vectors<T>(s, v, THREADS, raw);
 #pragma unroll
-      for (int q = 0; q < TS_FLIGHT; ++q) noted |= (uint32_t)(v + q * THREADS < s.hi && reaches<T>(raw[q], floor_value)) << (b * TS_FLIGHT + q);
+        for (int q = 0; q < TS_FLIGHT; ++q) noted |= (uint32_t)(v + q * THREADS < s.hi && reaches<T>(raw[q], floor_value)) << (b * TS_FLIGHT + q);
+      }
     }
     int mine = __popc(noted), before = mine;
     if (__any_sync(0xffffffffu, mine)) {
@@ -665,8 +685,12 @@ int top_launch(TopParams& p, cudaStream_t s) {
     p.shape = row_shape(p.rows, p.vocab, sizeof(T), lists + 8 * TOP_MAX_K, 3, 8192);
     if (p.shape.stages) return launch_pipe<top_pipe_kernel<T, 512, 1>>("top_logits", p.shape, p.rows, 512 + 32, s, p);
   }
-  if (bytes <= 8192) top_stream_kernel<T, 64><<<(unsigned)p.rows, 64, lists, s>>>(p);
-  else top_stream_kernel<T, 256><<<(unsigned)p.rows, 256, lists, s>>>(p);
+  const long long vectors = bytes / 16 + 2;  // a row that starts inside a vector touches one more
+  p.keyed = vectors <= TS_KEYS;
+  const int smem = lists + (p.keyed ? (int)vectors * 2 : 0);
+  // a warp's four shares per lane are too few for a threshold near the k-th largest where k is more than half of them
+  if (bytes <= 8192 && p.k <= 64) top_stream_kernel<T, 32><<<(unsigned)p.rows, 32, smem, s>>>(p);
+  else top_stream_kernel<T, 128><<<(unsigned)p.rows, 128, smem, s>>>(p);
   return check_launch("top_logits");
 }
 
@@ -686,6 +710,6 @@ extern "C" int eisen_top_logits(void* stream, const void* logits, long long ld, 
   if (rows == 0) return 0;
   if (!logits || !values || !ids) return fail(EISEN_ERR_INVALID, "top_logits: logits, values and ids must not be null");
   if (reinterpret_cast<uintptr_t>(logits) % (dtype == DT_F32 ? 4 : 2)) return fail(EISEN_ERR_INVALID, "top_logits: unaligned pointer");
-  TopParams p = {logits, ld, values, ids, lse, rows, (int)vocab, (int)k, 1.0f / temperature, {}};
+  TopParams p = {logits, ld, values, ids, lse, rows, (int)vocab, (int)k, 1.0f / temperature, 0, {}};
   EISEN_DISPATCH_DTYPE(dtype, T, { return top_launch<T>(p, (cudaStream_t)stream); });
 }
