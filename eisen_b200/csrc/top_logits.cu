@@ -237,9 +237,10 @@ top_pipe_kernel(const TopParams p) {
     ring_load<T>(ring, smem, p.shape.stages, p.shape.stage_bytes, n_mine, row0, stride, slice_of, [](long long) { return false; });
   } else {
     const int g = tid / GT, gt = tid % GT, warp = gt >> 5;
-    uint64_t* list = reinterpret_cast<uint64_t*>(smem + (size_t)p.shape.stages * p.shape.stage_bytes) + (size_t)g * (cap + cap / 2 + TOP_MAX_K);
+    uint64_t* list = reinterpret_cast<uint64_t*>(smem + (size_t)p.shape.stages * p.shape.stage_bytes) + (size_t)g * (cap + cap / 2 + 9 * TOP_MAX_K);
     int* hits = reinterpret_cast<int*>(list + cap);  // vectors with an element that reaches the threshold
     uint64_t* best = list + cap + cap / 2;  // this slice's k largest in descending order (clusters)
+    uint64_t* all = best + TOP_MAX_K;       // every slice's, in the first CTA
     int stage = g - G;  // the stage of row i, and its phase; a ring has at least G stages
     uint32_t phase = 0, turn = 0;
     for (int i = g; i < n_mine; i += G, ++turn) {
@@ -420,18 +421,24 @@ top_pipe_kernel(const TopParams p) {
           const uint32_t b0 = smem_u32(best), s0 = smem_u32(&s_slice[g][0]);
           top = -INFINITY;
           for (int o = 0; o < C; ++o) top = fmaxf(top, __uint_as_float((uint32_t)ld_cluster_u64(mapa_cluster(s0, o))));
+          // the slices' lists into this CTA's memory: a search over there costs its latency step by step
+          for (int j = gt; j < C * k; j += GT) {
+            const int from = j / k;
+            all[j] = ld_cluster_u64(mapa_cluster(b0 + 8 * (j - from * k), from));
+          }
+          group_sync<GT>(g);
           for (int j = gt; j < C * k; j += GT) {
             const int from = j / k, at = j - from * k;
-            const uint64_t c = ld_cluster_u64(mapa_cluster(b0 + 8 * at, from));
+            const uint64_t c = all[j];
             if (c == 0) continue;
             int r = at;  // before it in its own list, and in every other one
             for (int o = 0; o < C && r < k; ++o) {
               if (o == from) continue;
-              const uint32_t other = mapa_cluster(b0, o);
+              const uint64_t* other = all + o * k;
               int lo = 0, hi = k;
               while (lo < hi) {
                 const int mid = (lo + hi) >> 1;
-                if (ld_cluster_u64(other + 8 * mid) > c) lo = mid + 1;
+                if (other[mid] > c) lo = mid + 1;
                 else hi = mid;
               }
               r += lo;
@@ -682,7 +689,7 @@ int top_launch(TopParams& p, cudaStream_t s) {
   const int lists = 8 * (top_list(p.k) * 3 / 2);
   // few rows: all of a CTA's threads, and up to eight CTAs, for each of them
   if (p.rows <= 2LL * sm_count()) {
-    p.shape = row_shape(p.rows, p.vocab, sizeof(T), lists + 8 * TOP_MAX_K, 3, 8192);
+    p.shape = row_shape(p.rows, p.vocab, sizeof(T), lists + 9 * 8 * TOP_MAX_K, 3, 8192);
     if (p.shape.stages) return launch_pipe<top_pipe_kernel<T, 512, 1>>("top_logits", p.shape, p.rows, 512 + 32, s, p);
   }
   const long long vectors = bytes / 16 + 2;  // a row that starts inside a vector touches one more

@@ -132,6 +132,15 @@ def test_top_logits_many_rows(dtype, rows, vocab, k):
     check_top(x.to(dtype), k, 1.5)
 
 
+@pytest.mark.parametrize("dtype,vocab", [(torch.bfloat16, 131056), (torch.bfloat16, 131065), (torch.bfloat16, 131072), (torch.bfloat16, 131073),
+                                         (torch.float32, 65528), (torch.float32, 65533), (torch.float32, 65537), (torch.float32, 99999)])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_top_logits_around_the_longest_noted_row(dtype, vocab, shift):
+    """Rows in numbers, with as many vectors as are noted one by one, and a few more or less."""
+    x = torch.randn(300, vocab, generator=gen(vocab), device=dev()).to(dtype)
+    check_top(rows_at(x, vocab, shift), 9)
+
+
 def test_top_logits_longer_than_shared_memory():
     x = torch.randn(2, 700001, generator=gen(2), device=dev())
     x[1, 5000:6000] = 9.0
@@ -350,6 +359,18 @@ def test_distill_many_rows(dtype, rows, vocab, k, ignored):
     c.check_grad(d, fused=True)
     loss, row, lse = c.fwd()
     c.check_loss(loss, row, lse)
+    d.fill_(5.0)
+    c.bwd(lse, d)
+    c.check_grad(d)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_distill_row_longer_than_shared_memory(dtype):
+    c = Case(dtype, 2, 1000003, 70, 2.0, 0.5, 0.5, ignored=0.0).expected()
+    d = torch.full_like(c.x, 5.0)
+    loss, row, lse = c.fused(d)
+    c.check_loss(loss, row, lse)
+    c.check_grad(d, fused=True)
     d.fill_(5.0)
     c.bwd(lse, d)
     c.check_grad(d)
