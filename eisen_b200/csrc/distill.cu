@@ -22,7 +22,6 @@ namespace {
 
 constexpr int DS_MAX_K = 1024;
 
-
 struct DistillParams {
   const void* logits;
   long long ld;
@@ -40,7 +39,7 @@ struct DistillParams {
   float temperature, inv_t, kd_weight, ce_weight, grad_scale;
   int accumulate;
   int* bad_id_flag;
-  int sum_kind, grad_kind;  // distill_pipe_kernel: see RowExp
+  int sum_kind, grad_kind;  // see RowExp
   RowShape shape;
 };
 
@@ -50,13 +49,14 @@ constexpr int DS_FWD = 1, DS_BWD = 2;
 //   ONE     et alone (temperature 1, or no cross-entropy term and one log-sum-exp), as h^2 with h = exp((x - ref) / 2T)
 //   3 .. 8  bf16 rows with 2T a whole number: et = h^2, e1 = h^2T with the same h
 //   TWO     both, each by itself
-//   PLAIN1, PLAIN2   (x - ref) first and expf, et alone or both: rows of f32 logits, and rows whose largest entry is near
-//           the end of the type's range (all of it masked by the lowest value), where the products with ref would overflow
+//   PLAIN1, PLAIN2   (x - ref) first and expf, et alone or both: rows of f32 logits, and bf16 rows whose largest entry is
+//           beyond 1e4 (all of it masked by the type's lowest value, say): there the rounding of ref / T is felt
 // The special-function unit gives 16 results per clock and SM, 2000 clocks for 32000 entries.  Two exponentials in both
-// passes over a row would take 8000 where the memory needs 5600.  So the first pass of the fused form leaves h in the
+// passes over a row would take 8000 where the memory needs 5600.  So the first pass of the staged form leaves h in the
 // row's place in shared memory for the second: f32 rows keep et itself, bf16 rows h in fp16 (half a step is 2^-11 of h;
-// et has twice that, a quarter of bf16's own half step, e1 2T <= 8 times, at most as much as bf16's half step).  h, not its square, so that fp16's
-// range covers et down to 2^-38 (2T = 8) or 2^-54 (2T <= 3) of the row's largest; smaller ones fade to 0.
+// et has twice that, a quarter of bf16's own half step, e1 2T <= 8 times, at most as much as bf16's half step).  h, not
+// its square, so that fp16's range covers et down to 2^-38 (2T = 8) or 2^-54 (2T <= 3) of the row's largest; smaller
+// ones fade to 0.
 constexpr int ONE = 2, TWO = 1, PLAIN1 = 10, PLAIN2 = 11;
 
 template <typename T, int KIND>
@@ -128,7 +128,7 @@ __device__ __forceinline__ void with_exp(int kind, float ref, float inv_t, F f) 
     if (kind == ONE) f(RowExp<T, PLAIN1>(ref, inv_t));
     else f(RowExp<T, PLAIN2>(ref, inv_t));
   } else {
-    if (fabsf(ref) > 1e30f) {
+    if (fabsf(ref) * fmaxf(inv_t, 1.0f) > 1e4f) {
       if (kind == ONE) f(RowExp<T, PLAIN1>(ref, inv_t));
       else f(RowExp<T, PLAIN2>(ref, inv_t));
       return;
@@ -144,6 +144,13 @@ __device__ __forceinline__ void with_exp(int kind, float ref, float inv_t, F f) 
       default: return f(RowExp<T, TWO>(ref, inv_t));
     }
   }
+}
+
+// What a gradient alone takes its exponentials relative to, given the row's two log-sum-exps: at least its largest entry, and
+// not so far above it that exp((ref - x) / T) or exp(ref - x) of that entry leaves the range (T lse(x / T) and lse(x) are
+// at most T ln n and ln n above it; divided by a small T the latter may be thousands).
+__device__ __forceinline__ float grad_ref(const DistillParams& p, float lt, float l1) {
+  return p.temperature < 1.0f ? fminf(l1, lt * p.temperature) : l1;
 }
 
 // the kind for both exponentials at a temperature other than 1
@@ -533,7 +540,7 @@ distill_pipe_kernel(const DistillParams p) {
       if (own0) vec[0] = edge0;
       if (own1) vec[cnt - 1] = edge1;
 
-      float ref = l1_given, own_ref = ref, st = 0.0f, s1 = 0.0f, own_st = 1.0f;
+      float ref = FWD ? 0.0f : grad_ref(p, lt_given, l1_given), own_ref = ref, st = 0.0f, s1 = 0.0f, own_st = 1.0f;
       if constexpr (FWD) {
         float m = -INFINITY;
         if constexpr (sizeof(T) == 2) {
@@ -625,7 +632,7 @@ distill_pipe_kernel(const DistillParams p) {
       if constexpr (BWD) {
         const float Q = s_teacher[g][set].Q;
         if (has_kd) kt = FWD ? __fdividef(kq * Q, st) : kq * Q * expf(ref * p.inv_t - lt_given);
-        if (has_ce) k1 = FWD ? __fdividef(c1, p.grad_kind == ONE ? st : s1) : c1;
+        if (has_ce) k1 = FWD ? __fdividef(c1, p.grad_kind == ONE ? st : s1) : c1 * expf(ref - l1_given);
         if (p.grad_kind == ONE) { kt += k1; k1 = 0.0f; }  // temperature 1: one exponential for both terms
       }
       if (gt == 0) {
@@ -689,8 +696,14 @@ distill_pipe_kernel(const DistillParams p) {
       }
     }
   }
-  if (ring.abort_flag)
+  if (ring.abort_flag) {  // a wait ran out: nothing of this CTA's rows can be relied on, and they say so
     for (int i = 0; i < 64; ++i) __nanosleep(1000);  // copies in flight end before the CTA does
+    for (int i = tid; i < n_mine; i += blockDim.x) {
+      const long long row = row0 + (long long)i * stride;
+      if (FWD) p.row_loss[row] = NAN;
+      if (BWD) dlogits[row * p.ldd] = from_f32<T>(NAN);
+    }
+  }
   if (C > 1) {
     __syncwarp();
     cluster_sync_all();  // nobody leaves while a peer may still write to it
@@ -815,7 +828,7 @@ distill_stream_kernel(const DistillParams p) {
   tm = warp_max(tm);
   if (lane == 0) s_red[1][warp] = tm;
   __syncthreads();
-  float ref = FWD ? lanes_max<WARPS>(s_red[0][lane % WARPS]) : p.lse[p.rows + row];
+  float ref = FWD ? lanes_max<WARPS>(s_red[0][lane % WARPS]) : grad_ref(p, p.lse[row], p.lse[p.rows + row]);
   if (ref == -INFINITY) ref = 0.0f;
   // exp(t - tref) = q_j S, where tref is the teacher's given log-sum-exp (S = 1) or its maximum
   float tref = lanes_max<WARPS>(s_red[1][lane % WARPS]);
@@ -889,7 +902,7 @@ distill_stream_kernel(const DistillParams p) {
     const float Q = p.t_lse || S == 0.0f ? S : 1.0f;
     float kt = 0.0f, k1 = 0.0f;
     if (has_kd) kt = FWD ? __fdividef(kq * Q, st) : kq * Q * expf(ref * p.inv_t - p.lse[row]);
-    if (has_ce) k1 = FWD ? __fdividef(c1, p.grad_kind == ONE ? st : s1) : c1;
+    if (has_ce) k1 = FWD ? __fdividef(c1, p.grad_kind == ONE ? st : s1) : c1 * expf(ref - p.lse[p.rows + row]);
     if (p.grad_kind == ONE) { kt += k1; k1 = 0.0f; }  // temperature 1: one exponential for both terms
 #pragma unroll 1
     for (int v0 = tid; v0 < s.hi; v0 += DF_FLIGHT * DF_THREADS) {

@@ -314,7 +314,7 @@ top_pipe_kernel(const TopParams p) {
       // every element whose key reaches tau; NaN does, and so does everything where tau is 0
       const float floor_value = key_value(tau << 16);
       const float c2 = 1.4426950408889634f * p.inv_t, off = -ref * c2;
-      const bool far = sizeof(T) == 4 || fabsf(ref) > 1e30f;
+      const bool far = sizeof(T) == 4 || fabsf(ref) * p.inv_t > 1e4f;
       float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
       uint4 next = gt < cnt ? vec[gt] : make_uint4(0, 0, 0, 0);
       // a thread notes which of its vectors hold such an element (32 at a time); looking into them here would hold up
@@ -461,8 +461,10 @@ top_pipe_kernel(const TopParams p) {
       }
     }
   }
-  if (ring.abort_flag)
+  if (ring.abort_flag) {  // a wait ran out: nothing of this CTA's rows can be relied on, and they say so
     for (int i = 0; i < 64; ++i) __nanosleep(1000);  // copies in flight end before the CTA does
+    for (int i = tid; i < n_mine; i += blockDim.x) p.values[(row0 + (long long)i * stride) * k] = NAN;
+  }
   if (C > 1) {
     __syncwarp();
     cluster_sync_all();  // nobody leaves while a peer may still read its lists
@@ -522,7 +524,7 @@ top_stream_kernel(const TopParams p) {
         ref = bm;
       }
       const float off = -r0 * scale;
-      const bool far = sizeof(T) == 4 || fabsf(r0) > 1e30f;
+      const bool far = sizeof(T) == 4 || fabsf(r0) * p.inv_t > 1e4f;
       float acc[2] = {0.0f, 0.0f};
 #pragma unroll
       for (int q = 0; q < TS_FLIGHT; ++q) {

@@ -364,6 +364,29 @@ def test_distill_many_rows(dtype, rows, vocab, k, ignored):
     c.check_grad(d)
 
 
+@pytest.mark.parametrize("rows", [3, 400])
+@pytest.mark.parametrize("temperature", [0.5, 1.0, 2.0, 1e-3])
+def test_distill_large_logits(rows, temperature):
+    """bf16 logits of 2e4 and more: the row's largest, over T, is far beyond what a product with it would keep of a
+    difference.  One step of these logits is 128, so all probabilities but the largest ones' are 0."""
+    c = Case(torch.bfloat16, rows, 3000, 6, temperature, 0.5, 0.5, ignored=0.0, absent=0.0)
+    c.x = (c.x.float() * 10 + 20000).to(torch.bfloat16)
+    c.ids[:, 0] = c.x.float().argmax(1).int()
+    c.tv[:] = -math.inf
+    c.tv[:, 0] = 1.0  # the teacher is sure of the student's first choice, whose loss is that of the ties
+    c.expected()
+    d = torch.full_like(c.x, 5.0)
+    loss, row, lse = c.fused(d)
+    assert torch.isfinite(loss)
+    assert ((lse.double() - c.lse).abs() <= EPS_P + 8 * 2.0 ** -24 * c.lse.abs()).all()
+    c.check_grad(d, fused=True)
+    d.fill_(5.0)
+    c.bwd(lse, d)
+    # the log-sum-exps themselves are rounded to 32 bits: 2^-24 of 2e4 / T is the relative error of every probability
+    c.d_tol = c.d_tol * (1 + c.lse.abs().max(0).values[:, None] * 2.0 ** -23 / EPS_P)
+    c.check_grad(d)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_distill_row_longer_than_shared_memory(dtype):
     c = Case(dtype, 2, 1000003, 70, 2.0, 0.5, 0.5, ignored=0.0).expected()
@@ -593,6 +616,13 @@ def test_linear_ce_accumulates_and_takes_an_upstream_gradient(tied, dw_dtype):
     only_h, none = c.bwd(lse, 512, grad=g, dw=False)
     assert none is None
     c.within(only_h, c.dh, c.dh_tol, 2.0 ** -8)
+
+
+@pytest.mark.parametrize("tied", [False, True])
+def test_linear_ce_forward_of_any_width(tied):
+    """The loss alone takes widths that are no multiple of 8 (rows still are)."""
+    c = Head(70, 60, 333, tied, pad_h=4).expected()
+    c.check_loss(*c.fwd())
 
 
 def test_linear_ce_does_not_touch_what_is_beside_its_outputs():
