@@ -1015,6 +1015,8 @@ int distill_launch(const char* what, DistillParams& p, cudaStream_t s) {
   if constexpr (MODE == (DS_FWD | DS_BWD)) {
     if (bytes > 16384 && shape(2, 1 << 30))
       return launch_pipe<distill_pipe_kernel<T, 256, 2, MODE>>(what, p.shape, p.rows, pipe_threads(256, 2), s, p);
+    if (bytes > 16384 && shape(1, 1 << 30))  // one row at a time in a CTA
+      return launch_pipe<distill_pipe_kernel<T, 512, 1, MODE>>(what, p.shape, p.rows, pipe_threads(512, 1), s, p);
   }
   const int smem = stream_bytes(p.k);
   if (bytes <= 8192) distill_stream_kernel<T, 32, MODE><<<(unsigned)p.rows, 32, smem, s>>>(p);

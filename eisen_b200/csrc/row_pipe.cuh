@@ -243,8 +243,9 @@ struct RowShape {
 constexpr int RP_SMEM = 216 * 1024;
 
 // `extra`: dynamic shared memory beside the stages.  A row of up to a third of the stage memory stays whole (three
-// stages keep the memory busy while two groups work); longer rows are split over 2, 4 or 8 CTAs, and so are rows that
-// alone leave SMs idle, down to slices of `least` bytes.  stages == 0: no split fits.
+// stages keep the memory busy while two groups work); longer rows are split over 2, 4 or 8 CTAs, but for those
+// that would take 4 and fit one CTA whole (1024 x 100003 bf16, loss and gradient: 107 us whole, 128 in four slices that meet
+// for every row), and so are rows that alone leave SMs idle, down to slices of `least` bytes.  stages == 0: no split fits.
 inline RowShape row_shape(long long rows, long long vocab, int elem, int extra, int want_stages, int least) {
   RowShape s = {};
   const long long row_bytes = (vocab * elem + 31) / 16 * 16;
@@ -252,6 +253,7 @@ inline RowShape row_shape(long long rows, long long vocab, int elem, int extra, 
   int c = 1;
   auto slice = [&](int cl) { return ((row_bytes / 16 + cl - 1) / cl * 16 + 127) / 128 * 128; };
   while (c < 8 && slice(c) * 3 > room) c *= 2;
+  if (c >= 4 && slice(1) <= room) c = 1;
   while (c < 8 && rows * c * 2 <= sm_count() && row_bytes / (2 * c) >= least) c *= 2;
   if (slice(c) > room || slice(c) > (1 << 20)) return s;
   s.cluster = c;
