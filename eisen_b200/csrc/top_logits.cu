@@ -80,22 +80,44 @@ __device__ __forceinline__ bool reaches(const uint4& r, float floor) {
   }
 }
 
-// f(rank, key) for the listed keys: how many of them are larger.  2 or 4 threads share a key's comparisons where there
-// are threads enough.
-template <int GT, typename F>
-__device__ __forceinline__ void each_rank(const uint64_t* list, int listed, int gt, F f) {
-  const int share = 4 * listed <= GT ? 2 : 2 * listed <= GT ? 1 : 0;  // log2
-  const int part = gt & ((1 << share) - 1);
-  for (int j0 = 0; j0 < listed; j0 += GT >> share) {
-    const int j = j0 + (gt >> share);
-    const uint64_t c = j < listed ? list[j] : ~0ull;
-    int r = 0;
+// f(rank, key) for the listed keys, at least for the `most` largest of them.  Up to 96 keys by counting those that are larger
+// (2 or 4 threads share a key's comparisons where there are threads enough); more are sorted in place, which takes
+// log^2 steps instead of `listed`: 8192 x 16000 bf16, k 128: 162 us by counting, 140 sorted.  The list has room up to the next
+// power of two.  sync(): a barrier of the THREADS threads.
+template <int THREADS, typename Sync, typename F>
+__device__ __forceinline__ void each_rank(uint64_t* list, int listed, int most, int tid, Sync sync, F f) {
+  if (listed <= 96) {
+    const int share = 4 * listed <= THREADS ? 2 : 2 * listed <= THREADS ? 1 : 0;  // log2
+    const int part = tid & ((1 << share) - 1);
+    for (int j0 = 0; j0 < listed; j0 += THREADS >> share) {
+      const int j = j0 + (tid >> share);
+      const uint64_t c = j < listed ? list[j] : ~0ull;
+      int r = 0;
 #pragma unroll 4
-    for (int o = part; o < listed; o += 1 << share) r += list[o] > c;
-    if (share > 0) r += __shfl_xor_sync(0xffffffffu, r, 1);
-    if (share > 1) r += __shfl_xor_sync(0xffffffffu, r, 2);
-    if (j < listed && part == 0) f(r, c);
+      for (int o = part; o < listed; o += 1 << share) r += list[o] > c;
+      if (share > 0) r += __shfl_xor_sync(0xffffffffu, r, 1);
+      if (share > 1) r += __shfl_xor_sync(0xffffffffu, r, 2);
+      if (j < listed && part == 0) f(r, c);
+    }
+    return;
   }
+  int all = 128;
+  while (all < listed) all *= 2;
+  for (int j = listed + tid; j < all; j += THREADS) list[j] = 0;  // below every key
+  for (int size = 2; size <= all; size *= 2)
+    for (int stride = size / 2; stride > 0; stride /= 2) {
+      sync();
+      for (int i = tid; i < all / 2; i += THREADS) {
+        const int lo = 2 * i - (i & (stride - 1)), hi = lo + stride;
+        const uint64_t a = list[lo], b = list[hi];
+        if ((a < b) == ((lo & size) == 0)) {  // runs of `size` fall and rise in turn; the last one falls
+          list[lo] = b;
+          list[hi] = a;
+        }
+      }
+    }
+  sync();
+  for (int j = tid; j < min(listed, most); j += THREADS) f(j, list[j]);
 }
 
 // how many of a group's threads say so (a barrier of the group)
@@ -408,12 +430,12 @@ top_pipe_kernel(const TopParams p) {
       };
       if (C == 1) {
         if (gt == 0 && p.lse && top != INFINITY) p.lse[row] = ref * p.inv_t + logf(sum);
-        each_rank<GT>(list, listed, gt, [&](int r, uint64_t c) { if (r < k) put(r, c); });
+        each_rank<GT>(list, listed, k, gt, [&]() { group_sync<GT>(g); }, [&](int r, uint64_t c) { if (r < k) put(r, c); });
         group_sync<GT>(g);  // the list is read before the next row's takes its place
       } else {
         if (gt == 0) { s_slice[g][0] = sum == 0.0f ? -INFINITY : ref; s_slice[g][1] = sum; }
         for (int j = gt + kk; j < k; j += GT) best[j] = 0;
-        each_rank<GT>(list, listed, gt, [&](int r, uint64_t c) { if (r < k) best[r] = c; });
+        each_rank<GT>(list, listed, k, gt, [&]() { group_sync<GT>(g); }, [&](int r, uint64_t c) { if (r < k) best[r] = c; });
         group_sync<GT>(g);
         if (gt == 0) mbar_arrive_release_cluster(mapa_cluster(smem_u32(&xbar[g]), 0));
         if (rank == 0) {
@@ -477,7 +499,7 @@ top_pipe_kernel(const TopParams p) {
 // are read again for that, out of the L2 cache for the most part.  Ten CTAs of 128 threads per SM (32 of
 // one warp for short rows: 16384 x 1000 bf16 31 us, 54 with two) cover each other's latencies, where the staged form above has three rows at work on an SM; and a thread's
 // work beside its elements, some 500 instructions, is shared by more of them than in larger CTAs (4096 x 32000 bf16, k 64:
-// 92 us with 256 threads, 78 with 128).
+// 92 us with 256 threads, 79 with 128).
 constexpr int TS_FLIGHT = 4, TS_KEYS = 16384;
 
 template <typename T, int THREADS>
@@ -487,7 +509,7 @@ top_stream_kernel(const TopParams p) {
   extern __shared__ __align__(16) uint64_t list[];
   __shared__ float s_max[WARPS], s_sum[WARPS];
   __shared__ uint32_t s_range[WARPS];
-  __shared__ int s_count, s_hits;
+  __shared__ int s_count, s_hits, s_cnt[2][WARPS];
   __shared__ TopSelect s_sel;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int k = p.k, n = p.vocab, cap = top_list(k);
@@ -551,7 +573,12 @@ top_stream_kernel(const TopParams p) {
   const uint32_t top_key = max(max(m[0], m[1]), max(m[2], m[3]));
   const float wm = warp_max(ref);
   const uint32_t k_hi = __reduce_max_sync(0xffffffffu, top_key);
-  const uint32_t k_lo = __reduce_min_sync(0xffffffffu, tid < s.hi ? top_key : 0xffffu);
+  const bool by_thread = 2 * k <= min(s.hi, THREADS);  // the threshold goes by the threads' maxima, else by the shares'
+  uint32_t least = 0xffffu;
+#pragma unroll
+  for (int q = 0; q < TS_FLIGHT; ++q)
+    if (m[q]) least = min(least, m[q]);
+  const uint32_t k_lo = __reduce_min_sync(0xffffffffu, by_thread && top_key ? top_key : least);
   if (lane == 0) { s_max[warp] = wm; s_range[warp] = (k_hi << 16) | k_lo; }
   if (tid == 0) { s_count = 0; s_hits = 0; }
   __syncthreads();
@@ -566,7 +593,7 @@ top_stream_kernel(const TopParams p) {
   }
   const int bits = 32 - __clz(hi16 ^ lo16);
   uint32_t tau = 0;
-  if (2 * k <= min(s.hi, THREADS)) {
+  if (by_thread) {
     tau = (hi16 >> bits) << bits;
 #pragma unroll 1
     for (int bit = bits - 1; bit >= 0; --bit) {
@@ -574,12 +601,19 @@ top_stream_kernel(const TopParams p) {
       if (__syncthreads_count(top_key >= trial) >= k) tau = trial;
     }
   } else if (k <= min(s.hi, TS_FLIGHT * THREADS)) {
+    tau = (hi16 >> bits) << bits;
 #pragma unroll 1
-    for (int bit = 15; bit >= 0; --bit) {
-      const uint32_t trial = tau | (1u << bit);
+    for (int bit = bits - 1; bit >= 0; --bit) {
+      const uint32_t trial = tau | (1u << bit);  // not 0: places without a share do not count
+      int c = 0;
+#pragma unroll
+      for (int q = 0; q < TS_FLIGHT; ++q) c += m[q] >= trial;
+      c = __reduce_add_sync(0xffffffffu, c);
+      if (lane == 0) s_cnt[bit & 1][warp] = c;
+      __syncthreads();
       int total = 0;
 #pragma unroll
-      for (int q = 0; q < TS_FLIGHT; ++q) total += __syncthreads_count(m[q] >= trial);
+      for (int w = 0; w < WARPS; ++w) total += s_cnt[bit & 1][w];
       if (total >= k) tau = trial;
     }
   }
@@ -676,7 +710,7 @@ top_stream_kernel(const TopParams p) {
     __syncthreads();
     listed = min(s_count, cap);
   }
-  each_rank<THREADS>(list, listed, tid, [&](int r, uint64_t c) {
+  each_rank<THREADS>(list, listed, k, tid, []() { __syncthreads(); }, [&](int r, uint64_t c) {
     if (r >= k) return;
     const float v = key_value((uint32_t)(c >> 32));
     p.values[row * k + r] = v;
