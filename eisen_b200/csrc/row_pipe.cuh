@@ -87,6 +87,15 @@ struct RowSlice {
 // cache: a row does not fit there.
 template <typename T, int N>
 __device__ __forceinline__ void load_vectors(const RowSlice<T>& s, int v0, int step, uint4 (&raw)[N]) {
+  if (v0 >= s.w0 && v0 + (N - 1) * step < s.w1) {
+    const T* at = s.base + (long long)v0 * RowSlice<T>::V;
+#pragma unroll
+    for (int q = 0; q < N; ++q)
+      asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(raw[q].x), "=r"(raw[q].y), "=r"(raw[q].z), "=r"(raw[q].w)
+                   : "l"(at + (long long)q * step * RowSlice<T>::V));
+    return;
+  }
   constexpr uint32_t low = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
 #pragma unroll
   for (int q = 0; q < N; ++q) {

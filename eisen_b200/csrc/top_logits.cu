@@ -80,6 +80,24 @@ __device__ __forceinline__ bool reaches(const uint4& r, float floor) {
   }
 }
 
+// Upper 16 bits of the key of a vector's largest element; `most` takes that element into a maximum without NaN.  bf16: the key
+// from the element's own 16 bits (adding 0 makes one zero of the two; a NaN of the packed maximum is 0x7fff).
+template <typename T>
+__device__ __forceinline__ uint32_t vec_key(const uint4& r, float& most) {
+  if constexpr (sizeof(T) == 2) {
+    auto pair = [](uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); };
+    __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(pair(r.x), pair(r.y)), __hmax2_nan(pair(r.z), pair(r.w)));
+    m = __hadd2(__hmax2_nan(m, __lowhigh2highlow(m)), pair(0u));
+    const uint32_t u = *reinterpret_cast<const uint32_t*>(&m) & 0xffffu;
+    most = fmaxf(most, __uint_as_float(u << 16));
+    return (u & 0x8000u) ? u ^ 0xffffu : u | 0x8000u;
+  } else {
+    const float x = vec_max<T>(r);
+    most = fmaxf(most, x);
+    return order_key(x) >> 16;
+  }
+}
+
 // f(rank, key) for the listed keys, at least for the `most` largest of them.  Up to 96 keys by counting those that are larger
 // (2 or 4 threads share a key's comparisons where there are threads enough); more are sorted in place, which takes
 // log^2 steps instead of `listed`: 8192 x 16000 bf16, k 128: 162 us by counting, 140 sorted.  The list has room up to the next
@@ -531,13 +549,11 @@ top_stream_kernel(const TopParams p) {
 #pragma unroll
     for (int q = 0; q < TS_FLIGHT; ++q) {
       const int v = v0 + q * THREADS;
-      const float x = vec_max<T>(raw[q]);
+      const uint32_t key = vec_key<T>(raw[q], bm);
       if (v < s.hi) {
-        const uint32_t key = order_key(x) >> 16;
         m[q] = max(m[q], key);
         if (keyed) keys[v] = (uint16_t)key;
       }
-      bm = fmaxf(bm, x);
     }
     if (p.lse) {
       const float r0 = bm == -INFINITY ? 0.0f : bm;
