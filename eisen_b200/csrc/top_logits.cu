@@ -111,8 +111,13 @@ __device__ __forceinline__ void each_rank(uint64_t* list, int listed, int most, 
       const int j = j0 + (tid >> share);
       const uint64_t c = j < listed ? list[j] : ~0ull;
       int r = 0;
+      const ulonglong2* two = reinterpret_cast<const ulonglong2*>(list);
 #pragma unroll 4
-      for (int o = part; o < listed; o += 1 << share) r += list[o] > c;
+      for (int o = part; o < listed / 2; o += 1 << share) {
+        const ulonglong2 l = two[o];
+        r += (l.x > c) + (l.y > c);
+      }
+      if ((listed & 1) && part == 0) r += list[listed - 1] > c;
       if (share > 0) r += __shfl_xor_sync(0xffffffffu, r, 1);
       if (share > 1) r += __shfl_xor_sync(0xffffffffu, r, 2);
       if (j < listed && part == 0) f(r, c);
@@ -589,7 +594,7 @@ top_stream_kernel(const TopParams p) {
   const uint32_t top_key = max(max(m[0], m[1]), max(m[2], m[3]));
   const float wm = warp_max(ref);
   const uint32_t k_hi = __reduce_max_sync(0xffffffffu, top_key);
-  const bool by_thread = 2 * k <= min(s.hi, THREADS);  // the threshold goes by the threads' maxima, else by the shares'
+  const bool by_thread = (THREADS == 32 ? 2 : 4) * k <= min(s.hi, THREADS);  // the threshold goes by the threads' maxima, else by the shares'
   uint32_t least = 0xffffu;
 #pragma unroll
   for (int q = 0; q < TS_FLIGHT; ++q)
