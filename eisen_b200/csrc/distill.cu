@@ -192,11 +192,11 @@ __device__ __forceinline__ void kept_vec(const uint4& r, float (&x)[VecOf<T>::N]
 }
 
 // The frame of row_pipe.cuh.  A group of GT threads walks over its row three times: maximum, sums of the exponentials,
-// gradient, which goes from registers to global memory: a row of 64 KB sent off from shared memory would hold its stage,
-// one of three, for another 5000 clocks.  Beside it two warps see to what the row has of single entries: one reads, a
+// gradient, which goes from registers to global memory: a row of 64 KB sent off from shared memory holds its stage,
+// one of three, until it has been read (16384 x 32000 bf16: 454 us, 417 from registers).  Beside it two warps see to what the row has of single entries: one reads, a
 // row ahead, the teacher's ids and logits and forms their distribution; the other one, when the group has been through
 // the row, forms the loss and rewrites the entries that have a term of their own, the ids and the target.  In the
-// group's hands these were half of a row's time, latency after latency with most of its threads idle.
+// group's hands these took a quarter of a row's time (4200 of 17000 clocks), latency after latency with most threads idle.
 constexpr int pipe_threads(int gt, int groups) { return (gt + 64) * groups + 32; }
 __host__ __device__ constexpr int entry_pad(int k) { return (k + 4) & ~3; }
 // slots of the table that finds equal ids: at least four times the entries
