@@ -751,3 +751,52 @@ def test_teacher_to_student():
     want = -w * 2.0 * (1 - rest) * rest
     tol = (c.d_tol + c.kept_tol).gather(1, i.long()).sum(1)
     assert ((got - want).abs() <= tol + 2.0 ** -8 * (d.double().gather(1, i.long()).abs().sum(1) + tol)).all()
+
+
+@pytest.mark.parametrize("tied", [False, True])
+@pytest.mark.parametrize("dw_dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("accumulate", [0, 1])
+def test_linear_ce_weight_gradient_with_any_row_stride(tied, dw_dtype, accumulate):
+    """The weight gradient's rows may start at any element, unlike the weight's."""
+    c = Head(300, 136, 1203, tied).expected()
+    loss, row, lse = c.fwd()
+    start = (torch.randn(tuple(c.w.shape), generator=gen(5), device=dev()) * 1e-2).to(dw_dtype)
+    cols = c.w.shape[1]
+    buf = torch.full((c.w.shape[0], cols + 3), 3.0, dtype=dw_dtype, device=dev())
+    buf[:, :cols] = start
+    eb.call("eisen_linear_ce_bwd", stream(), *c.operands(), P(lse), None, None, 0, P(buf), cols + 3, DT[dw_dtype], accumulate,
+            P(c.workspace(512)), c.rows, c.k, c.vocab, 512, -1, c.norm, P(c.status))
+    assert int(c.status[0]) == 0
+    # a bf16 sum may round the product before it is added
+    c.within(buf[:, :cols], c.dw + accumulate * start.double(), c.dw_tol + accumulate * 2.0 ** -8 * c.dw.abs(), STEP[dw_dtype])
+    assert (buf[:, cols:] == 3.0).all()
+
+
+def test_linear_ce_no_rows():
+    c = Head(0, 64, 100, False)
+    loss, _, lse = c.fwd()
+    assert float(loss) == 0.0
+    _, dw = c.bwd(lse)
+    assert (dw == 0).all()
+    _, dw = c.bwd(lse, acc_w=1, dw0=torch.full((64, 100), 2.0, dtype=torch.bfloat16, device=dev()))
+    assert (dw == 2).all()
+
+
+@pytest.mark.parametrize("rows", [260, 320])
+def test_rows_more_than_two_to_the_31_elements_apart(rows):
+    """Element offsets pass 32 bits in both row forms, in reading and in writing."""
+    ld = (2 ** 31 + 2 ** 20) // (rows - 1) + 5
+    buf = torch.empty(rows * ld, dtype=torch.bfloat16, device=dev())
+    c = Case(torch.bfloat16, rows, 1000, 7, temperature=2.0).expected()
+    far = buf.view(rows, ld)[:, :1000]
+    far.copy_(c.x)
+    assert (rows - 1) * ld > 2 ** 31
+    check_top(far, 9)
+    c.x = far
+    loss, row, lse = c.fwd()
+    c.check_loss(loss, row, lse)
+    d = torch.empty(rows, 1000, dtype=torch.bfloat16, device=dev())
+    c.bwd(lse, d)
+    c.check_grad(d)
+    c.check_loss(*c.fused(far))  # the gradient over the logits
+    c.check_grad(far, fused=True)
