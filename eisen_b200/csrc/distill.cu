@@ -370,13 +370,10 @@ distill_pipe_kernel(const DistillParams p) {
           }
         }
       }
-      // exp(t - ref) = q_j S, where ref is the teacher's given log-sum-exp (S = 1) or its maximum
-      if (p.t_lse) {
-        ref = tl_given;
-      } else {
-        ref = warp_max(ref);
-        if (ref == -INFINITY) ref = 0.0f;
-      }
+      // exp(t - ref) = q_j S, where ref is the teacher's given log-sum-exp (S = 1) or its maximum.  A row without an entry
+      // above -inf has no weight whatever was given for it: the log-sum-exp of a teacher that masks everything is -inf too
+      const float most = warp_max(ref);
+      ref = most == -INFINITY ? 0.0f : p.t_lse ? tl_given : most;
       if constexpr (BWD)
         for (int c = lane; c < slots / 8; c += 32) reinterpret_cast<uint4*>(table)[c] = make_uint4(~0u, ~0u, ~0u, ~0u);
       __syncwarp();
@@ -830,10 +827,10 @@ distill_stream_kernel(const DistillParams p) {
   __syncthreads();
   float ref = FWD ? lanes_max<WARPS>(s_red[0][lane % WARPS]) : grad_ref(p, p.lse[row], p.lse[p.rows + row]);
   if (ref == -INFINITY) ref = 0.0f;
-  // exp(t - tref) = q_j S, where tref is the teacher's given log-sum-exp (S = 1) or its maximum
+  // exp(t - tref) = q_j S, where tref is the teacher's given log-sum-exp (S = 1) or its maximum; 0 without an entry above -inf
   float tref = lanes_max<WARPS>(s_red[1][lane % WARPS]);
-  if (p.t_lse) tref = p.t_lse[row];
-  else if (tref == -INFINITY) tref = 0.0f;
+  if (tref == -INFINITY) tref = 0.0f;
+  else if (p.t_lse) tref = p.t_lse[row];
   float S = 0.0f;
   bool again = false;
   for (int j = tid; j < k; j += DF_THREADS) {

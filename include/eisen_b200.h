@@ -314,7 +314,8 @@ int eisen_top_logits(void* stream, const void* logits, long long ld, float* valu
  * Gradient of a row: kd_weight T (Q p_i - sum of q_j with id_j = i) + ce_weight (softmax(x)_i - [i = y]), Q = sum q_j;
  * the 1e-8 takes no part in it (as in eisen_ce_bwd).
  *   teacher_ids [rows, k] int32: negative entries are absent (their teacher_logits are not read); ids may repeat.
- *     An id >= vocab raises *bad_id_flag and counts as absent.  A row without entries has no distillation term.
+ *     An id >= vocab raises *bad_id_flag and counts as absent.  A row without entries above -inf has no
+ *     distillation term, whatever its teacher_lse.
  *   teacher_logits [rows, k] f32.  1 <= k <= 1024.
  *   targets [rows] int32, or null (every row counts; ce_weight must then be 0).  Rows whose target is ignore_index
  *     have loss 0 and gradient 0, whatever their logits hold; a target outside [0, vocab) raises *bad_id_flag and its

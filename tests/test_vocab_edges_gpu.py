@@ -1,0 +1,63 @@
+"""The vocabulary-end operators on rows and calls at the edge of what their documentation allows: teacher rows without
+entries, rows whose logits are all the lowest of their type, every kind of exponential in both row forms, sums in a fixed order,
+tensors that take no gradient, refusals."""
+import math
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+import eisen_b200 as eb  # noqa: E402
+from eisen_b200.graph import BF16_MIXED, FP32  # noqa: E402
+from test_vocab_graph_gpu import CFG, data, f64_distill, model, new_graph  # noqa: E402
+from test_vocab_ops_gpu import Case, EPS_P, Head, P, STEP, dev, gen, top  # noqa: E402
+
+FORMS = [(4, 500), (3, 40000), (700, 500), (400, 12000)]  # few rows (one CTA, several CTAs each), rows in numbers, and in numbers and long
+
+
+# ------------------------------------------------------------------------------------------ teacher rows without entries
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab", FORMS)
+def test_rows_without_teacher_entries_whatever_their_log_sum_exp(dtype, rows, vocab):
+    """Entries that are absent or -inf have no weight, and a row of them has no distillation term: its given log-sum-exp
+    (-inf for a teacher that masks everything, or nothing that was ever set) is not looked at."""
+    c = Case(dtype, rows, vocab, 6, 2.0, 0.6, 0.4, full=True, ignored=0.0, absent=0.0)
+    empty = [0, 1, rows - 1]
+    c.ids[0] = -1
+    c.tv[1] = -math.inf
+    c.ids[rows - 1, :3] = -1
+    c.tv[rows - 1, 3:] = -math.inf
+    c.tlse[0], c.tlse[1], c.tlse[rows - 1] = math.nan, -math.inf, -math.inf
+    given, c.tlse = c.tlse, c.tlse.clone()
+    c.tlse[empty] = 0.0  # in the formula the term is 0 whatever stands here
+    c.expected()
+    c.tlse = given
+    loss, row, lse = c.fwd()
+    c.check_loss(loss, row, lse)
+    d = torch.full_like(c.x, 5.0)
+    c.bwd(lse, d)
+    c.check_grad(d)
+    d.fill_(5.0)
+    c.check_loss(*c.fused(d))
+    c.check_grad(d, fused=True)
+
+
+@pytest.mark.parametrize("rows", [5, 700])
+def test_masked_teacher_row_to_student(rows):
+    """A teacher row of nothing but -inf through the top logits into the loss."""
+    teacher = torch.randn(rows, 900, generator=gen(3), device=dev())
+    teacher[2] = -math.inf
+    v, i, s = top(teacher, 4, 2.0)
+    assert (v[2] == -math.inf).all() and float(s[2]) == -math.inf
+    c = Case(torch.float32, rows, 900, 4, 2.0, 1.0, 0.0, ignored=0.0, absent=0.0)
+    c.ids, c.tv = i, v
+    c.tlse = torch.where(torch.isfinite(s), s, torch.zeros_like(s))
+    c.expected()
+    c.tlse = s
+    d = torch.full_like(c.x, 5.0)
+    loss, row, _ = c.fused(d)
+    c.check_loss(loss, row)
+    c.check_grad(d)
+    assert float(row[2]) == 0.0 and (d[2] == 0).all()
