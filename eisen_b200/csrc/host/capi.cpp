@@ -300,6 +300,7 @@ int eisen_graph_copy_from(void* g, void* src, long long src_id, long long* out) 
     Graph& to = G(g);
     Graph& from = G(src);
     const HTensor t = from.tensors.at(src_id);
+    if (t.dtype == 1 && to.precision == Precision::Fp32) throw EisenException(EISEN_ERR_INVALID, "copy_from: a bf16 tensor has no place in an Fp32 graph");
     const bool apart = to.stream != from.stream;
     if (apart && (to.capturing || from.capturing)) throw EisenException(EISEN_ERR_INVALID, "copy_from: a capture may not wait on another graph's stream");
     cudaEvent_t ev = nullptr;

@@ -431,6 +431,9 @@ void Graph::backward_from(int64_t begin) {
 }
 
 const void* Graph::operand(const HTensor& t) const {
+  // the kernels read numel elements of the graph's activation type, whatever stands here
+  if (t.dtype == DT_I32) invalid("a tensor of ids used as an operand");
+  if (precision == Precision::Fp32 && t.dtype == 1) invalid("a bf16 tensor used in Fp32 mode");
   if (precision == Precision::Bf16Mixed && t.dtype == 0) {
     if (!t.shadow) throw EisenException(EISEN_ERR_INVALID, "f32 tensor without a bf16 shadow used in Bf16Mixed mode");
     return t.shadow;

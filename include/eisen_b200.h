@@ -589,7 +589,8 @@ int eisen_graph_lm_head_distill(void* g, long long h, long long w, long long tea
                                 long long chunk_rows, long long* out);
 int eisen_graph_sync_ids_to_cpu(void* g, long long id, int* out);   /* an id tensor to the host */
 /* A tensor of another graph (a teacher's top logits) as an activation without gradient of this one: a copy on this graph's
- * stream, ordered behind the other stream's work so far. */
+ * stream, ordered behind the other stream's work so far.  Types stay as they are: f32 and ids go anywhere, a bf16 activation only
+ * into another Bf16Mixed graph. */
 int eisen_graph_copy_from(void* g, void* src_graph, long long src_id, long long* out);
 int eisen_graph_rms_norm(void* g, long long x, long long w, float eps, long long* out);
 int eisen_graph_rope(void* g, long long a, long long head_dim, long long* out);

@@ -61,3 +61,27 @@ def test_masked_teacher_row_to_student(rows):
     c.check_loss(loss, row)
     c.check_grad(d)
     assert float(row[2]) == 0.0 and (d[2] == 0).all()
+
+
+# ------------------------------------------------------------------------------------------ tensors of another type
+def test_tensors_of_another_type_are_not_read_as_logits():
+    """A kernel reads as many elements of the graph's own type as the tensor has: a bf16 buffer is half of that in f32."""
+    x, ids, tv, _ = data(4, 64, 3)
+    b, f = new_graph(BF16_MIXED), new_graph(FP32)
+    act = b.alloc_pooled([4, 64])
+    b.load_tensor_data(act, x)
+    with pytest.raises(eb.EisenError, match="copy_from"):
+        f.copy_from(b, act)
+    again = new_graph(BF16_MIXED)
+    same = again.copy_from(b, act)
+    v, i, s = again.top_logits(same, 3)
+    assert (again.ids_to_cpu(i).reshape(4, 3) == np.argsort(-b.data(act).reshape(4, 64), axis=1, kind="stable")[:, :3]).all()
+    for g in (b, f):
+        t, lg = g.alloc_ids([4, 64], np.zeros(256)), g.alloc([4, 3], tv)
+        for call in (lambda: g.top_logits(t, 3), lambda: g.distill(t, g.alloc_ids([4, 3], ids), lg, 4)):
+            with pytest.raises(eb.EisenError, match="ids"):
+                call()
+    teacher = b.copy_from(f, f.alloc([4, 3], tv))  # f32 values go anywhere ...
+    with pytest.raises(eb.EisenError, match="shadow"):
+        b.top_logits(teacher, 2)  # ... but are no bf16 logits
+    assert np.isfinite(b.data(b.distill(act, b.alloc_ids([4, 3], ids), teacher, 4))[0])
