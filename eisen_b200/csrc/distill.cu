@@ -40,6 +40,7 @@ struct DistillParams {
   int accumulate;
   int* bad_id_flag;
   int sum_kind, grad_kind;  // see RowExp
+  int* fault_word;
   RowShape shape;
 };
 
@@ -693,17 +694,12 @@ distill_pipe_kernel(const DistillParams p) {
       }
     }
   }
-  if (ring.abort_flag) {  // a wait ran out: nothing of this CTA's rows can be relied on, and they say so
-    for (int i = 0; i < 64; ++i) __nanosleep(1000);  // copies in flight end before the CTA does
+  if (ring_gave_up(ring, C, p.fault_word)) {
     for (int i = tid; i < n_mine; i += blockDim.x) {
       const long long row = row0 + (long long)i * stride;
       if (FWD) p.row_loss[row] = NAN;
       if (BWD) dlogits[row * p.ldd] = from_f32<T>(NAN);
     }
-  }
-  if (C > 1) {
-    __syncwarp();
-    cluster_sync_all();  // nobody leaves while a peer may still write to it
   }
 }
 
@@ -1023,6 +1019,7 @@ int distill_launch(const char* what, DistillParams& p, cudaStream_t s) {
 }
 
 int distill_run(const char* what, int mode, DistillParams& p, int dtype, cudaStream_t s) {
+  p.fault_word = fault_word();
   // both exponentials are summed where the caller takes both log-sum-exps or the cross-entropy needs its own
   const bool one = p.temperature == 1.0f;
   p.sum_kind = one || (!p.lse && p.ce_weight == 0.0f) ? ONE : exp_kind(p.temperature, dtype);

@@ -13,6 +13,15 @@ void set_error(const char* msg);
 int fail(int code, const char* msg);
 int check_launch(const char* what);  // also counts the launch
 void count_launch();
+// Where kernels whose entry points take no status argument leave their fault code: the current device's own word
+// (eisen_pending_fault; null where it cannot be had), or the one that the calling thread has set
+int* fault_word();
+struct FaultWordScope {
+  int* before;
+  explicit FaultWordScope(int* word);
+  ~FaultWordScope();
+  FaultWordScope(const FaultWordScope&) = delete;
+};
 
 // Index of the current device for per-device one-time set-up (kernel attributes and occupancy
 // are properties of a device, not of the process).  Devices beyond 63 share the last slot.

@@ -91,6 +91,16 @@ int eisen_graph_selftest_bounded_wait(void* g, long long budget_cycles) {
     if (rc) throw EisenException(rc, eisen_last_error());
   });
 }
+int eisen_graph_selftest_row_frame(void* g, long long budget_cycles) {
+  return guarded([&] {
+    Graph& gr = G(g);
+    FaultWordScope faults(gr.status_dev);
+    float* out = static_cast<float*>(gr.pool_get(64 * 4));
+    const int rc = eisen_selftest_row_frame(gr.stream, out, 64, budget_cycles);
+    gr.pool_put(out, 64 * 4);
+    if (rc) throw EisenException(rc, eisen_last_error());
+  });
+}
 int eisen_graph_set_vram_budget(void* g, long long budget_bytes, long long activation_reserve_bytes) {
   return guarded([&] {
     if (budget_bytes < 0 || activation_reserve_bytes < 0) throw EisenException(EISEN_ERR_INVALID, "set_vram_budget: negative size");

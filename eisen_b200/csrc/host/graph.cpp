@@ -9,6 +9,7 @@
 #include <cstring>
 
 #include "../../../include/eisen_b200.h"
+#include "../errors.h"
 
 namespace eisen {
 
@@ -346,7 +347,7 @@ void Graph::check_status() {
   cuck(cudaMemcpy(h, status_dev, sizeof(h), cudaMemcpyDeviceToHost), "read status");
   if (h[0] != 0) {
     cudaMemset(status_dev, 0, 4);
-    throw EisenException(EISEN_ERR_KERNEL, "a tensor-core kernel gave up on a bounded wait (fault code " + std::to_string(h[0]) + ")");
+    throw EisenException(EISEN_ERR_KERNEL, "a kernel gave up on a bounded wait (fault code " + std::to_string(h[0]) + ")");
   }
   if (h[16] != 0) {
     cudaMemset(bad_id_dev, 0, 4);
@@ -1369,6 +1370,7 @@ void Graph::top_logits(int64_t logits, int64_t k, float temperature, int64_t out
   out3[1] = alloc_pooled_dtype(ks, DT_I32);
   out3[2] = alloc_pooled_dtype(ls, 0);
   for (int i = 0; i < 3; ++i) tensors[out3[i]].constant = true;
+  FaultWordScope faults(status_dev);
   ck(eisen_top_logits(stream, operand(tensors[logits]), vocab, (float*)tensors[out3[0]].data, (int*)tensors[out3[1]].data,
                       (float*)tensors[out3[2]].data, rows, vocab, k, temperature, act_dtype()),
      "top_logits");
@@ -1393,6 +1395,7 @@ void Graph::lm_head_top_logits(int64_t h, int64_t w, int64_t k, float temperatur
     const int64_t m = std::min(chunk_rows, d.rows - r0);
     gemm(*this, false, !trans_b, m, d.vocab, d.k, (const char*)operand(tensors[h]) + (size_t)r0 * d.k * dsize(dt), weight_operand(w), slab,
          dt, false);
+    FaultWordScope faults(status_dev);
     ck(eisen_top_logits(stream, slab, d.vocab, (float*)tensors[out3[0]].data + r0 * k, (int*)tensors[out3[1]].data + r0 * k,
                         (float*)tensors[out3[2]].data + r0, m, d.vocab, k, temperature, dt),
        "lm_head_top_logits");
@@ -1421,6 +1424,7 @@ int64_t Graph::distill(int64_t logits, const Teacher& t, int64_t tid, float norm
   tensors[lse].constant = tensors[row_loss].constant = true;
   const int* targets = tid >= 0 ? (const int*)tensors[tid].data : nullptr;
   const float* t_lse = t.lse >= 0 ? (const float*)tensors[t.lse].data : nullptr;
+  FaultWordScope faults(status_dev);
   ck(eisen_distill_fwd(stream, operand(tensors[logits]), vocab, (const int*)tensors[t.ids].data, (const float*)tensors[t.logits].data, t_lse,
                        targets, (float*)tensors[o].data, (float*)tensors[row_loss].data, (float*)tensors[lse].data, rows, vocab, k, -1,
                        t.temperature, t.kd_weight * normalizer, t.ce_weight * normalizer, dt, bad_id_dev + 1),
@@ -1430,6 +1434,7 @@ int64_t Graph::distill(int64_t logits, const Teacher& t, int64_t tid, float norm
       OUT_GRAD_OR_RETURN(o);
       HTensor& gl = tensors[logits];
       ensure_grad(logits);
+      FaultWordScope faults(status_dev);
       ck(eisen_distill_bwd(stream, operand(gl), vocab, (const int*)tensors[t.ids].data, (const float*)tensors[t.logits].data,
                            t.lse >= 0 ? (const float*)tensors[t.lse].data : nullptr, tid >= 0 ? (const int*)tensors[tid].data : nullptr,
                            (const float*)tensors[lse].data, gl.grad, vocab, (const float*)to.grad, rows, vocab, k, -1, t.temperature,
@@ -1467,6 +1472,7 @@ int64_t Graph::lm_head_distill(int64_t h, int64_t w, const Teacher& t, int64_t t
     const float* t_lse = t.lse >= 0 ? (const float*)tensors[t.lse].data + r0 : nullptr;
     const int* targets = tid >= 0 ? (const int*)tensors[tid].data + r0 : nullptr;
     const float kd = t.kd_weight * normalizer, ce = t.ce_weight * normalizer;
+    FaultWordScope faults(status_dev);
     if (!grads) {
       ck(eisen_distill_fwd(stream, slab, d.vocab, ids, tv, t_lse, targets, nullptr, rl + r0, nullptr, m, d.vocab, k, -1, t.temperature, kd, ce,
                            dt, bad_id_dev + 1),

@@ -21,6 +21,7 @@ enum KernelFault : int {
   FAULT_WAIT_TMEM_FULL = 3,
   FAULT_WAIT_TMEM_EMPTY = 4,
   FAULT_WAIT_ATTN = 5,
+  FAULT_WAIT_ROWS = 6,  // a wait of the row kernels (row_pipe.cuh), in the device's own word
   FAULT_WAIT_SELFTEST = 99,  // the wait of eisen_selftest_bounded_wait, which is meant to run out
 };
 

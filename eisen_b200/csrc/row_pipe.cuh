@@ -194,16 +194,29 @@ __device__ __forceinline__ void ring_init(RowRing& r, int stages, int group_warp
 // Waits until the copy of this CTA's i-th row has landed.  Successive rows of a stage may belong to different groups, and
 // a group that runs ahead (over rows that are skipped) must not take the end of the stage's row before for its own: a
 // row is sent for only after that one was used up, so once it is, the phase of its own copy is the current one.
-__device__ __forceinline__ void ring_wait_row(RowRing& r, int i, int stage, uint32_t phase) {
+__device__ __forceinline__ void ring_wait_row(RowRing& r, int i, int stage, uint32_t phase, long long budget = EISEN_WAIT_CYCLES) {
   if (r.issued <= i) {
     const long long t0 = clock64();
     while (r.issued <= i) {
       if (*(volatile int*)&r.abort_flag) return;
-      if (clock64() - t0 > EISEN_WAIT_CYCLES) { *(volatile int*)&r.abort_flag = 1; return; }
+      if (clock64() - t0 > budget) { *(volatile int*)&r.abort_flag = 1; return; }
     }
   }
   __threadfence_block();
-  mbar_wait(&r.full[stage], phase, &r.abort_flag, nullptr, FAULT_WAIT_FULL);
+  mbar_wait(&r.full[stage], phase, &r.abort_flag, nullptr, FAULT_WAIT_FULL, budget);
+}
+
+// The end of a kernel, for all of its threads: true where a wait of this CTA ran out, so that the rows it shares in cannot be
+// relied on and are to be marked.  Groups go on after such a wait, so every warp of the CTA, and of the cluster's other CTAs, has to be
+// through before anything is marked, or a row would be written over its mark.  (A cluster's CTAs do not leave before that
+// anyway: a peer may still write to them or read their lists.)  The copies in flight end before the CTA does.
+__device__ __forceinline__ bool ring_gave_up(RowRing& r, int cluster, int* fault_word) {
+  __syncthreads();
+  if (cluster > 1) cluster_sync_all();
+  if (!*(volatile int*)&r.abort_flag) return false;
+  if (threadIdx.x == 0 && fault_word) atomicCAS(fault_word, 0, FAULT_WAIT_ROWS);
+  for (int i = 0; i < 64; ++i) __nanosleep(1000);
+  return true;
 }
 
 // The loading warp.  slice(row) -> RowSlice; skip(row): the row's logits are not looked at (its stage passes

@@ -5,6 +5,7 @@
 // spins without a limit: no TMA, no tensor memory, no other CTA is involved.
 #include "ptx.cuh"
 #include "errors.h"
+#include "row_pipe.cuh"
 #include "../../include/eisen_b200.h"
 
 namespace eisen {
@@ -35,8 +36,35 @@ __global__ void __launch_bounds__(32) bounded_wait_selftest_kernel(int* status, 
   }
 }
 
+// The row kernels' frame (row_pipe.cuh) when a wait runs out: two groups of one warp take rows in turn, the first one is through
+// its rows and gone, the second waits, with a short budget, for a row that the loading warp never sends for, and then goes on as a
+// group does.  All rows must be marked in the end, those of the first group too.
+__global__ void __launch_bounds__(96) row_frame_selftest_kernel(float* out, int rows, long long budget, int* fault_word) {
+  __shared__ RowRing ring;
+  const int g = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  ring_init(ring, 2, 1);
+  __syncthreads();
+  if (g < 2) {
+    for (int i = g; i < rows; i += 2) {
+      if (g == 1) ring_wait_row(ring, i, 1, 0, budget);
+      if (lane == 0) out[i] = 1.0f;
+      __syncwarp();
+    }
+  }
+  if (ring_gave_up(ring, 1, fault_word))
+    for (int i = threadIdx.x; i < rows; i += blockDim.x) out[i] = NAN;
+}
+
 }  // namespace
 }  // namespace eisen
+
+extern "C" int eisen_selftest_row_frame(void* stream, float* out, int rows, long long budget_cycles) {
+  if (!out || rows < 1 || rows > 4096) return eisen::fail(EISEN_ERR_INVALID, "selftest_row_frame: out is null, or rows not in [1, 4096]");
+  if (budget_cycles < 1000 || budget_cycles > 200000000ll)
+    return eisen::fail(EISEN_ERR_INVALID, "selftest_row_frame: budget must be between 1e3 and 2e8 cycles");
+  eisen::row_frame_selftest_kernel<<<1, 96, 0, (cudaStream_t)stream>>>(out, rows, budget_cycles, eisen::fault_word());
+  return eisen::check_launch("selftest_row_frame");
+}
 
 extern "C" int eisen_selftest_bounded_wait(void* stream, int* status, long long budget_cycles, int* report5) {
   if (!status) return eisen::fail(EISEN_ERR_INVALID, "selftest_bounded_wait: status is null");

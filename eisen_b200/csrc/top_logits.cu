@@ -32,6 +32,7 @@ struct TopParams {
   long long rows;
   int vocab, k;
   float inv_t;
+  int* fault_word;
   int keyed;  // top_stream_kernel: there is room for the vectors' keys
   RowShape shape;
 };
@@ -506,13 +507,15 @@ top_pipe_kernel(const TopParams p) {
       }
     }
   }
-  if (ring.abort_flag) {  // a wait ran out: nothing of this CTA's rows can be relied on, and they say so
-    for (int i = 0; i < 64; ++i) __nanosleep(1000);  // copies in flight end before the CTA does
-    for (int i = tid; i < n_mine; i += blockDim.x) p.values[(row0 + (long long)i * stride) * k] = NAN;
-  }
-  if (C > 1) {
-    __syncwarp();
-    cluster_sync_all();  // nobody leaves while a peer may still read its lists
+  if (ring_gave_up(ring, C, p.fault_word)) {
+    for (int i = 0; i < n_mine; ++i) {
+      const long long row = row0 + (long long)i * stride;
+      for (int j = tid; j < k; j += blockDim.x) {
+        p.values[row * k + j] = NAN;
+        p.ids[row * k + j] = -1;  // an absent entry to whoever reads on
+      }
+      if (tid == 0 && p.lse) p.lse[row] = NAN;
+    }
   }
 }
 
@@ -774,6 +777,6 @@ extern "C" int eisen_top_logits(void* stream, const void* logits, long long ld, 
   if (rows == 0) return 0;
   if (!logits || !values || !ids) return fail(EISEN_ERR_INVALID, "top_logits: logits, values and ids must not be null");
   if (reinterpret_cast<uintptr_t>(logits) % (dtype == DT_F32 ? 4 : 2)) return fail(EISEN_ERR_INVALID, "top_logits: unaligned pointer");
-  TopParams p = {logits, ld, values, ids, lse, rows, (int)vocab, (int)k, 1.0f / temperature, 0, {}};
+  TopParams p = {logits, ld, values, ids, lse, rows, (int)vocab, (int)k, 1.0f / temperature, fault_word(), 0, {}};
   EISEN_DISPATCH_DTYPE(dtype, T, { return top_launch<T>(p, (cudaStream_t)stream); });
 }

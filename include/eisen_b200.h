@@ -70,6 +70,14 @@ int eisen_get_deterministic(void);
  * would.  report5 (device int[5], may be null): first wait succeeded, second wait succeeded, abort
  * flag, first wait used its budget, second wait returned at once. */
 int eisen_selftest_bounded_wait(void* stream, int* status, long long budget_cycles, int* report5);
+/* The same for the frame of the row kernels (eisen_top_logits, eisen_distill_*): out [rows] holds 1 where a group of threads went
+ * through a row; the second group's wait runs out, so all of out must be NaN in the end and eisen_pending_fault say 6. */
+int eisen_selftest_row_frame(void* stream, float* out, int rows, long long budget_cycles);
+/* *code (host) = fault code of kernels on the current device that take no status argument (eisen_top_logits, eisen_distill_*: 6, a
+ * wait ran out), 0 = none; waits for the device, reads the code and clears it.  The rows of such a kernel are marked besides: NaN in
+ * row_loss, in a gradient row's first element, in values and lse, -1 in ids.  Graphs have a word of their own, which
+ * eisen_graph_synchronize looks at. */
+int eisen_pending_fault(int* code);
 
 /* ------------------------------------------------------------------------------------------
  * Dense contractions
@@ -536,6 +544,7 @@ int eisen_graph_exec_destroy(void* exec);
 /* runs eisen_selftest_bounded_wait on the graph's stream against the graph's own fault word: the
  * next eisen_graph_synchronize must return EISEN_ERR_KERNEL and clear the word */
 int eisen_graph_selftest_bounded_wait(void* g, long long budget_cycles);
+int eisen_graph_selftest_row_frame(void* g, long long budget_cycles); /* likewise with eisen_selftest_row_frame */
 int eisen_graph_counts(void* g, long long* num_tensors, long long* tape_len, long long* num_params);
 /* out5: pool bytes in use, pool bytes cached, device bytes allocated, pool hits, pool misses */
 int eisen_graph_pool_stats(void* g, long long* out5);

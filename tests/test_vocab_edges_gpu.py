@@ -85,3 +85,30 @@ def test_tensors_of_another_type_are_not_read_as_logits():
     with pytest.raises(eb.EisenError, match="shadow"):
         b.top_logits(teacher, 2)  # ... but are no bf16 logits
     assert np.isfinite(b.data(b.distill(act, b.alloc_ids([4, 3], ids), teacher, 4))[0])
+
+
+# ------------------------------------------------------------------------------------------ a wait that runs out
+@pytest.mark.parametrize("rows", [2, 31, 50, 1000])
+def test_rows_are_marked_when_a_wait_runs_out(rows):
+    """A group that gives up marks the rows of the groups that were through long before, and the device's word says so."""
+    out = torch.zeros(rows, device=dev())
+    code = torch.zeros(1, dtype=torch.int32)
+    eb.call("eisen_pending_fault", code.data_ptr())
+    eb.call("eisen_selftest_row_frame", torch.cuda.current_stream().cuda_stream, P(out), rows, 200000)
+    eb.call("eisen_pending_fault", code.data_ptr())
+    assert int(code) == 6 and torch.isnan(out).all()
+    eb.call("eisen_pending_fault", code.data_ptr())
+    assert int(code) == 0
+
+
+def test_a_graph_reports_the_wait_of_its_own_row_kernel():
+    g = new_graph()
+    eb.call("eisen_graph_selftest_row_frame", g._h, 200000)
+    with pytest.raises(eb.EisenError, match="bounded wait"):
+        g.synchronize()
+    g.synchronize()
+    code = torch.zeros(1, dtype=torch.int32)
+    eb.call("eisen_pending_fault", code.data_ptr())
+    assert int(code) == 0
+    with pytest.raises(eb.EisenError):
+        eb.call("eisen_selftest_row_frame", None, None, 5, 200000)
