@@ -154,6 +154,11 @@ __device__ __forceinline__ float grad_ref(const DistillParams& p, float lt, floa
   return p.temperature < 1.0f ? fminf(l1, lt * p.temperature) : l1;
 }
 
+// Rows whose log-sum-exps are no use to a gradient alone: a 32-bit number beyond 512 is off by 2^-16 and more, and so would every
+// probability be by that of itself (a row that is masked all over by its type's lowest value has them at 1 instead of
+// 1 / n).  Their sums are formed again, relative to the row's largest entry.
+__device__ __forceinline__ bool sums_again(float lt, float l1) { return !(fabsf(lt) <= 512.0f && fabsf(l1) <= 512.0f); }
+
 // the kind for both exponentials at a temperature other than 1
 int exp_kind(float temperature, int dtype) {
   if (dtype == DT_BF16)
@@ -226,8 +231,8 @@ struct Entries {
 struct RowTeacher {  // exp(t - tref) = q_j S;  Q = sum of the q_j
   float tref, S, Q;
 };
-struct RowStats {  // what the group found
-  float ref, kt, k1, lt, l1;
+struct RowStats {  // what the group found; nt, n1: logarithms of the two sums relative to ref
+  float ref, kt, k1, nt, n1;
 };
 
 template <typename T, int GT, int G, int MODE>
@@ -462,19 +467,23 @@ distill_pipe_kernel(const DistillParams p) {
         if (has_ce && !met && lane == 0 && y >= e_lo && y < e_hi) rewrite(k, y, c1);
       }
       if (FWD && rank == 0) {
-        const float tl = p.t_lse || S == 0.0f ? te.tref : te.tref + logf(S);  // ln q_j = t_j - tl
+        // in differences: far from 0 the log-sum-exps themselves are rounded too coarsely
+        const float ns = p.t_lse || S == 0.0f ? 0.0f : logf(S);
         float kl = 0.0f;
         for (int j = lane; j < k; j += 32) {
-          const float t = e.t[j], q = expf(t - tl);
-          if (q > 0.0f || q != q) kl += q * (t - tl - (e.x[j] * p.inv_t - st.lt));
+          const float lq = e.t[j] - te.tref - ns, q = expf(lq);
+          if (q > 0.0f || q != q) kl += q * (lq - ((e.x[j] - st.ref) * p.inv_t - st.nt));
         }
         kl = warp_sum(kl);
         if (lane == 0) {
           float l = 0.0f;
           if (has_kd) l = p.kd_weight * p.temperature * p.temperature * kl;
-          if (has_ce) l -= p.ce_weight * logf(expf(e.x[k] - st.l1) + 1e-8f);
+          if (has_ce) l -= p.ce_weight * logf(expf(e.x[k] - st.ref - st.n1) + 1e-8f);
           p.row_loss[row] = l;
-          if (p.lse) { p.lse[row] = st.lt; p.lse[p.rows + row] = st.l1; }
+          if (p.lse) {
+            p.lse[row] = st.ref * p.inv_t + st.nt;
+            p.lse[p.rows + row] = st.ref + st.n1;
+          }
         }
       }
       mbar_arrive_warp(&finished[g][set]);
@@ -494,6 +503,7 @@ distill_pipe_kernel(const DistillParams p) {
     };
     request(g);
     int turn = -1;       // rows this group has worked on (skipped ones do not count)
+    int met_rows = 0;    // those of them whose slices have met
     int stage = g - G;   // the stage of row i, and its phase; a ring has at least G stages
     uint32_t phase = 0;
     for (int i = g; i < n_mine; i += G) {
@@ -538,8 +548,9 @@ distill_pipe_kernel(const DistillParams p) {
       if (own0) vec[0] = edge0;
       if (own1) vec[cnt - 1] = edge1;
 
+      const bool sums = FWD || sums_again(lt_given, l1_given);
       float ref = FWD ? 0.0f : grad_ref(p, lt_given, l1_given), own_ref = ref, st = 0.0f, s1 = 0.0f, own_st = 1.0f;
-      if constexpr (FWD) {
+      if (sums) {
         float m = -INFINITY;
         if constexpr (sizeof(T) == 2) {
           auto pair = [](uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); };
@@ -585,7 +596,7 @@ distill_pipe_kernel(const DistillParams p) {
               x[c] = h0;
               x[c + 1] = h1;
             }
-            if constexpr (BWD && Ex::KEEPS) vec[v] = keep_vec<T>(x);
+            if constexpr (FWD && BWD && Ex::KEEPS) vec[v] = keep_vec<T>(x);
           }
           st = (sa[0] + sa[1]) * Ex::scale_t;
           s1 = (sb[0] + sb[1]) * Ex::scale_1;
@@ -604,7 +615,7 @@ distill_pipe_kernel(const DistillParams p) {
           own_st = st;
           // the entry warp has read its logits: after the exchange the other CTAs may write theirs over them
           mbar_wait(&ready[g][set], set_phase, &ring.abort_flag, nullptr, FAULT_WAIT_FULL);
-          float(*met)[3] = s_xch[g][set];
+          float(*met)[3] = s_xch[g][met_rows & 1];
           if (gt < C) {
             const uint32_t to = mapa_cluster(smem_u32(&met[rank][0]), gt);
             st_cluster_f32(to, st == 0.0f ? -INFINITY : ref);  // a slice without a finite entry has no say in the maximum
@@ -612,7 +623,8 @@ distill_pipe_kernel(const DistillParams p) {
             st_cluster_f32(to + 8, s1);
             mbar_arrive_release_cluster(mapa_cluster(smem_u32(&xbar[g]), gt));
           }
-          mbar_wait_cluster(&xbar[g], (uint32_t)(turn & 1), &ring.abort_flag);
+          mbar_wait_cluster(&xbar[g], (uint32_t)(met_rows & 1), &ring.abort_flag);
+          ++met_rows;
           float gm = -INFINITY;
           for (int r = 0; r < C; ++r) gm = fmaxf(gm, met[r][0]);
           ref = gm == -INFINITY ? 0.0f : gm;
@@ -624,13 +636,13 @@ distill_pipe_kernel(const DistillParams p) {
           }
         }
       }
-      if (!(FWD && C > 1)) mbar_wait(&ready[g][set], set_phase, &ring.abort_flag, nullptr, FAULT_WAIT_FULL);
+      if (!(sums && C > 1)) mbar_wait(&ready[g][set], set_phase, &ring.abort_flag, nullptr, FAULT_WAIT_FULL);
       // d = kt exp((x - ref) / T) + k1 exp(x - ref): kt, k1 turn the exponentials into weighted probabilities
       float kt = 0.0f, k1 = 0.0f;
       if constexpr (BWD) {
         const float Q = s_teacher[g][set].Q;
-        if (has_kd) kt = FWD ? __fdividef(kq * Q, st) : kq * Q * expf(ref * p.inv_t - lt_given);
-        if (has_ce) k1 = FWD ? __fdividef(c1, p.grad_kind == ONE ? st : s1) : c1 * expf(ref - l1_given);
+        if (has_kd) kt = sums ? __fdividef(kq * Q, st) : kq * Q * expf(ref * p.inv_t - lt_given);
+        if (has_ce) k1 = sums ? __fdividef(c1, p.grad_kind == ONE ? st : s1) : c1 * expf(ref - l1_given);
         if (p.grad_kind == ONE) { kt += k1; k1 = 0.0f; }  // temperature 1: one exponential for both terms
       }
       if (gt == 0) {
@@ -639,8 +651,8 @@ distill_pipe_kernel(const DistillParams p) {
         o.kt = kt;
         o.k1 = k1;
         if constexpr (FWD) {
-          o.lt = ref * p.inv_t + logf(st);
-          o.l1 = p.sum_kind == ONE ? (p.temperature == 1.0f ? o.lt : 0.0f) : ref + logf(s1);
+          o.nt = logf(st);
+          o.n1 = p.sum_kind == ONE ? o.nt : logf(s1);  // temperature 1: the same sum; otherwise there is no use for a second one
         }
       }
       if constexpr (!BWD) {
@@ -649,8 +661,8 @@ distill_pipe_kernel(const DistillParams p) {
         // vectors that go to dlogits as they are
         const int w0 = like(s, dr) ? s.w0 : s.hi, w1 = like(s, dr) ? s.w1 : s.hi;
         // a slice without a finite entry has nothing but zeros
-        const float at = C > 1 && FWD ? (own_st == 0.0f ? 0.0f : expf((own_ref - ref) * p.inv_t)) : 1.0f;
-        const float a1 = C > 1 && FWD ? (own_st == 0.0f ? 0.0f : expf(own_ref - ref)) : 1.0f;
+        const float at = C > 1 && sums ? (own_st == 0.0f ? 0.0f : expf((own_ref - ref) * p.inv_t)) : 1.0f;
+        const float a1 = C > 1 && sums ? (own_st == 0.0f ? 0.0f : expf(own_ref - ref)) : 1.0f;
         with_exp<T>(FWD ? p.sum_kind : p.grad_kind, own_ref, p.inv_t, [&](const auto& ex) {
           using Ex = std::remove_cv_t<std::remove_reference_t<decltype(ex)>>;
           const float mt = kt * at * Ex::scale_t, m1 = k1 * a1 * Ex::scale_1;
@@ -779,7 +791,8 @@ distill_stream_kernel(const DistillParams p) {
   if constexpr (BWD)
     for (int c = tid; c < entry_slots(k) / 8; c += DF_THREADS) reinterpret_cast<uint4*>(table)[c] = make_uint4(~0u, ~0u, ~0u, ~0u);
   float m = -INFINITY, st = 0.0f, s1 = 0.0f;
-  if constexpr (FWD) {
+  const bool sums = FWD || sums_again(p.lse[row], p.lse[p.rows + row]);
+  if (sums) {
 #pragma unroll 1
     for (int v0 = tid; v0 < s.hi; v0 += DF_FLIGHT * DF_THREADS) {
       uint4 raw[DF_FLIGHT];
@@ -814,14 +827,14 @@ distill_stream_kernel(const DistillParams p) {
     }
   }
   // maxima, then the sums relative to them
-  if constexpr (FWD) {
+  if (sums) {
     const float wm = warp_max(m);
     if (lane == 0) s_red[0][warp] = wm;
   }
   tm = warp_max(tm);
   if (lane == 0) s_red[1][warp] = tm;
   __syncthreads();
-  float ref = FWD ? lanes_max<WARPS>(s_red[0][lane % WARPS]) : grad_ref(p, p.lse[row], p.lse[p.rows + row]);
+  float ref = sums ? lanes_max<WARPS>(s_red[0][lane % WARPS]) : grad_ref(p, p.lse[row], p.lse[p.rows + row]);
   if (ref == -INFINITY) ref = 0.0f;
   // exp(t - tref) = q_j S, where tref is the teacher's given log-sum-exp (S = 1) or its maximum; 0 without an entry above -inf
   float tref = lanes_max<WARPS>(s_red[1][lane % WARPS]);
@@ -850,7 +863,7 @@ distill_stream_kernel(const DistillParams p) {
     }
   }
   S = warp_sum(S);
-  if constexpr (FWD) {
+  if (sums) {
     const float mine = m == -INFINITY ? 0.0f : m - ref;
     st = warp_sum(st * expf(mine * p.inv_t));
     s1 = warp_sum(s1 * expf(mine));
@@ -865,11 +878,11 @@ distill_stream_kernel(const DistillParams p) {
   float kl = 0.0f;
   if constexpr (FWD) {
     if (warp == 0 || !BWD) {  // the loss; beside a gradient in the hands of one warp
-      const float lt = ref * p.inv_t + logf(st);
-      const float tl = p.t_lse || S == 0.0f ? tref : tref + logf(S);  // ln q_j = t_j - tl
+      // in differences: far from 0 the log-sum-exps themselves are rounded too coarsely
+      const float nt = logf(st), ns = p.t_lse || S == 0.0f ? 0.0f : logf(S);
       for (int j = BWD ? lane : tid; j < k; j += BWD ? 32 : DF_THREADS) {
-        const float q = expf(e.t[j] - tl);
-        if (q > 0.0f || q != q) kl += q * (e.t[j] - tl - (e.x[j] * p.inv_t - lt));
+        const float lq = e.t[j] - tref - ns, q = expf(lq);
+        if (q > 0.0f || q != q) kl += q * (lq - ((e.x[j] - ref) * p.inv_t - nt));
       }
       kl = warp_sum(kl);
     }
@@ -879,13 +892,15 @@ distill_stream_kernel(const DistillParams p) {
       kl = lanes_sum<WARPS>(s_red[3][lane % WARPS]);
     }
     if (tid == 0) {
-      const float lt = ref * p.inv_t + logf(st);
-      const float l1 = p.sum_kind == ONE ? (p.temperature == 1.0f ? lt : 0.0f) : ref + logf(s1);
+      const float nt = logf(st), n1 = p.sum_kind == ONE ? nt : logf(s1);
       float l = 0.0f;
       if (has_kd) l = p.kd_weight * p.temperature * p.temperature * kl;
-      if (has_ce) l -= p.ce_weight * logf(expf(e.x[k] - l1) + 1e-8f);
+      if (has_ce) l -= p.ce_weight * logf(expf(e.x[k] - ref - n1) + 1e-8f);
       p.row_loss[row] = l;
-      if (p.lse) { p.lse[row] = lt; p.lse[p.rows + row] = l1; }
+      if (p.lse) {
+        p.lse[row] = ref * p.inv_t + nt;
+        p.lse[p.rows + row] = ref + n1;
+      }
     }
   }
   if constexpr (BWD) {
@@ -894,8 +909,8 @@ distill_stream_kernel(const DistillParams p) {
     const float kq = has_kd ? p.kd_weight * p.temperature * g : 0.0f, c1 = has_ce ? p.ce_weight * g : 0.0f;
     const float Q = p.t_lse || S == 0.0f ? S : 1.0f;
     float kt = 0.0f, k1 = 0.0f;
-    if (has_kd) kt = FWD ? __fdividef(kq * Q, st) : kq * Q * expf(ref * p.inv_t - p.lse[row]);
-    if (has_ce) k1 = FWD ? __fdividef(c1, p.grad_kind == ONE ? st : s1) : c1 * expf(ref - p.lse[p.rows + row]);
+    if (has_kd) kt = sums ? __fdividef(kq * Q, st) : kq * Q * expf(ref * p.inv_t - p.lse[row]);
+    if (has_ce) k1 = sums ? __fdividef(c1, p.grad_kind == ONE ? st : s1) : c1 * expf(ref - p.lse[p.rows + row]);
     if (p.grad_kind == ONE) { kt += k1; k1 = 0.0f; }  // temperature 1: one exponential for both terms
 #pragma unroll 1
     for (int v0 = tid; v0 < s.hi; v0 += DF_FLIGHT * DF_THREADS) {

@@ -330,7 +330,7 @@ int eisen_top_logits(void* stream, const void* logits, long long ld, float* valu
  *     row is skipped the same way.
  *   A weight of 0 removes its term.  A counted row needs a finite logit.
  *   lse [2, rows]: log-sum-exp of x / T, then of x (0 for skipped rows); may be null except in eisen_distill_bwd,
- *   which takes what the forward left.  *loss = sum of row_loss in a fixed order; loss may be null.
+ *   which takes what the forward left (and forms the sums of a row again where they are beyond 512 and so too coarse).  *loss = sum of row_loss in a fixed order; loss may be null.
  * eisen_distill_fused forms loss and dlogits (times grad_scale) in one pass over the logits, for an op that ends in
  * the loss; eisen_distill_bwd forms dlogits (op)= gradient * (*grad_out) (null: 1).  dlogits may alias logits
  * (same pointer, same row stride); otherwise the two must not overlap.  ld / ld_d: row strides in entries. */

@@ -112,3 +112,79 @@ def test_a_graph_reports_the_wait_of_its_own_row_kernel():
     assert int(code) == 0
     with pytest.raises(eb.EisenError):
         eb.call("eisen_selftest_row_frame", None, None, 5, 200000)
+
+
+# ------------------------------------------------------------------------------------------ logits far from 0
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab", FORMS)
+@pytest.mark.parametrize("temperature", [0.5, 1.0, 2.0, 3.5])
+def test_rows_of_nothing_but_the_lowest_value(dtype, rows, vocab, temperature):
+    """A row masked all over by its type's lowest value has equal logits: probabilities 1 / n, whatever its log-sum-exp rounds
+    to.  Differences from the row's largest entry are exact here, so the bounds do not grow with the logits."""
+    c = Case(dtype, rows, vocab, 6, temperature, 0.6, 0.4, ignored=0.0, absent=0.0)
+    low = [0, rows // 2, rows - 1]
+    c.x[low] = 0.0
+    c.expected()  # the same for any constant
+    c.x[low] = torch.finfo(dtype).min
+    loss, row, lse = c.fwd()
+    c.check_loss(loss, row)
+    d = torch.full_like(c.x, 5.0)
+    c.bwd(lse, d)
+    c.check_grad(d)
+    base = torch.ones_like(c.x)
+    c.bwd(lse, base, accumulate=1)
+    want = 1.0 + c.d
+    assert ((base.double() - want).abs() <= c.d_tol + STEP[dtype] * (want.abs() + c.d_tol)).all()
+    d.fill_(5.0)
+    loss, row, _ = c.fused(d)
+    c.check_loss(loss, row)
+    c.check_grad(d, fused=True)
+    x = c.x.clone()  # the gradient over the logits, from the log-sum-exps
+    keep, c.x = c.x, x
+    c.bwd(lse, x)
+    c.x = keep
+    c.check_grad(x)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab", FORMS)
+@pytest.mark.parametrize("shift", [3000.0, -70000.0])
+def test_logits_far_from_zero(dtype, rows, vocab, shift):
+    """Loss and gradient depend on differences of logits only: far rows meet the bounds of rows around 0, moved as they
+    are rounded."""
+    c = Case(dtype, rows, vocab, 6, 2.0, 0.6, 0.4, ignored=0.0, absent=0.0)
+    if dtype == torch.bfloat16:  # a few steps of the type apart
+        c.x = (c.x.float() / 3).round() * (2.0 ** -7 * abs(shift))
+    c.x = (c.x.float() + shift).to(dtype)
+    far = c.x
+    c.x = (far.double() - far.double().amax(1, keepdim=True)).float()  # exact
+    assert torch.equal(c.x.double() + far.double().amax(1, keepdim=True), far.double())
+    c.expected()
+    c.x = far
+    loss, row, lse = c.fwd()
+    c.check_loss(loss, row)
+    d = torch.full_like(c.x, 5.0)
+    c.bwd(lse, d)
+    c.check_grad(d)
+    d.fill_(5.0)
+    loss, row, _ = c.fused(d)
+    c.check_loss(loss, row)
+    c.check_grad(d, fused=True)
+
+
+@pytest.mark.parametrize("rows", [3, 400])
+@pytest.mark.parametrize("temperature", [0.5, 1.0, 2.0, 1e-3])
+def test_losses_of_large_logits(rows, temperature):
+    """bf16 logits of 2e4: the row losses, which lie in differences of at most a few hundred."""
+    c = Case(torch.bfloat16, rows, 3000, 6, temperature, 0.5, 0.5, ignored=0.0, absent=0.0)
+    c.x = (c.x.float() * 10 + 20000).to(torch.bfloat16)
+    c.ids[:, 0] = c.x.float().argmax(1).int()
+    c.tv[:] = -math.inf
+    c.tv[:, 0] = 1.0
+    whole, c.x = c.x, c.x.double() - c.x.double().amax(1, keepdim=True)
+    c.expected()
+    c.x = whole
+    loss, row, lse = c.fwd()
+    c.check_loss(loss, row)
+    loss, row, _ = c.fused(torch.empty_like(c.x))
+    c.check_loss(loss, row)
