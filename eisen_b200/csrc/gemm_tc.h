@@ -21,11 +21,14 @@ int gemm_bf16_tc(cudaStream_t stream, int a_mn, int b_mn, int M, int N, int K, c
                  long long lda, const void* B, long long ldb, void* C, long long ldc, const void* R, long long ldr,
                  int out_mode, int split_k, float alpha, int* status, const char** err);
 
-// paired-CTA (cta_group::2) variant: 256 x 256 tile per cluster of two CTAs (gemm_tc2.cu).  alpha_dev: a device scalar that
-// alpha is multiplied by, null for none
+// paired-CTA (cta_group::2) variant: 256 x 256 tile per cluster of two CTAs (gemm_tc2.cu).  With `scale` alpha is multiplied by a
+// device scalar (null: 1), and GEMM_OUT_BF16_ACC adds before it rounds
+struct PairScale {
+  const float* alpha_dev;
+};
 int gemm_bf16_tc_pair(cudaStream_t stream, int a_mn, int b_mn, int M, int N, int K, const void* A, long long lda,
                       const void* B, long long ldb, void* C, long long ldc, const void* R, long long ldr, int out_mode,
-                      int split_k, float alpha, int* status, const char** err, const float* alpha_dev = nullptr);
+                      int split_k, float alpha, int* status, const char** err, const PairScale* scale = nullptr);
 // gate / up projections with the SwiGLU product in the epilogue (dual mode of the paired kernel)
 int gemm_bf16_pair_swiglu(cudaStream_t stream, int M, int N, int K, const void* A, long long lda, const void* Bg,
                           const void* Bu, long long ldb, void* G, void* U, void* H, long long ldo, int* status,

@@ -56,7 +56,7 @@ struct PairParams {
   // cross-entropy epilogues (the LCE instantiations): the product is a tile of logits that is never stored
   const int* targets;
   const float* lse;       // LCE_GRAD
-  const float* grad_out;  // LCE_SCALED, device scalar
+  const float* grad_out;  // LCE_SCALED, device scalar or null
   float2* stats;          // LCE_STATS: [n_tiles][M] (maximum, sum of exp(x - maximum)) of a row's 256 columns
   float* target_logit;    // LCE_STATS: [M]
   int ignore_index, vocab, col_base;  // col_base: vocabulary index of column 0
@@ -99,7 +99,8 @@ struct SegMaps {
 //     products) -> C = D.  Rows that do not count are written as zeros whatever their accumulators hold.  The factor
 //     normalizer * grad_out comes in behind the products: on D it would take every target's entry, about -1, off the
 //     numbers that bf16 has, all of them by the same rounding error.
-//   LCE_SCALED: the plain epilogues with alpha times *grad_out, for the products whose operand D is.
+//   LCE_SCALED: the plain epilogues for the products whose operand D is: alpha times *grad_out, and a bf16 addend is added in
+//     f32 before the one rounding (row by row, without the staging tile).
 constexpr int LCE_NONE = 0, LCE_STATS = 1, LCE_GRAD = 2, LCE_SCALED = 3;
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -173,7 +174,7 @@ gemm_bf16_tc2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
   grid_launch_dependents();
   grid_dependency_wait();
 
-  const float alpha = LCE == LCE_SCALED ? p.alpha * *p.grad_out : p.alpha;
+  const float alpha = LCE == LCE_SCALED && p.grad_out ? p.alpha * *p.grad_out : p.alpha;
   const int tiles_mn = p.m_tiles * p.n_tiles;
   const int cluster_id = blockIdx.x >> 1;
   const int n_clusters = gridDim.x >> 1;
@@ -306,7 +307,7 @@ gemm_bf16_tc2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
       const bool staged = has_k && (out_mode == GEMM_OUT_BF16 || out_mode == GEMM_OUT_BF16_ACC || rope) &&
                           row0 + 32 <= p.M && n0 + PN <= Nn && (ldc % 8) == 0 &&
                           (reinterpret_cast<uintptr_t>(Cp) & 15) == 0 &&
-                          (!acc_bf16 || ((ldr % 8) == 0 && (reinterpret_cast<uintptr_t>(Rp) & 15) == 0));
+                          (!acc_bf16 || (LCE != LCE_SCALED && (ldr % 8) == 0 && (reinterpret_cast<uintptr_t>(Rp) & 15) == 0));
       if constexpr (LCE == LCE_STATS) {
         const int at = row_ok ? p.targets[row] : -1;
         float m = -INFINITY, sum = 0.0f, xt = 0.0f;
@@ -839,7 +840,7 @@ int gemm_bf16_pair_multi_n(cudaStream_t stream, int a_mn, int b_mn, int M, int K
 
 int gemm_bf16_tc_pair(cudaStream_t stream, int a_mn, int b_mn, int M, int N, int K, const void* A, long long lda,
                       const void* B, long long ldb, void* C, long long ldc, const void* R, long long ldr, int out_mode, int split_k,
-                      float alpha, int* status, const char** err, const float* alpha_dev) {
+                      float alpha, int* status, const char** err, const PairScale* scale) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
   if ((lda % 8) || (ldb % 8) || (reinterpret_cast<uintptr_t>(A) & 15) || (reinterpret_cast<uintptr_t>(B) & 15)) {
     if (err) *err = "gemm_bf16_tc: operand rows must be 16-byte aligned (leading dimension % 8 == 0)";
@@ -877,8 +878,8 @@ int gemm_bf16_tc_pair(cudaStream_t stream, int a_mn, int b_mn, int M, int N, int
   p.status = status;
   p.dual = 0; p.C2 = nullptr; p.H = nullptr;
   p.rope_tab = nullptr; p.rope_s = 1; p.rope_hd = 2;
-  p.grad_out = alpha_dev;
-  return pair_launch(stream, tmA, tmB, tmB, p, err, nullptr, alpha_dev ? LCE_SCALED : LCE_NONE);
+  p.grad_out = scale ? scale->alpha_dev : nullptr;
+  return pair_launch(stream, tmA, tmB, tmB, p, err, nullptr, scale ? LCE_SCALED : LCE_NONE);
 }
 
 // Gate / up projections with the SwiGLU product in the epilogue (dual mode of the kernel):

@@ -206,9 +206,10 @@ int eisen_linear_ce_bwd(void* stream, const void* h, long long ldh, const void* 
   auto product = [&](int a_mn, int b_mn, long long M, long long N, long long K, const void* A, long long lda, const void* B,
                      long long ldb, void* C, long long ldc, int mode) {
     const int split = mode == GEMM_OUT_F32_ATOMIC && !deterministic() ? gemm_pair_auto_split_k((int)M, (int)N, (int)K) : 1;
+    const PairScale scale = {grad_out};
     const char* err = nullptr;
     if (gemm_bf16_tc_pair(s, a_mn, b_mn, (int)M, (int)N, (int)K, A, lda, B, ldb, C, ldc, nullptr, 0, mode, split, normalizer, status, &err,
-                          grad_out))
+                          &scale))
       return fail(EISEN_ERR_CUDA, err ? err : "linear_ce_bwd failed");
     count_launch();
     return 0;

@@ -188,3 +188,19 @@ def test_losses_of_large_logits(rows, temperature):
     c.check_loss(loss, row)
     loss, row, _ = c.fused(torch.empty_like(c.x))
     c.check_loss(loss, row)
+
+
+# ------------------------------------------------------------------------------------------ one rounding
+@pytest.mark.parametrize("rows,k,vocab", [(2048, 2048, 500), (300, 136, 1203), (1024, 4096, 256)])
+@pytest.mark.parametrize("tied", [False, True])
+def test_linear_ce_adds_before_it_rounds(rows, k, vocab, tied):
+    """What a gradient's bf16 rounding left off comes back when the rounded gradient is taken away from it again: a product that is
+    rounded before it is added would leave nothing."""
+    c = Head(rows, k, vocab, tied)
+    _, _, lse = c.fwd()
+    dh, dw = c.bwd(lse)
+    rest_h, rest_w = c.bwd(lse, acc_h=1, acc_w=1, dh0=-dh, dw0=-dw)
+    for rest, whole in ((rest_h, dh), (rest_w, dw)):
+        assert (rest.double().abs() <= 2.0 ** -8 * whole.double().abs() + 1e-30).all()
+        counted = rest[whole != 0]  # rows that do not count have no gradient
+        assert float((counted != 0).double().mean()) > 0.9
