@@ -22,9 +22,11 @@ int gemm_bf16_tc(cudaStream_t stream, int a_mn, int b_mn, int M, int N, int K, c
                  int out_mode, int split_k, float alpha, int* status, const char** err);
 
 // paired-CTA (cta_group::2) variant: 256 x 256 tile per cluster of two CTAs (gemm_tc2.cu).  With `scale` alpha is multiplied by a
-// device scalar (null: 1), and GEMM_OUT_BF16_ACC adds before it rounds
+// device scalar (null: 1), GEMM_OUT_BF16_ACC adds before it rounds, and the k slices of an f32 output lie slice_stride elements
+// apart instead of adding up in one place (0: they add up)
 struct PairScale {
   const float* alpha_dev;
+  long long slice_stride;
 };
 int gemm_bf16_tc_pair(cudaStream_t stream, int a_mn, int b_mn, int M, int N, int K, const void* A, long long lda,
                       const void* B, long long ldb, void* C, long long ldc, const void* R, long long ldr, int out_mode,
@@ -56,6 +58,9 @@ int gemm_bf16_pair_ce(cudaStream_t stream, int b_mn, int M, int N, int K, const 
 // columns of the output tile one statistics entry of gemm_bf16_pair_ce covers
 constexpr int GEMM_CE_COLS = 256;
 int gemm_pair_auto_split_k(int M, int N, int K);
+// ... with outputs of their own that are added up afterwards: the number of slices worth their traffic, at most `most`.  The traffic is
+// paid once for `K_all` elements of k, `K` of them in the launch in question
+int gemm_pair_split_k_apart(long long M, long long N, long long K, long long K_all, int most);
 // m-tiles per band of the paired kernel's tile order; 0 = chosen by the DRAM-traffic model
 void gemm_pair_set_band(int band);
 int gemm_num_sms();

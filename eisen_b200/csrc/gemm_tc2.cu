@@ -14,6 +14,7 @@
 
 #include <cuda.h>
 
+#include <algorithm>
 #include <climits>
 
 namespace eisen {
@@ -57,6 +58,7 @@ struct PairParams {
   const int* targets;
   const float* lse;       // LCE_GRAD
   const float* grad_out;  // LCE_SCALED, device scalar or null
+  long long slice_stride; // LCE_SCALED: elements between the f32 outputs of two k slices
   float2* stats;          // LCE_STATS: [n_tiles][M] (maximum, sum of exp(x - maximum)) of a row's 256 columns
   float* target_logit;    // LCE_STATS: [M]
   int ignore_index, vocab, col_base;  // col_base: vocabulary index of column 0
@@ -100,7 +102,7 @@ struct SegMaps {
 //     normalizer * grad_out comes in behind the products: on D it would take every target's entry, about -1, off the
 //     numbers that bf16 has, all of them by the same rounding error.
 //   LCE_SCALED: the plain epilogues for the products whose operand D is: alpha times *grad_out, and a bf16 addend is added in
-//     f32 before the one rounding (row by row, without the staging tile).
+//     f32 before the one rounding (row by row, without the staging tile).  The k slices may have outputs of their own.
 constexpr int LCE_NONE = 0, LCE_STATS = 1, LCE_GRAD = 2, LCE_SCALED = 3;
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -293,6 +295,7 @@ gemm_bf16_tc2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         Cp = p.Cs[sg]; ldc = p.ldcs[sg]; Nn = p.Ns[sg]; out_mode = p.out_modes[sg];
         if (sg > 0) { Rp = Cp; ldr = ldc; }
       }
+      if (LCE == LCE_SCALED) Cp = reinterpret_cast<float*>(Cp) + ks * p.slice_stride;
       const int kb0 = ks * p.kblocks_per_split;
       const bool has_k = kb0 < p.kblocks_total;
       mbar_wait(&tmem_full_bar[acc], acc_phase, abort_flag, p.status, FAULT_WAIT_TMEM_FULL);
@@ -847,7 +850,8 @@ int gemm_bf16_tc_pair(cudaStream_t stream, int a_mn, int b_mn, int M, int N, int
     return 1;
   }
   if (split_k < 1) split_k = 1;
-  if (split_k > 1 && out_mode != GEMM_OUT_F32_ATOMIC) {
+  const long long apart = scale ? scale->slice_stride : 0;
+  if (split_k > 1 && out_mode != GEMM_OUT_F32_ATOMIC && !(apart > 0 && out_mode == GEMM_OUT_F32)) {
     if (err) *err = "gemm_bf16_tc: split_k > 1 needs the f32 atomic output mode";
     return 1;
   }
@@ -879,6 +883,7 @@ int gemm_bf16_tc_pair(cudaStream_t stream, int a_mn, int b_mn, int M, int N, int
   p.dual = 0; p.C2 = nullptr; p.H = nullptr;
   p.rope_tab = nullptr; p.rope_s = 1; p.rope_hd = 2;
   p.grad_out = scale ? scale->alpha_dev : nullptr;
+  p.slice_stride = apart;
   return pair_launch(stream, tmA, tmB, tmB, p, err, nullptr, scale ? LCE_SCALED : LCE_NONE);
 }
 
@@ -1000,6 +1005,21 @@ int gemm_pair_clusters_hint() { return gemm_num_sms() / 2; }
 // tile per cluster, so the split is chosen to fill the last wave (176 tiles on 74 clusters are
 // 2.4 waves = 79 % busy; split in two they are 4.8 waves = 95 %).  Every extra split costs one
 // more pass of f32 atomics over C, charged as 1.5 % each.
+// A slice writes and reads 8 bytes per output element, which takes (at 5 TB/s) as long as 2400 FLOPs (at 1.5 PFLOP/s): 1200 / K_all of the
+// element's 2 K_all.  What it buys is a fuller machine.
+int gemm_pair_split_k_apart(long long M, long long N, long long K, long long K_all, int most) {
+  const long long tiles = ((M + 2 * PM - 1) / (2 * PM)) * ((N + PN - 1) / PN), kblocks = (K + BK - 1) / BK;
+  const int clusters = gemm_num_sms() / 2;
+  int best_s = 1;
+  double best = -1e30;
+  for (int s = 1; s <= std::max(1LL, std::min(kblocks / 8, (long long)most)); ++s) {
+    const long long t = tiles * s, waves = (t + clusters - 1) / clusters;
+    const double score = (double)t / (double)(waves * clusters) - (s - 1) * 1200.0 / (double)K_all;
+    if (score > best + 1e-9) { best = score; best_s = s; }
+  }
+  const long long per = (kblocks + best_s - 1) / best_s;
+  return (int)((kblocks + per - 1) / per);  // none of them is empty
+}
 int gemm_pair_auto_split_k(int M, int N, int K) {
   const int tiles = ((M + 2 * PM - 1) / (2 * PM)) * ((N + PN - 1) / PN);
   return pair_auto_split(tiles, (K + BK - 1) / BK);

@@ -85,11 +85,33 @@ ce_join_kernel(const float2* __restrict__ stats, const float* __restrict__ targe
   }
 }
 
+// dst [n] (op)= the sum of `slices` f32 vectors that lie n elements apart, in their order, rounded once.  Eight elements per thread.
+__global__ void __launch_bounds__(256)
+ce_slices_kernel(__nv_bfloat16* __restrict__ dst, const float* __restrict__ src, int slices, long long n, int accumulate) {
+  for (long long i = ((long long)blockIdx.x * blockDim.x + threadIdx.x) * 8; i < n; i += (long long)gridDim.x * blockDim.x * 8) {
+    float x[8], o[8];
+    ld16(src + i, *reinterpret_cast<float(*)[4]>(x));
+    ld16(src + i + 4, *reinterpret_cast<float(*)[4]>(x + 4));
+    for (int s = 1; s < slices; ++s) {
+      ld16(src + s * n + i, *reinterpret_cast<float(*)[4]>(o));
+      ld16(src + s * n + i + 4, *reinterpret_cast<float(*)[4]>(o + 4));
+#pragma unroll
+      for (int c = 0; c < 8; ++c) x[c] += o[c];
+    }
+    if (accumulate) {
+      ld16(dst + i, o);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) x[c] += o[c];
+    }
+    st16(dst + i, x);
+  }
+}
+
 struct CePlan {
   long long piece, ld;                 // vocabulary entries of a piece, row stride of D
   long long stats_bytes, fwd_bytes;    // forward: tile statistics, then the target logits
   long long d_bytes, bwd_bytes;        // backward: D, then dH in f32
-  bool dh_f32;                         // dH is added up in f32 over the pieces (or k slices) and then rounded
+  int dh_slices;                       // f32 sums of dH, one per k slice, added up over the pieces; 0: dH leaves the product as it is
 };
 
 constexpr long long up256(long long n) { return (n + 255) & ~255LL; }
@@ -109,10 +131,12 @@ CePlan ce_plan(long long rows, long long k, long long vocab, long long piece) {
   p.stats_bytes = up256(tiles * rows * 8);
   p.fwd_bytes = p.stats_bytes + up256(rows * 4);
   p.d_bytes = up256(rows * p.ld * 2);
-  // one piece and enough output tiles to fill the machine: dH leaves the product in bf16
-  const long long tiles_dh = ((rows + 255) / 256) * ((k + 255) / 256);
-  p.dh_f32 = n > 1 || tiles_dh < 48;
-  p.bwd_bytes = p.d_bytes + (p.dh_f32 ? up256(rows * k * 4) : 0);
+  // Few output tiles of dH and a long sum: in k slices, with sums of their own that are added up in order at the end, so that the
+  // result is the same every time.  Their memory stays within 64 MB.
+  const int most = (int)std::min<long long>(32, (64LL << 20) / (rows * k * 4));
+  p.dh_slices = gemm_pair_split_k_apart(rows, k, std::min(piece, vocab), vocab, most);
+  if (n == 1 && p.dh_slices == 1) p.dh_slices = 0;
+  p.bwd_bytes = p.d_bytes + up256(p.dh_slices * rows * k * 4);
   return p;
 }
 
@@ -200,13 +224,10 @@ int eisen_linear_ce_bwd(void* stream, const void* h, long long ldh, const void* 
   const CePlan p = ce_plan(rows, k, vocab, piece);
   char* d = (char*)workspace;
   float* dh32 = (float*)(d + p.d_bytes);
-  if (dh && p.dh_f32 && cudaMemsetAsync(dh32, 0, (size_t)rows * k * 4, s) != cudaSuccess)
-    return fail(EISEN_ERR_CUDA, "linear_ce_bwd: memset");
   // C (op)= normalizer * (*grad_out) * A B^T on the paired-CTA kernel, whatever the size: its k slices fill the machine
   auto product = [&](int a_mn, int b_mn, long long M, long long N, long long K, const void* A, long long lda, const void* B,
-                     long long ldb, void* C, long long ldc, int mode) {
-    const int split = mode == GEMM_OUT_F32_ATOMIC && !deterministic() ? gemm_pair_auto_split_k((int)M, (int)N, (int)K) : 1;
-    const PairScale scale = {grad_out};
+                     long long ldb, void* C, long long ldc, int mode, int split, long long apart) {
+    const PairScale scale = {grad_out, apart};
     const char* err = nullptr;
     if (gemm_bf16_tc_pair(s, a_mn, b_mn, (int)M, (int)N, (int)K, A, lda, B, ldb, C, ldc, nullptr, 0, mode, split, normalizer, status, &err,
                           &scale))
@@ -223,20 +244,25 @@ int eisen_linear_ce_bwd(void* stream, const void* h, long long ldh, const void* 
     if (rc) return fail(EISEN_ERR_CUDA, err ? err : "linear_ce_bwd failed");
     count_launch();
     if (dh) {  // dH[rows, k] += D[rows, n] W_piece^T
-      const int mode = p.dh_f32 ? GEMM_OUT_F32_ATOMIC : accumulate_dh ? GEMM_OUT_BF16_ACC : GEMM_OUT_BF16;
-      rc = product(0, trans_b ? 1 : 0, rows, k, n, d, p.ld, wp, ldw, p.dh_f32 ? (void*)dh32 : dh, k, mode);
+      // (atomically where there is something to add to: one add per element and piece)
+      const int mode = p.dh_slices ? (c0 == 0 ? GEMM_OUT_F32 : GEMM_OUT_F32_ATOMIC) : accumulate_dh ? GEMM_OUT_BF16_ACC : GEMM_OUT_BF16;
+      rc = product(0, trans_b ? 1 : 0, rows, k, n, d, p.ld, wp, ldw, p.dh_slices ? (void*)dh32 : dh, k, mode, std::max(p.dh_slices, 1), rows * k);
       if (rc) return rc;
     }
     if (dw) {  // dW[k, piece] = H^T D, or with the tied table dW[piece, k] = D^T H
       char* out = (char*)dw + (dw_dtype == DT_F32 ? 4 : 2) * (trans_b ? c0 * lddw : c0);
       const int mode = dw_dtype == DT_F32 ? (accumulate_dw ? GEMM_OUT_F32_ATOMIC : GEMM_OUT_F32)
                                           : (accumulate_dw ? GEMM_OUT_BF16_ACC : GEMM_OUT_BF16);
-      rc = trans_b ? product(1, 1, n, k, rows, d, p.ld, h, ldh, out, lddw, mode) : product(1, 1, k, n, rows, h, ldh, d, p.ld, out, lddw, mode);
+      const int split = mode == GEMM_OUT_F32_ATOMIC && !deterministic()
+                            ? gemm_pair_auto_split_k((int)(trans_b ? n : k), (int)(trans_b ? k : n), (int)rows) : 1;
+      rc = trans_b ? product(1, 1, n, k, rows, d, p.ld, h, ldh, out, lddw, mode, split, 0)
+                   : product(1, 1, k, n, rows, h, ldh, d, p.ld, out, lddw, mode, split, 0);
       if (rc) return rc;
     }
   }
-  if (dh && p.dh_f32) return eisen_accumulate(stream, dh, DT_BF16, dh32, DT_F32, rows * k, accumulate_dh);
-  return 0;
+  if (!dh || !p.dh_slices) return 0;
+  ce_slices_kernel<<<grid_for(rows * k, 256 * 8, 8), 256, 0, s>>>((__nv_bfloat16*)dh, dh32, p.dh_slices, rows * k, accumulate_dh);
+  return check_launch("linear_ce_bwd(dh)");
 }
 
 }  // extern "C"

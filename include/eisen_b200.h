@@ -53,8 +53,8 @@ long long eisen_launch_count(void);
 /* Fixed-order arithmetic (process-wide, default off).  Some kernels of the Bf16Mixed path add f32 values in
  * an order that varies from run to run: weight-gradient GEMMs that split the token dimension over several
  * SM clusters (red.global.add), the attention backward, whose key-tile CTAs add their dQ tiles to one
- * buffer, the staged RMSNorm backward on bf16 rows, whose CTAs add their column sums of dw to one vector, and the k slices
- * of the gradients of eisen_linear_ce_bwd.  With the
+ * buffer, the staged RMSNorm backward on bf16 rows, whose CTAs add their column sums of dw to one vector, and
+ * eisen_linear_ce_bwd's weight gradient where it is added to an f32 one.  With the
  * switch on, a weight-gradient GEMM whose split is left to the library uses one slice per tile, the
  * attention backward writes every key tile's dQ to its own slice of the workspace
  * (eisen_attn_bwd_workspace_bytes grows by the number of key tiles) and sums the slices in key order, and
@@ -360,8 +360,8 @@ int eisen_distill_fused(void* stream, const void* logits, long long ld, const in
  * rows that do not count must be finite where dw is asked for (their zero gradient multiplies them).
  * ldh and ldw must be multiples of 8, k one of 8 in the backward; h, w, dh, dw and workspace 16-byte aligned.
  * `workspace` holds eisen_linear_ce_workspace_bytes(rows, k, vocab, piece, backward) bytes of scratch; the amount
- * for backward = 1 serves both calls.  Outside the fixed-order mode dh (and an f32 dw that is accumulated) may be
- * summed over k slices in an order that varies.  status as in eisen_gemm_bf16. */
+ * for backward = 1 serves both calls.  Outside the fixed-order mode an f32 dw that is accumulated
+ * may be summed over k slices in an order that varies; all else is the same every time.  status as in eisen_gemm_bf16. */
 long long eisen_linear_ce_workspace_bytes(long long rows, long long k, long long vocab, long long piece, int backward);
 int eisen_linear_ce_fwd(void* stream, const void* h, long long ldh, const void* w, long long ldw, int trans_b, const int* targets,
                         float* loss, float* row_loss, float* lse, void* workspace, long long rows, long long k, long long vocab,

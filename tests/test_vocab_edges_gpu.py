@@ -204,3 +204,30 @@ def test_linear_ce_adds_before_it_rounds(rows, k, vocab, tied):
         assert (rest.double().abs() <= 2.0 ** -8 * whole.double().abs() + 1e-30).all()
         counted = rest[whole != 0]  # rows that do not count have no gradient
         assert float((counted != 0).double().mean()) > 0.9
+
+
+# ------------------------------------------------------------------------------------------ sums in a fixed order
+@pytest.mark.parametrize("rows,k,vocab,tied,piece", [(700, 512, 3000, False, 1024), (1021, 1000, 50001, True, 0), (2048, 2048, 32000, False, 0),
+                                                     (5, 384, 8192, True, 0), (300, 256, 20000, False, 4096)])
+def test_linear_ce_repeats_bit_for_bit(rows, k, vocab, tied, piece):
+    """Without the fixed-order switch too: the k slices of dh have a buffer each and are added up in order."""
+    c = Head(rows, k, vocab, tied)
+    _, _, lse = c.fwd()
+    dh, dw = c.bwd(lse, piece)
+    for _ in range(3):
+        again = c.bwd(lse, piece)
+        assert torch.equal(dh, again[0]) and torch.equal(dw, again[1])
+
+
+@pytest.mark.parametrize("rows,k,vocab,piece", [(1024, 520, 20001, 0), (200, 1032, 9000, 0), (700, 512, 9000, 2048), (64, 64, 40000, 8192)])
+@pytest.mark.parametrize("accumulate", [0, 1])
+def test_linear_ce_hidden_gradient_in_slices(rows, k, vocab, piece, accumulate):
+    """Few output tiles and a long vocabulary: slices, a ragged last one, pieces that add to them; a last piece shorter than the first."""
+    c = Head(rows, k, vocab, True).expected()
+    _, _, lse = c.fwd()
+    ws = c.workspace(piece)
+    size = eb.lib().eisen_linear_ce_workspace_bytes(rows, k, vocab, piece, 1)
+    dh0 = (torch.randn(rows, k, generator=gen(1), device=dev()) * 1e-2).to(torch.bfloat16)
+    dh, _ = c.bwd(lse, piece, dw=False, acc_h=accumulate, dh0=dh0, ws=ws)
+    c.within(dh, c.dh + accumulate * dh0.double(), c.dh_tol, 2.0 ** -8)
+    assert (ws[size:] == 0x7f).all()
