@@ -1005,17 +1005,17 @@ int gemm_pair_clusters_hint() { return gemm_num_sms() / 2; }
 // tile per cluster, so the split is chosen to fill the last wave (176 tiles on 74 clusters are
 // 2.4 waves = 79 % busy; split in two they are 4.8 waves = 95 %).  Every extra split costs one
 // more pass of f32 atomics over C, charged as 1.5 % each.
-// A slice writes and reads 8 bytes per output element, which takes (at 5 TB/s) as long as 2400 FLOPs (at 1.5 PFLOP/s): 1200 / K_all of the
-// element's 2 K_all.  What it buys is a fuller machine.
+// In units of the time of a full machine: the product takes 1 / (busy clusters); a slice writes and reads 8 bytes per output element,
+// which takes (at 5 TB/s) as long as 2400 FLOPs (at 1.5 PFLOP/s), 1200 / K_all of the element's 2 K_all.
 int gemm_pair_split_k_apart(long long M, long long N, long long K, long long K_all, int most) {
   const long long tiles = ((M + 2 * PM - 1) / (2 * PM)) * ((N + PN - 1) / PN), kblocks = (K + BK - 1) / BK;
   const int clusters = gemm_num_sms() / 2;
   int best_s = 1;
-  double best = -1e30;
+  double best = 1e30;
   for (int s = 1; s <= std::max(1LL, std::min(kblocks / 8, (long long)most)); ++s) {
     const long long t = tiles * s, waves = (t + clusters - 1) / clusters;
-    const double score = (double)t / (double)(waves * clusters) - (s - 1) * 1200.0 / (double)K_all;
-    if (score > best + 1e-9) { best = score; best_s = s; }
+    const double time = (double)(waves * clusters) / (double)t + s * 1200.0 / (double)K_all;
+    if (time < best - 1e-9) { best = time; best_s = s; }
   }
   const long long per = (kblocks + best_s - 1) / best_s;
   return (int)((kblocks + per - 1) / per);  // none of them is empty

@@ -132,7 +132,8 @@ CePlan ce_plan(long long rows, long long k, long long vocab, long long piece) {
   p.fwd_bytes = p.stats_bytes + up256(rows * 4);
   p.d_bytes = up256(rows * p.ld * 2);
   // Few output tiles of dH and a long sum: in k slices, with sums of their own that are added up in order at the end, so that the
-  // result is the same every time.  Their memory stays within 64 MB.
+  // result is the same every time (forward and backward of 64 x 384 x 8192: 58 us, 88 in one slice; of 1021 x 1000 x 50001, tied:
+  // 475-483, slices that add up atomically in one place 480-499).  Their memory stays within 64 MB.
   const int most = (int)std::min<long long>(32, (64LL << 20) / (rows * k * 4));
   p.dh_slices = gemm_pair_split_k_apart(rows, k, std::min(piece, vocab), vocab, most);
   if (n == 1 && p.dh_slices == 1) p.dh_slices = 0;
