@@ -1336,22 +1336,23 @@ int64_t Graph::linear_cross_entropy(int64_t h, int64_t w, int64_t tid, float nor
   if (!no_grad) {
     tape.push_back({{h, w}, o, [this, h, w, tid, lse, o, d, ldw, trans_b, piece, normalizer]() {
       OUT_GRAD_OR_RETURN(o);
-      const bool dw = !tensors[w].constant;
-      ensure_grad(h);
+      const bool dh = !tensors[h].constant, dw = !tensors[w].constant;
+      if (!dh && !dw) return;
+      if (dh) ensure_grad(h);
       if (dw) ensure_grad(w);
       HTensor& gh = tensors[h];
       HTensor& gw = tensors[w];
-      if (gh.grad_dtype != 1) invalid("linear_cross_entropy: the hidden-state gradient must be bf16");
+      if (dh && gh.grad_dtype != 1) invalid("linear_cross_entropy: the hidden-state gradient must be bf16");
       const size_t bytes = (size_t)eisen_linear_ce_workspace_bytes(d.rows, d.k, d.vocab, piece, 1);
       void* ws = pool_get(bytes);
       struct Release { Graph& g; void* p; size_t b; ~Release() { g.pool_put(p, b); } } release{*this, ws, bytes};
-      prof_begin(0, (dw ? 6.0 : 4.0) * (double)d.rows * (double)d.k * (double)d.vocab);
+      prof_begin(0, (2.0 + 2.0 * dh + 2.0 * dw) * (double)d.rows * (double)d.k * (double)d.vocab);
       ck(eisen_linear_ce_bwd(stream, operand(gh), d.k, operand(gw), ldw, trans_b, (const int*)tensors[tid].data,
-                             (const float*)tensors[lse].data, (const float*)to.grad, gh.grad, gh.grad_init, dw ? gw.grad : nullptr, ldw,
+                             (const float*)tensors[lse].data, (const float*)to.grad, dh ? gh.grad : nullptr, gh.grad_init, dw ? gw.grad : nullptr, ldw,
                              gw.grad_dtype, gw.grad_init, ws, d.rows, d.k, d.vocab, piece, -1, normalizer, status_dev),
          "linear_cross_entropy.bwd");
       prof_end();
-      gh.grad_init = true;
+      if (dh) gh.grad_init = true;
       if (dw) gw.grad_init = true;
     }});
   }
@@ -1433,6 +1434,7 @@ int64_t Graph::distill(int64_t logits, const Teacher& t, int64_t tid, float norm
     tape.push_back({{logits}, o, [this, logits, t, tid, lse, o, rows, vocab, k, normalizer, dt]() {
       OUT_GRAD_OR_RETURN(o);
       HTensor& gl = tensors[logits];
+      if (gl.constant) return;
       ensure_grad(logits);
       FaultWordScope faults(status_dev);
       ck(eisen_distill_bwd(stream, operand(gl), vocab, (const int*)tensors[t.ids].data, (const float*)tensors[t.logits].data,
@@ -1451,14 +1453,14 @@ int64_t Graph::lm_head_distill(int64_t h, int64_t w, const Teacher& t, int64_t t
   const int64_t k = teacher_k(*this, "lm_head_distill", t, tid, d.rows);
   if (chunk_rows <= 0 || chunk_rows > d.rows) chunk_rows = d.rows;
   const int dt = act_dtype();
-  const bool grads = !no_grad;
+  const bool gives_dh = !no_grad && !tensors[h].constant, gives_dw = !no_grad && !tensors[w].constant, grads = gives_dh || gives_dw;
   const int64_t row_loss = alloc_pooled_dtype({d.rows}, 0), o = alloc_pooled_dtype({}, 0);
   tensors[row_loss].constant = true;
-  if (grads) {
+  if (gives_dh) {
     ensure_grad(h);
-    if (!tensors[w].constant) ensure_grad(w);
     if (tensors[h].grad_dtype != dt) invalid("lm_head_distill: the hidden-state gradient must have the activation dtype");
   }
+  if (gives_dw) ensure_grad(w);
   const size_t slab_bytes = (size_t)chunk_rows * d.vocab * dsize(dt);
   void* slab = pool_get(slab_bytes);
   struct Release { Graph& g; void* p; size_t b; ~Release() { g.pool_put(p, b); } } release{*this, slab, slab_bytes};
@@ -1482,15 +1484,17 @@ int64_t Graph::lm_head_distill(int64_t h, int64_t w, const Teacher& t, int64_t t
     ck(eisen_distill_fused(stream, slab, d.vocab, ids, tv, t_lse, targets, slab, d.vocab, nullptr, rl + r0, nullptr, m, d.vocab, k, -1,
                            t.temperature, kd, ce, 1.0f, dt, bad_id_dev + 1),
        "lm_head_distill");
-    HTensor& gh = tensors[h];
-    char* dh = (char*)gh.grad + (size_t)r0 * d.k * dsize(gh.grad_dtype);
-    gemm(*this, false, trans_b, m, d.k, d.vocab, slab, weight_operand(w), dh, gh.grad_dtype, gh.grad_init);
-    if (!tensors[w].constant) {
+    if (gives_dh) {
+      HTensor& gh = tensors[h];
+      char* dh = (char*)gh.grad + (size_t)r0 * d.k * dsize(gh.grad_dtype);
+      gemm(*this, false, trans_b, m, d.k, d.vocab, slab, weight_operand(w), dh, gh.grad_dtype, gh.grad_init);
+    }
+    if (gives_dw) {
       if (!trans_b) dw_gemm(*this, true, true, d.k, d.vocab, m, hrows, slab, w);
       else dw_gemm(*this, true, true, d.vocab, d.k, m, slab, hrows, w);
     }
   }
-  if (grads) tensors[h].grad_init = true;
+  if (gives_dh) tensors[h].grad_init = true;
   ck(eisen_ce_loss_reduce(stream, rl, (float*)tensors[o].data, d.rows), "lm_head_distill(reduce)");
   if (grads) {
     tape.push_back({{h, w}, o, [this, o]() {

@@ -591,7 +591,9 @@ int eisen_graph_lm_head_top_logits(void* g, long long h, long long w, long long 
                                    long long* out3);
 /* eisen_distill_* as graph ops: mean over n_valid rows (both weights are divided by it).  teacher_ids (int32) and
  * teacher_logits (f32) [rows, k]; teacher_lse (f32 [rows]) and target_ids (int32 [rows], -1 = ignored) may be -1.  The second
- * form is eisen_graph_lm_head_cross_entropy with this loss: one [chunk_rows, vocab] slab, gradients formed in the forward. */
+ * form is eisen_graph_lm_head_cross_entropy with this loss: one [chunk_rows, vocab] slab, gradients formed in the forward.
+ * Of hidden states, head and logits those get a gradient that take one (a copy from another graph does not); this holds for
+ * eisen_graph_linear_cross_entropy too. */
 int eisen_graph_distill(void* g, long long logits, long long teacher_ids, long long teacher_logits, long long teacher_lse,
                         long long target_ids, long long n_valid, float temperature, float kd_weight, float ce_weight, long long* out);
 int eisen_graph_lm_head_distill(void* g, long long h, long long w, long long teacher_ids, long long teacher_logits, long long teacher_lse,

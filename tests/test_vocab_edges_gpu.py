@@ -231,3 +231,67 @@ def test_linear_ce_hidden_gradient_in_slices(rows, k, vocab, piece, accumulate):
     dh, _ = c.bwd(lse, piece, dw=False, acc_h=accumulate, dh0=dh0, ws=ws)
     c.within(dh, c.dh + accumulate * dh0.double(), c.dh_tol, 2.0 ** -8)
     assert (ws[size:] == 0x7f).all()
+
+
+# ------------------------------------------------------------------------------------------ tensors that take no gradient
+def frozen(g, H):
+    """Hidden states that come from another graph: an activation without a gradient."""
+    src = new_graph(BF16_MIXED)
+    base = src.alloc_pooled(list(H.shape))
+    src.load_tensor_data(base, H)
+    out = g.copy_from(src, base)
+    g.synchronize()
+    return out
+
+
+@pytest.mark.parametrize("tied", [False, True])
+def test_head_trained_on_frozen_hidden_states(tied):
+    """linear_cross_entropy and lm_head_distill form the head's gradient alone where the hidden states take none."""
+    r = np.random.default_rng(5)
+    H, W = r.standard_normal((70, 64)).astype(np.float32), (r.standard_normal((64, 1000)) * 0.2).astype(np.float32)
+    _, ids, tv, y = data(70, 1000, 5)
+    n = int((y >= 0).sum())
+    bf = [torch.tensor(a).to(torch.bfloat16).double() for a in (H, W)]
+    for how in ("linear", "distill"):
+        g = new_graph(BF16_MIXED)
+        w = g.alloc([1000, 64] if tied else [64, 1000], W.T if tied else W)
+        g.mark_params()
+        tid, h = g.alloc_ids([70], y), frozen(g, H)
+        if how == "linear":
+            loss = g.linear_cross_entropy(h, w, tid, n, tied, 256)
+            kd = 0.0
+        else:
+            kd = 0.6
+            loss = g.lm_head_distill(h, w, g.alloc_ids([70, 5], ids), g.alloc([70, 5], tv), n, target_ids=tid, temperature=2.0, kd_weight=kd,
+                                     ce_weight=1.0 - kd, trans_b=tied, chunk_rows=32)
+        want, dx = f64_distill((bf[0] @ bf[1]).numpy(), ids, tv, y, 2.0, kd, 1.0 - kd)
+        # the distillation's logits are rounded to bf16: at most 2^-8 of a logit of size 8 in its part of a loss of about 7
+        assert abs(g.data(loss)[0] - want) < (2e-5 if how == "linear" else 1e-2) * want
+        g.backward(loss)
+        dw = bf[0].T.numpy() @ dx
+        got = g.grad(w).reshape(g.shape(w))
+        want_w = dw.T if tied else dw
+        assert np.linalg.norm(got - want_w) < (2.0 ** -8 if how == "linear" else 2e-2) * np.linalg.norm(want_w)
+
+
+def test_nothing_takes_a_gradient():
+    """A frozen head over frozen hidden states, and a loss of frozen logits: backward leaves them alone."""
+    x, ids, tv, y = data(6, 300, 4)
+    g = new_graph(FP32)
+    g.mark_params()
+    src = new_graph(FP32)
+    l = g.copy_from(src, src.alloc([6, 300], x))
+    g.synchronize()
+    loss = g.distill(l, g.alloc_ids([6, 4], ids), g.alloc([6, 4], tv), int((y >= 0).sum()), target_ids=g.alloc_ids([6], y), temperature=1.5)
+    want, _ = f64_distill(x, ids, tv, y, 1.5, 1.0, 0.0)
+    assert abs(g.data(loss)[0] - want) < 1e-5 * abs(want) + 1e-6
+    g.backward(loss)
+    r = np.random.default_rng(1)
+    g = new_graph(BF16_MIXED)
+    g.mark_params()
+    h = frozen(g, r.standard_normal((6, 64)).astype(np.float32))
+    w = frozen(g, r.standard_normal((64, 304)).astype(np.float32))
+    tid = g.alloc_ids([6], y)
+    g.backward(g.linear_cross_entropy(h, w, tid, 6))
+    g.backward(g.lm_head_distill(h, w, g.alloc_ids([6, 4], ids), g.alloc([6, 4], tv), 6))
+    g.synchronize()
