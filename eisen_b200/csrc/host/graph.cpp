@@ -1319,6 +1319,7 @@ int64_t Graph::linear_cross_entropy(int64_t h, int64_t w, int64_t tid, float nor
   if (tensors.at(tid).dtype != DT_I32 || tensors[tid].numel != d.rows) invalid("linear_cross_entropy: one int32 target per row expected");
   if (tensors[w].host_homed) invalid("linear_cross_entropy: the head weight must be on the device");
   if (piece < 0) invalid("linear_cross_entropy: piece must be >= 0");
+  if (!no_grad && !tensors[h].constant && tensors[h].grad_dtype != 1) invalid("linear_cross_entropy: the hidden-state gradient must be bf16");
   const int64_t ldw = trans_b ? d.k : d.vocab;
   const int64_t lse = alloc_pooled_dtype({d.rows}, 0), row_loss = alloc_pooled_dtype({d.rows}, 0), o = alloc_pooled_dtype({}, 0);
   tensors[lse].constant = tensors[row_loss].constant = true;
@@ -1342,7 +1343,6 @@ int64_t Graph::linear_cross_entropy(int64_t h, int64_t w, int64_t tid, float nor
       if (dw) ensure_grad(w);
       HTensor& gh = tensors[h];
       HTensor& gw = tensors[w];
-      if (dh && gh.grad_dtype != 1) invalid("linear_cross_entropy: the hidden-state gradient must be bf16");
       const size_t bytes = (size_t)eisen_linear_ce_workspace_bytes(d.rows, d.k, d.vocab, piece, 1);
       void* ws = pool_get(bytes);
       struct Release { Graph& g; void* p; size_t b; ~Release() { g.pool_put(p, b); } } release{*this, ws, bytes};
@@ -1421,6 +1421,7 @@ int64_t Graph::distill(int64_t logits, const Teacher& t, int64_t tid, float norm
   if (tl.shape.size() != 2) invalid("distill: logits must be [rows, vocab]");
   const int64_t rows = tl.shape[0], vocab = tl.shape[1], k = teacher_k(*this, "distill", t, tid, rows);
   const int dt = act_dtype();
+  if (!no_grad && !tl.constant && tl.grad_dtype != dt) invalid("distill: the logits' gradient must have the activation dtype");
   const int64_t lse = alloc_pooled_dtype({2, rows}, 0), row_loss = alloc_pooled_dtype({rows}, 0), o = alloc_pooled_dtype({}, 0);
   tensors[lse].constant = tensors[row_loss].constant = true;
   const int* targets = tid >= 0 ? (const int*)tensors[tid].data : nullptr;

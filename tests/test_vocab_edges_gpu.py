@@ -295,3 +295,21 @@ def test_nothing_takes_a_gradient():
     g.backward(g.linear_cross_entropy(h, w, tid, 6))
     g.backward(g.lm_head_distill(h, w, g.alloc_ids([6, 4], ids), g.alloc([6, 4], tv), 6))
     g.synchronize()
+
+
+# ------------------------------------------------------------------------------------------ refusals leave nothing behind
+def test_gradients_of_another_type_are_refused_at_once():
+    """A Bf16Mixed parameter's gradient is f32: as logits, or as hidden states, it cannot take the kernels' bf16."""
+    x, ids, tv, y = data(6, 304, 4)
+    g = new_graph(BF16_MIXED)
+    l = g.alloc([6, 304], x)
+    w = g.alloc([304, 64], np.zeros(304 * 64))
+    g.mark_params()
+    t, v, tid = g.alloc_ids([6, 4], ids), g.alloc([6, 4], tv), g.alloc_ids([6], y)
+    n = g.tape_len()
+    for f in (lambda: g.distill(l, t, v, 6), lambda: g.linear_cross_entropy(l, w, tid, 6), lambda: g.lm_head_distill(l, w, t, v, 6)):
+        with pytest.raises(eb.EisenError, match="gradient"):
+            f()
+    assert g.tape_len() == n
+    g.set_no_grad(True)
+    assert np.isfinite(g.data(g.distill(l, t, v, 6))[0])
