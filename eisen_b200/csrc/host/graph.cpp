@@ -1359,11 +1359,15 @@ int64_t Graph::linear_cross_entropy(int64_t h, int64_t w, int64_t tid, float nor
   return o;
 }
 
+void Graph::check_top_logits(const char* what, int64_t vocab, int64_t k, float temperature) const {
+  ck(eisen_top_logits(stream, nullptr, vocab, nullptr, nullptr, nullptr, 0, vocab, k, temperature, act_dtype()), what);
+}
+
 void Graph::top_logits(int64_t logits, int64_t k, float temperature, int64_t out3[3]) {
   const std::vector<int64_t> shape = tensors.at(logits).shape;
   if (shape.empty()) invalid("top_logits: logits must be [.., vocab]");
   const int64_t vocab = shape.back(), rows = tensors[logits].numel / std::max<int64_t>(vocab, 1);
-  if (k < 1 || k > vocab) invalid("top_logits: k must be in [1, vocab]");
+  check_top_logits("top_logits", vocab, k, temperature);
   std::vector<int64_t> ks = shape, ls = shape;
   ks.back() = k;
   ls.pop_back();
@@ -1379,7 +1383,7 @@ void Graph::top_logits(int64_t logits, int64_t k, float temperature, int64_t out
 
 void Graph::lm_head_top_logits(int64_t h, int64_t w, int64_t k, float temperature, bool trans_b, int64_t chunk_rows, int64_t out3[3]) {
   const HeadShape d = head_shape("lm_head_top_logits", tensors.at(h), tensors.at(w), trans_b);
-  if (k < 1 || k > d.vocab) invalid("lm_head_top_logits: k must be in [1, vocab]");
+  check_top_logits("lm_head_top_logits", d.vocab, k, temperature);
   if (chunk_rows <= 0 || chunk_rows > d.rows) chunk_rows = d.rows;
   const int dt = act_dtype();
   std::vector<int64_t> ks = tensors[h].shape, ls = ks;

@@ -186,6 +186,7 @@ class Graph {
   // ids int32 [.., k], lse f32 [..]}, none of which takes a gradient.  The second form works through the head in chunks of
   // token rows, so that only a [chunk_rows, vocab] slab of logits exists.
   void top_logits(int64_t logits, int64_t k, float temperature, int64_t out3[3]);
+  void check_top_logits(const char* what, int64_t vocab, int64_t k, float temperature) const;  // throws what the kernel would refuse
   void lm_head_top_logits(int64_t h, int64_t w, int64_t k, float temperature, bool trans_b, int64_t chunk_rows, int64_t out3[3]);
   // Distillation from a teacher's top logits (eisen_distill_*).  teacher.lse and target_ids may be -1.
   struct Teacher { int64_t ids = -1, logits = -1, lse = -1; float temperature = 1.0f, kd_weight = 1.0f, ce_weight = 0.0f; };

@@ -242,21 +242,21 @@ int64_t TransformerLM::hidden_forward(Graph& g, int64_t x) {
 }
 
 void TransformerLM::top_logits(Graph& g, int64_t x, int64_t k, float temperature, int64_t chunk_rows, int64_t out3[3]) {
-  if (k < 1 || k > vocab) throw EisenException(EISEN_ERR_INVALID, "lm_top_logits: k must be in [1, vocab]");
   const int64_t rows = g.tensors.at(x).numel;
+  g.check_top_logits("lm_top_logits", vocab, k, temperature);  // before the forward pass
+  // the forward pass leaves nothing behind, and one that fails no results either
+  struct Unwind { Graph& g; int64_t to; ~Unwind() { g.restore_save_point(to); } } unwind{g, g.mark_save_point()};
   int64_t keep[3] = {g.alloc_pooled_dtype({rows, k}, 0), g.alloc_pooled_dtype({rows, k}, DT_I32), g.alloc_pooled_dtype({rows}, 0)};
   const int64_t sp = g.mark_save_point();
-  {
-    FlagGuard ng(g.no_grad, true);
-    int64_t made[3];
-    g.lm_head_top_logits(hidden_forward(g, x), tie ? emb : head, k, temperature, tie, chunk_rows, made);
-    for (int i = 0; i < 3; ++i) {
-      std::swap(g.tensors[keep[i]].data, g.tensors[made[i]].data);
-      g.tensors[keep[i]].constant = true;
-      out3[i] = keep[i];
-    }
+  FlagGuard ng(g.no_grad, true);
+  int64_t made[3];
+  g.lm_head_top_logits(hidden_forward(g, x), tie ? emb : head, k, temperature, tie, chunk_rows, made);
+  for (int i = 0; i < 3; ++i) {
+    std::swap(g.tensors[keep[i]].data, g.tensors[made[i]].data);
+    g.tensors[keep[i]].constant = true;
+    out3[i] = keep[i];
   }
-  g.restore_save_point(sp);  // the forward pass leaves nothing behind
+  unwind.to = sp;
 }
 
 int64_t TransformerLM::forward(Graph& g, int64_t x) {

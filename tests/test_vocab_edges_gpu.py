@@ -313,3 +313,33 @@ def test_gradients_of_another_type_are_refused_at_once():
     assert g.tape_len() == n
     g.set_no_grad(True)
     assert np.isfinite(g.data(g.distill(l, t, v, 6))[0])
+
+
+def teacher_state(g):
+    return g.num_tensors(), g.tape_len(), g.pool_stats()["live_bytes"]
+
+
+@pytest.mark.parametrize("precision", [FP32, BF16_MIXED])
+def test_top_logits_refused_before_the_forward_pass(precision):
+    g, lm = model(precision, 1)
+    ids = np.random.default_rng(0).integers(0, CFG["vocab"], (2, 64)).astype(np.int32)
+    x = g.alloc_ids([2, 64], ids)
+    h = g.alloc_pooled([128, CFG["hidden"]])
+    before, launches = teacher_state(g), eb.lib().eisen_launch_count()
+    for k, temperature in ((300, 1.0), (0, 1.0), (5, 0.0), (5, float("nan"))):
+        with pytest.raises(eb.EisenError):
+            lm.top_logits(x, k, temperature)
+        assert teacher_state(g) == before and eb.lib().eisen_launch_count() == launches
+        with pytest.raises(eb.EisenError):
+            g.lm_head_top_logits(h, lm.params()[-1], k, temperature)
+        assert teacher_state(g) == before and eb.lib().eisen_launch_count() == launches
+    lm.top_logits(x, 5)
+
+
+def test_top_logits_leaves_nothing_behind_when_the_forward_pass_fails():
+    g, lm = model(FP32, 1)
+    bad = g.alloc_ids([128], np.zeros(128, dtype=np.int32))  # no batch axis: the first attention refuses it
+    before = teacher_state(g)
+    with pytest.raises(eb.EisenError):
+        lm.top_logits(bad, 5)
+    assert teacher_state(g) == before
