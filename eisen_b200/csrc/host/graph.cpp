@@ -1313,13 +1313,21 @@ static HeadShape head_shape(const char* what, const HTensor& th, const HTensor& 
   return {th.numel / k, k, trans_b ? tw.shape[0] : tw.shape[1]};
 }
 
-int64_t Graph::linear_cross_entropy(int64_t h, int64_t w, int64_t tid, float normalizer, bool trans_b, int64_t piece) {
+void Graph::check_linear_cross_entropy(int64_t w) const {
+  const HTensor& tw = tensors.at(w);
   if (precision != Precision::Bf16Mixed) invalid("linear_cross_entropy: bf16 operands only (Bf16Mixed)");
+  if (tw.host_homed) invalid("linear_cross_entropy: the head weight must be on the device");
+  if (tw.shape.size() != 2) invalid("linear_cross_entropy: the head weight must have rank 2");
+  if (tw.shape[1] % 8) invalid("linear_cross_entropy: rows of the head weight must be a multiple of 8 long");
+}
+
+int64_t Graph::linear_cross_entropy(int64_t h, int64_t w, int64_t tid, float normalizer, bool trans_b, int64_t piece) {
+  check_linear_cross_entropy(w);
   const HeadShape d = head_shape("linear_cross_entropy", tensors.at(h), tensors.at(w), trans_b);
   if (tensors.at(tid).dtype != DT_I32 || tensors[tid].numel != d.rows) invalid("linear_cross_entropy: one int32 target per row expected");
-  if (tensors[w].host_homed) invalid("linear_cross_entropy: the head weight must be on the device");
   if (piece < 0) invalid("linear_cross_entropy: piece must be >= 0");
   if (!no_grad && !tensors[h].constant && tensors[h].grad_dtype != 1) invalid("linear_cross_entropy: the hidden-state gradient must be bf16");
+  if (d.k % 8) invalid("linear_cross_entropy: the width must be a multiple of 8");
   const int64_t ldw = trans_b ? d.k : d.vocab;
   const int64_t lse = alloc_pooled_dtype({d.rows}, 0), row_loss = alloc_pooled_dtype({d.rows}, 0), o = alloc_pooled_dtype({}, 0);
   tensors[lse].constant = tensors[row_loss].constant = true;

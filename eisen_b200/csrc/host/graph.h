@@ -181,6 +181,7 @@ class Graph {
   // The same loss without logits (Bf16Mixed): head projection and cross-entropy in pieces of `piece` vocabulary entries
   // (0 = the library's choice), eisen_linear_ce_fwd here and eisen_linear_ce_bwd in the backward pass.  Any loss gradient
   // may come in: nothing is formed ahead.
+  void check_linear_cross_entropy(int64_t w) const;  // throws where the head's weight has not the form it needs
   int64_t linear_cross_entropy(int64_t h, int64_t w, int64_t target_ids, float normalizer, bool trans_b, int64_t piece);
   // The k largest logits of every row, their ids and the row's log-sum-exp at a temperature: {values f32 [.., k],
   // ids int32 [.., k], lse f32 [..]}, none of which takes a gradient.  The second form works through the head in chunks of

@@ -281,6 +281,7 @@ int64_t TransformerLM::train_micro_step(Graph& g, int64_t x, const int64_t* targ
 int64_t TransformerLM::train_micro_step_dev(Graph& g, int64_t x, int64_t target_ids, int64_t n_valid, bool checkpoint,
                                             const std::function<void(int64_t)>& after_block) {
   const int64_t n_targets = g.tensors.at(target_ids).numel;
+  if (head_piece >= 0) g.check_linear_cross_entropy(tie ? emb : head);  // before the blocks run
   // src/graph/ops/reduction.rs:724-737: mean over the valid rows; all rows masked -> loss 0, no gradient
   const float normalizer = n_valid > 0 ? 1.0f / (float)n_valid : 0.0f;
   return micro_step(g, x, checkpoint, after_block, [&](int64_t hn) {

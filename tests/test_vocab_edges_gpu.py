@@ -343,3 +343,19 @@ def test_top_logits_leaves_nothing_behind_when_the_forward_pass_fails():
     with pytest.raises(eb.EisenError):
         lm.top_logits(bad, 5)
     assert teacher_state(g) == before
+
+
+@pytest.mark.parametrize("precision,vocab,tie", [(FP32, 1024, False), (BF16_MIXED, 1020, False)])
+def test_head_pieces_refused_before_the_blocks_run(precision, vocab, tie):
+    """f32 operands, or an untied head whose rows do not start on 16 bytes."""
+    g, lm = model(precision, 1, tie, vocab=vocab)
+    lm.set_head_pieces(0)
+    ids = np.random.default_rng(0).integers(0, vocab, (2, 64)).astype(np.int32)
+    x, t = g.alloc_ids([2, 64], ids), g.alloc_ids([128], ids.reshape(-1))
+    before, launches = teacher_state(g), eb.lib().eisen_launch_count()
+    with pytest.raises(eb.EisenError, match="linear_cross_entropy"):
+        lm.train_micro_step_dev(x, t, 128)
+    assert teacher_state(g) == before and eb.lib().eisen_launch_count() == launches
+    if precision == FP32:  # the other head takes it (no bf16 head takes such rows)
+        lm.set_head_pieces(None)
+        assert np.isfinite(g.data(lm.train_micro_step_dev(x, t, 128))[0])
