@@ -994,6 +994,9 @@ int distill_check(const char* what, const DistillParams& p, int dtype, bool bwd)
   if ((reinterpret_cast<uintptr_t>(p.logits) % es) || (bwd && (reinterpret_cast<uintptr_t>(p.dlogits) % es)))
     return bad(EISEN_ERR_INVALID, "unaligned pointer");
   if (bwd && !p.dlogits) return bad(EISEN_ERR_INVALID, "dlogits must not be null");
+  // a row's gradient would go over the logits of another one
+  if (bwd && p.dlogits == p.logits && p.ldd != p.ld && p.rows > 1)
+    return bad(EISEN_ERR_INVALID, "dlogits over the logits needs their row stride");
   if (p.k < 1 || p.k > DS_MAX_K) return bad(EISEN_ERR_LIMIT, "k must be in [1, 1024]");
   if (!(p.temperature > 0.0f) || !(p.temperature <= FLT_MAX) || !(1.0f / p.temperature <= FLT_MAX))
     return bad(EISEN_ERR_INVALID, "the temperature must be positive and finite");
