@@ -359,3 +359,57 @@ def test_head_pieces_refused_before_the_blocks_run(precision, vocab, tie):
     if precision == FP32:  # the other head takes it (no bf16 head takes such rows)
         lm.set_head_pieces(None)
         assert np.isfinite(g.data(lm.train_micro_step_dev(x, t, 128))[0])
+
+
+# ------------------------------------------------------------------------------------------ kinds of exponentials
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("temperature", [0.7, 1.0, 1.5, 2.5, 3.0, 3.5, 4.0, 5.0])
+@pytest.mark.parametrize("rows,vocab", [(3, 9001), (2, 40000), (1300, 600), (330, 9001)])
+def test_every_kind_of_exponential_in_every_row_form(dtype, temperature, rows, vocab):
+    c = Case(dtype, rows, vocab, 9, temperature, 0.6, 0.4).expected()
+    loss, row, lse = c.fwd()
+    c.check_loss(loss, row, lse)
+    d = torch.full_like(c.x, 5.0)
+    c.bwd(lse, d)
+    c.check_grad(d)
+    d.fill_(5.0)
+    c.check_loss(*c.fused(d))
+    c.check_grad(d, fused=True)
+    c.ce = 0.0  # one exponential where no log-sum-exps are asked for
+    c.expected()
+    d.fill_(5.0)
+    loss, row, _ = c.fused(d, lse=False)
+    c.check_loss(loss, row)
+    c.check_grad(d, fused=True)
+
+
+# ------------------------------------------------------------------------------------------ the steps in a data-parallel run
+@pytest.mark.parametrize("how", ["pieces", "distill"])
+def test_steps_announce_finished_blocks(how):
+    """after_block comes for every block, last one first, when that block's gradients are final: what buckets are reduced by."""
+    r = np.random.default_rng(0)
+    g, lm = model(BF16_MIXED, 3)
+    ids = r.integers(0, CFG["vocab"], (1, 128)).astype(np.int32)
+    y = r.integers(0, CFG["vocab"], 128).astype(np.int32)
+    x, t = g.alloc_ids([1, 128], ids), g.alloc_ids([128], y)
+    teacher = g.alloc_ids([128, 4], r.integers(0, CFG["vocab"], (128, 4)).astype(np.int32)), g.alloc([128, 4], r.standard_normal((128, 4)))
+    seen = []
+
+    def announce(layer):
+        seen.append((layer, {p: g.grad(p).copy() for p in lm.params()}))
+
+    if how == "pieces":
+        lm.set_head_pieces(256)
+        lm.train_micro_step_dev(x, t, 128, checkpoint=True, after_block=announce)
+    else:
+        lm.distill_micro_step_dev(x, *teacher, 128, target_ids_id=t, kd_weight=0.5, ce_weight=0.5, checkpoint=True, after_block=announce)
+    final = {p: g.grad(p) for p in lm.params()}
+    layers = [l for l, _ in seen]
+    assert sorted(l for l in layers if 0 <= l < CFG["layers"]) == list(range(CFG["layers"]))
+    assert layers == sorted(layers, reverse=True)
+    done = set()  # parameters whose gradient was already as it is in the end
+    for layer, grads in seen:
+        now = {p for p in grads if np.array_equal(grads[p], final[p]) and np.any(final[p])}
+        assert done <= now
+        done = now
+    assert len(seen[0][1]) == len(lm.params()) and len(done) >= len(lm.params()) - 2
