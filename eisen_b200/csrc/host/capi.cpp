@@ -342,6 +342,7 @@ int eisen_graph_sync_ids_to_cpu(void* g, long long id, int* out) {
     if (cudaMemcpyAsync(out, t.data, (size_t)t.numel * 4, cudaMemcpyDefault, gr.stream) != cudaSuccess ||
         cudaStreamSynchronize(gr.stream) != cudaSuccess)
       throw EisenException(EISEN_ERR_CUDA, "sync_ids_to_cpu: copy failed");
+    gr.check_status();  // like sync_to_cpu
   });
 }
 int eisen_graph_rms_norm(void* g, long long x, long long w, float eps, long long* out) {

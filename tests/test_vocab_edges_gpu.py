@@ -114,6 +114,17 @@ def test_a_graph_reports_the_wait_of_its_own_row_kernel():
         eb.call("eisen_selftest_row_frame", None, None, 5, 200000)
 
 
+def test_ids_are_not_handed_out_past_a_wait_that_ran_out():
+    """Reading ids back looks at the graph's fault word as reading values does."""
+    g = new_graph()
+    _, i, _ = g.top_logits(g.alloc([2, 50], np.arange(100)), 3)
+    assert (g.ids_to_cpu(i).reshape(2, 3) == [49, 48, 47]).all()
+    eb.call("eisen_graph_selftest_row_frame", g._h, 200000)
+    with pytest.raises(eb.EisenError, match="bounded wait"):
+        g.ids_to_cpu(i)
+    assert (g.ids_to_cpu(i).reshape(2, 3) == [49, 48, 47]).all()
+
+
 # ------------------------------------------------------------------------------------------ logits far from 0
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("rows,vocab", FORMS)
