@@ -3,8 +3,9 @@
 //   distribution over the entries it gives; gradient
 //   kd T (Q p_i - sum_{id_j = i} q_j) + ce (softmax(x)_i - [i = y]),  Q = sum_j q_j
 //
-// A row of `vocab` logits is read once, and written once where there is a gradient: bound by that traffic.  Maxima,
-// sums and statistics are f32.
+// Bound by the traffic of the rows of `vocab` logits.  Few rows, and loss and gradient together over rows of more than 16 KB, are read
+// once into shared memory and written once (distill_pipe_kernel); all else is read from global memory, and for a gradient beside
+// the loss a second time out of the L2 cache (distill_stream_kernel); distill_launch has the rule.  Maxima, sums and statistics are f32.
 #include <algorithm>
 #include <cfloat>
 #include <cstdio>
@@ -48,7 +49,7 @@ constexpr int DS_FWD = 1, DS_BWD = 2;
 
 // A row's exponentials et = exp((x - ref) / T) and e1 = exp(x - ref).  KIND says how they are formed:
 //   ONE     et alone (temperature 1, or no cross-entropy term and one log-sum-exp), as h^2 with h = exp((x - ref) / 2T)
-//   3 .. 8  bf16 rows with 2T a whole number: et = h^2, e1 = h^2T with the same h
+//   3 .. 8  bf16 rows, 2T = 3, 4 .. 8 (T = 1.5, 2 .. 4): et = h^2, e1 = h^2T with the same h
 //   TWO     both, each by itself
 //   PLAIN1, PLAIN2   (x - ref) first and expf, et alone or both: rows of f32 logits, and bf16 rows whose largest entry is
 //           beyond 1e4 (all of it masked by the type's lowest value, say): there the rounding of ref / T is felt

@@ -61,7 +61,6 @@ struct RowSlice {
     w1 = max(min(hi, (lead + n) / V), w0);
   }
   __device__ __forceinline__ int first(int vec) const { return vec * V - lead; }  // row index of its first element
-  __device__ __forceinline__ bool edges() const { return w0 > lo || w1 < hi; }
   // a vector that reaches beyond an end of the row, -inf in the places outside
   __device__ __noinline__ uint4 load_edge(int vec) const {
     uint32_t u[4];
@@ -120,11 +119,6 @@ __device__ __forceinline__ uint64_t ld_cluster_u64(uint32_t addr) {
   asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
-  int v;
-  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-  return v;
-}
 // arrival that publishes this thread's earlier writes to the peer that waits on the barrier
 __device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
@@ -154,8 +148,7 @@ __device__ __forceinline__ void mbar_wait_cluster(uint64_t* bar, uint32_t parity
 // ---- one group of GT threads
 template <int GT>
 __device__ __forceinline__ void group_sync(int g) {
-  if constexpr (GT == 32) __syncwarp();
-  else asm volatile("bar.sync %0, %1;" ::"r"(1 + g), "n"(GT) : "memory");
+  asm volatile("bar.sync %0, %1;" ::"r"(1 + g), "n"(GT) : "memory");
 }
 // sum / maximum over W consecutive lanes
 template <int W>

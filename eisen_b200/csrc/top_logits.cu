@@ -1,11 +1,14 @@
 // The k largest logits of every row in descending order (equal values: the lowest index first), and the row's
 // log-sum-exp at a temperature: what a teacher hands to a student (distill.cu).
 //
-// A row is read once, into shared memory (row_pipe.cuh).  A group of GT threads then
-//   1. takes the largest element of every thread's share: the k-th largest of these is a threshold that at least k
+// The threads of a CTA
+//   1. take the largest element of every thread's share: the k-th largest of these is a threshold that at least k
 //      elements of the row reach and, on rows in no special order, few more do;
-//   2. lists the elements that reach it, and adds up the exponentials in the same pass;
-//   3. ranks the listed ones against each other.
+//   2. list the elements that reach it;
+//   3. rank the listed ones against each other.
+// Few rows (two per SM at most) are read once, into shared memory (row_pipe.cuh, split over a cluster's CTAs where they alone
+// leave SMs idle), and the exponentials are added up in the second pass.  Rows in numbers stay where they are: many small CTAs read
+// them once for the maxima and the sum, and note which vectors to look into again (top_stream_kernel).
 // Keys are 64 bits, value above complemented index, so every two differ and nothing depends on the order of arrival.
 // Rows whose large values sit in a few threads' shares (or are equal in thousands) overflow the list; for them the
 // exact threshold is found digit by digit over all elements, first of the value, then of the index.
@@ -147,17 +150,13 @@ __device__ __forceinline__ void each_rank(uint64_t* list, int listed, int most, 
 // how many of a group's threads say so (a barrier of the group)
 template <int GT>
 __device__ __forceinline__ int group_count(int g, bool yes) {
-  if constexpr (GT == 32) {
-    return __popc(__ballot_sync(0xffffffffu, yes));
-  } else {
-    int n;
-    asm volatile(
-        "{\n.reg .pred p;\nsetp.ne.u32 p, %1, 0;\nbar.red.popc.u32 %0, %2, %3, p;\n}"
-        : "=r"(n)
-        : "r"((uint32_t)yes), "r"(1 + g), "n"(GT)
-        : "memory");
-    return n;
-  }
+  int n;
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.u32 p, %1, 0;\nbar.red.popc.u32 %0, %2, %3, p;\n}"
+      : "=r"(n)
+      : "r"((uint32_t)yes), "r"(1 + g), "n"(GT)
+      : "memory");
+  return n;
 }
 
 // One warp: the bin of 256 at which the count from the top reaches `want`.  out = bin, count above it, count in it.
@@ -250,18 +249,18 @@ __device__ __forceinline__ void each_element(const RowSlice<T>& s, const uint4* 
 
 __host__ __device__ constexpr int top_list(int k) { return k <= 64 ? 256 : 1024; }  // entries of a group's list
 
-template <typename T, int GT, int G>
-__global__ void __launch_bounds__(GT * G + 32, 1)
+template <typename T, int GT>
+__global__ void __launch_bounds__(GT + 32, 1)
 top_pipe_kernel(const TopParams p) {
   constexpr int V = VecOf<T>::N, GW = GT / 32;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ RowRing ring;
-  __shared__ uint64_t xbar[G], xdone[G];  // all slices' lists are there; the first CTA has read them
-  __shared__ float s_max[G][GW], s_sum[G][GW];
-  __shared__ uint32_t s_range[G][GW];
-  __shared__ int s_count[G], s_hits[G];
-  __shared__ __align__(8) float s_slice[G][2];  // a slice's maximum and sum
-  __shared__ TopSelect s_sel[G];
+  __shared__ uint64_t xbar, xdone;  // all slices' lists are there; the first CTA has read them
+  __shared__ float s_max[GW], s_sum[GW];
+  __shared__ uint32_t s_range[GW];
+  __shared__ int s_count, s_hits;
+  __shared__ __align__(8) float s_slice[2];  // a slice's maximum and sum
+  __shared__ TopSelect s_sel;
   const int tid = threadIdx.x, lane = tid & 31;
   const int C = p.shape.cluster, k = p.k, n = p.vocab, cap = top_list(k);
   const int rank = C > 1 ? (int)cluster_ctarank() : 0;
@@ -269,29 +268,26 @@ top_pipe_kernel(const TopParams p) {
   const int n_mine = row0 < p.rows ? (int)((p.rows - row0 + stride - 1) / stride) : 0;
   ring_init(ring, p.shape.stages, GW);
   if (tid == 0) {
-    for (int g = 0; g < G; ++g) {
-      mbar_init(&xbar[g], C);
-      mbar_init(&xdone[g], 1);
-    }
+    mbar_init(&xbar, C);
+    mbar_init(&xdone, 1);
     fence_mbar_init();
   }
   __syncthreads();
   if (C > 1) cluster_sync_all();
   const T* logits = reinterpret_cast<const T*>(p.logits);
   auto slice_of = [&](long long row) { return RowSlice<T>(logits + row * p.ld, n, rank, p.shape.cluster_log2); };
-  if (tid >= GT * G) {
+  if (tid >= GT) {
     ring_load<T>(ring, smem, p.shape.stages, p.shape.stage_bytes, n_mine, row0, stride, slice_of, [](long long) { return false; });
   } else {
-    const int g = tid / GT, gt = tid % GT, warp = gt >> 5;
-    uint64_t* list = reinterpret_cast<uint64_t*>(smem + (size_t)p.shape.stages * p.shape.stage_bytes) + (size_t)g * (cap + cap / 2 + 9 * TOP_MAX_K);
+    const int gt = tid, warp = gt >> 5;
+    uint64_t* list = reinterpret_cast<uint64_t*>(smem + (size_t)p.shape.stages * p.shape.stage_bytes);
     int* hits = reinterpret_cast<int*>(list + cap);  // vectors with an element that reaches the threshold
     uint64_t* best = list + cap + cap / 2;  // this slice's k largest in descending order (clusters)
     uint64_t* all = best + TOP_MAX_K;       // every slice's, in the first CTA
-    int stage = g - G;  // the stage of row i, and its phase; a ring has at least G stages
+    int stage = -1;  // the stage of row i, and its phase
     uint32_t phase = 0, turn = 0;
-    for (int i = g; i < n_mine; i += G, ++turn) {
-      stage += G;
-      if (stage >= p.shape.stages) { stage -= p.shape.stages; phase ^= 1; }
+    for (int i = 0; i < n_mine; ++i, ++turn) {
+      if (++stage == p.shape.stages) { stage = 0; phase ^= 1; }
       const long long row = row0 + (long long)i * stride;
       const RowSlice<T> s = slice_of(row);
       // the vectors at the row's ends, by the threads that walk over them
@@ -316,19 +312,19 @@ top_pipe_kernel(const TopParams p) {
           if (v + q * GT < cnt) m[q] = max_nan(m[q], vec_max<T>(vec[v + q * GT]));
       }
       const float most = max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3]));
-      if (gt == 0) { s_count[g] = 0; s_hits[g] = 0; }
+      if (gt == 0) { s_count = 0; s_hits = 0; }
       const uint32_t top_key = gt < cnt ? order_key(most) >> 16 : 0;
       const float wm = warp_max(most);  // drops NaN, which the sum brings back
       const uint32_t k_hi = __reduce_max_sync(0xffffffffu, top_key);
       const uint32_t k_lo = __reduce_min_sync(0xffffffffu, gt < cnt ? top_key : 0xffffu);
-      if (lane == 0) { s_max[g][warp] = wm; s_range[g][warp] = (k_hi << 16) | k_lo; }
-      group_sync<GT>(g);
+      if (lane == 0) { s_max[warp] = wm; s_range[warp] = (k_hi << 16) | k_lo; }
+      group_sync<GT>(0);
       // the bits in which the threads' maxima agree are the threshold's too
       uint32_t hi16 = 0, lo16 = 0xffffu;
 #pragma unroll
       for (int w = 0; w < GW; ++w) {
-        hi16 = max(hi16, s_range[g][w] >> 16);
-        lo16 = min(lo16, s_range[g][w] & 0xffffu);
+        hi16 = max(hi16, s_range[w] >> 16);
+        lo16 = min(lo16, s_range[w] & 0xffffu);
       }
       const int bits = 32 - __clz(hi16 ^ lo16);
       // ---- threshold: the kk-th largest of the threads' maxima in their upper 16 bits, by bisection.  Where kk is more than
@@ -339,7 +335,7 @@ top_pipe_kernel(const TopParams p) {
 #pragma unroll 1
         for (int bit = bits - 1; bit >= 0; --bit) {
           const uint32_t trial = tau | (1u << bit);
-          if (group_count<GT>(g, top_key >= trial) >= kk) tau = trial;  // trial is not 0: threads without a share do not count
+          if (group_count<GT>(0, top_key >= trial) >= kk) tau = trial;  // trial is not 0: threads without a share do not count
         }
       } else if (kk <= min(cnt, 4 * GT)) {
         uint32_t key[4];
@@ -350,12 +346,12 @@ top_pipe_kernel(const TopParams p) {
           const uint32_t trial = tau | (1u << bit);  // never 0: places without a share do not count
           int total = 0;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) total += group_count<GT>(g, key[q] >= trial);
+          for (int q = 0; q < 4; ++q) total += group_count<GT>(0, key[q] >= trial);
           if (total >= kk) tau = trial;
         }
       }
-      group_sync<GT>(g);
-      float ref = lanes_max<GW>(s_max[g][lane % GW]);
+      group_sync<GT>(0);
+      float ref = lanes_max<GW>(s_max[lane % GW]);
       if (ref == -INFINITY) ref = 0.0f;
       // every element whose key reaches tau; NaN does, and so does everything where tau is 0
       const float floor_value = key_value(tau << 16);
@@ -395,17 +391,17 @@ top_pipe_kernel(const TopParams p) {
           if (lane >= o) before += up;
         }
         int at = 0;
-        if (lane == 31 && before) at = atomicAdd(&s_hits[g], before);
+        if (lane == 31 && before) at = atomicAdd(&s_hits, before);
         at = __shfl_sync(0xffffffffu, at, 31) + before - mine;
         for (; noted; noted &= noted - 1, ++at)
           if (at < cap) hits[at] = v0 + (__ffs(noted) - 1) * GT;
       }
       float sum = (acc[0] + acc[1]) + (acc[2] + acc[3]);
       sum = warp_sum(sum);
-      if (lane == 0) s_sum[g][warp] = sum;
-      group_sync<GT>(g);
-      sum = lanes_sum<GW>(s_sum[g][lane % GW]);
-      const int noted = s_hits[g];
+      if (lane == 0) s_sum[warp] = sum;
+      group_sync<GT>(0);
+      sum = lanes_sum<GW>(s_sum[lane % GW]);
+      const int noted = s_hits;
       if (noted <= cap) {
         for (int j = gt; j < noted; j += GT) {
           float x[V];
@@ -414,7 +410,7 @@ top_pipe_kernel(const TopParams p) {
           uint32_t in = 0;
 #pragma unroll
           for (int c = 0; c < V; ++c) in |= (uint32_t)(!(x[c] < floor_value) && e + c >= 0 && e + c < n) << c;
-          int at = atomicAdd(&s_count[g], __popc(in));
+          int at = atomicAdd(&s_count, __popc(in));
 #pragma unroll
           for (int c = 0; c < V; ++c)
             if ((in >> c) & 1) {
@@ -423,23 +419,23 @@ top_pipe_kernel(const TopParams p) {
             }
         }
       }
-      group_sync<GT>(g);
-      int listed = noted <= cap ? s_count[g] : cap + 1;
+      group_sync<GT>(0);
+      int listed = noted <= cap ? s_count : cap + 1;
       if (listed > cap) {
         uint32_t value, last;
-        exact_threshold<GT>(s_sel[g], gt, kk, here, value, last, [&](auto f) { each_element<T, GT>(s, vec, gt, f); },
-                            [&]() { group_sync<GT>(g); });
-        if (gt == 0) s_count[g] = 0;
-        group_sync<GT>(g);
+        exact_threshold<GT>(s_sel, gt, kk, here, value, last, [&](auto f) { each_element<T, GT>(s, vec, gt, f); },
+                            [&]() { group_sync<GT>(0); });
+        if (gt == 0) s_count = 0;
+        group_sync<GT>(0);
         each_element<T, GT>(s, vec, gt, [&](int e, float x) {
           const uint32_t q = order_key(x);
           if (q > value || (q == value && (uint32_t)e <= last)) {
-            const int at = atomicAdd(&s_count[g], 1);
+            const int at = atomicAdd(&s_count, 1);
             if (at < cap) list[at] = ((uint64_t)q << 32) | (uint32_t)~e;
           }
         });
-        group_sync<GT>(g);
-        listed = min(s_count[g], cap);
+        group_sync<GT>(0);
+        listed = min(s_count, cap);
       }
       fence_proxy_async_smem();  // the vectors at the ends, before a copy takes their place
       mbar_arrive_warp(&ring.empty[stage]);
@@ -454,17 +450,17 @@ top_pipe_kernel(const TopParams p) {
       };
       if (C == 1) {
         if (gt == 0 && p.lse && top != INFINITY) p.lse[row] = ref * p.inv_t + logf(sum);
-        each_rank<GT>(list, listed, k, gt, [&]() { group_sync<GT>(g); }, [&](int r, uint64_t c) { if (r < k) put(r, c); });
-        group_sync<GT>(g);  // the list is read before the next row's takes its place
+        each_rank<GT>(list, listed, k, gt, [&]() { group_sync<GT>(0); }, [&](int r, uint64_t c) { if (r < k) put(r, c); });
+        group_sync<GT>(0);  // the list is read before the next row's takes its place
       } else {
-        if (gt == 0) { s_slice[g][0] = sum == 0.0f ? -INFINITY : ref; s_slice[g][1] = sum; }
+        if (gt == 0) { s_slice[0] = sum == 0.0f ? -INFINITY : ref; s_slice[1] = sum; }
         for (int j = gt + kk; j < k; j += GT) best[j] = 0;
-        each_rank<GT>(list, listed, k, gt, [&]() { group_sync<GT>(g); }, [&](int r, uint64_t c) { if (r < k) best[r] = c; });
-        group_sync<GT>(g);
-        if (gt == 0) mbar_arrive_release_cluster(mapa_cluster(smem_u32(&xbar[g]), 0));
+        each_rank<GT>(list, listed, k, gt, [&]() { group_sync<GT>(0); }, [&](int r, uint64_t c) { if (r < k) best[r] = c; });
+        group_sync<GT>(0);
+        if (gt == 0) mbar_arrive_release_cluster(mapa_cluster(smem_u32(&xbar), 0));
         if (rank == 0) {
-          mbar_wait_cluster(&xbar[g], turn & 1, &ring.abort_flag);
-          const uint32_t b0 = smem_u32(best), s0 = smem_u32(&s_slice[g][0]);
+          mbar_wait_cluster(&xbar, turn & 1, &ring.abort_flag);
+          const uint32_t b0 = smem_u32(best), s0 = smem_u32(&s_slice[0]);
           top = -INFINITY;
           for (int o = 0; o < C; ++o) top = fmaxf(top, __uint_as_float((uint32_t)ld_cluster_u64(mapa_cluster(s0, o))));
           // the slices' lists into this CTA's memory: a search over there costs its latency step by step
@@ -472,7 +468,7 @@ top_pipe_kernel(const TopParams p) {
             const int from = j / k;
             all[j] = ld_cluster_u64(mapa_cluster(b0 + 8 * (j - from * k), from));
           }
-          group_sync<GT>(g);
+          group_sync<GT>(0);
           for (int j = gt; j < C * k; j += GT) {
             const int from = j / k, at = j - from * k;
             const uint64_t c = all[j];
@@ -500,10 +496,10 @@ top_pipe_kernel(const TopParams p) {
             }
             p.lse[row] = r0 * p.inv_t + logf(gs);
           }
-          group_sync<GT>(g);
-          if (gt < C) mbar_arrive_release_cluster(mapa_cluster(smem_u32(&xdone[g]), gt));
+          group_sync<GT>(0);
+          if (gt < C) mbar_arrive_release_cluster(mapa_cluster(smem_u32(&xdone), gt));
         }
-        mbar_wait_cluster(&xdone[g], turn & 1, &ring.abort_flag);  // `best` may be written again
+        mbar_wait_cluster(&xdone, turn & 1, &ring.abort_flag);  // `best` may be written again
       }
     }
   }
@@ -750,7 +746,7 @@ int top_launch(TopParams& p, cudaStream_t s) {
   // few rows: all of a CTA's threads, and up to eight CTAs, for each of them
   if (p.rows <= 2LL * sm_count()) {
     p.shape = row_shape(p.rows, p.vocab, sizeof(T), lists + 9 * 8 * TOP_MAX_K, 3, 8192);
-    if (p.shape.stages) return launch_pipe<top_pipe_kernel<T, 512, 1>>("top_logits", p.shape, p.rows, 512 + 32, s, p);
+    if (p.shape.stages) return launch_pipe<top_pipe_kernel<T, 512>>("top_logits", p.shape, p.rows, 512 + 32, s, p);
   }
   const long long vectors = bytes / 16 + 2;  // a row that starts inside a vector touches one more
   p.keyed = vectors <= TS_KEYS;
