@@ -224,6 +224,7 @@ int eisen_linear_ce_bwd(void* stream, const void* h, long long ldh, const void* 
   if (!lse || (!dh && !dw)) return fail(EISEN_ERR_INVALID, "linear_ce_bwd: lse and one of dh, dw must not be null");
   if (!aligned16(dh) || !aligned16(dw)) return fail(EISEN_ERR_INVALID, "linear_ce_bwd: dh and dw must be 16-byte aligned");
   if (k % 8) return fail(EISEN_ERR_INVALID, "linear_ce_bwd: k must be a multiple of 8");
+  if ((dh && dh == h) || (dw && dw == w)) return fail(EISEN_ERR_INVALID, "linear_ce_bwd: a gradient may not go over its operand");
   const CePlan p = ce_plan(rows, k, vocab, piece);
   char* d = (char*)workspace;
   float* dh32 = (float*)(d + p.d_bytes);

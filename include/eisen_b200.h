@@ -360,7 +360,8 @@ int eisen_distill_fused(void* stream, const void* logits, long long ld, const in
  * The backward forms the logits again, `piece` vocabulary entries at a time (rounded to a multiple of 256; 0 = chosen
  * so that one [rows, piece] bf16 slab takes about 256 MB), and
  *   dh [rows, k] bf16 (op)= c D W^T,  dw (layout of w, leading dimension lddw, dw_dtype EISEN_BF16 or EISEN_F32) (op)= c H^T D,
- *   D = bf16(softmax(x) - onehot), zero for rows that do not count, c = normalizer * (*grad_out); dh or dw may be null.
+ *   D = bf16(softmax(x) - onehot), zero for rows that do not count, c = normalizer * (*grad_out); dh or dw may be null, and neither may lie over
+ *   an operand.
  * Sums over tokens and vocabulary are f32; dh is added up in f32 over the pieces, and dh and dw are rounded once, what they are
  * added to included.  Hidden states of
  * rows that do not count must be finite where dw is asked for (their zero gradient multiplies them).
